@@ -494,6 +494,66 @@ int64_t npamd_dense_gemm_workspace_bytes(int M, int N, int K);
 /* 1 where npamd_dense_gemm is the better choice for this shape against a library GEMM.  Host-only arithmetic. */
 int npamd_dense_gemm_preferred(int M, int N, int K);
 
+/* ------------------------------------- around the feed-forward half of a block ---- */
+/*
+ * Layer norm over the last dimension: out[m, i] = round((x[m, i] - mean) * rstd * weight[i] + bias[i]), f32 arithmetic, the variance
+ * (over H, not H - 1) taken around the mean.  x, weight, bias, out share `dtype` (NPAMD_F16 / NPAMD_BF16 / NPAMD_F32); weight and bias
+ * may be NULL; any H >= 1 and any alignment.  mean, rstd: NULL, or f32 [M] each, what the backward pass reads.  out may be x.
+ */
+int npamd_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, void* out, int64_t ldo,
+                     float* mean, float* rstd, int M, int H, float eps, int dtype, void* stream);
+
+/*
+ * Its backward pass: with xh = (x - mean) * rstd and g = dy * weight,
+ *   dx = rstd * (g - mean_i(g) - xh * mean_i(g * xh)),  dweight = sum_m dy * xh,  dbias = sum_m dy,
+ * all of `dtype`, f32 arithmetic, each rounded once.  dx, dweight and dbias may be NULL: not asked for.  dx may be dy or x (with the
+ * same row distance).  dweight and dbias are sums over strips of rows, added in a fixed order: the same from run to run; zero with M = 0.
+ * workspace: npamd_layer_norm_workspace_bytes(M, H) bytes of 16-byte aligned device memory where dweight or dbias is asked for,
+ * contents irrelevant; calls that overlap must not share one.
+ */
+int npamd_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
+                              const float* mean, const float* rstd, void* dx, int64_t lddx, void* dweight, void* dbias,
+                              int M, int H, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t npamd_layer_norm_workspace_bytes(int M, int H);
+
+/*
+ * Dense product with an epilogue: y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n], f32 up to one rounding.
+ * x, w, residual, y: act_dtype (NPAMD_F16 or NPAMD_BF16); bias: NULL, or bias_dtype NPAMD_F32 or act_dtype; residual: NULL, or
+ * [M, N] with row stride ldr, and may be y itself (same row distance).  activation: one of NPAMD_ACT_*; GELU is v * (1 + erf(v / sqrt 2)) / 2, GELU_TANH
+ * its form with tanh, SILU v / (1 + exp(-v)).  Any shape up to 32 tokens; past that K has to be a multiple of 8, x and w 16-byte
+ * aligned, ldx and ldw multiples of 8 and below NPAMD_TILE_MAX_STRIDE.
+ * workspace: optional, npamd_dense_gemm_act_workspace_bytes of them, 16-byte aligned, contents irrelevant; with less, K is not
+ * split over blocks.  Calls that overlap must not share one.
+ */
+#define NPAMD_ACT_NONE 0
+#define NPAMD_ACT_RELU 1
+#define NPAMD_ACT_GELU 2
+#define NPAMD_ACT_GELU_TANH 3
+#define NPAMD_ACT_SILU 4
+int npamd_dense_gemm_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
+                         int activation, const void* residual, int64_t ldr, void* y, int64_t ldy, int M, int N, int K,
+                         int act_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t npamd_dense_gemm_act_workspace_bytes(int M, int N, int K);
+
+/*
+ * A whole mixture-of-experts layer, M <= NPAMD_GEMV_MAX_M tokens:
+ *   p[m, :] = softmax(x[m] . router^T) over all E experts; the top_k largest are taken (ties: the lower index; NaN counts as largest), with
+ *   renormalize divided by their sum;  y[m] = sum over them of p[m, e] * down_e . (silu(gate_e . x[m]) * up_e . x[m]).
+ * x, router [E, H], y: act_dtype (NPAMD_F16 or NPAMD_BF16).  gate_up: [E, 2 I, H], an expert's I gate rows before its I up rows;
+ * down: [E, H, I].  nbits 16: dense, act_dtype.  nbits 4 / 8: codes packed as for npamd_q_gemv, w = (q - zero) * scale, scale f16
+ * [E, rows, K / group_size], zero f16 of the same shape or NULL (2^(nbits - 1)).  f32 accumulate; w is not rounded, silu(gate) * up is
+ * rounded to act_dtype, y once.
+ * H and I multiples of 64, group_size a power of two from 32 on that divides both, E <= 512, top_k <= 16, 16-byte aligned x,
+ * router and weights, ldx a multiple of 8; others are NPAMD_ERR_UNSUPPORTED or NPAMD_ERR_INVALID.
+ * workspace: npamd_moe_workspace_bytes bytes of 16-byte aligned device memory, contents irrelevant before and after; calls that
+ * overlap must not share one.
+ */
+int npamd_moe_layer(const void* x, int64_t ldx, const void* router, const void* gate_up, const void* gate_up_scale_f16,
+                    const void* gate_up_zero_f16, const void* down, const void* down_scale_f16, const void* down_zero_f16,
+                    void* y, int64_t ldy, int M, int E, int top_k, int H, int I, int nbits, int group_size, int renormalize,
+                    int act_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t npamd_moe_workspace_bytes(int M, int E, int top_k, int H, int I);
+
 #ifdef __cplusplus
 }
 #endif

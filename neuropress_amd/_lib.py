@@ -72,6 +72,13 @@ SIGNATURES: dict[str, list] = {
     "npamd_dense_gemm": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _i64, _vp],
     "npamd_dense_gemm_ragged": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _i64, _vp],
     "npamd_dense_gemm_workspace_bytes": [_int, _int, _int],
+    "npamd_layer_norm": [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _int, _int, ctypes.c_float, _int, _vp],
+    "npamd_layer_norm_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _int, _int, _int, _vp, _i64, _vp],
+    "npamd_layer_norm_workspace_bytes": [_int, _int],
+    "npamd_dense_gemm_act": [_vp, _i64, _vp, _i64, _vp, _int, _int, _vp, _i64, _vp, _i64, _int, _int, _int, _int, _vp, _i64, _vp],
+    "npamd_dense_gemm_act_workspace_bytes": [_int, _int, _int],
+    "npamd_moe_layer": [_vp, _i64] + [_vp] * 8 + [_i64] + [_int] * 9 + [_vp, _i64, _vp],
+    "npamd_moe_workspace_bytes": [_int] * 5,
     "npamd_dense_gemm_preferred": [_int, _int, _int],
     "npamd_gemv_blocks_preferred": [_int] * 7,
     "npamd_gather_columns": [_vp, _i64, _vp, _vp, _i64, _int, _int, _vp],
@@ -86,7 +93,8 @@ SIGNATURES: dict[str, list] = {
 }
 
 _RESTYPES = {"npamd_vq_sliced_workspace_bytes": _i64, "npamd_gemm_tile_workspace_bytes": _i64, "npamd_dense_gemm_workspace_bytes": _i64,
-             "npamd_vq_slice_workspace_bytes": _i64,
+             "npamd_vq_slice_workspace_bytes": _i64, "npamd_layer_norm_workspace_bytes": _i64, "npamd_dense_gemm_act_workspace_bytes": _i64,
+             "npamd_moe_workspace_bytes": _i64,
              "npamd_diag_reload_tuning": None}
 SLICED_HEADER_BYTES = 128
 SLICED_STATIC_WORKSPACE_BYTES = 4 * 1024 * 1024

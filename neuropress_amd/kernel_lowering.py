@@ -8,7 +8,8 @@ norm_backend).apply(model)`` / ``.from_config(src)``, ``is_lowered`` and
 
 ``apply`` runs the lowering passes in the reference's order (kernel_lowering.py:200-219):
 scalar-quantized embeddings, scalar-quantized linears, VQ linears, VQ embeddings and -- with
-``norm_backend`` ``"auto"`` or ``"cuda"`` -- the RMSNorms that live on a GPU.  When the lowered
+``norm_backend`` ``"auto"`` or ``"cuda"`` -- the RMSNorms that live on a GPU; ``"all"``: those and the
+``nn.LayerNorm`` there (no counterpart in the reference).  When the lowered
 model already sits on a GPU it then makes the tensors the decode kernels derive from the
 module buffers (:func:`prepare_decode`), so that no forward call has host work left to do.
 
@@ -121,6 +122,7 @@ def _meta_embedding(module: nn.Module, vocab: int, scale: float) -> nn.Module:
 
 def _kinds() -> tuple[_Kind, ...]:
     from .nn.np_embedding import NPEmbedding
+    from .nn.np_layer_norm import NPLayerNorm
     from .nn.np_linear import NPLinear
     from .nn.np_rms_norm import NPRMSNorm
     from .nn.np_vq_embedding import NPVQEmbedding
@@ -135,6 +137,7 @@ def _kinds() -> tuple[_Kind, ...]:
         _Kind(NPEmbedding, with_backend, lambda m: _meta_embedding(m, m.num_embeddings, m.embed_scale)),
         _Kind(NPVQEmbedding, lambda m: "NPVQEmbedding", lambda m: _meta_embedding(m, m.all_indices.shape[0], m.scale)),
         _Kind(NPRMSNorm, lambda m: "NPRMSNorm", lambda m: m.to_source_module()),
+        _Kind(NPLayerNorm, lambda m: "NPLayerNorm", lambda m: m.to_source_module()),
     )
 
 
@@ -181,6 +184,7 @@ class AutoKernelLowering(KernelLowering):
 
     def _passes(self) -> list[Callable[[nn.Module], object]]:
         from .nn.np_embedding import linearize_qtensor_embeddings
+        from .nn.np_layer_norm import linearize_layer_norms
         from .nn.np_linear import linearize_qtensor_weights
         from .nn.np_rms_norm import linearize_rms_norms
         from .nn.np_vq_embedding import linearize_vq_embeddings
@@ -192,8 +196,10 @@ class AutoKernelLowering(KernelLowering):
             lambda model: linearize_vq_weights(model, backend=self.vq_backend),
             linearize_vq_embeddings,
         ]
-        if self.norm_backend in ("auto", "cuda"):
+        if self.norm_backend in ("auto", "cuda", "all"):
             passes.append(linearize_rms_norms)
+        if self.norm_backend == "all":
+            passes.append(linearize_layer_norms)
         return passes
 
     def apply(self, model: nn.Module) -> None:
@@ -231,9 +237,12 @@ def unlower_model(model: nn.Module) -> None:
     """
     kinds = _kinds()
     restored: dict[str, nn.Module] = {}
-    for path, module in model.named_modules():
+    originals: dict[int, nn.Module | None] = {}  # a module that stands in several places is restored once
+    for path, module in model.named_modules(remove_duplicate=False):
         kind = _kind_of(module, kinds)
-        original = kind.restore(module) if kind is not None else None
+        if kind is not None and id(module) not in originals:
+            originals[id(module)] = kind.restore(module)
+        original = originals.get(id(module))
         if original is not None:
             restored[path] = original
     for path, original in restored.items():

@@ -1098,6 +1098,263 @@ def q_embedding(
     return out.reshape(*input_ids.shape, dim)
 
 
+# ---------------------------------------------------------------------------
+# Around the feed-forward half of a block: layer norm, the product with its epilogue, experts
+# ---------------------------------------------------------------------------
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on_device(t: torch.Tensor):
+    """A context in which *t*'s device is the current one (launches go to the current device whatever the stream's)."""
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _lead2d(t: torch.Tensor, rows: int, width: int) -> torch.Tensor:
+    """*t* ``[..., width]`` as *rows* rows for a kernel: a view where they lie at one distance, else a copy."""
+    return _rows(t if t.dim() == 2 else t.reshape(rows, width))
+
+
+def _norm_args(what: str, x: torch.Tensor, *params: torch.Tensor | None) -> int:
+    """The checks that the layer norm's functions share; returns the length of the normed dimension."""
+    _check_device(what, x, *params)
+    _dt(x.dtype, what)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"{what}: x must be [..., H] with H of at least 1")
+    h = x.shape[-1]
+    for p in params:
+        if p is None:
+            continue
+        if p.dim() != 1 or p.shape[0] != h:
+            raise RuntimeError(f"{what}: weight and bias must be 1-D [H] matching x.size(-1)")
+        if p.dtype != x.dtype:
+            raise RuntimeError(f"{what}: x, weight and bias must share dtype")
+    return h
+
+
+def _layer_norm(what, x, weight, bias, eps, stats):
+    h = _norm_args(what, x, weight, bias)
+    m = x.numel() // h
+    x2 = _lead2d(x, m, h)
+    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
+    out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    mean = rstd = None
+    if stats:
+        mean, rstd = (torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) for _ in range(2))
+    with _on_device(x):
+        _lib.call("npamd_layer_norm", x2.data_ptr(), x2.stride(0), _ptr(weight), _ptr(bias), out.data_ptr(), h, _ptr(mean), _ptr(rstd), m, h, float(eps),
+                  _DT[x.dtype], _stream(x))  # fmt: skip
+    return out, mean, rstd
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        out, mean, rstd = _layer_norm("layer_norm", x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        return *layer_norm_backward(dy, x, weight, mean, rstd, needs=ctx.needs_input_grad[:3]), None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension of *x* ``[..., H]`` (``npamd_layer_norm``): *weight* and *bias* ``[H]`` of its dtype or None; the result has x's dtype.
+
+    Where a gradient of x, weight or bias is recorded, the backward pass is :func:`layer_norm_backward`'s kernels (first derivatives).  Calls that torch follows in
+    other ways (forward mode, ``torch.func``, traces, autocast to another type) go through ``torch.nn.functional.layer_norm``.
+    """
+    followed = [t for t in (x, weight, bias) if t is not None and tracked(t)]
+    if not followed:
+        return _layer_norm("layer_norm", x, weight, bias, eps, False)[0]
+    _norm_args("layer_norm", x, weight, bias)
+    with torch.no_grad():  # what is left of it when no gradient is recorded
+        otherwise = any(tracked(t) for t in followed)
+    if otherwise:
+        return torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps)
+    return _LayerNorm.apply(x, weight, bias, eps)
+
+
+def layer_norm_stats(
+    x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`layer_norm` without a recorded gradient, and the mean and reciprocal standard deviation (float32 ``[...]``) that :func:`layer_norm_backward` takes."""
+    return _layer_norm("layer_norm_stats", x, weight, bias, eps, True)
+
+
+def layer_norm_backward(
+    dy: torch.Tensor,
+    x: torch.Tensor,
+    weight: torch.Tensor | None,
+    mean: torch.Tensor,
+    rstd: torch.Tensor,
+    needs: tuple[bool, bool, bool] = (True, True, True),
+) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of x, weight and bias (``npamd_layer_norm_backward``), in x's dtype; None where *needs* says no.  *mean*, *rstd*: of
+    :func:`layer_norm_stats`.  The same bits from run to run."""
+    what = "layer_norm_backward"
+    h = _norm_args(what, x, weight)
+    _check_device(what, x, dy, mean, rstd)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise RuntimeError(f"{what}: dy must have x's shape and dtype")
+    m = x.numel() // h
+    x2, dy2 = _lead2d(x, m, h), _lead2d(dy, m, h)
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.numel() != m:
+            raise RuntimeError(f"{what}: mean and rstd must be float32, one for each row of x")
+    weight = None if weight is None else weight.contiguous()
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if needs[0] else None
+    dw, db = (torch.empty(h, device=x.device, dtype=x.dtype) if need else None for need in needs[1:])
+    need = int(_lib.load().npamd_layer_norm_workspace_bytes(m, h)) if needs[1] or needs[2] else 0
+    ws = torch.empty(need // 4, device=x.device, dtype=torch.float32) if need else None
+    with _on_device(x):
+        _lib.call("npamd_layer_norm_backward", dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dx),
+                  h, _ptr(dw), _ptr(db), m, h, _DT[x.dtype], _ptr(ws), need, _stream(x))  # fmt: skip
+    return dx, dw, db
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _torch_linear_act(x, w, bias, activation, residual):
+    f = torch.nn.functional
+    y = f.linear(x, w, None if bias is None else bias.to(w.dtype))
+    if activation is not None:
+        y = f.gelu(y, approximate="tanh") if activation == "gelu_tanh" else getattr(f, activation)(y)
+    return y if residual is None else y + residual
+
+
+def dense_linear_act(
+    x: torch.Tensor,
+    w: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    activation: str | None = None,
+    residual: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``act(x @ w.T + bias) + residual`` of an fp16 / bf16 *x* ``[..., K]`` and a dense weight ``[N, K]`` of its dtype, rounded once (``npamd_dense_gemm_act``).
+
+    *activation*: None, ``"relu"``, ``"gelu"`` (with erf), ``"gelu_tanh"`` or ``"silu"``; *bias* ``[N]`` in float32 or x's dtype; *residual* ``[..., N]`` in x's
+    dtype.  Any sizes.  Calls that torch follows (:func:`tracked`) go through torch's own operations, which round in between.
+    """
+    what = "dense_linear_act"
+    _check_device(what, x, w, bias, residual)
+    if x.dtype not in (torch.float16, torch.bfloat16) or w.dtype != x.dtype or w.dim() != 2 or x.dim() < 1 or w.shape[1] != x.shape[-1]:
+        raise RuntimeError(f"{what}: x and w must be float16 or bfloat16 [..., K] and [N, K]")
+    if activation not in ACTIVATIONS:
+        raise RuntimeError(f"{what}: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    n, k = w.shape
+    if k < 1:
+        raise RuntimeError(f"{what}: K must be at least 1")
+    if bias is not None and (bias.dtype not in (torch.float32, x.dtype) or bias.shape != (n,)):
+        raise RuntimeError(f"{what}: bias must be [N] in float32 or x's dtype")
+    shape = (*x.shape[:-1], n)
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != shape):
+        raise RuntimeError(f"{what}: residual must be {list(shape)} in x's dtype")
+    if any(t is not None and tracked(t) for t in (x, w, bias, residual)):
+        return _torch_linear_act(x, w, bias, activation, residual)
+    m = x.numel() // k
+    x2 = _lead2d(x, m, k)
+    w = _rows(w)
+    bias = None if bias is None else bias.contiguous()
+    r2 = None if residual is None else _lead2d(residual, m, n)
+    y = torch.empty(shape, device=x.device, dtype=x.dtype)
+    need = int(_lib.load().npamd_dense_gemm_act_workspace_bytes(m, n, k))
+    ws = torch.empty(need // 4, device=x.device, dtype=torch.float32) if need > 0 else None
+    with _on_device(x):
+        _lib.call("npamd_dense_gemm_act", x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _ptr(bias), _lib.F32 if bias is None else _DT[bias.dtype],
+                  ACTIVATIONS[activation], _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), n, m, n, k, _DT[x.dtype], _ptr(ws), need, _stream(x))  # fmt: skip
+    return y
+
+
+class MoEExperts:
+    """The weights of a mixture-of-experts layer, checked once, for :func:`moe_layer`.
+
+    *router* ``[E, H]``.  *gate_up* ``[E, 2 I, H]`` (an expert's I gate rows, then its I up rows) and *down* ``[E, H, I]``: dense in router's dtype
+    (*nbits* 16), or uint8 codes of *nbits* 4 or 8 with the row length ``H * nbits / 8`` and ``I * nbits / 8`` (low nibble = even column), float16 scales
+    ``[E, rows, columns / group_size]`` and, for both weights or neither, float16 zero points of the scales' shape (default ``2 ** (nbits - 1)``).
+    """
+
+    def __init__(
+        self,
+        router: torch.Tensor,
+        gate_up: torch.Tensor,
+        down: torch.Tensor,
+        *,
+        nbits: int = 16,
+        group_size: int = 32,
+        gate_up_scale: torch.Tensor | None = None,
+        gate_up_zero: torch.Tensor | None = None,
+        down_scale: torch.Tensor | None = None,
+        down_zero: torch.Tensor | None = None,
+    ):
+        what = "MoEExperts"
+        _check_device(what, router, gate_up, down, gate_up_scale, gate_up_zero, down_scale, down_zero)
+        if nbits not in (4, 8, 16):
+            raise RuntimeError(f"{what}: nbits must be 4, 8 or 16 (dense), got {nbits}")
+        if router.dtype not in (torch.float16, torch.bfloat16) or router.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
+            raise RuntimeError(f"{what}: router must be float16 or bfloat16 [E, H], gate_up [E, 2 I, H] and down [E, H, I]")
+        e, h = router.shape
+        i = gate_up.shape[1] // 2
+        if nbits != 16 and group_size < 1:
+            raise RuntimeError(f"{what}: group_size must be positive, got {group_size}")
+        dtype = router.dtype if nbits == 16 else torch.uint8
+        for name, w, rows, cols, scale, zero in (("gate_up", gate_up, 2 * i, h, gate_up_scale, gate_up_zero), ("down", down, h, i, down_scale, down_zero)):
+            if w.dtype != dtype or w.shape != (e, rows, cols if nbits == 16 else cols * nbits // 8):
+                raise RuntimeError(f"{what}: {name} must be {dtype} {[e, rows, cols if nbits == 16 else cols * nbits // 8]}, got {w.dtype} {list(w.shape)}")
+            if nbits == 16:
+                if scale is not None or zero is not None:
+                    raise RuntimeError(f"{what}: dense weights have no scales or zero points")
+                continue
+            if scale is None or (zero is None) != (gate_up_zero is None):
+                raise RuntimeError(f"{what}: codes need scales for both weights, and zero points for both or neither")
+            for t in (scale, zero):
+                if t is not None and (t.dtype != torch.float16 or t.shape != (e, rows, cols // group_size) or cols % group_size):
+                    raise RuntimeError(f"{what}: scales and zero points of {name} must be float16 {[e, rows, cols // group_size]}")
+        self.experts, self.hidden, self.inter, self.nbits, self.group_size = e, h, i, int(nbits), int(group_size)
+        self.router, self.gate_up, self.down = router.detach().contiguous(), gate_up.detach().contiguous(), down.detach().contiguous()
+        self.gate_up_scale, self.gate_up_zero, self.down_scale, self.down_zero = (
+            None if t is None else t.detach().contiguous() for t in (gate_up_scale, gate_up_zero, down_scale, down_zero)
+        )
+
+
+def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: bool = True) -> torch.Tensor:
+    """A whole mixture-of-experts layer for up to 32 tokens *x* ``[..., H]`` (``npamd_moe_layer``): softmax router over all experts, the *top_k* largest (ties: the
+    lower index; divided by their sum with *renormalize*), ``down(silu(gate(x)) * up(x))`` of each, weighted sum.  For inference: calls that torch follows
+    (:func:`tracked`) are refused."""
+    what = "moe_layer"
+    _check_device(what, x, experts.router)
+    h = experts.hidden
+    if x.dtype != experts.router.dtype or x.dim() < 1 or x.shape[-1] != h:
+        raise RuntimeError(f"{what}: x must be {experts.router.dtype} [..., {h}], got {x.dtype} {list(x.shape)}")
+    if tracked(x):
+        raise RuntimeError(f"{what}: for inference only: no gradient, trace or transform of torch can follow it")
+    m, e, i = x.numel() // h, experts.experts, experts.inter
+    x2 = _lead2d(x, m, h)
+    if x2.stride(0) % 8 or x2.data_ptr() % 16:
+        x2 = torch.clone(x2, memory_format=torch.contiguous_format)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    need = int(_lib.load().npamd_moe_workspace_bytes(m, e, int(top_k), h, i))
+    ws = torch.empty(need // 4, device=x.device, dtype=torch.float32) if need > 0 else None
+    with _on_device(x):
+        _lib.call("npamd_moe_layer", x2.data_ptr(), x2.stride(0), experts.router.data_ptr(), experts.gate_up.data_ptr(), _ptr(experts.gate_up_scale),
+                  _ptr(experts.gate_up_zero), experts.down.data_ptr(), _ptr(experts.down_scale), _ptr(experts.down_zero), y.data_ptr(), h, m, e, int(top_k), h, i,
+                  experts.nbits, experts.group_size, int(bool(renormalize)), _DT[x.dtype], _ptr(ws), need, _stream(x))  # fmt: skip
+    return y
+
+
 # The functions a lowered module's call plan stands in for.  Replacing one (instrumentation, a test's spy) makes the
 # plans step aside, so that the replacement is called.
 WRAPPERS = {

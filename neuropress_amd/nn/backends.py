@@ -89,11 +89,12 @@ class EmbeddingBackend(_StrEnum):
 
 
 class NormBackend(_StrEnum):
-    """Valid backends for RMSNorm modules (:class:`.NPRMSNorm`)."""
+    """Valid backends for norms (:class:`.NPRMSNorm`, and with ``"all"`` :class:`.NPLayerNorm`)."""
 
     AUTO = "auto"
     DEFAULT = "default"
     CUDA = "cuda"
+    ALL = "all"
 
 
 class VQBackend(_StrEnum):

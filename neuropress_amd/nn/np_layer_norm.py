@@ -1,0 +1,73 @@
+"""NPLayerNorm: layer norm as one HIP kernel, its backward pass as three, and the pass that installs it.
+
+A neighbour of :mod:`.np_rms_norm` for models that norm with mean and variance.  It replaces ``nn.LayerNorm`` over the last dimension on a GPU; the
+parameters stay the module's own objects, so optimizers and ``state_dict`` keys go on as before.  ``AutoKernelLowering`` runs the pass with
+``norm_backend="all"``.
+"""
+
+from __future__ import annotations
+
+import logging
+
+import torch
+from torch import nn
+
+__all__ = ["NPLayerNorm", "linearize_layer_norms"]
+
+log = logging.getLogger(__name__)
+
+
+class NPLayerNorm(nn.Module):
+    """``(x - mean) * rstd * weight + bias`` over the last dimension in f32 arithmetic, rounded once to x's dtype; differentiable."""
+
+    def __init__(self, weight: nn.Parameter | None, bias: nn.Parameter | None, width: int, eps: float = 1e-5, source: nn.Module | None = None) -> None:
+        super().__init__()
+        self.register_parameter("weight", weight)
+        self.register_parameter("bias", bias)
+        self.width = width
+        self.eps = eps
+        self.__dict__["_source"] = source  # outside the module tree: no state_dict entries
+
+    def to_source_module(self) -> nn.Module | None:
+        """The module this one replaced, with this one's parameters."""
+        source = self.__dict__.get("_source")
+        if source is not None:
+            source.weight, source.bias = self.weight, self.bias
+            source.train(self.training)
+        return source
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        w, b = (p if p is None or p.dtype == x.dtype else p.to(x.dtype) for p in (self.weight, self.bias))
+        if x.is_cuda:
+            from .. import kernels
+
+            if x.shape[-1:] != (self.width,):
+                raise RuntimeError(f"NPLayerNorm: x must be [..., {self.width}], got {list(x.shape)}")
+            return kernels.layer_norm(x, w, b, self.eps)
+        return nn.functional.layer_norm(x, (self.width,), w, b, self.eps)
+
+    def extra_repr(self) -> str:
+        return f"H={self.width}, eps={self.eps}, weight={self.weight is not None}, bias={self.bias is not None}"
+
+
+def _on_gpu(module: nn.Module) -> bool:
+    return module.weight is not None and module.weight.device.type == "cuda"
+
+
+def linearize_layer_norms(model: nn.Module) -> int:
+    """Replace every ``nn.LayerNorm`` inside *model* that has a weight on a GPU and norms one dimension; returns how many.  Subclasses are left alone: what
+    they override is theirs."""
+    from .backends import is_hip_backend_available
+
+    if not is_hip_backend_available():
+        log.debug("linearize_layer_norms: HIP kernel library unavailable - skipping")
+        return 0
+    fused: dict[int, NPLayerNorm] = {}  # a module that stands in several places is replaced by one
+    for name, mod in list(model.named_modules(remove_duplicate=False)):
+        if not name or type(mod) is not nn.LayerNorm or len(mod.normalized_shape) != 1 or not _on_gpu(mod):
+            continue
+        if id(mod) not in fused:
+            fused[id(mod)] = NPLayerNorm(mod.weight, mod.bias, mod.normalized_shape[0], mod.eps, source=mod).train(mod.training)
+        parent_name, _, attr = name.rpartition(".")
+        setattr(model.get_submodule(parent_name) if parent_name else model, attr, fused[id(mod)])
+    return len(fused)

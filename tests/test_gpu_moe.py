@@ -1,0 +1,237 @@
+"""The mixture-of-experts layer against the formulas in 64 bits.
+
+Tolerances: half a step of the output type; the rounding of silu(gate) * up, half a step e / 2 of each value, independent of each other: eight standard deviations of
+their sum through the down-projection, 8 (e / 2) / sqrt(3) sqrt(sum (p w h)^2); what f32 adds to sums of n terms, n 2^-24 of the sum of magnitudes with n at
+most K / 16 + 40 -- for codes times 2^7, as they are summed with an offset of up to 128 times their spread."""
+
+import pytest
+import torch
+
+from neuropress_amd.t2n.packing import BitPacking
+from tests import cases
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float16, torch.bfloat16]
+FORMATS = [(16, 32, False), (4, 32, False), (4, 128, True), (8, 64, False), (8, 32, True), (4, 64, False)]
+
+
+def _layer(seed, e, h, i, dtype, nbits, group=32, zero=False):
+    g = cases.gen(seed)
+    layer = {"router": (torch.randn(e, h, generator=g) * 2 * h**-0.5).to(dtype), "nbits": nbits, "group_size": group}
+    dense = {}
+    for name, rows, cols in (("gate_up", 2 * i, h), ("down", h, i)):
+        if nbits == 16:
+            layer[name] = (torch.randn(e, rows, cols, generator=g) * cols**-0.5).to(dtype)
+            dense[name] = layer[name].double()
+            continue
+        codes = torch.randint(0, 1 << nbits, (e * rows, cols), generator=g, dtype=torch.int64).to(torch.uint8)
+        layer[name] = BitPacking(nbits).compress(codes).reshape(e, rows, -1)
+        s = ((torch.rand(e, rows, cols // group, generator=g) + 0.5) * 3.5 / (1 << nbits) * cols**-0.5).half()
+        layer[name + "_scale"] = s
+        z = torch.full_like(s, float(1 << (nbits - 1)))
+        if zero:
+            z = layer[name + "_zero"] = (torch.randn(e, rows, cols // group, generator=g) * (1 << nbits) / 16 + (1 << (nbits - 1))).half()
+        wide = lambda t: t.double().repeat_interleave(group, -1)
+        dense[name] = (codes.reshape(e, rows, cols).double() - wide(z)) * wide(s)
+    return layer, dense
+
+
+def _experts(layer):
+    from neuropress_amd import kernels
+
+    return kernels.MoEExperts(**{k: v.to("cuda") if isinstance(v, torch.Tensor) else v for k, v in layer.items()})
+
+
+def _reference(x, layer, dense, top_k, renormalize):
+    """The result and how far f32 sums and the rounding of h may take it, all in 64 bits on the CPU."""
+    xd, dtype = x.double(), x.dtype
+    logits = xd @ layer["router"].double().T
+    p = torch.softmax(logits, -1)
+    order = torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    p = p.gather(1, order)
+    if renormalize:
+        p = p / p.sum(-1, keepdim=True)
+    h, i = dense["down"].shape[1:]
+    wide = 1.0 if layer["nbits"] == 16 else 128.0
+    y, rounding, slack = (torch.zeros_like(xd) for _ in range(3))
+    for m in range(x.shape[0]):
+        for t in range(top_k):
+            e = int(order[m, t])
+            both, spread = dense["gate_up"][e] @ xd[m], dense["gate_up"][e].abs() @ xd[m].abs()
+            gate, up = both[:i], both[i:]
+            v = torch.nn.functional.silu(gate) * up
+            dv = 2.0**-24 * wide * (h / 16 + 40) * (1.1 * spread[:i] * up.abs() + gate.abs() * spread[i:]) + 2.0**-20 * v.abs()
+            w, share = dense["down"][e], p[m, t]
+            y[m] += share * (w @ v)
+            rounding[m] += share**2 * (w.square() @ v.square())
+            # the router's own sum moves p by 2 n 2^-24 sum |x r| relative
+            moved = 2.0**-23 * (h / 16 + 40) * (xd[m].abs() @ layer["router"][e].double().abs())
+            slack[m] += share * (w.abs() @ (dv + 2.0**-24 * wide * (i / 16 + 40) * v.abs())) + moved * share * (w @ v).abs()
+    eps = torch.finfo(dtype).eps
+    return y, y.abs() * eps / 2 * 1.0001 + 8 * eps / 2 / 3**0.5 * rounding.sqrt() + slack + torch.finfo(dtype).smallest_normal * eps * (1 + i**0.5)
+
+
+def _check(y, ref, tol, dtype):
+    assert y.dtype == dtype and y.shape == ref.shape
+    err = (y.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), f"{(err / tol).max().item():.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nbits,group,zero", FORMATS)
+@pytest.mark.parametrize("m,top_k", [(1, 2), (2, 1), (7, 3), (16, 2), (17, 4), (32, 8)])
+def test_formats_and_tokens(gpu, dtype, nbits, group, zero, m, top_k):
+    from neuropress_amd import kernels
+
+    e, h, i = 8, 256, 384
+    layer, dense = _layer(m + nbits, e, h, i, dtype, nbits, group, zero)
+    x = torch.randn(m, h, generator=cases.gen(m)).to(dtype)
+    experts = _experts(layer)
+    for renormalize in (True, False):
+        y = kernels.moe_layer(x.to(gpu), experts, top_k, renormalize)
+        _check(y, *_reference(x, layer, dense, top_k, renormalize), dtype)
+    assert torch.equal(kernels.moe_layer(x.to(gpu), experts, top_k, False), y), "the same inputs, other bits"
+
+
+@pytest.mark.parametrize("nbits,group,zero", FORMATS[:4])
+@pytest.mark.parametrize("e,top_k,h,i,m", [(1, 1, 64, 64, 3), (1, 1, 128, 128, 32), (3, 3, 128, 640, 5), (64, 8, 384, 128, 9), (60, 4, 128, 1408, 2), (130, 5, 192, 192, 31),
+                                           (512, 16, 128, 128, 4), (4, 2, 1152, 2304, 1)])  # fmt: skip
+def test_sizes(gpu, nbits, group, zero, e, top_k, h, i, m):
+    from neuropress_amd import kernels
+
+    if nbits != 16 and (h % group or i % group):
+        group = 64
+    layer, dense = _layer(e, e, h, i, torch.bfloat16, nbits, group, zero)
+    x = torch.randn(m, h, generator=cases.gen(m)).to(torch.bfloat16)
+    _check(kernels.moe_layer(x.to(gpu), _experts(layer), top_k), *_reference(x, layer, dense, top_k, True), torch.bfloat16)
+
+
+@pytest.mark.parametrize("nbits,group", [(16, 32), (4, 64)])
+@pytest.mark.parametrize("m", [1, 8, 32])
+def test_every_token_to_the_same_experts(gpu, nbits, group, m):
+    """One row of tokens: two experts take all of them, the others none; then each token an expert of its own."""
+    from neuropress_amd import kernels
+
+    e, h, i = 32, 256, 256
+    layer, dense = _layer(5, e, h, i, torch.float16, nbits, group)
+    x = torch.randn(1, h, generator=cases.gen(9)).half()
+    y = kernels.moe_layer(x.to(gpu).expand(m, h), _experts(layer), 2)
+    _check(y, *(t.expand(m, h) for t in _reference(x, layer, dense, 2, True)), torch.float16)
+    layer["router"] = torch.zeros(e, h).half()
+    layer["router"][:, :e] = torch.eye(e).half()
+    x = torch.randn(m, h, generator=cases.gen(9)).half()
+    x[:, :e] = 0
+    x[torch.arange(m), torch.arange(m)] = 12.0
+    _check(kernels.moe_layer(x.to(gpu), _experts(layer), 1), *_reference(x, layer, dense, 1, True), torch.float16)
+
+
+def test_ties_go_to_the_lower_index(gpu):
+    from neuropress_amd import kernels
+
+    e, h, i = 70, 128, 64
+    layer, dense = _layer(6, e, h, i, torch.bfloat16, 16)
+    for row in (torch.zeros(h), torch.ones(h) / 16):  # every expert has the same logit, zero or not
+        layer["router"] = row.to(torch.bfloat16).expand(e, h).contiguous()
+        x = torch.randn(4, h, generator=cases.gen(2)).to(torch.bfloat16)
+        for top_k in (1, 5, 16):
+            _check(kernels.moe_layer(x.to(gpu), _experts(layer), top_k, False), *_reference(x, layer, dense, top_k, False), torch.bfloat16)
+
+
+def test_values_that_are_not_finite_stay_where_they_are(gpu):
+    from neuropress_amd import kernels
+
+    for nbits in (16, 4):
+        layer, dense = _layer(7, 8, 128, 128, torch.float16, nbits)
+        x = torch.randn(6, 128, generator=cases.gen(4)).half()
+        clean = kernels.moe_layer(x.to(gpu), _experts(layer), 2)
+        order = torch.sort(x.double() @ layer["router"].double().T, dim=-1, descending=True, stable=True).indices[:, :2]
+        # an expert with infinite weights or scales reaches only the tokens that meet it
+        bad = int(order[0, 0])
+        if nbits == 16:
+            layer["down"][bad, 3, 5] = float("inf")
+        else:
+            layer["down_scale"][bad, 3, 1] = float("inf")
+        y = kernels.moe_layer(x.to(gpu), _experts(layer), 2).cpu()
+        meets = (order == bad).any(-1)
+        assert torch.equal(y[~meets], clean.cpu()[~meets]) and not y[meets][:, 3].isfinite().any()
+        others = [c for c in range(128) if c != 3]
+        assert torch.equal(y[:, others], clean.cpu()[:, others])
+        # a token that is not a number: its own row, and it picks experts that exist
+        x[2, 7] = float("nan")
+        y = kernels.moe_layer(x.to(gpu), _experts(_layer(7, 8, 128, 128, torch.float16, nbits)[0]), 2).cpu()
+        assert y[2].isnan().all() and torch.equal(y[[0, 1, 3, 4, 5]], clean.cpu()[[0, 1, 3, 4, 5]])
+
+
+def test_shapes_strides_and_no_tokens(gpu):
+    from neuropress_amd import kernels
+
+    layer, dense = _layer(8, 8, 128, 192, torch.bfloat16, 4)
+    experts = _experts(layer)
+    x = torch.randn(2, 6, 128, generator=cases.gen(1)).to(torch.bfloat16).to(gpu)
+    y = kernels.moe_layer(x, experts, 2)
+    assert y.shape == x.shape and torch.equal(y.view(12, 128), kernels.moe_layer(x.view(12, 128), experts, 2))
+    assert torch.equal(kernels.moe_layer(x[0, 0], experts, 2), kernels.moe_layer(x[0, :1], experts, 2)[0])
+    assert kernels.moe_layer(x[:, :0], experts, 2).shape == (2, 0, 128)
+    wide = torch.full((12, 136 + 3), float("nan"), dtype=torch.bfloat16, device=gpu)
+    for ld in (136, 139):
+        view = wide.view(-1)[: 12 * ld].view(12, ld)[:, :128]
+        view.copy_(x.view(12, 128))
+        assert torch.equal(kernels.moe_layer(view, experts, 2), y.view(12, 128))
+        wide.fill_(float("nan"))
+
+
+def test_captured_twice_and_on_two_streams(gpu):
+    """Two captured calls and eager ones, replayed in turn and side by side: each has scratch of its own."""
+    from neuropress_amd import kernels
+
+    layer, _ = _layer(9, 16, 256, 512, torch.float16, 4)
+    experts = _experts(layer)
+    xs = [torch.randn(m, 256, generator=cases.gen(m)).half().to(gpu) for m in (3, 12)]
+    for x in xs:
+        kernels.moe_layer(x, experts, 4)
+    torch.cuda.synchronize()
+    streams, graphs, outs = [torch.cuda.Stream() for _ in xs], [torch.cuda.CUDAGraph() for _ in xs], []
+    for x, st, graph in zip(xs, streams, graphs):
+        with torch.cuda.graph(graph, stream=st):
+            outs.append(kernels.moe_layer(x, experts, 4))
+    for seed in range(5):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=cases.gen(seed)).half())
+        want = [kernels.moe_layer(x, experts, 4) for x in xs]
+        torch.cuda.synchronize()
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_refusals(gpu):
+    from neuropress_amd import kernels
+
+    layer, _ = _layer(1, 4, 128, 128, torch.float16, 4)
+    experts = _experts(layer)
+    x = torch.randn(2, 128, device=gpu).half()
+    with pytest.raises(RuntimeError, match="at most 32 tokens"):
+        kernels.moe_layer(x[:1].expand(33, 128), experts, 2)
+    for top_k in (0, 5):
+        with pytest.raises(RuntimeError, match="bad shape"):
+            kernels.moe_layer(x, experts, top_k)
+    with pytest.raises(RuntimeError, match="x must be"):
+        kernels.moe_layer(x.float(), experts, 2)
+    with pytest.raises(RuntimeError, match="x must be"):
+        kernels.moe_layer(x[:, :64], experts, 2)
+    with pytest.raises(RuntimeError, match="inference only"):
+        kernels.moe_layer(x.clone().requires_grad_(), experts, 2)
+    odd = {k: v.to(gpu) if isinstance(v, torch.Tensor) else v for k, v in layer.items()}
+    with pytest.raises(RuntimeError, match="scales"):
+        kernels.MoEExperts(**{**odd, "down_scale": None})
+    with pytest.raises(RuntimeError, match="must be"):
+        kernels.MoEExperts(**{**odd, "down": odd["down"][:, :64].contiguous()})
+    with pytest.raises(RuntimeError, match="zero points"):
+        kernels.MoEExperts(**odd, gate_up_zero=odd["gate_up_scale"])
+    with pytest.raises(RuntimeError, match="nbits"):
+        kernels.MoEExperts(**{**odd, "nbits": 2})
+    dense, _ = _layer(1, 4, 96, 128, torch.float16, 16)
+    with pytest.raises(RuntimeError, match="multiples of 64"):
+        kernels.moe_layer(x[:, :96], _experts(dense), 2)
