@@ -1324,10 +1324,15 @@ class MoEExperts:
                 if t is not None and (t.dtype != torch.float16 or t.shape != (e, rows, cols // group_size) or cols % group_size):
                     raise RuntimeError(f"{what}: scales and zero points of {name} must be float16 {[e, rows, cols // group_size]}")
         self.experts, self.hidden, self.inter, self.nbits, self.group_size = e, h, i, int(nbits), int(group_size)
-        self.router, self.gate_up, self.down = router.detach().contiguous(), gate_up.detach().contiguous(), down.detach().contiguous()
-        self.gate_up_scale, self.gate_up_zero, self.down_scale, self.down_zero = (
-            None if t is None else t.detach().contiguous() for t in (gate_up_scale, gate_up_zero, down_scale, down_zero)
-        )
+
+        def kept(t: torch.Tensor | None) -> torch.Tensor | None:  # rows one behind the other, from a 16-byte address on
+            if t is None:
+                return None
+            t = t.detach().contiguous()
+            return t if t.data_ptr() % 16 == 0 else t.clone()
+
+        self.router, self.gate_up, self.down = kept(router), kept(gate_up), kept(down)
+        self.gate_up_scale, self.gate_up_zero, self.down_scale, self.down_zero = kept(gate_up_scale), kept(gate_up_zero), kept(down_scale), kept(down_zero)
 
 
 def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: bool = True) -> torch.Tensor:
@@ -1343,8 +1348,6 @@ def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: boo
         raise RuntimeError(f"{what}: for inference only: no gradient, trace or transform of torch can follow it")
     m, e, i = x.numel() // h, experts.experts, experts.inter
     x2 = _lead2d(x, m, h)
-    if x2.stride(0) % 8 or x2.data_ptr() % 16:
-        x2 = torch.clone(x2, memory_format=torch.contiguous_format)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     need = int(_lib.load().npamd_moe_workspace_bytes(m, e, int(top_k), h, i))
     ws = torch.empty(need // 4, device=x.device, dtype=torch.float32) if need > 0 else None

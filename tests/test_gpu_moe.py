@@ -178,6 +178,16 @@ def test_shapes_strides_and_no_tokens(gpu):
         view.copy_(x.view(12, 128))
         assert torch.equal(kernels.moe_layer(view, experts, 2), y.view(12, 128))
         wide.fill_(float("nan"))
+    odd = torch.empty(12 * 128 + 1, dtype=torch.bfloat16, device=gpu)[1:].view(12, 128)  # rows between two 16-byte addresses
+    odd.copy_(x.view(12, 128))
+    assert torch.equal(kernels.moe_layer(odd, experts, 2), y.view(12, 128))
+
+    def shifted(v):
+        if not isinstance(v, torch.Tensor):
+            return v
+        return torch.cat([v.reshape(-1)[:1], v.reshape(-1)]).to(gpu)[1:].view(v.shape)
+
+    assert torch.equal(kernels.moe_layer(x, kernels.MoEExperts(**{k: shifted(v) for k, v in layer.items()}), 2), y)
 
 
 def test_captured_twice_and_on_two_streams(gpu):
