@@ -23,8 +23,8 @@ using namespace npamd;
 
 namespace {
 
-constexpr int kMoeMaxTokens = NPAMD_GEMV_MAX_M, kMoeMaxExperts = 512, kMoeMaxTopK = 16, kMoeMaxPairs = kMoeMaxTokens * kMoeMaxTopK;
-constexpr int kMoeMaxWaves = 8;  // of a block
+constexpr int kMoeMaxTokens = NPAMD_GEMV_MAX_M, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
+constexpr int kMoeMaxWaves = 8, kMoeMaxParts = 8;  // of a block
 
 struct MoeArgs {
   const void *x, *router;
@@ -34,11 +34,40 @@ struct MoeArgs {
   int64_t ldx, ldy;
   int M, E, top_k, H, I, shift, renormalize;  // shift: log2(group / 32)
   float* logits;   // [M][E]
-  int32_t* ids;    // [M][top_k]
+  uint16_t* ids;   // [M][top_k]
   float* share;    // [M][top_k]
+  uint32_t* done;  // [H / 32] blocks of the down kernel that have left their part
+  float* parts;    // [part][H / 32][M * 32]
   uint16_t* xs;    // [M][H], rows as the up kernel reads them
   uint16_t* h;     // [M][top_k][I]
 };
+
+// Over a wave without LDS: each step takes a lane's value from another lane's register.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_move(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, lane_move<0x111, 0xF>(v));  // from 1, 2, 4, 8 lanes before, within 16 lanes
+  v = max(v, lane_move<0x112, 0xF>(v));
+  v = max(v, lane_move<0x114, 0xF>(v));
+  v = max(v, lane_move<0x118, 0xF>(v));
+  v = max(v, lane_move<0x142, 0xA>(v));  // lane 15 to the next 16, lane 31 to the upper half
+  v = max(v, lane_move<0x143, 0xC>(v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// The sum, in lane 63.
+__device__ __forceinline__ float wave_sum_last(float v) {
+  auto add = [&](uint32_t from) { v += __builtin_bit_cast(float, from); };
+  auto bits = [&] { return __builtin_bit_cast(uint32_t, v); };
+  add(lane_move<0x111, 0xF>(bits()));
+  add(lane_move<0x112, 0xF>(bits()));
+  add(lane_move<0x114, 0xF>(bits()));
+  add(lane_move<0x118, 0xF>(bits()));
+  add(lane_move<0x142, 0xA>(bits()));
+  add(lane_move<0x143, 0xC>(bits()));
+  return v;
+}
 
 // Eight 16-bit values at any even address.
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
@@ -60,137 +89,159 @@ __device__ __forceinline__ float dot8(const u32x4& a, const u32x4& b, float sum)
   return sum;
 }
 
-// The logits of one expert, TB tokens at a time; and every row of x, copied to where the up kernel reads it (NIBBLES: each octet in int4's order), by one block each.
+// The logits of one expert for TB tokens (blockIdx.y); and every row of x, copied to where the up kernel reads it (NIBBLES: each octet in int4's order), by one block
+// each.  It clears the down kernel's counters.
 template <int ACT, int TB, bool NIBBLES>
 __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a) {
-  __shared__ float part[4][kMoeMaxTokens];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x, octets = a.H / 8;
+  __shared__ float part[4][TB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x, octets = a.H / 8, m0 = blockIdx.y * TB;
   const auto* x = reinterpret_cast<const uint16_t*>(a.x);
   const u32x4* const router = reinterpret_cast<const u32x4*>(a.router) + (int64_t)e * octets;
-  for (int m0 = 0; m0 < a.M; m0 += TB) {
-    float v[TB];
+  if (e == 0 && m0 == 0)
+    for (int i = threadIdx.x; i < a.H / 32; i += 256) a.done[i] = 0;
+  float v[TB];
 #pragma unroll
-    for (int t = 0; t < TB; ++t) v[t] = 0.f;
-    for (int k = threadIdx.x; k < octets; k += 256) {
-      const u32x4 r = router[k];
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        const u32x4 xv = *reinterpret_cast<const u32x4_any*>(x + min(m0 + t, a.M - 1) * a.ldx + 8 * k);
-        v[t] = dot8<ACT>(xv, r, v[t]);
-      }
-    }
+  for (int t = 0; t < TB; ++t) v[t] = 0.f;
+#pragma unroll 2
+  for (int k = threadIdx.x; k < octets; k += 256) {
+    const u32x4 r = router[k];
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
-      const float s = wave_reduce_sum(v[t]);
-      if (lane == 0 && m0 + t < a.M) part[wave][m0 + t] = s;
+      const u32x4 xv = *reinterpret_cast<const u32x4_any*>(x + min(m0 + t, a.M - 1) * a.ldx + 8 * k);
+      v[t] = dot8<ACT>(xv, r, v[t]);
     }
   }
-  for (int m = e; m < a.M; m += a.E)
+#pragma unroll
+  for (int t = 0; t < TB; ++t) {
+    const float s = wave_sum_last(v[t]);
+    if (lane == 63) part[wave][t] = s;
+  }
+  for (int m = m0 + e; m < min(m0 + TB, a.M); m += a.E)
     for (int k = threadIdx.x; k < octets; k += 256) {
       const u32x4 xv = *reinterpret_cast<const u32x4_any*>(x + m * a.ldx + 8 * k);
       reinterpret_cast<u32x4*>(a.xs)[(int64_t)m * octets + k] = NIBBLES ? octet_order(xv) : xv;
     }
   __syncthreads();
-  if ((int)threadIdx.x < a.M) a.logits[threadIdx.x * a.E + e] = part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
+  const int t = threadIdx.x;
+  if (t < TB && m0 + t < a.M) a.logits[(m0 + t) * a.E + e] = part[0][t] + part[1][t] + part[2][t] + part[3][t];
 }
 
-// The routing of all tokens in a block's LDS.
+// The routing of all tokens, in a block's LDS.  An entry is an expert and up to `cap` of its pairs.
 struct MoeRoute {
-  int32_t ids[kMoeMaxPairs];  // [M][top_k]
-  float share[kMoeMaxPairs];
-  uint32_t met[kMoeMaxExperts / 32];  // bit e: some token meets expert e
-  uint16_t experts[kMoeMaxExperts];   // those, in order
-  int n_experts;
+  uint32_t* entries;  // [pairs] expert, and from bit 16 on the number of its first pair
+  uint32_t* met;      // [E] pairs of each expert, while the entries are made
+  int* counts;        // [wave][2] how many pairs the wave's lists hold
+  int* n_entries;
+  uint16_t* lists;    // [wave][2][16] the pairs of the entries that a wave is at
+  uint16_t* ids;      // [M][top_k]
+  static __host__ __device__ int bytes(int pairs, int waves) { return pairs * 4 + waves * 2 * (4 + 32) + 16 + (pairs + 1) / 2 * 4; }
+  // `met` lies where weights will.
+  __device__ __forceinline__ MoeRoute(uint8_t* at, int pairs, int waves, uint8_t* scratch) {
+    entries = reinterpret_cast<uint32_t*>(at);
+    counts = reinterpret_cast<int*>(entries + pairs);
+    n_entries = counts + waves * 2;
+    lists = reinterpret_cast<uint16_t*>(n_entries + 4);
+    ids = lists + waves * 32;
+    met = reinterpret_cast<uint32_t*>(scratch);
+  }
 };
 
-// One wave picks the experts of token m.
-__device__ __forceinline__ void pick_experts(const MoeArgs& a, int m, int lane, MoeRoute& route) {
+// One wave picks the experts of token m; `first`: and writes them down for the down kernel.
+__device__ __forceinline__ void pick_experts(const MoeArgs& a, int m, int lane, const MoeRoute& route, bool first) {
   constexpr int kPer = kMoeMaxExperts / 64;
   float v[kPer];
-  float most = -INFINITY, sum = 0.f;
+  uint32_t key[kPer];  // in the order of the logits, NaN above all; 0: none
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    v[i] = -INFINITY;
-    if (64 * i < a.E) v[i] = lane + 64 * i < a.E ? a.logits[m * a.E + lane + 64 * i] : -INFINITY;
-    most = fmaxf(most, v[i]);
+    key[i] = 0;
+    if (64 * i >= a.E) continue;
+    v[i] = lane + 64 * i < a.E ? a.logits[m * a.E + lane + 64 * i] : -INFINITY;
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v[i] + 0.f);  // minus zero is zero
+    if (lane + 64 * i < a.E) key[i] = v[i] != v[i] ? 0xFFFFFFFFu : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
   }
-#pragma unroll
-  for (int off = 32; off; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (64 * i < a.E && lane + 64 * i < a.E) sum += expf(v[i] - most);
-  sum = wave_reduce_sum(sum);
-  uint32_t taken = 0;
-  float mine = 0.f, total = 0.f;
+  float most = 0.f, sum = 0.f, mine = 0.f, total = 0.f;
   int id = 0;
   for (int t = 0; t < a.top_k; ++t) {
-    // the largest of what is left, NaN above all: an order of (value, -index) as one 64-bit number
-    uint64_t best = 0;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (64 * i < a.E) top = max(top, key[i]);
+    top = wave_max(top);
+    int e = 0;
+    bool found = false;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (64 * i >= a.E) break;
-      if (lane + 64 * i >= a.E || (taken >> i & 1)) continue;
-      const float l = v[i];
-      const uint32_t bits = __builtin_bit_cast(uint32_t, l + 0.f);  // minus zero is zero
-      const uint32_t order = l != l ? 0xFFFFFFFFu : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-      const uint64_t key = ((uint64_t)order << 32) | (uint32_t)(0xFFFFFFFFu - (lane + 64 * i));
-      best = key > best ? key : best;
+      if (64 * i >= a.E || found) continue;
+      const uint64_t with = __ballot(key[i] == top);
+      if (!with) continue;
+      found = true;
+      const int at = __ffsll((unsigned long long)with) - 1;
+      e = 64 * i + at;
+      if (lane == at) key[i] = 0;
     }
+    const float l = top == 0xFFFFFFFFu ? NAN : __builtin_bit_cast(float, top & 0x80000000u ? top & 0x7FFFFFFFu : ~top);
+    if (t == 0) {
+      most = l;
 #pragma unroll
-    for (int off = 32; off; off >>= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)best, off, 64);
-      best = other > best ? other : best;
+      for (int i = 0; i < kPer; ++i)
+        if (64 * i < a.E && lane + 64 * i < a.E) sum += __expf(v[i] - most);
+      sum = wave_sum_last(sum);
+      sum = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
     }
-    const int e = (int)(0xFFFFFFFFu - (uint32_t)best);
-    if ((e & 63) == lane) taken |= 1u << (e >> 6);
-    const uint32_t order = (uint32_t)(best >> 32), bits = order & 0x80000000u ? order & 0x7FFFFFFFu : ~order;
-    const float l = order == 0xFFFFFFFFu ? NAN : __builtin_bit_cast(float, bits);
-    const float p = expf(l - most) / sum;
+    const float p = __expf(l - most) / sum;
     total += p;
     if (lane == t) mine = p, id = e;
   }
   if (lane < a.top_k) {
-    route.ids[m * a.top_k + lane] = id;
-    route.share[m * a.top_k + lane] = a.renormalize ? mine / total : mine;
+    route.ids[m * a.top_k + lane] = (uint16_t)id;
+    if (first) {
+      a.ids[m * a.top_k + lane] = (uint16_t)id;
+      a.share[m * a.top_k + lane] = a.renormalize ? mine / total : mine;
+    }
   }
 }
 
-// The list of the experts that are met, from the pairs; all threads of the block, behind a barrier that follows the ids.
-__device__ __forceinline__ void list_experts(const MoeArgs& a, MoeRoute& route) {
-  constexpr int kWords = kMoeMaxExperts / 32;
-  if (threadIdx.x < kWords) route.met[threadIdx.x] = 0;
+// The entries, from the pairs; all threads of the block, behind a barrier that follows the ids.
+__device__ __forceinline__ void list_entries(const MoeArgs& a, const MoeRoute& route, int cap) {
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) route.met[e] = 0;
   __syncthreads();
-  for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) atomicOr(&route.met[route.ids[p] >> 5], 1u << (route.ids[p] & 31));
+  for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) atomicAdd(&route.met[route.ids[p]], 1u);
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
-    if (!(route.met[e >> 5] >> (e & 31) & 1)) continue;
-    int before = __popc(route.met[e >> 5] & ((1u << (e & 31)) - 1u));
-    for (int w = 0; w < e >> 5; ++w) before += __popc(route.met[w]);
-    route.experts[before] = (uint16_t)e;
-  }
-  if (threadIdx.x == 0) {
-    int n = 0;
-    for (int w = 0; w < kWords; ++w) n += __popc(route.met[w]);
-    route.n_experts = n;
+  if (threadIdx.x < 64) {
+    int before = 0;
+    for (int e0 = 0; e0 < a.E; e0 += 64) {
+      const int e = e0 + threadIdx.x, mine = e < a.E ? ((int)route.met[e] + cap - 1) / cap : 0;
+      int upto = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int other = __shfl_up(upto, off, 64);
+        if ((int)threadIdx.x >= off) upto += other;
+      }
+      for (int i = 0; i < mine; ++i) route.entries[before + upto - mine + i] = (uint32_t)(e | (i * cap) << 16);
+      before += __shfl(upto, 63, 64);
+    }
+    if (threadIdx.x == 0) *route.n_entries = before;
   }
   __syncthreads();
 }
 
-// The pairs of expert e in their order, into a wave's own list; returns how many.
-__device__ __forceinline__ int list_pairs(const MoeArgs& a, const MoeRoute& route, int e, int lane, uint16_t* list) {
+// The pairs of an entry in their order, into a wave's list; returns how many.
+__device__ __forceinline__ int list_pairs(const MoeArgs& a, const MoeRoute& route, uint32_t entry, int cap, int lane, uint16_t* list) {
+  const int e = entry & 0xFFFF, first = entry >> 16;
   int n = 0;
   for (int p0 = 0; p0 < a.M * a.top_k; p0 += 64) {
     const bool is = p0 + lane < a.M * a.top_k && route.ids[p0 + lane] == e;
     const uint64_t all = __ballot(is);
-    if (is) list[n + __popcll(all & ((1ull << lane) - 1ull))] = (uint16_t)(p0 + lane);
+    const int at = n + __popcll(all & ((1ull << lane) - 1ull)) - first;
+    if (is && at >= 0 && at < cap) list[at] = (uint16_t)(p0 + lane);
     n += __popcll(all);
   }
-  return n;
+  return min(n - first, cap);
 }
 
-// A step: KSTEP columns of 16 R rows of weights and of an expert's tokens, in a wave's own LDS: its tokens, 1024 / kXRow to a KiB (16-byte piece p of
-// token j in place p ^ (j & 15) of its row), then for each of the R row tiles its 16 rows (piece p of row r in place p ^ (r >> 1 & 7) of eight or p ^ r of 16) and its
-// scales and zero points, a dword for each row and 64 columns.
+// A step: kColumns columns of 16 R rows of weights and of an entry's tokens, in LDS in one of two places: the tokens, 1024 / kXRow to a KiB (16-byte piece p of
+// token j in place p ^ j of its row), and for each of a wave's R row tiles its 16 rows (piece p of row r in place p ^ (r >> 1 & 7) of eight or p ^ r of 16) and its
+// scales and zero points, a dword for each row and 64 columns.  All of it comes in whole lines, straight into LDS, a step ahead of the MFMAs.
 template <int FMT, bool ASYM>
 struct MoeStep {
   static constexpr int kColumns = FMT == 16 ? 128 : 256, kMfmas = kColumns / 32;
@@ -202,76 +253,99 @@ struct MoeStep {
   static constexpr int x_loads(int tokens) { return (tokens + kTokensPerLoad - 1) / kTokensPerLoad; }
 };
 
-template <int ACT, int FMT, bool ASYM, int MT, int R>
+// (v & MASK) | BITS in one instruction, which takes constants from registers only: one of them scalar.
+template <uint32_t MASK, uint32_t BITS>
+__device__ __forceinline__ uint32_t masked_or(uint32_t v) {
+  uint32_t mask = MASK, bits = BITS;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(bits));
+  return (v & mask) | bits;
+}
+
+// GROUP: MFMAs that see one scale group, one after the other into one sum.
+template <int ACT, int FMT, bool ASYM, int R, int GROUP>
 struct MoeWalk {
   using S = MoeStep<FMT, ASYM>;
-  static constexpr int kXLoads = S::x_loads(16 * MT);
-  uint8_t* mine;
-  uint32_t mine_lds;
-  int lane, c, q, K, chunks, groups, shift, x_bytes;  // x_bytes: LDS of the tokens
+  static constexpr int kXLoads = S::x_loads(16), kPlace = R * S::kItem;
+  uint8_t *own, *shared;  // LDS: the weights (two places of kPlace), the tokens (two of x_bytes)
+  int lane, c, q, K, groups, shift, x_bytes;
+  int x_first, x_stride;  // the loads of the tokens that this wave makes
   const uint8_t *w[R], *x;
-  const uint16_t *scale[R], *zero[R];
-  int count;  // tokens
-  uint32_t x_off[kXLoads];
-  f32x4 acc[R][MT];
+  const uint8_t *scale[R], *zero[R];
+  int x_loads;
+  uint32_t x_row[kXLoads], w_off[S::kCodeLoads];
+  f32x4 acc[R];
 
-  __device__ __forceinline__ MoeWalk(uint8_t* lds, int x_loads, int columns, int shift_) : mine(lds), K(columns), shift(shift_) {
+  __device__ __forceinline__ MoeWalk(uint8_t* weights_lds, uint8_t* tokens_lds, int most_x_loads, int columns, int shift_, int x_first_, int x_stride_)
+      : own(weights_lds), shared(tokens_lds), K(columns), shift(shift_), x_first(x_first_), x_stride(x_stride_) {
     lane = threadIdx.x & 63;
     c = lane & 15, q = lane >> 4;
-    mine_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    chunks = K / 64;
     groups = (K / 32) >> shift;
-    x_bytes = x_loads * 1024;
+    x_bytes = most_x_loads * 1024;
+#pragma unroll
+    for (int t = 0; t < S::kCodeLoads; ++t) {
+      const int row = t * S::kRowsPerLoad + lane / S::kSlots;
+      w_off[t] = (uint32_t)row * (uint32_t)(K / 8 * FMT);
+    }
     clear();
   }
+  static __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < R; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   // Row tile r: 16 rows from `row` on.
   __device__ __forceinline__ void rows(int r, const uint8_t* weights, const uint16_t* scales, const uint16_t* zeros, int64_t row) {
-    w[r] = weights + row * (int64_t)(K / 8 * FMT);
-    if constexpr (FMT != 16) scale[r] = scales + row * groups;
-    if constexpr (ASYM) zero[r] = zeros + row * groups;
+    w[r] = uniform_ptr(weights + row * (int64_t)(K / 8 * FMT));
+    if constexpr (FMT != 16) scale[r] = uniform_ptr((const uint8_t*)(scales + row * groups));
+    if constexpr (ASYM) zero[r] = uniform_ptr((const uint8_t*)(zeros + row * groups));
   }
-  // The tokens: row list[j] / divide of x.
+  // The tokens: rows list[j] / divide of x.
   __device__ __forceinline__ void tokens(const uint16_t* rows_of_x, const uint16_t* list, int n, int divide) {
     x = reinterpret_cast<const uint8_t*>(rows_of_x);
-    count = __builtin_amdgcn_readfirstlane(n);
+    x_loads = __builtin_amdgcn_readfirstlane(S::x_loads(n));
 #pragma unroll
     for (int i = 0; i < kXLoads; ++i) {
       const int j = min(i * S::kTokensPerLoad + lane / S::kXSlots, n - 1);
-      x_off[i] = (uint32_t)((int)list[j] / divide) * (uint32_t)(K * 2);
+      x_row[i] = (uint32_t)((int)list[j] / divide) * (uint32_t)(K * 2);
     }
   }
-  __device__ __forceinline__ void load(int step) {
+  __device__ __forceinline__ void load(int step, int place) {
+    int lane = this->lane;
+    asm volatile("" : "+v"(lane));  // as in multiply()
+    // pieces past the rows' end: the last one again
+    const int last_x = (K - step * S::kColumns) / 8 - 1, last_w = (K - step * S::kColumns) / 8 * FMT / 16 - 1;
+    const uint8_t* const xs = x + (int64_t)step * S::kXRow;
+    const uint32_t to_x = lds_address(shared) + (uint32_t)(place * x_bytes), to = lds_address(own) + (uint32_t)(place * kPlace);
 #pragma unroll
     for (int i = 0; i < kXLoads; ++i) {
-      if (i * S::kTokensPerLoad >= count) break;
-      const int j = i * S::kTokensPerLoad + lane / S::kXSlots;
-      const int p = step * S::kXSlots + ((lane % S::kXSlots) ^ (j & 15));
-      lds_load16(mine_lds + (uint32_t)(i * 1024), x_off[i] + (uint32_t)(min(p, K / 8 - 1) * 16), uniform_ptr(x));
+      if (i >= x_loads) break;
+      if (i % x_stride != x_first) continue;
+      const int p = (lane % S::kXSlots) ^ (i * S::kTokensPerLoad + lane / S::kXSlots);
+      lds_load16(to_x + (uint32_t)(i * 1024), x_row[i] + (uint32_t)(min(p, last_x) * 16), xs);
     }
-    const uint32_t row_bytes = (uint32_t)(K / 8 * FMT);
+    uint32_t at_scale = 0;
+    if constexpr (FMT != 16) {
+      const int kc = min(step * 4 + (lane & 3), K / 64 - 1);
+      at_scale = (((uint32_t)(lane >> 2) * (uint32_t)groups + (uint32_t)((2 * kc) >> shift)) * 2u) & ~3u;
+    }
+    uint32_t at[S::kCodeLoads];
+#pragma unroll
+    for (int t = 0; t < S::kCodeLoads; ++t) {
+      const int row = t * S::kRowsPerLoad + lane / S::kSlots, p = (lane % S::kSlots) ^ (S::kSlots == 8 ? (row >> 1) & 7 : row);
+      at[t] = w_off[t] + (uint32_t)min(p, last_w) * 16u;
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t dst = mine_lds + (uint32_t)(x_bytes + r * S::kItem);
+      const uint32_t dst = to + (uint32_t)(r * S::kItem);
 #pragma unroll
-      for (int t = 0; t < S::kCodeLoads; ++t) {
-        const int row = t * S::kRowsPerLoad + lane / S::kSlots;
-        const int p = step * S::kSlots + ((lane % S::kSlots) ^ (S::kSlots == 8 ? (row >> 1) & 7 : row));
-        lds_load16(dst + (uint32_t)(t * 1024), (uint32_t)row * row_bytes + (uint32_t)min(p, (int)row_bytes / 16 - 1) * 16u, uniform_ptr(w[r]));
-      }
-      if constexpr (FMT != 16) {
-        const int kc = min(step * 4 + (lane & 3), chunks - 1);
-        const uint32_t at = (((uint32_t)(lane >> 2) * (uint32_t)groups + (uint32_t)((2 * kc) >> shift)) * 2u) & ~3u;
-        lds_load4(dst + 16 * S::kRow, at, uniform_ptr(reinterpret_cast<const uint8_t*>(scale[r])));
-        if constexpr (ASYM) lds_load4(dst + 16 * S::kRow + 256, at, uniform_ptr(reinterpret_cast<const uint8_t*>(zero[r])));
-      }
+      for (int t = 0; t < S::kCodeLoads; ++t) lds_load16(dst + (uint32_t)(t * 1024), at[t], w[r] + (int64_t)step * S::kRow);
+      if constexpr (FMT != 16) lds_load4(dst + 16 * S::kRow, at_scale, scale[r]);
+      if constexpr (ASYM) lds_load4(dst + 16 * S::kRow + 256, at_scale, zero[r]);
     }
   }
+  // This wave's loads have arrived.
+  static __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
   // A constant operand: `even` and `odd` dwords.
   static __device__ __forceinline__ u32x4 constant(uint32_t even, uint32_t odd) { return u32x4{even, odd, even, odd}; }
 
@@ -291,11 +365,11 @@ struct MoeWalk {
       }
       return u32x4{o[0], o[1], o[2], o[3]};
     } else if constexpr (ACT == NPAMD_F16) {  // 1024 + q, 64 + q
-      return u32x4{(v[0] & 0x000F000Fu) | 0x64006400u, (v[0] & 0x00F000F0u) | 0x54005400u, ((v[0] >> 8) & 0x000F000Fu) | 0x64006400u,
-                   ((v[0] >> 8) & 0x00F000F0u) | 0x54005400u};
+      return u32x4{masked_or<0x000F000Fu, 0x64006400u>(v[0]), masked_or<0x00F000F0u, 0x54005400u>(v[0]), masked_or<0x000F000Fu, 0x64006400u>(v[0] >> 8),
+                   masked_or<0x00F000F0u, 0x54005400u>(v[0] >> 8)};
     } else {  // 128 + q
-      return u32x4{(v[0] & 0x000F000Fu) | 0x43004300u, ((v[0] >> 4) & 0x000F000Fu) | 0x43004300u, ((v[0] >> 8) & 0x000F000Fu) | 0x43004300u,
-                   ((v[0] >> 12) & 0x000F000Fu) | 0x43004300u};
+      return u32x4{masked_or<0x000F000Fu, 0x43004300u>(v[0]), masked_or<0x000F000Fu, 0x43004300u>(v[0] >> 4), masked_or<0x000F000Fu, 0x43004300u>(v[0] >> 8),
+                   masked_or<0x000F000Fu, 0x43004300u>(v[0] >> 12)};
     }
   }
   static constexpr bool kOffset = FMT == 4 || (FMT == 8 && (ACT == NPAMD_F16 || !ASYM));
@@ -311,226 +385,275 @@ struct MoeWalk {
   }
   static __device__ __forceinline__ u32x4 ones() { return ACT == NPAMD_F16 ? constant(0x3C003C00u, 0x3C003C00u) : constant(0x3F803F80u, 0x3F803F80u); }
 
-  // The step that has been loaded; `next` issues the loads of the one behind it, as soon as this one is in registers.
-  template <class Next>
-  __device__ __forceinline__ void compute(int step, Next&& next) {
-    const int in_lds = count;  // next() may go on to other tokens
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    u32x4 xa[MT][S::kMfmas];
-    uint32_t raw[R][S::kMfmas][S::kWords];
-    u32x4 sc[R], zp[R];
+
+
+
+  // The step in `place`, with `n` tokens.
+  __device__ __forceinline__ void multiply(int step, int place, int n) {
+    // Places in LDS are worked out anew every time: kept, they would take more registers than the waves that hide the waits can spare.
+    int c = this->c;
+    asm volatile("" : "+v"(c));
+    const int j = min(c, n - 1);  // rows past the tokens: one that nobody stores again
+    const uint8_t* const xrow = shared + place * x_bytes + j * S::kXRow;
+    const uint8_t* const base = own + place * kPlace;
+    const int swizzle = S::kSlots == 8 ? (c >> 1) & 7 : c;
+    const f32x4 zero4{0.f, 0.f, 0.f, 0.f};
+    auto group = [&](int g) __attribute__((always_inline)) {
+      u32x4 xa[GROUP];
+      f32x4 d[R], from = zero4, sum = zero4;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int j = min(16 * t + c, in_lds - 1);  // rows past the tokens: one that nobody stores again
-      const uint8_t* const row = mine + j * S::kXRow;
-#pragma unroll
-      for (int i = 0; i < S::kMfmas; ++i) xa[t][i] = *reinterpret_cast<const u32x4*>(row + (((4 * i + q) ^ (j & 15)) << 4));
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const uint8_t* const item = mine + x_bytes + r * S::kItem;
-      const uint8_t* const row = item + c * S::kRow;
-      const int swizzle = S::kSlots == 8 ? (c >> 1) & 7 : c;
-#pragma unroll
-      for (int i = 0; i < S::kMfmas; ++i) {
-        if constexpr (FMT == 4) {
-          raw[r][i][0] = *reinterpret_cast<const uint32_t*>(row + ((i ^ swizzle) << 4) + 4 * q);
-        } else if constexpr (FMT == 8) {
-          const u32x2 v = *reinterpret_cast<const u32x2*>(row + (((2 * i + (q >> 1)) ^ swizzle) << 4) + 8 * (q & 1));
-          raw[r][i][0] = v.x, raw[r][i][1] = v.y;
-        } else {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(row + (((4 * i + q) ^ swizzle) << 4));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) raw[r][i][e] = v[e];
-        }
-      }
-      if constexpr (FMT != 16) sc[r] = *reinterpret_cast<const u32x4*>(item + 16 * S::kRow + 16 * c);
-      if constexpr (ASYM) zp[r] = *reinterpret_cast<const u32x4*>(item + 16 * S::kRow + 256 + 16 * c);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    next();
-    const int live = min(S::kMfmas, (K - step * S::kColumns) / 32);  // MFMAs in front of the rows' end
-#pragma unroll
-    for (int i = 0; i < S::kMfmas; ++i) {
-      if (i >= live) break;
-      f32x4 from[MT], sum[MT];
-      if constexpr (FMT != 16) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          from[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if constexpr (kOffset) from[t] = mfma16<ACT>(xa[t][i], offset(), from[t]);
-          if constexpr (ASYM) sum[t] = mfma16<ACT>(xa[t][i], ones(), f32x4{0.f, 0.f, 0.f, 0.f});
-        }
+      for (int i = 0; i < GROUP; ++i) {
+        xa[i] = *reinterpret_cast<const u32x4*>(xrow + (((4 * (g * GROUP + i) + q) ^ j) << 4));
+        if constexpr (FMT != 16 && kOffset) from = mfma16<ACT>(xa[i], offset(), from);
+        if constexpr (ASYM) sum = mfma16<ACT>(xa[i], ones(), sum);
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const u32x4 b = operand(raw[r][i]);
-        if constexpr (FMT == 16) {
+        const uint8_t* const row = base + r * S::kItem + c * S::kRow;
+        d[r] = from;
 #pragma unroll
-          for (int t = 0; t < MT; ++t) acc[r][t] = mfma16<ACT>(xa[t][i], b, acc[r][t]);
-        } else {
-          // groups of 32: a dword has both scales of its 64 columns; larger: the one scale, in either half of it
-          const uint32_t index = (uint32_t)c * (uint32_t)groups + (uint32_t)((2 * (step * 4 + (i >> 1))) >> shift);
-          const uint32_t half = shift ? index & 1u : (uint32_t)(i & 1);
-          const float s = f16_bits_to_f32((sc[r][i >> 1] >> (16u * half)) & 0xFFFFu);
+        for (int i = 0; i < GROUP; ++i) {
+          const int at = g * GROUP + i;
+          uint32_t raw[S::kWords];
+          if constexpr (FMT == 4) {
+            raw[0] = *reinterpret_cast<const uint32_t*>(row + ((at ^ swizzle) << 4) + 4 * q);
+          } else if constexpr (FMT == 8) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(row + (((2 * at + (q >> 1)) ^ swizzle) << 4) + 8 * (q & 1));
+            raw[0] = v.x, raw[1] = v.y;
+          } else {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(row + (((4 * at + q) ^ swizzle) << 4));
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            f32x4 d = mfma16<ACT>(xa[t][i], b, from[t]);
-            if constexpr (ASYM) {
-              const float z = f16_bits_to_f32((zp[r][i >> 1] >> (16u * half)) & 0xFFFFu);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) d[e] = __builtin_fmaf(-z, sum[t][e], d[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[r][t][e] = __builtin_fmaf(s, d[e], acc[r][t][e]);
+            for (int e = 0; e < 4; ++e) raw[e] = v[e];
           }
+          if constexpr (FMT == 16) acc[r] = mfma16<ACT>(xa[i], operand(raw), acc[r]);
+          else d[r] = mfma16<ACT>(xa[i], operand(raw), d[r]);
         }
       }
+      if constexpr (FMT != 16) {
+        // groups of 32: a dword has both scales of its 64 columns; larger: the one scale, in either half of it
+        const int chunk = g * GROUP / 2;
+        uint32_t by = (uint32_t)(g & 1) * 16u;
+        if constexpr (GROUP > 1) by = (((uint32_t)c * (uint32_t)groups + (uint32_t)((2 * (step * 4 + chunk)) >> shift)) & 1u) * 16u;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint8_t* const at = base + r * S::kItem + 16 * S::kRow + 16 * c + 4 * chunk;
+          const float s = f16_bits_to_f32((*reinterpret_cast<const uint32_t*>(at) >> by) & 0xFFFFu);
+          if constexpr (ASYM) {
+            const float z = f16_bits_to_f32((*reinterpret_cast<const uint32_t*>(at + 256) >> by) & 0xFFFFu);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[r][e] = __builtin_fmaf(-z, sum[e], d[r][e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][e] = __builtin_fmaf(s, d[r][e], acc[r][e]);
+        }
+      }
+    };
+    const int live = (K - step * S::kColumns) / 32;  // MFMAs in front of the rows' end: whole groups
+    if (live >= S::kMfmas) {
+#pragma unroll
+      for (int g = 0; g < S::kMfmas / GROUP; ++g) group(g);
+    } else {
+#pragma unroll 1
+      for (int g = 0; g < live / GROUP; ++g) group(g);
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the place may be loaded again
   }
 };
 
 constexpr int kMoeRedRow = 36;  // floats of a token's row where the waves' sums meet: 32 and some to spread the banks
 
-template <int ACT, int FMT, bool ASYM, int MT>
-__global__ void __launch_bounds__(64 * kMoeMaxWaves) moe_up_kernel(const MoeArgs a, int x_loads) {
-  using Walk = MoeWalk<ACT, FMT, ASYM, MT, 2>;
+// Items: (entry, 16 gate rows and their 16 up rows for each wave or for all), dealt to the blocks in turn.  TOGETHER: the waves have row tiles of their own and share the
+// tokens, a barrier per step; else they share the columns of one pair of row tiles, each with tokens of its own, and their sums meet at the item's end.  Tokens
+// take LDS and come from the L2 once per wave or per block: few of them are best brought by each wave, many are not.
+template <int ACT, int FMT, bool ASYM, int GROUP, bool TOGETHER>
+__global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) moe_up_kernel(const MoeArgs a, int cap, int own_lds) {
+  using Walk = MoeWalk<ACT, FMT, ASYM, 2, GROUP>;
   using S = typename Walk::S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ MoeRoute route;
-  __shared__ uint16_t lists[kMoeMaxWaves][2][kMoeMaxTokens];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  float* const red = reinterpret_cast<float*>(lds + waves * (x_loads * 1024 + 2 * S::kItem));
-
-  for (int m = wave; m < a.M; m += waves) pick_experts(a, m, lane, route);
+  const MoeRoute route(lds + own_lds, a.M * a.top_k, waves, lds);
+  for (int m = wave; m < a.M; m += waves) pick_experts(a, m, lane, route, blockIdx.x == 0);
   __syncthreads();
-  if (blockIdx.x == 0)  // for the down kernel
-    for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) a.ids[p] = route.ids[p], a.share[p] = route.share[p];
-  list_experts(a, route);
+  list_entries(a, route, cap);
 
-  const int tiles = a.I / 16, items = route.n_experts * tiles, steps = (a.H + S::kColumns - 1) / S::kColumns;
-  const int first = steps * wave / waves, last = steps * (wave + 1) / waves;  // this wave's steps of an item
-  Walk walk(lds + wave * (x_loads * 1024 + 2 * S::kItem), x_loads, a.H, a.shift);
-  int parity = 0;
-  auto begin = [&](int item) {
-    const int e = route.experts[item / tiles], tile = item % tiles;
-    uint16_t* const list = lists[wave][parity];
-    const int n = list_pairs(a, route, e, lane, list);
-    walk.rows(0, a.gate_up, a.gate_up_scale, a.gate_up_zero, (int64_t)e * 2 * a.I + tile * 16);
-    walk.rows(1, a.gate_up, a.gate_up_scale, a.gate_up_zero, (int64_t)e * 2 * a.I + a.I + tile * 16);
-    walk.tokens(a.xs, list, n, a.top_k);
+  const int groups = TOGETHER ? waves : 1, tiles = a.I / 16 / groups, items = __builtin_amdgcn_readfirstlane(*route.n_entries) * tiles, steps = (a.H + S::kColumns - 1) / S::kColumns;
+  const int first = TOGETHER ? 0 : steps * wave / waves, last = TOGETHER ? steps : steps * (wave + 1) / waves;  // this wave's steps of an item: one at least
+  const int x_bytes = S::x_loads(cap) * 1024;
+  uint8_t* const tokens = lds + waves * 2 * Walk::kPlace;
+  Walk walk(lds + wave * 2 * Walk::kPlace, tokens + (TOGETHER ? 0 : wave * 2 * x_bytes), S::x_loads(cap), a.H, a.shift, TOGETHER ? wave : 0, groups);
+  float* const red = reinterpret_cast<float*>(tokens + (TOGETHER ? 1 : waves) * 2 * x_bytes);
+
+  // What is requested next: a step ahead of what is multiplied, so it may be the next item's.
+  int ahead = blockIdx.x, ahead_step = first, ahead_entry = -1, ahead_slot = 1;
+  auto request = [&](int place) __attribute__((always_inline)) {
+    if (ahead >= items) return;
+    if (ahead_step == first) {
+      const int at = ahead / tiles;
+      const uint32_t entry = __builtin_amdgcn_readfirstlane(route.entries[at]);
+      if (at != ahead_entry) {  // the entries that a block meets take the two lists in turn
+        ahead_entry = at;
+        ahead_slot ^= 1;
+        uint16_t* const list = route.lists + (wave * 2 + ahead_slot) * 16;
+        const int n = list_pairs(a, route, entry, cap, lane, list);
+        if (lane == 0) route.counts[wave * 2 + ahead_slot] = n;
+        walk.tokens(a.xs, list, n, a.top_k);
+      }
+      const int64_t row = (int64_t)(entry & 0xFFFF) * 2 * a.I + (ahead % tiles * groups + (TOGETHER ? wave : 0)) * 16;
+      walk.rows(0, a.gate_up, a.gate_up_scale, a.gate_up_zero, row);
+      walk.rows(1, a.gate_up, a.gate_up_scale, a.gate_up_zero, row + a.I);
+    }
+    walk.load(ahead_step, place);
+    if (++ahead_step == last) {
+      ahead_step = first;
+      ahead += gridDim.x;
+    }
   };
-  int item = blockIdx.x;
-  if (item < items) {
-    begin(item);
-    if (first < last) walk.load(first);
-  }
-  for (; item < items; item += gridDim.x) {
-    const int count = walk.count;
-    const uint16_t* const list = lists[wave][parity];
-    const int following = item + gridDim.x;
-    auto go_on = [&] {
-      if (following >= items) return;
-      parity ^= 1;
-      begin(following);
-      if (first < last) walk.load(first);
-    };
+  request(0);
+  int place = 0, slot = 1, entry_now = -1;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    if (item / tiles != entry_now) slot ^= 1;
+    entry_now = item / tiles;
+    const int count = __builtin_amdgcn_readfirstlane(route.counts[wave * 2 + slot]);
+    const uint16_t* const list = route.lists + (wave * 2 + slot) * 16;
     walk.clear();
-    for (int step = first; step < last - 1; ++step) walk.compute(step, [&] { walk.load(step + 1); });
-    // The last step of an item brings the next item's first on its way; `count` tokens are this one's.
-    if (first < last) walk.compute(last - 1, go_on);
-    else go_on();
-    block_sync_lds();  // nobody reads the sums of the item before any more
+    for (int step = first; step < last; ++step) {
+      Walk::arrived();
+      if constexpr (TOGETHER) block_sync_lds();  // everybody's tokens are there, and nobody reads the other place any more
+      request(place ^ 1);
+      walk.multiply(step, place, count);
+      place ^= 1;
+    }
+    const int tile = item % tiles;
+    auto store = [&](int j, int k, float gate, float up) __attribute__((always_inline)) {
+      const int to = FMT == 4 ? (k & ~7) | octet_place(k & 7) : k;
+      store_from_f32<ACT>(a.h, (int64_t)list[j] * a.I + to, silu_f32(gate) * up);
+    };
+    if constexpr (TOGETHER) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+      for (int i = 0; i < 4; ++i) {
+        const int j = 4 * (lane >> 4) + i;
+        if (j < count) store(j, (tile * groups + wave) * 16 + (lane & 15), walk.acc[0][i], walk.acc[1][i]);
+      }
+    } else {
+      block_sync_lds();  // nobody reads the sums of the item before any more
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int j = 16 * t + 4 * (lane >> 4) + i;
-          if (j < count) red[(wave * 16 * MT + j) * kMoeRedRow + r * 16 + (lane & 15)] = walk.acc[r][t][i];
+          const int j = 4 * (lane >> 4) + i;
+          if (j < count) red[(wave * cap + j) * kMoeRedRow + r * 16 + (lane & 15)] = walk.acc[r][i];
         }
-    block_sync_lds();
-    const int tile = item % tiles;
-    for (int o = threadIdx.x; o < count * 16; o += blockDim.x) {
-      const int j = o >> 4, n = o & 15;
-      float gate = 0.f, up = 0.f;
-      for (int w = 0; w < waves; ++w) {
-        gate += red[(w * 16 * MT + j) * kMoeRedRow + n];
-        up += red[(w * 16 * MT + j) * kMoeRedRow + 16 + n];
+      block_sync_lds();
+      for (int o = threadIdx.x; o < count * 16; o += blockDim.x) {
+        const int j = o >> 4, n = o & 15;
+        float gate = 0.f, up = 0.f;
+        for (int w = 0; w < waves; ++w) {
+          gate += red[(w * cap + j) * kMoeRedRow + n];
+          up += red[(w * cap + j) * kMoeRedRow + 16 + n];
+        }
+        store(j, tile * 16 + n, gate, up);
       }
-      const int k = tile * 16 + n;
-      const int at = FMT == 4 ? (k & ~7) | octet_place(k & 7) : k;
-      store_from_f32<ACT>(a.h, (int64_t)list[j] * a.I + at, silu_f32(gate) * up);
     }
   }
 }
 
-template <int ACT, int FMT, bool ASYM, int MT>
-__global__ void __launch_bounds__(64 * kMoeMaxWaves) moe_down_kernel(const MoeArgs a, int x_loads) {
-  using Walk = MoeWalk<ACT, FMT, ASYM, MT, 1>;
+// A block per 32 rows of y and part of the columns of all entries, laid one behind the other; its waves share those.  Parts leave their sums in the workspace, past the
+// L2 (agent scope), and the last of a row tile's blocks to do so adds them in their order.
+template <int ACT, int FMT, bool ASYM, int GROUP>
+__global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const MoeArgs a, int cap, int own_lds) {
+  using Walk = MoeWalk<ACT, FMT, ASYM, 2, GROUP>;
   using S = typename Walk::S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ MoeRoute route;
-  __shared__ uint16_t lists[kMoeMaxWaves][2][kMoeMaxTokens];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  float* const sums = reinterpret_cast<float*>(lds + waves * (x_loads * 1024 + S::kItem));  // [wave][M][16]
-  for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) route.ids[p] = a.ids[p], route.share[p] = a.share[p];
-  for (int o = threadIdx.x; o < waves * a.M * 16; o += blockDim.x) sums[o] = 0.f;
+  const int x_bytes = S::x_loads(cap) * 1024;
+  const MoeRoute route(lds + own_lds, a.M * a.top_k, waves, lds);
+  uint8_t* const tokens = lds + waves * 2 * Walk::kPlace;
+  Walk walk(lds + wave * 2 * Walk::kPlace, tokens + wave * 2 * x_bytes, S::x_loads(cap), a.I, a.shift, 0, 1);
+  float* const sums = reinterpret_cast<float*>(tokens + waves * 2 * x_bytes);  // [wave][M][32]
+  for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) route.ids[p] = a.ids[p];
+  for (int o = threadIdx.x; o < waves * a.M * 32; o += blockDim.x) sums[o] = 0.f;
   __syncthreads();
-  list_experts(a, route);
-  const int n0 = blockIdx.x * 16, steps = (a.I + S::kColumns - 1) / S::kColumns, all = route.n_experts * steps;
-  const int first = (int)((int64_t)all * wave / waves), last = (int)((int64_t)all * (wave + 1) / waves);
-  Walk walk(lds + wave * (x_loads * 1024 + S::kItem), x_loads, a.I, a.shift);
-  int parity = 0;
-  auto begin = [&](int at) {
-    const int e = route.experts[at / steps];
-    const int n = list_pairs(a, route, e, lane, lists[wave][parity]);
-    walk.rows(0, a.down, a.down_scale, a.down_zero, (int64_t)e * a.H + n0);
-    walk.tokens(a.h, lists[wave][parity], n, 1);
+  list_entries(a, route, cap);
+
+  const int n0 = blockIdx.x * 32, steps = (a.I + S::kColumns - 1) / S::kColumns, all = __builtin_amdgcn_readfirstlane(*route.n_entries) * steps;
+  const int shares = waves * gridDim.y, of = blockIdx.y * waves + wave;
+  const int first = (int)((int64_t)all * of / shares), last = (int)((int64_t)all * (of + 1) / shares);
+  int left_to_ask = last - first, ahead_entry = first / steps, ahead_step = first - ahead_entry * steps, ahead_slot = 1;
+  bool ahead_new = true;
+  auto request = [&](int place) __attribute__((always_inline)) {
+    if (left_to_ask <= 0) return;
+    --left_to_ask;
+    if (ahead_new) {
+      ahead_new = false;
+      ahead_slot ^= 1;
+      const uint32_t entry = __builtin_amdgcn_readfirstlane(route.entries[ahead_entry]);
+      uint16_t* const list = route.lists + (wave * 2 + ahead_slot) * 16;
+      const int n = list_pairs(a, route, entry, cap, lane, list);
+      if (lane == 0) route.counts[wave * 2 + ahead_slot] = n;
+      const int64_t row = (int64_t)(entry & 0xFFFF) * a.H + n0;
+      walk.rows(0, a.down, a.down_scale, a.down_zero, row);
+      walk.rows(1, a.down, a.down_scale, a.down_zero, row + 16);
+      walk.tokens(a.h, list, n, 1);
+    }
+    walk.load(ahead_step, place);
+    if (++ahead_step == steps) {
+      ahead_step = 0;
+      ++ahead_entry;
+      ahead_new = true;
+    }
   };
-  if (first < last) {
-    begin(first);
-    walk.load(first % steps);
-  }
-  float* const mine = sums + wave * a.M * 16;
-  for (int at = first; at < last; ++at) {
-    const int step = at % steps, count = walk.count;
-    const uint16_t* const list = lists[wave][parity];
-    const bool ends = step == steps - 1 || at == last - 1;
-    walk.compute(step, [&] {
-      if (at == last - 1) return;
-      if (ends) {
-        parity ^= 1;
-        begin(at + 1);
-      }
-      walk.load(ends ? 0 : step + 1);
-    });
-    if (!ends) continue;
-    // the expert's tokens, each times its share: a token's place is written by one lane
+  request(0);
+  int slot = 0, place = 0, step = first % steps;
+  float* const mine = sums + wave * a.M * 32;
+  for (int i = first; i < last; ++i) {
+    const int count = __builtin_amdgcn_readfirstlane(route.counts[wave * 2 + slot]);
+    Walk::arrived();
+    request(place ^ 1);
+    walk.multiply(step, place, count);
+    place ^= 1;
+    if (++step != steps && i != last - 1) continue;
+    // the entry's tokens, each times its share: a token's place is written by one lane
+    step = 0;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int e = 0; e < 4; ++e) {
+      const int j = 4 * (lane >> 4) + e;
+      if (j < count) {
+        const int pair = route.lists[(wave * 2 + slot) * 16 + j];
+        const float share = a.share[pair];
+        float* const to = mine + pair / a.top_k * 32 + (lane & 15);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 16 * t + 4 * (lane >> 4) + i;
-        if (j < count) {
-          const int pair = list[j];
-          float* const to = mine + pair / a.top_k * 16 + (lane & 15);
-          *to = __builtin_fmaf(route.share[pair], walk.acc[0][t][i], *to);
-        }
+        for (int r = 0; r < 2; ++r) to[16 * r] = __builtin_fmaf(share, walk.acc[r][e], to[16 * r]);
       }
+    }
+    slot ^= 1;
     walk.clear();
   }
   __syncthreads();
-  for (int o = threadIdx.x; o < a.M * 16; o += blockDim.x) {
+  const int values = a.M * 32;
+  float* const left = a.parts + (int64_t)blockIdx.x * values;
+  const int64_t part_stride = (int64_t)gridDim.x * values;
+  for (int o = threadIdx.x; o < values; o += blockDim.x) {
     float v = 0.f;
-    for (int w = 0; w < waves; ++w) v += sums[w * a.M * 16 + o];
-    store_from_f32<ACT>(a.y, (o >> 4) * a.ldy + n0 + (o & 15), v);
+    for (int w = 0; w < waves; ++w) v += sums[w * values + o];
+    if (gridDim.y == 1) store_from_f32<ACT>(a.y, (o >> 5) * a.ldy + n0 + (o & 31), v);
+    else __hip_atomic_store(left + blockIdx.y * part_stride + o, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (gridDim.y == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the part is where the others will read it
+  __syncthreads();
+  int* const order = route.n_entries;
+  if (threadIdx.x == 0) *order = (int)__hip_atomic_fetch_add(a.done + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (*order != (int)gridDim.y - 1) return;
+  for (int o = threadIdx.x; o < values; o += blockDim.x) {
+    float v = 0.f;
+    for (unsigned p = 0; p < gridDim.y; ++p) v += __hip_atomic_load(left + p * part_stride + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    store_from_f32<ACT>(a.y, (o >> 5) * a.ldy + n0 + (o & 31), v);
   }
 }
 
 struct MoeSpace {
-  int64_t logits, ids, share, xs, h, bytes;
+  int64_t logits, ids, share, xs, h, done, parts, bytes;
   MoeSpace(int M, int E, int top_k, int H, int I) {
     int64_t at = 0;
     auto take = [&](int64_t n) {
@@ -539,54 +662,61 @@ struct MoeSpace {
       return was;
     };
     logits = take((int64_t)M * E * 4);
-    ids = take((int64_t)M * top_k * 4);
+    ids = take((int64_t)M * top_k * 2);
     share = take((int64_t)M * top_k * 4);
     xs = take((int64_t)M * H * 2);
     h = take((int64_t)M * top_k * I * 2);
+    done = take((int64_t)H / 32 * 4);
+    parts = take((int64_t)kMoeMaxParts * M * H * 4);
     bytes = at;
   }
 };
 
-template <int ACT, int FMT, bool ASYM, int MT>
-int launch_moe_mt(const MoeArgs& a, hipStream_t st) {
+// Four waves to a block of the up kernel (us of the layer with two / four / eight: int4 4096 x 14336, one token 54 / 50 / 56; dense 2048 x 2048, four tokens 67 / 65 / 66)
+// and eight of the down kernel (four / eight / 16: 54 / 50 / 52, 65 / 65 / 66), whose blocks split the columns where there are fewer row tiles than compute units (one part /
+// two: 57 / 50; hidden size 2048, seven tokens int8 one / four: 103 / 73).  From five tokens on the up kernel's waves share them: 16 tokens int4 271 / 219, one token 54 / 57.
+constexpr int kMoeUpWaves = 4, kMoeDownWaves = 8, kMoeTogether = 5, kMoeBlocks = 256, kMoeBlocksPerCu = 4;
+
+template <int ACT, int FMT, bool ASYM, int GROUP>
+int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   const char* what = "npamd_moe_layer";
   using S = MoeStep<FMT, ASYM>;
-  constexpr bool kNibbles = FMT == 4;
-  const int x_loads = S::x_loads(a.M);
-  auto up_lds_of = [&](int waves) { return waves * (x_loads * 1024 + 2 * S::kItem) + waves * 16 * MT * kMoeRedRow * 4; };
-  auto down_lds_of = [&](int waves) { return waves * (x_loads * 1024 + S::kItem) + waves * a.M * 16 * 4; };
-  constexpr int kRoom = 160 * 1024 - 8192;  // next to what the kernels have of their own
-  static const int env_up = getenv("UPW") ? atoi(getenv("UPW")) : 4, env_down = getenv("DNW") ? atoi(getenv("DNW")) : 8, env_cu = getenv("UPC") ? atoi(getenv("UPC")) : 4;
-  int up_waves = env_up, down_waves = env_down;
-  while (up_lds_of(up_waves) > kRoom) --up_waves;
-  while (down_lds_of(down_waves) > kRoom) --down_waves;
-  const int up_lds = up_lds_of(up_waves), down_lds = down_lds_of(down_waves);
-  static LdsLatch up_latch, down_latch;
-  const auto up = moe_up_kernel<ACT, FMT, ASYM, MT>;
-  const auto down = moe_down_kernel<ACT, FMT, ASYM, MT>;
-  hipError_t e = enable_dynamic_lds(up_latch, reinterpret_cast<const void*>(up), up_lds);
+  constexpr int kRoom = 160 * 1024;
+  const bool together = a.M >= kMoeTogether;
+  const int cap = std::min(a.M, 16), pairs = a.M * a.top_k, x_bytes = 2 * S::x_loads(cap) * 1024;
+  auto up_own = [&](int waves) { return waves * 4 * S::kItem + (together ? x_bytes : waves * (x_bytes + cap * kMoeRedRow * 4)); };
+  auto down_own = [&](int waves) { return waves * (x_bytes + 4 * S::kItem + a.M * 32 * 4); };
+  const int up_waves = together ? kMoeUpWaves : std::min(kMoeUpWaves, (a.H + S::kColumns - 1) / S::kColumns);
+  int down_waves = kMoeDownWaves;
+  while (down_own(down_waves) + MoeRoute::bytes(pairs, down_waves) > kRoom) --down_waves;
+  const int up_lds = up_own(up_waves) + MoeRoute::bytes(pairs, up_waves), down_lds = down_own(down_waves) + MoeRoute::bytes(pairs, down_waves);
+  static LdsLatch up_latch[2], down_latch;
+  const auto up = together ? moe_up_kernel<ACT, FMT, ASYM, GROUP, true> : moe_up_kernel<ACT, FMT, ASYM, GROUP, false>;
+  const auto down = moe_down_kernel<ACT, FMT, ASYM, GROUP>;
+  hipError_t e = enable_dynamic_lds(up_latch[together], reinterpret_cast<const void*>(up), up_lds);
   if (e == hipSuccess) e = enable_dynamic_lds(down_latch, reinterpret_cast<const void*>(down), down_lds);
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve LDS: %s", what, hipGetErrorString(e));
-  const auto logits = a.M == 1 ? moe_logits_kernel<ACT, 1, kNibbles> : a.M <= 4 ? moe_logits_kernel<ACT, 4, kNibbles> : moe_logits_kernel<ACT, 8, kNibbles>;
-  launch(logits, a.E, 256, 0, st, a);
-  const int most = a.E < a.M * a.top_k ? a.E : a.M * a.top_k;  // experts that can be met
-  const int64_t items = (int64_t)most * (a.I / 16);
-  const int per_cu = std::min(env_cu, (160 * 1024) / (up_lds + 8192));
-  launch(up, (unsigned)std::min<int64_t>(items, 256 * std::max(per_cu, 1)), 64 * up_waves, up_lds, st, a, x_loads);
-  launch(down, a.H / 16, 64 * down_waves, down_lds, st, a, x_loads);
+  if (a.M == 1) launch(moe_logits_kernel<ACT, 1, FMT == 4>, a.E, 256, 0, st, a);
+  else launch(moe_logits_kernel<ACT, 4, FMT == 4>, dim3(a.E, (a.M + 3) / 4), 256, 0, st, a);
+  const int64_t items = (int64_t)std::min(pairs, a.E + pairs / cap) * (a.I / 16 / (together ? up_waves : 1));  // no more than that
+  const int per_cu = std::max(1, std::min(kMoeBlocksPerCu, kRoom / up_lds));
+  launch(up, (unsigned)std::min<int64_t>(items, kMoeBlocks * per_cu), 64 * up_waves, up_lds, st, a, cap, up_own(up_waves));
+  const int parts = std::max(1, std::min(kMoeMaxParts, kMoeBlocks / (a.H / 32)));
+  launch(down, dim3(a.H / 32, parts), 64 * down_waves, down_lds, st, a, cap, down_own(down_waves));
   return check_launch(what);
 }
 
+template <int ACT, int FMT, bool ASYM>
+int launch_moe_codes(const MoeArgs& a, hipStream_t st) {
+  if (a.shift == 0) return launch_moe_format<ACT, FMT, ASYM, 1>(a, st);
+  if (a.shift == 1) return launch_moe_format<ACT, FMT, ASYM, 2>(a, st);
+  return launch_moe_format<ACT, FMT, ASYM, 4>(a, st);
+}
 template <int ACT>
 int launch_moe(const MoeArgs& a, int nbits, hipStream_t st) {
-  const bool two = a.M > 16;
-#define NPAMD_MOE(FMT, ASYM) return two ? launch_moe_mt<ACT, FMT, ASYM, 2>(a, st) : launch_moe_mt<ACT, FMT, ASYM, 1>(a, st)
-  if (nbits == 16) NPAMD_MOE(16, false);
-  if (nbits == 8 && a.gate_up_zero) NPAMD_MOE(8, true);
-  if (nbits == 8) NPAMD_MOE(8, false);
-  if (a.gate_up_zero) NPAMD_MOE(4, true);
-  NPAMD_MOE(4, false);
-#undef NPAMD_MOE
+  if (nbits == 16) return launch_moe_format<ACT, 16, false, 2>(a, st);
+  if (nbits == 8) return a.gate_up_zero ? launch_moe_codes<ACT, 8, true>(a, st) : launch_moe_codes<ACT, 8, false>(a, st);
+  return a.gate_up_zero ? launch_moe_codes<ACT, 4, true>(a, st) : launch_moe_codes<ACT, 4, false>(a, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -631,7 +761,7 @@ extern "C" int npamd_moe_layer(const void* x, int64_t ldx, const void* router, c
   int shift = 0;
   while (codes && (32 << shift) < group_size) ++shift;
   const MoeArgs a{x, router, (const uint8_t*)gate_up, (const uint8_t*)down, half(gate_up_scale_f16), half(gate_up_zero_f16), half(down_scale_f16),
-                  half(down_zero_f16), y, ldx, ldy, M, E, top_k, H, I, shift, renormalize, (float*)(at + space.logits), (int32_t*)(at + space.ids),
-                  (float*)(at + space.share), (uint16_t*)(at + space.xs), (uint16_t*)(at + space.h)};
+                  half(down_zero_f16), y, ldx, ldy, M, E, top_k, H, I, shift, renormalize, (float*)(at + space.logits), (uint16_t*)(at + space.ids),
+                  (float*)(at + space.share), (uint32_t*)(at + space.done), (float*)(at + space.parts), (uint16_t*)(at + space.xs), (uint16_t*)(at + space.h)};
   return act_dtype == NPAMD_BF16 ? launch_moe<NPAMD_BF16>(a, nbits, (hipStream_t)stream) : launch_moe<NPAMD_F16>(a, nbits, (hipStream_t)stream);
 }

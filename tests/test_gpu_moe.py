@@ -74,7 +74,8 @@ def _reference(x, layer, dense, top_k, renormalize):
 def _check(y, ref, tol, dtype):
     assert y.dtype == dtype and y.shape == ref.shape
     err = (y.double().cpu() - ref).abs()
-    assert bool((err <= tol).all()), f"{(err / tol).max().item():.2f} of the tolerance"
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert worst <= 1, f"{worst:.2f} of the tolerance"
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
