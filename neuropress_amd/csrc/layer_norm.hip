@@ -3,11 +3,17 @@
 //   y = xh w + b
 //   backward, g = dy w:  dx = rstd (g - sum(g) / H - xh sum(g xh) / H),  dw = sum over rows of dy xh,  db = sum over rows of dy
 // All arithmetic in f32, one rounding at the store; the variance is taken around the mean, in a second pass over the row.
+#include <algorithm>
+
 #include "common.hpp"
+#include "wave_ops.hpp"
 
 using namespace npamd;
 
 namespace {
+
+// Below so many waves a row gets more of them: 1100 x 4096 7.3 -> 6.7 us, 300 x 2048 4.0 -> 2.8.
+constexpr int kFewWaves = 4096;
 
 // The sum over a block of 256 threads, in every one of them.  `part`: four floats of the block's own for this sum.
 __device__ __forceinline__ float block_sum(float v, float* part) {
@@ -17,7 +23,139 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return part[0] + part[1] + part[2] + part[3];
 }
 
-// Any H, any alignment: a block per row, which it reads three times.
+// A row in registers goes in pieces of 16 bytes, V values, at whatever address; a row that does not end with a piece has its last one end with the row, and the values
+// that the piece before has too count once (and are stored twice, the same).
+template <int DT>
+struct Pieces {
+  static constexpr int V = DT == NPAMD_F32 ? 4 : 8, kBytes = DT == NPAMD_F32 ? 4 : 2;
+  // Value `at` of a row, which is the same for all lanes.
+  static __device__ __forceinline__ u32x4 load(const uint8_t* row, int at) { return *reinterpret_cast<const u32x4_any*>(row + (uint32_t)at * kBytes); }
+  static __device__ __forceinline__ void store(uint8_t* row, int at, const u32x4& v) { *reinterpret_cast<u32x4_any*>(row + (uint32_t)at * kBytes) = v; }
+  static __device__ __forceinline__ const uint8_t* row_of(const void* p, int64_t row, int64_t ld) { return (const uint8_t*)p + row * ld * kBytes; }
+  // What is made of a piece from here on is made anew: kept since it was made before, it would take two to four times the registers.
+  static __device__ __forceinline__ void forget(u32x4& v) {
+    if constexpr (DT != NPAMD_F32) asm volatile("" : "+v"(v));
+  }
+  static __device__ __forceinline__ void unpack(const u32x4& v, float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == NPAMD_F32) {
+        f[i] = __builtin_bit_cast(float, (uint32_t)v[i]);
+      } else {
+        f[2 * i] = act_bits_to_f32<DT>(v[i] & 0xFFFFu);
+        f[2 * i + 1] = act_bits_to_f32<DT>(v[i] >> 16);
+      }
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float (&f)[V]) {
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == NPAMD_F32) v[i] = __builtin_bit_cast(uint32_t, f[i]);
+      else if constexpr (DT == NPAMD_BF16) v[i] = f32_to_bf16_bits(f[2 * i]) | (f32_to_bf16_bits(f[2 * i + 1]) << 16);
+      else v[i] = f32_to_f16_bits(f[2 * i]) | (f32_to_f16_bits(f[2 * i + 1]) << 16);
+    }
+    return v;
+  }
+};
+
+// RW waves to a row, 4 / RW rows to a block, NV pieces to a lane, so that x is read once.  Bound by HBM: 4096 x 4096 bf16 14.7 us (a copy of x 12.7; one wave to a row, eight
+// pieces to a lane 15.4: too few waves for the registers), 8192 x 2048 14.1 (12.9); by the launch and one round trip below that: 300 x 2048 2.8, one row 2.2.
+template <int DT, int NV, int RW>
+__global__ void __launch_bounds__(256)
+layer_norm_row_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* __restrict__ out, int64_t ldo,
+                      float* __restrict__ mean_out, float* __restrict__ rstd_out, int M, int H, float eps) {
+  using P = Pieces<DT>;
+  constexpr int V = P::V, kLanes = 64 * RW;
+  __shared__ float part[2][4];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kLanes - 1);
+  const int64_t row_of_wave = (int64_t)blockIdx.x * (4 / RW) + wave / RW, row = min(row_of_wave, (int64_t)M - 1);  // past the end: the last row, not stored
+  const int pieces = (H + V - 1) / V;
+  const uint8_t* const xr = P::row_of(x, row, ldx);
+  u32x4 xv[NV], wv[NV], bv[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = lane + kLanes * i;
+    xv[i] = u32x4{0, 0, 0, 0};
+    if (p < pieces) xv[i] = P::load(xr, min(p * V, H - V));
+  }
+  auto parameters = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = lane + kLanes * i, at = min(p * V, H - V);
+      wv[i] = bv[i] = u32x4{0, 0, 0, 0};
+      if (w && p < pieces) wv[i] = P::load((const uint8_t*)w, at);
+      if (b && p < pieces) bv[i] = P::load((const uint8_t*)b, at);
+    }
+  };
+  // Few rows wait for memory once: w and b are requested with x.  Many need the registers for waves: w and b come from the L1 when they are used.
+  constexpr bool kEarly = NV <= 2;
+  if constexpr (kEarly) parameters();
+  // f(value) for the lane's values of the row, each once.
+  auto values = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = lane + kLanes * i;
+      if (p >= pieces) continue;
+      float v[V];
+      P::forget(xv[i]);
+      P::unpack(xv[i], v);
+      if (p * V + V <= H) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f(v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e >= p * V + V - H) f(v[e]);
+      }
+    }
+  };
+  auto over_row = [&](float v, float* meet) __attribute__((always_inline)) {
+    v = wave_sum(v);
+    if constexpr (RW > 1) {
+      if ((threadIdx.x & 63) == 0) meet[wave] = v;
+      __syncthreads();
+      v = 0.f;
+#pragma unroll
+      for (int i = 0; i < RW; ++i) v += meet[wave / RW * RW + i];
+    }
+    return v;
+  };
+  float s = 0.f, ss = 0.f;
+  values([&](float v) __attribute__((always_inline)) { s += v; });
+  const float mean = over_row(s, part[0]) / (float)H;
+  values([&](float v) __attribute__((always_inline)) { ss = __builtin_fmaf(v - mean, v - mean, ss); });
+  const float rstd = 1.0f / __builtin_sqrtf(over_row(ss, part[1]) / (float)H + eps);
+  if constexpr (!kEarly) parameters();
+  if (row_of_wave >= M) return;
+  if (lane == 0) {
+    if (mean_out) mean_out[row] = mean;
+    if (rstd_out) rstd_out[row] = rstd;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = lane + kLanes * i;
+    if (p >= pieces) continue;
+    float f[V], g[V];
+    P::forget(xv[i]);
+    P::unpack(xv[i], f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = (f[e] - mean) * rstd;
+    if (w) {
+      P::unpack(wv[i], g);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] *= g[e];
+    }
+    if (b) {
+      P::unpack(bv[i], g);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] += g[e];
+    }
+    P::store(const_cast<uint8_t*>(P::row_of(out, row, ldo)), min(p * V, H - V), P::pack(f));
+  }
+}
+
+// Rows too short for a piece or too long for the registers: a block per row, which it reads three times.
 template <int DT>
 __global__ void __launch_bounds__(256)
 layer_norm_block_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* __restrict__ out,
@@ -53,7 +191,7 @@ struct LayerNormBack {
   int M, H;
 };
 
-// The gradient of the input, any H and alignment: a block per row.
+// Rows too short for a piece or too long for the registers.  The gradient of the input: a block per row.
 template <int DT>
 __global__ void __launch_bounds__(256)
 layer_norm_back_block_kernel(const LayerNormBack a) {
@@ -74,7 +212,7 @@ layer_norm_back_block_kernel(const LayerNormBack a) {
   }
 }
 
-// Sums over strips of rows for the gradients of weight and bias: partials [parts][2][H], a lane per column.
+// And sums over strips of rows for the gradients of weight and bias: partials [parts][2][H], a lane per column.
 template <int DT>
 __global__ void __launch_bounds__(256)
 layer_norm_back_columns_kernel(const LayerNormBack a, float* __restrict__ partials, int parts) {
@@ -95,20 +233,168 @@ layer_norm_back_columns_kernel(const LayerNormBack a, float* __restrict__ partia
     partials[((int64_t)blockIdx.y * 2 + wave) * a.H + col] = sums[0][wave][lane] + sums[1][wave][lane] + sums[2][wave][lane] + sums[3][wave][lane];
 }
 
-// The parts' sums, in the order of the parts: 64 columns of one of the two gradients (blockIdx.y) to a block, its 16 waves each a sixteenth of the parts.
+// All of it in one pass over x and dy, 8192 x 4096 bf16 41.7 us in all, 4.8 TB/s, as fast as a copy (with masks for every value and pieces unpacked twice, 48: the vector
+// instructions were the limit): RW waves to a row, G rows to a block at a time, a lane has NV pieces of every row that its group meets, the weight's at hand, and adds up
+// its columns' part of the weight's and bias's gradients in registers.  The next rows are requested before the two sums of these meet in LDS (one barrier a turn).
+template <int DT, int NV>
+__global__ void __launch_bounds__(1024)
+layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, int RW, int G) {
+  using P = Pieces<DT>;
+  constexpr int V = P::V;
+  extern __shared__ __attribute__((aligned(16))) float back_lds[];
+  __shared__ float meet[2][16][2];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave / RW, lanes = 64 * RW;
+  const int lane = (int)threadIdx.x - group * lanes, pieces = (a.H + V - 1) / V;
+  const float inv = 1.f / (float)a.H;
+  u32x4 xv[NV], dv[NV], wv[NV];
+  float dw[NV][V], db[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = lane + lanes * i;
+    xv[i] = dv[i] = wv[i] = u32x4{0, 0, 0, 0};
+    if (a.w && p < pieces) wv[i] = P::load((const uint8_t*)a.w, min(p * V, a.H - V));
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[i][e] = db[i][e] = 0.f;
+  }
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto request = [&](int64_t row) __attribute__((always_inline)) {
+    if (row >= a.M) return;
+    int64_t at_row = row;  // by vector loads: scalar ones would be waited for in front of the barrier
+    asm volatile("" : "+v"(at_row));
+    next_mean = a.mean[at_row];
+    next_rstd = a.rstd[at_row];
+    const uint8_t* const xr = P::row_of(a.x, row, a.ldx);
+    const uint8_t* const dr = P::row_of(a.dy, row, a.lddy);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = lane + lanes * i, at = min(p * V, a.H - V);
+      if (p >= pieces) continue;
+      xv[i] = P::load(xr, at);
+      dv[i] = P::load(dr, at);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t row = (int64_t)blockIdx.x * G + group;
+  request(row);
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * G; first < a.M; first += step, row += step, turn ^= 1) {
+    const bool live = row < a.M;
+    const float mean = next_mean, rstd = next_rstd;
+    u32x4 xc[NV], dc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) xc[i] = xv[i], dc[i] = dv[i];
+    request(row + step);
+    const float shift = -mean * rstd;  // (x - mean) rstd, rounded once: it is off by 2^-24 mean rstd, as it is by the mean's own rounding
+    float s1 = 0.f, s2 = 0.f, xh[NV][V], g[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = lane + lanes * i;
+      if (!live || p >= pieces) continue;
+      float wf[V], d[V];
+      P::unpack(xc[i], xh[i]);
+      P::unpack(dc[i], d);
+      P::unpack(wv[i], wf);
+      auto value = [&](int e) __attribute__((always_inline)) {
+        dw[i][e] = __builtin_fmaf(d[e], xh[i][e], dw[i][e]);
+        db[i][e] += d[e];
+        s1 += g[i][e];
+        s2 = __builtin_fmaf(g[i][e], xh[i][e], s2);
+      };
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        xh[i][e] = __builtin_fmaf(xh[i][e], rstd, shift);
+        g[i][e] = a.w ? d[e] * wf[e] : d[e];
+      }
+      if (p * V + V <= a.H) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) value(e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e >= p * V + V - a.H) value(e);
+      }
+    }
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if (RW > 1) {
+      if ((threadIdx.x & 63) == 0) meet[turn][wave][0] = s1, meet[turn][wave][1] = s2;
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the loads stay on their way
+      s1 = s2 = 0.f;
+      for (int i = 0; i < RW; ++i) s1 += meet[turn][group * RW + i][0], s2 += meet[turn][group * RW + i][1];
+    }
+    if (!live || !a.dx) continue;
+    const float c1 = -s1 * inv * rstd, c2 = -s2 * inv * rstd;
+    uint8_t* const to = const_cast<uint8_t*>(P::row_of(a.dx, row, a.lddx));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = lane + lanes * i;
+      if (p >= pieces) continue;
+      if constexpr (NV > 1) {  // not kept
+        float wf[V];
+        P::forget(xc[i]);
+        P::forget(dc[i]);
+        P::forget(wv[i]);
+        P::unpack(xc[i], xh[i]);
+        P::unpack(dc[i], g[i]);
+        P::unpack(wv[i], wf);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          xh[i][e] = __builtin_fmaf(xh[i][e], rstd, shift);
+          if (a.w) g[i][e] *= wf[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[i][e] = __builtin_fmaf(xh[i][e], c2, __builtin_fmaf(g[i][e], rstd, c1));
+      P::store(to, min(p * V, a.H - V), P::pack(g[i]));
+    }
+  }
+  if (!partials) return;
+  // The groups' sums meet in the first group, in their order.
+  float* const mine = back_lds + (int64_t)(group - 1) * 2 * NV * V * lanes + lane;
+  if (group > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) mine[(2 * (i * V + e)) * lanes] = dw[i][e], mine[(2 * (i * V + e) + 1) * lanes] = db[i][e];
+  }
+  __syncthreads();
+  if (group > 0) return;
+  for (int o = 0; o < G - 1; ++o) {
+    const float* const theirs = back_lds + (int64_t)o * 2 * NV * V * lanes + lane;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) dw[i][e] += theirs[(2 * (i * V + e)) * lanes], db[i][e] += theirs[(2 * (i * V + e) + 1) * lanes];
+  }
+  // Rows of whole pieces, as the lanes have them.
+  float* const to = partials + (int64_t)blockIdx.x * 2 * pieces * V;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = lane + lanes * i;
+    if (p >= pieces) continue;
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      *reinterpret_cast<f32x4*>(to + p * V + e) = f32x4{dw[i][e], dw[i][e + 1], dw[i][e + 2], dw[i][e + 3]};
+      *reinterpret_cast<f32x4*>(to + (pieces + p) * V + e) = f32x4{db[i][e], db[i][e + 1], db[i][e + 2], db[i][e + 3]};
+    }
+  }
+}
+
+// The parts' sums, in the order of the parts: 64 columns of one of the two gradients (blockIdx.y) to a block, its 16 waves each a sixteenth of the parts.  A part has `width`
+// columns for each, whole pieces: the last one's lie at its end.
 template <int DT>
 __global__ void __launch_bounds__(1024)
-layer_norm_back_sum_kernel(const float* __restrict__ partials, int parts, int H, void* __restrict__ dw, void* __restrict__ db) {
+layer_norm_back_sum_kernel(const float* __restrict__ partials, int parts, int H, int width, int last, void* __restrict__ dw, void* __restrict__ db) {
   __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
   void* const out = blockIdx.y ? db : dw;
   if (!out) return;
-  const int first = parts * wave / 16, last = parts * (wave + 1) / 16;
+  const int first = parts * wave / 16, end = parts * (wave + 1) / 16;
   float v = 0.f;
   if (col < H) {
-    const float* p = partials + ((int64_t)first * 2 + blockIdx.y) * H + col;
+    const float* p = partials + ((int64_t)first * 2 + blockIdx.y) * width + (col < last ? col : col + width - H);
 #pragma unroll 8
-    for (int i = first; i < last; ++i, p += 2 * (int64_t)H) v += *p;
+    for (int i = first; i < end; ++i, p += 2 * (int64_t)width) v += *p;
   }
   sums[wave][lane] = v;
   __syncthreads();
@@ -118,26 +404,75 @@ layer_norm_back_sum_kernel(const float* __restrict__ partials, int parts, int H,
   store_from_f32<DT>(out, col, v);
 }
 
-// Strips of rows whose sums the backward pass keeps apart.
-int back_parts(int M) { return M <= 0 ? 0 : M < 64 * 64 ? (M + 63) / 64 : 64; }
+// Turns of a block at least, where rows are few: every block leaves sums of two rows' bytes in f32, and a turn takes 1.3 us (509 x 3003 with one / two / three turns
+// 11.7 / 9.9 / 12.2 us, 64 x 4096 7.0 / 7.9 / 9.3); and no more blocks than compute units (8192 x 4096 with 192 / 256 / 512 55 / 48 / 54 us).
+constexpr int kTurns = 2;
+// Which kernel the backward pass takes.  parts: sums over rows that it leaves to be added.
+struct BackPlan {
+  int nv = 0, row_waves = 0, groups = 0, parts = 0;  // nv 0: rows that do not fit the registers
+  BackPlan(int M, int H, int dtype) {
+    const int V = dtype == NPAMD_F32 ? 4 : 8, pieces = (H + V - 1) / V;
+    if (H < V || pieces > 64 * 16 * 2) {
+      parts = std::min(64, (M + 63) / 64);
+      return;
+    }
+    nv = pieces <= 1024 ? 1 : 2;
+    row_waves = 1;
+    while (row_waves * 64 * nv < pieces) row_waves *= 2;
+    groups = 16 / row_waves;
+    parts = std::min(256, (M + groups * kTurns - 1) / (groups * kTurns));
+  }
+};
 
 template <int DT>
 int launch_forward(const void* x, int64_t ldx, const void* w, const void* b, void* out, int64_t ldo, float* mean, float* rstd, int M, int H, float eps,
                    hipStream_t st) {
-  launch(layer_norm_block_kernel<DT>, M, 256, 0, st, x, ldx, w, b, out, ldo, mean, rstd, H, eps);
+  constexpr int V = Pieces<DT>::V;
+  const int pieces = (H + V - 1) / V;
+  if (H < V || pieces > 256 * 16) {
+    launch(layer_norm_block_kernel<DT>, M, 256, 0, st, x, ldx, w, b, out, ldo, mean, rstd, H, eps);
+    return check_launch("npamd_layer_norm");
+  }
+#define NPAMD_LN(NV, RW) launch(layer_norm_row_kernel<DT, NV, RW>, (unsigned)((M + 4 / RW - 1) / (4 / RW)), 256, 0, st, x, ldx, w, b, out, ldo, mean, rstd, M, H, eps)
+  int rw = 1;
+  while (rw < 4 && (pieces > 64 * 4 * rw || (pieces > 64 * rw && (int64_t)M * rw < kFewWaves))) rw *= 2;
+  const int nv = (pieces + 64 * rw - 1) / (64 * rw);
+  if (rw == 1) {
+    if (nv <= 1) NPAMD_LN(1, 1);
+    else if (nv <= 2) NPAMD_LN(2, 1);
+    else NPAMD_LN(4, 1);
+  } else if (rw == 2) {
+    if (nv <= 1) NPAMD_LN(1, 2);
+    else if (nv <= 2) NPAMD_LN(2, 2);
+    else NPAMD_LN(4, 2);
+  } else {
+    if (nv <= 1) NPAMD_LN(1, 4);
+    else if (nv <= 2) NPAMD_LN(2, 4);
+    else if (nv <= 4) NPAMD_LN(4, 4);
+    else if (nv <= 8) NPAMD_LN(8, 4);
+    else NPAMD_LN(16, 4);
+  }
+#undef NPAMD_LN
   return check_launch("npamd_layer_norm");
 }
 
 template <int DT>
 int launch_backward(const LayerNormBack& a, void* dw, void* db, float* partials, hipStream_t st) {
   const char* what = "npamd_layer_norm_backward";
-  if (a.M && a.dx) launch(layer_norm_back_block_kernel<DT>, a.M, 256, 0, st, a);
-  if (dw || db) {
-    const int parts = back_parts(a.M);
-    const unsigned columns = (unsigned)(a.H + 63) / 64;
-    if (parts) launch(layer_norm_back_columns_kernel<DT>, dim3(columns, parts), 256, 0, st, a, partials, parts);
-    launch(layer_norm_back_sum_kernel<DT>, dim3(columns, 2), 1024, 0, st, partials, parts, a.H, dw, db);
+  const bool sums = dw || db;
+  const BackPlan p(a.M, a.H, DT);
+  const unsigned columns = (unsigned)(a.H + 63) / 64;
+  if (a.M && p.nv) {
+    const int lds = sums ? (p.groups - 1) * 2 * p.nv * Pieces<DT>::V * 64 * p.row_waves * 4 : 0;
+    const auto kernel = p.nv == 1 ? layer_norm_back_kernel<DT, 1> : layer_norm_back_kernel<DT, 2>;
+    if (sums || a.dx) launch(kernel, p.parts, 1024, lds, st, a, sums ? partials : nullptr, p.row_waves, p.groups);
+  } else if (a.M) {
+    if (a.dx) launch(layer_norm_back_block_kernel<DT>, a.M, 256, 0, st, a);
+    if (sums) launch(layer_norm_back_columns_kernel<DT>, dim3(columns, p.parts), 256, 0, st, a, partials, p.parts);
   }
+  constexpr int V = Pieces<DT>::V;
+  const int width = p.nv ? (a.H + V - 1) / V * V : a.H, last = p.nv ? a.H / V * V : a.H;
+  if (sums) launch(layer_norm_back_sum_kernel<DT>, dim3(columns, 2), 1024, 0, st, partials, p.parts, a.H, width, last, dw, db);
   return check_launch(what);
 }
 
@@ -159,7 +494,7 @@ extern "C" int npamd_layer_norm(const void* x, int64_t ldx, const void* weight, 
 
 extern "C" int64_t npamd_layer_norm_workspace_bytes(int M, int H) {
   if (M < 1 || H < 1) return 0;
-  return (int64_t)back_parts(M) * 2 * H * 4;
+  return (int64_t)std::max(BackPlan(M, H, NPAMD_F16).parts, BackPlan(M, H, NPAMD_F32).parts) * 2 * ((H + 7) / 8 * 8) * 4;
 }
 
 extern "C" int npamd_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, const float* mean,

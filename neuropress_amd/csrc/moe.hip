@@ -18,6 +18,7 @@
 #include "common.hpp"
 #include "gemm_tile.hpp"
 #include "lds_transfer.hpp"
+#include "wave_ops.hpp"
 
 using namespace npamd;
 
@@ -41,36 +42,6 @@ struct MoeArgs {
   uint16_t* xs;    // [M][H], rows as the up kernel reads them
   uint16_t* h;     // [M][top_k][I]
 };
-
-// Over a wave without LDS: each step takes a lane's value from another lane's register.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t lane_move(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  v = max(v, lane_move<0x111, 0xF>(v));  // from 1, 2, 4, 8 lanes before, within 16 lanes
-  v = max(v, lane_move<0x112, 0xF>(v));
-  v = max(v, lane_move<0x114, 0xF>(v));
-  v = max(v, lane_move<0x118, 0xF>(v));
-  v = max(v, lane_move<0x142, 0xA>(v));  // lane 15 to the next 16, lane 31 to the upper half
-  v = max(v, lane_move<0x143, 0xC>(v));
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-// The sum, in lane 63.
-__device__ __forceinline__ float wave_sum_last(float v) {
-  auto add = [&](uint32_t from) { v += __builtin_bit_cast(float, from); };
-  auto bits = [&] { return __builtin_bit_cast(uint32_t, v); };
-  add(lane_move<0x111, 0xF>(bits()));
-  add(lane_move<0x112, 0xF>(bits()));
-  add(lane_move<0x114, 0xF>(bits()));
-  add(lane_move<0x118, 0xF>(bits()));
-  add(lane_move<0x142, 0xA>(bits()));
-  add(lane_move<0x143, 0xC>(bits()));
-  return v;
-}
-
-// Eight 16-bit values at any even address.
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 // int4 operands hold the columns of an octet in the order 0 4 1 5 2 6 3 7 (the nibbles 4 i and 4 i + 16 of a dword are a pair): where column k of it lies.
 __device__ __forceinline__ int octet_place(int k) { return ((k & 3) << 1) | ((k >> 2) & 1); }
@@ -185,8 +156,7 @@ __device__ __forceinline__ void pick_experts(const MoeArgs& a, int m, int lane, 
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (64 * i < a.E && lane + 64 * i < a.E) sum += __expf(v[i] - most);
-      sum = wave_sum_last(sum);
-      sum = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
+      sum = wave_sum(sum);
     }
     const float p = __expf(l - most) / sum;
     total += p;
