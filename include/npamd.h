@@ -520,7 +520,7 @@ int64_t npamd_layer_norm_workspace_bytes(int M, int H);
  * Dense product with an epilogue: y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n], f32 up to one rounding.
  * x, w, residual, y: act_dtype (NPAMD_F16 or NPAMD_BF16); bias: NULL, or bias_dtype NPAMD_F32 or act_dtype; residual: NULL, or
  * [M, N] with row stride ldr, and may be y itself (same row distance).  activation: one of NPAMD_ACT_*; GELU is v * (1 + erf(v / sqrt 2)) / 2, GELU_TANH
- * its form with tanh, SILU v / (1 + exp(-v)).  Any shape up to 32 tokens; past that K has to be a multiple of 8, x and w 16-byte
+ * its form with tanh, SILU v / (1 + exp(-v)).  Any shape and alignment up to NPAMD_GEMV_MAX_M tokens; past that K has to be a multiple of 8, x and w 16-byte
  * aligned, ldx and ldw multiples of 8 and below NPAMD_TILE_MAX_STRIDE.
  * workspace: optional, npamd_dense_gemm_act_workspace_bytes of them, 16-byte aligned, contents irrelevant; with less, K is not
  * split over blocks.  Calls that overlap must not share one.

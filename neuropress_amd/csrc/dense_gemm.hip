@@ -30,6 +30,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "activation.hpp"
 #include "dense_gemm.hpp"
 #include "gemm_tile.hpp"
 #include "lds_transfer.hpp"
@@ -58,8 +59,8 @@ struct DenseTile {
 };
 
 // SHORT: rows end inside the last step.  Loads past their end bring the last piece again, and the operands there are zeroed
-// as they are used, in the one step that has any.
-template <int ACT, int WGM, int WGN, int KG, bool SHORT>
+// as they are used, in the one step that has any.  EPILOGUE: s.ep is applied to the sums where they lie.
+template <int ACT, int WGM, int WGN, int KG, bool SHORT, bool EPILOGUE>
 __global__ void __launch_bounds__((DenseTile<WGM, WGN, KG>::kThreads))
 dense_gemm_kernel(const DenseShape s) {
   using T = DenseTile<WGM, WGN, KG>;
@@ -233,10 +234,31 @@ dense_gemm_kernel(const DenseShape s) {
     }
     return;
   }
-  store_wave_tile<ACT, 1, 2>(acc, lds + T::kRedBytes + wave * 4096, lane, s.y, s.ldy, m0 + wm * 32, n0 + wn * 64, s.M, s.N, s.bias);
+  if constexpr (EPILOGUE) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int n = min(n0 + wn * 64 + t * 32 + c, s.N - 1);
+      float bias = 0.f;
+      if (s.ep.bias) bias = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, n) : ((const float*)s.ep.bias)[n];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[0][t][i] += bias;
+      activate_all(s.ep.act, [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[0][t][i] = f(acc[0][t][i]);
+      });
+      if (s.ep.residual) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = min(m0 + wm * 32 + 8 * (i / 4) + 4 * h + (i % 4), s.M - 1);
+          acc[0][t][i] += load_as_f32<ACT>(s.ep.residual, (int64_t)m * s.ep.ldr + n);
+        }
+      }
+    }
+  }
+  store_wave_tile<ACT, 1, 2>(acc, lds + T::kRedBytes + wave * 4096, lane, s.y, s.ldy, m0 + wm * 32, n0 + wn * 64, s.M, s.N, EPILOGUE ? nullptr : s.bias);
 }
 
-template <int ACT, int WGM, int WGN, int KG>
+template <int ACT, int WGM, int WGN, int KG, bool EPILOGUE>
 int launch_dense_tile(DenseShape s, hipStream_t st) {
   using T = DenseTile<WGM, WGN, KG>;
   s.row_tiles = (s.M + T::kBM - 1) / T::kBM;
@@ -246,7 +268,7 @@ int launch_dense_tile(DenseShape s, hipStream_t st) {
   if (blocks > 0x7FFFFFFF) return fail(NPAMD_ERR_UNSUPPORTED, "npamd_dense_gemm: too many tiles");
   static LdsLatch latches[2];
   const bool ends_inside = s.pieces % 8 != 0;
-  const auto kernel = ends_inside ? dense_gemm_kernel<ACT, WGM, WGN, KG, true> : dense_gemm_kernel<ACT, WGM, WGN, KG, false>;
+  const auto kernel = ends_inside ? dense_gemm_kernel<ACT, WGM, WGN, KG, true, EPILOGUE> : dense_gemm_kernel<ACT, WGM, WGN, KG, false, EPILOGUE>;
   const hipError_t e = enable_dynamic_lds(latches[ends_inside], reinterpret_cast<const void*>(kernel), T::kLds);
   if (e != hipSuccess)
     return fail(NPAMD_ERR_LAUNCH, "npamd_dense_gemm: cannot reserve %d bytes of LDS: %s", T::kLds, hipGetErrorString(e));
@@ -285,12 +307,75 @@ constexpr int kDenseTiles = sizeof(kDenseCost) / sizeof(kDenseCost[0]), kDenseTw
 
 template <int ACT>
 int launch_dense(const DenseShape& s, int tile, hipStream_t st) {
-  const int rc = tile == 0 ? launch_dense_tile<ACT, 1, 1, 4>(s, st)
-                 : tile == kDenseTwoGroups ? launch_dense_tile<ACT, 2, 2, 2>(s, st)
+  const int rc = tile == 0 ? launch_dense_tile<ACT, 1, 1, 4, false>(s, st)
+                 : tile == kDenseTwoGroups ? launch_dense_tile<ACT, 2, 2, 2, false>(s, st)
                                            : launch_wide(s, ACT, tile, st);
   if (rc != NPAMD_OK || s.splits == 1) return rc;
   launch_splitk_reduce<ACT>(s.partials, s.splits, s.M, s.N, s.bias, s.y, s.ldy, st);
   return check_launch("npamd_dense_gemm");
+}
+
+// splitk_reduce_kernel with an epilogue: four columns to a thread, the parts' loads in batches.
+template <int ACT>
+__global__ void __launch_bounds__(64) splitk_reduce_epilogue_kernel(const DenseShape s) {
+  const int n = ((int)blockIdx.x * 64 + (int)threadIdx.x) * 4, last = min(3, s.N - 1 - n);  // columns past N: the last one again, not stored
+  if (n >= s.N) return;
+  const bool vec = s.N % 4 == 0 && (reinterpret_cast<uintptr_t>(s.partials) & 15) == 0;
+  float bias[4] = {0.f, 0.f, 0.f, 0.f};
+  if (s.ep.bias) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[j] = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, n + min(j, last)) : ((const float*)s.ep.bias)[n + min(j, last)];
+  }
+  for (int m = blockIdx.y; m < s.M; m += gridDim.y) {
+    const float* const p = s.partials + (size_t)m * s.N + n;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int z0 = 0; z0 < s.splits; z0 += kReduceBatch) {
+      float v[kReduceBatch][4];
+#pragma unroll
+      for (int i = 0; i < kReduceBatch; ++i) {
+        const float* const q = p + (size_t)min(z0 + i, s.splits - 1) * s.M * s.N;
+        if (vec) {
+          const f32x4 t = *reinterpret_cast<const f32x4*>(q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i][j] = t[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i][j] = q[min(j, last)];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kReduceBatch; ++i)
+        if (z0 + i < s.splits) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[j] += v[i][j];
+        }
+    }
+    float res[4] = {0.f, 0.f, 0.f, 0.f};
+    if (s.ep.residual) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) res[j] = load_as_f32<ACT>(s.ep.residual, (int64_t)m * s.ep.ldr + n + min(j, last));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] += bias[j];
+    activate_all(s.ep.act, [&](auto f) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = f(sum[j]);
+    });
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j <= last) store_from_f32<ACT>(s.y, (int64_t)m * s.ldy + n + j, s.ep.residual ? sum[j] + res[j] : sum[j]);
+  }
+}
+
+template <int ACT>
+int launch_dense_epilogue(const DenseShape& s, int tile, hipStream_t st, const char* what) {
+  const int rc = tile == 0 ? launch_dense_tile<ACT, 1, 1, 4, true>(s, st)
+                 : tile == kDenseTwoGroups ? launch_dense_tile<ACT, 2, 2, 2, true>(s, st)
+                                           : launch_wide_epilogue(s, ACT, tile, st);
+  if (rc != NPAMD_OK || s.splits == 1) return rc;
+  const dim3 grid((unsigned)(((s.N + 3) / 4 + 63) / 64), (unsigned)(s.M < 65535 ? s.M : 65535));
+  launch(splitk_reduce_epilogue_kernel<ACT>, grid, 64, 0, st, s);
+  return check_launch(what);
 }
 
 constexpr int kDenseMaxSplits = 16;
@@ -392,7 +477,7 @@ static int dense_gemm(const char* what, const void* x, int64_t ldx, const void* 
   const bool wide = ldy < kDenseStrideMax;
   DensePlan p = plan_dense(M, N, width, tuning().dense_tile, kDenseMaxSplits, wide);
   if (p.splits > room) p = plan_dense(M, N, width, tuning().dense_tile, 1, wide);  // too little workspace: unsplit
-  const DenseShape s{x, w, bias, y, ldx, ldw, ldy, M, N, width / 64, 0, 0, p.splits, 0, (float*)workspace, K / 8, 0};
+  const DenseShape s{x, w, bias, y, ldx, ldw, ldy, M, N, width / 64, 0, 0, p.splits, 0, (float*)workspace, K / 8, 0, {}};
   const int tile = p.tile;
   return act_dtype == NPAMD_BF16 ? launch_dense<NPAMD_BF16>(s, tile, st) : launch_dense<NPAMD_F16>(s, tile, st);
 }
@@ -402,6 +487,19 @@ extern "C" int npamd_dense_gemm(const void* x, int64_t ldx, const void* w, int64
   const char* what = "npamd_dense_gemm";
   NPAMD_REQUIRE(M >= 0 && N >= 0 && K >= 64 && K % 64 == 0, "%s: bad shape M=%d N=%d K=%d (K has to be a multiple of 64)", what, M, N, K);
   return dense_gemm(what, x, ldx, w, ldw, bias, y, ldy, M, N, K, act_dtype, workspace, workspace_bytes, stream);
+}
+
+int npamd::dense_gemm_epilogue(const char* what, const DenseShape& shape, int K, int act, int64_t workspace_bytes, hipStream_t st) {
+  DenseShape s = shape;
+  const int64_t room = s.partials ? workspace_bytes / ((int64_t)s.M * s.N * 4) : 1;
+  const int width = (K + 63) / 64 * 64;
+  const bool wide = s.ldy < kDenseStrideMax;
+  DensePlan p = plan_dense(s.M, s.N, width, tuning().dense_tile, kDenseMaxSplits, wide);
+  if (p.splits > room) p = plan_dense(s.M, s.N, width, tuning().dense_tile, 1, wide);  // too little workspace: unsplit
+  s.steps = width / 64;
+  s.splits = p.splits;
+  s.pieces = K / 8;
+  return act == NPAMD_BF16 ? launch_dense_epilogue<NPAMD_BF16>(s, p.tile, st, what) : launch_dense_epilogue<NPAMD_F16>(s, p.tile, st, what);
 }
 
 // Rows of x and w that end inside a 64-k step, K a multiple of 8: neither is copied to whole steps first.

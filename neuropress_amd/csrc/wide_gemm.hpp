@@ -15,6 +15,7 @@
 
 #include <type_traits>
 
+#include "activation.hpp"
 #include "dense_gemm.hpp"
 #include "gemm_tile.hpp"
 #include "lds_transfer.hpp"
@@ -41,7 +42,8 @@ struct WideTile {
   static_assert(kLds <= kLdsPerBlockMax && SPAN <= 2 * kMfmas && (ST - 1) * kLoads < 64);
 };
 
-template <int ACT, class T>
+// EPILOGUE: s.ep is applied to the sums, which leave through LDS in f32, 16 rows of a wave at a time.
+template <int ACT, class T, bool EPILOGUE = false>
 __global__ void __launch_bounds__(T::kThreads, T::kThreads == 256 ? 2 : 1)
 wide_gemm_kernel(const DenseShape s) {
   constexpr int MT = T::MT, NT = T::NT, ST = T::ST, L = T::kLoads, kM = T::kMfmas, SPAN = T::SPAN;
@@ -210,6 +212,72 @@ wide_gemm_kernel(const DenseShape s) {
       }
     return;
   }
+  if constexpr (EPILOGUE) {
+    constexpr int kRow = 64 * NT + 16, kPerRow = 2 * NT, kRowsAtOnce = 64 / kPerRow;  // bytes of a row in LDS; pieces of eight values
+    static_assert(16 * kRow <= T::kLds / T::kWaves);
+    uint8_t* const ep = lds + wave * 16 * kRow;
+    const int r = lane / kPerRow, p = lane % kPerRow, n = p * 8;
+    float bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bias[e] = 0.f;
+      const int at = min(wn0 + n + e, s.N - 1);
+      if (s.ep.bias) bias[e] = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, at) : ((const float*)s.ep.bias)[at];
+    }
+    const bool whole = s.N % 8 == 0 && s.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(s.y) & 15) == 0 &&
+                       (!s.ep.residual || (s.ep.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(s.ep.residual) & 15) == 0));
+    uint16_t* const to = reinterpret_cast<uint16_t*>(s.y) + (int64_t)wm0 * s.ldy + wn0;
+    const uint16_t* const from = reinterpret_cast<const uint16_t*>(s.ep.residual) + (int64_t)wm0 * s.ep.ldr + wn0;
+#pragma unroll 1
+    for (int a = 0; a < MT; ++a) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (i != a) continue;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) *reinterpret_cast<f32x4*>(ep + c * kRow + 64 * b + 16 * h) = acc[i][b];
+      }
+#pragma unroll 1
+      for (int i = 0; i < (16 + kRowsAtOnce - 1) / kRowsAtOnce; ++i) {
+        const int row = i * kRowsAtOnce + r, m = 16 * a + row;
+        const bool in = r < kRowsAtOnce && row < 16 && m < rows && n < cols;
+        if (!in) continue;
+        u32x4 res{0, 0, 0, 0};
+        if (s.ep.residual) {
+          const uint16_t* const at = from + (int64_t)m * s.ep.ldr + n;
+          if (whole) {
+            res = *reinterpret_cast<const u32x4*>(at);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < cols) res[e >> 1] |= (uint32_t)at[e] << (16 * (e & 1));
+          }
+        }
+        float v[8];
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(ep + row * kRow + 32 * p), hi = *reinterpret_cast<const f32x4*>(ep + row * kRow + 32 * p + 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lo[e] + bias[e], v[4 + e] = hi[e] + bias[4 + e];
+        activate_all(s.ep.act, [&](auto f) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
+        });
+        uint32_t bits[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (s.ep.residual) v[e] += act_bits_to_f32<ACT>((res[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+          bits[e] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(v[e]) : f32_to_f16_bits(v[e]);
+        }
+        uint16_t* const at = to + (int64_t)m * s.ldy + n;
+        if (whole) {
+          *reinterpret_cast<u32x4*>(at) = u32x4{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16), bits[4] | (bits[5] << 16), bits[6] | (bits[7] << 16)};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < cols) at[e] = (uint16_t)bits[e];
+        }
+      }
+    }
+    return;
+  }
   // Through LDS, each wave in a part of its own: rows of 16 NT columns then leave whole.
   uint8_t* const ep = lds + wave * T::kEpBytes;
 #pragma unroll
@@ -257,7 +325,7 @@ wide_gemm_kernel(const DenseShape s) {
   }
 }
 
-template <int ACT, class T>
+template <int ACT, class T, bool EPILOGUE = false>
 int launch_wide_tile(DenseShape s, hipStream_t st) {
   s.row_tiles = (s.M + T::kBM - 1) / T::kBM;
   s.col_tiles = (s.N + T::kBN - 1) / T::kBN;
@@ -270,11 +338,31 @@ int launch_wide_tile(DenseShape s, hipStream_t st) {
   // x 1024 19.2 / 15.3; 1440 x 970 x 8832 53.4 / 59.2, 1956 x 1532 x 11008 102.2 / 108.5, 3575 x 703 x 1536 17.3 / 20.3.
   s.group = s.M > 1.2f * s.N ? 4 : 2048 / T::kBM;
   static LdsLatch latch;
-  const auto kernel = wide_gemm_kernel<ACT, T>;
+  const auto kernel = wide_gemm_kernel<ACT, T, EPILOGUE>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), T::kLds);
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "npamd_dense_gemm: cannot reserve %d bytes of LDS: %s", T::kLds, hipGetErrorString(e));
   launch(kernel, (unsigned)blocks, T::kThreads, T::kLds, st, s);
   return check_launch("npamd_dense_gemm");
+}
+
+// Which number of the plan's list (dense_gemm.hip) is which tile.
+template <int ACT, bool EPILOGUE>
+int launch_wide_on(const DenseShape& s, int tile, hipStream_t st) {
+  switch (tile) {
+    case 1: return launch_wide_tile<ACT, WideTile<2, 2, 2, 2, 6, 4>, EPILOGUE>(s, st);    // 64 x 64
+    case 2: return launch_wide_tile<ACT, WideTile<2, 2, 2, 4, 5, 12>, EPILOGUE>(s, st);   // 64 x 128
+    case 3: return launch_wide_tile<ACT, WideTile<2, 2, 4, 4, 4, 24>, EPILOGUE>(s, st);   // 128 x 128
+    case 4: return launch_wide_tile<ACT, WideTile<2, 2, 5, 4, 4, 24>, EPILOGUE>(s, st);   // 160 x 128
+    case 5: return launch_wide_tile<ACT, WideTile<4, 2, 4, 4, 3, 24>, EPILOGUE>(s, st);   // 256 x 128
+    case 6: return launch_wide_tile<ACT, WideTile<4, 2, 3, 4, 3, 20>, EPILOGUE>(s, st);   // 192 x 128
+    case 7: return launch_wide_tile<ACT, WideTile<2, 2, 3, 4, 4, 20>, EPILOGUE>(s, st);   // 96 x 128
+    case 8: return launch_wide_tile<ACT, WideTile<2, 4, 5, 4, 3, 24>, EPILOGUE>(s, st);   // 160 x 256
+    case 9: return launch_wide_tile<ACT, WideTile<2, 4, 6, 4, 2, 20>, EPILOGUE>(s, st);   // 192 x 256
+    case 10: return launch_wide_tile<ACT, WideTile<4, 2, 4, 7, 2, 24>, EPILOGUE>(s, st);  // 256 x 224
+    case 11: return launch_wide_tile<ACT, WideTile<2, 4, 8, 4, 2, 24>, EPILOGUE>(s, st);  // 256 x 256
+    case 12: return launch_wide_tile<ACT, WideTile<2, 2, 3, 2, 6, 6>, EPILOGUE>(s, st);   // 96 x 64
+    default: return launch_wide_tile<ACT, WideTile<2, 4, 6, 3, 3, 24>, EPILOGUE>(s, st);  // 192 x 192
+  }
 }
 
 }  // namespace npamd

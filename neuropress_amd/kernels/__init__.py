@@ -1266,8 +1266,12 @@ def dense_linear_act(
     if any(t is not None and tracked(t) for t in (x, w, bias, residual)):
         return _torch_linear_act(x, w, bias, activation, residual)
     m = x.numel() // k
-    x2 = _lead2d(x, m, k)
-    w = _rows(w)
+    x2, w = _lead2d(x, m, k), _rows(w)
+    if m > _lib.GEMV_MAX_M:  # the tiles read 16 bytes at a time: rows of whole pieces
+        if k % 8:
+            x2, w = (gather_columns(t, None, -(-k // 8) * 8) for t in (x2, w))
+            k = x2.shape[1]
+        x2, w = _aligned_rows(x2), _aligned_rows(w)
     bias = None if bias is None else bias.contiguous()
     r2 = None if residual is None else _lead2d(residual, m, n)
     y = torch.empty(shape, device=x.device, dtype=x.dtype)
