@@ -327,6 +327,11 @@ __global__ void __launch_bounds__(64) splitk_reduce_epilogue_kernel(const DenseS
     for (int j = 0; j < 4; ++j) bias[j] = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, n + min(j, last)) : ((const float*)s.ep.bias)[n + min(j, last)];
   }
   for (int m = blockIdx.y; m < s.M; m += gridDim.y) {
+    float res[4] = {0.f, 0.f, 0.f, 0.f};
+    if (s.ep.residual) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) res[j] = load_as_f32<ACT>(s.ep.residual, (int64_t)m * s.ep.ldr + n + min(j, last));
+    }
     const float* const p = s.partials + (size_t)m * s.N + n;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int z0 = 0; z0 < s.splits; z0 += kReduceBatch) {
@@ -349,11 +354,6 @@ __global__ void __launch_bounds__(64) splitk_reduce_epilogue_kernel(const DenseS
 #pragma unroll
           for (int j = 0; j < 4; ++j) sum[j] += v[i][j];
         }
-    }
-    float res[4] = {0.f, 0.f, 0.f, 0.f};
-    if (s.ep.residual) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) res[j] = load_as_f32<ACT>(s.ep.residual, (int64_t)m * s.ep.ldr + n + min(j, last));
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] += bias[j];

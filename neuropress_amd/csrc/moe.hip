@@ -50,16 +50,6 @@ __device__ __forceinline__ u32x4 octet_order(const u32x4& v) {  // (0 1) (2 3) (
                __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
 }
 
-template <int ACT>
-__device__ __forceinline__ float dot8(const u32x4& a, const u32x4& b, float sum) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    sum = __builtin_fmaf(act_bits_to_f32<ACT>(a[i] & 0xFFFFu), act_bits_to_f32<ACT>(b[i] & 0xFFFFu), sum);
-    sum = __builtin_fmaf(act_bits_to_f32<ACT>(a[i] >> 16), act_bits_to_f32<ACT>(b[i] >> 16), sum);
-  }
-  return sum;
-}
-
 // The logits of one expert for TB tokens (blockIdx.y); and every row of x, copied to where the up kernel reads it (NIBBLES: each octet in int4's order), by one block
 // each.  It clears the down kernel's counters.
 template <int ACT, int TB, bool NIBBLES>
@@ -79,7 +69,7 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a) {
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
       const u32x4 xv = *reinterpret_cast<const u32x4_any*>(x + min(m0 + t, a.M - 1) * a.ldx + 8 * k);
-      v[t] = dot8<ACT>(xv, r, v[t]);
+      v[t] = add_dot8<ACT>(xv, r, v[t]);
     }
   }
 #pragma unroll

@@ -1,4 +1,4 @@
-// Reductions over a wave in registers, and 16-byte loads at any address.
+// Reductions over a wave in registers, dot products of eight values, and 16-byte loads at any address.
 #pragma once
 
 #include "common.hpp"
@@ -35,6 +35,17 @@ __device__ __forceinline__ float wave_sum_last(float v) {
 // The sum, in every lane.
 __device__ __forceinline__ float wave_sum(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_sum_last(v)), 63));
+}
+
+// sum + the dot product of eight values each, in f32.
+template <int ACT>
+__device__ __forceinline__ float add_dot8(const u32x4& a, const u32x4& b, float sum) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum = __builtin_fmaf(act_bits_to_f32<ACT>(a[i] & 0xFFFFu), act_bits_to_f32<ACT>(b[i] & 0xFFFFu), sum);
+    sum = __builtin_fmaf(act_bits_to_f32<ACT>(a[i] >> 16), act_bits_to_f32<ACT>(b[i] >> 16), sum);
+  }
+  return sum;
 }
 
 // Four dwords at any even address: the card's memory takes them as they lie.

@@ -228,6 +228,30 @@ wide_gemm_kernel(const DenseShape s) {
                        (!s.ep.residual || (s.ep.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(s.ep.residual) & 15) == 0));
     uint16_t* const to = reinterpret_cast<uint16_t*>(s.y) + (int64_t)wm0 * s.ldy + wn0;
     const uint16_t* const from = reinterpret_cast<const uint16_t*>(s.ep.residual) + (int64_t)wm0 * s.ep.ldr + wn0;
+    constexpr int kTurns = (16 + kRowsAtOnce - 1) / kRowsAtOnce;
+    // Row i of the lane in rows 16 a ..: -1 where it has none.
+    auto row_of = [&](int a, int i) NPAMD_INLINE {
+      const int row = i * kRowsAtOnce + r, m = 16 * a + row;
+      return r < kRowsAtOnce && row < 16 && m < rows && n < cols ? row : -1;
+    };
+    u32x4 res[2][kTurns];
+    auto ask = [&](int set, int a) NPAMD_INLINE {
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int row = row_of(a, i);
+        res[set][i] = u32x4{0, 0, 0, 0};
+        if (row < 0) continue;
+        const uint16_t* const at = from + (int64_t)(16 * a + row) * s.ep.ldr + n;
+        if (whole) {
+          res[set][i] = *reinterpret_cast<const u32x4*>(at);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < cols) res[set][i][e >> 1] |= (uint32_t)at[e] << (16 * (e & 1));
+        }
+      }
+    };
+    if (s.ep.residual) ask(0, 0);
 #pragma unroll 1
     for (int a = 0; a < MT; ++a) {
 #pragma unroll
@@ -236,44 +260,41 @@ wide_gemm_kernel(const DenseShape s) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) *reinterpret_cast<f32x4*>(ep + c * kRow + 64 * b + 16 * h) = acc[i][b];
       }
-#pragma unroll 1
-      for (int i = 0; i < (16 + kRowsAtOnce - 1) / kRowsAtOnce; ++i) {
-        const int row = i * kRowsAtOnce + r, m = 16 * a + row;
-        const bool in = r < kRowsAtOnce && row < 16 && m < rows && n < cols;
-        if (!in) continue;
-        u32x4 res{0, 0, 0, 0};
-        if (s.ep.residual) {
-          const uint16_t* const at = from + (int64_t)m * s.ep.ldr + n;
-          if (whole) {
-            res = *reinterpret_cast<const u32x4*>(at);
-          } else {
+      if (s.ep.residual && a + 1 < MT) ask(1, a + 1);  // a round of rows ahead
+      float v[kTurns][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < cols) res[e >> 1] |= (uint32_t)at[e] << (16 * (e & 1));
-          }
-        }
-        float v[8];
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(ep + row * kRow + 32 * p), hi = *reinterpret_cast<const f32x4*>(ep + row * kRow + 32 * p + 16);
+      for (int i = 0; i < kTurns; ++i) {
+        const uint8_t* const at = ep + min(i * kRowsAtOnce + r, 15) * kRow + 32 * min(p, kPerRow - 1);
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(at), hi = *reinterpret_cast<const f32x4*>(at + 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = lo[e] + bias[e], v[4 + e] = hi[e] + bias[4 + e];
-        activate_all(s.ep.act, [&](auto f) {
+        for (int e = 0; e < 4; ++e) v[i][e] = lo[e] + bias[e], v[i][4 + e] = hi[e] + bias[4 + e];
+      }
+      activate_all(s.ep.act, [&](auto f) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
-        });
+        for (int i = 0; i < kTurns; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] = f(v[i][e]);
+      });
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int row = row_of(a, i);
         uint32_t bits[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (s.ep.residual) v[e] += act_bits_to_f32<ACT>((res[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
-          bits[e] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(v[e]) : f32_to_f16_bits(v[e]);
+          if (s.ep.residual) v[i][e] += act_bits_to_f32<ACT>((res[0][i][e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+          bits[e] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(v[i][e]) : f32_to_f16_bits(v[i][e]);
         }
-        uint16_t* const at = to + (int64_t)m * s.ldy + n;
-        if (whole) {
-          *reinterpret_cast<u32x4*>(at) = u32x4{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16), bits[4] | (bits[5] << 16), bits[6] | (bits[7] << 16)};
-        } else {
+        if (row >= 0) {
+          uint16_t* const at = to + (int64_t)(16 * a + row) * s.ldy + n;
+          if (whole) {
+            *reinterpret_cast<u32x4*>(at) = u32x4{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16), bits[4] | (bits[5] << 16), bits[6] | (bits[7] << 16)};
+          } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e < cols) at[e] = (uint16_t)bits[e];
+            for (int e = 0; e < 8; ++e)
+              if (n + e < cols) at[e] = (uint16_t)bits[e];
+          }
         }
+        res[0][i] = res[1][i];
       }
     }
     return;

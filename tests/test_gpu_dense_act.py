@@ -201,3 +201,29 @@ def test_the_residual_in_its_own_place(gpu):
         _lib.call("npamd_dense_gemm_act", x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), 0, 1, room.data_ptr(), n + 8, room.data_ptr(), n + 8, m, n, k, 0, None, 0,
                   torch.cuda.current_stream().cuda_stream)  # fmt: skip
         _check(room[:m, :n], x, w, b, "relu", r)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [2, 3, 15, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize("n,k", [(1, 8), (16, 120), (17, 128), (100, 1032), (8191, 136), (8192, 136), (8209, 1160)])
+def test_where_one_kernel_takes_over_from_another(gpu, dtype, m, n, k):
+    """Tokens and rows on both sides of where the kernel changes; columns that end inside a step, or before every wave has one."""
+    x, w, b, r = _inputs(m, n, k, dtype)
+    _check(_run(x, w, b, "silu", r), x, w, b, "silu", r)
+
+
+@pytest.mark.parametrize("n", [4096, 4112])  # 2^24 weights of 4096 columns, and some more
+@pytest.mark.parametrize("m", [16, 17, 32])
+def test_weights_on_both_sides_of_the_line(gpu, m, n):
+    x, w, b, r = _inputs(m, n, 4096, torch.bfloat16)
+    _check(_run(x, w, b, "gelu", r), x, w, b, "gelu", r)
+
+
+def test_nothing_of_other_rows_reaches_a_result(gpu):
+    """Infinities and NaN in the rows that a tile reads besides its own, and behind the columns."""
+    x, w, b, r = _inputs(32, 48, 200, torch.bfloat16)
+    for m, n in [(1, 48), (3, 47), (5, 17), (17, 33), (31, 1)]:
+        xs, ws = torch.full((32, 208), float("nan"), dtype=x.dtype), torch.full((48, 208), float("inf"), dtype=x.dtype)
+        xs[:m, :200], ws[:n, :200] = x[:m], w[:n]
+        xs, ws = xs.to("cuda")[:m, :200], ws.to("cuda")[:n, :200]
+        _check(_run(xs, ws, b[:n], "relu", r[:m, :n]), xs, ws, b[:n], "relu", r[:m, :n])
