@@ -69,7 +69,7 @@ def _compile(src: Path, force: bool) -> Path:
 def _compile_host(force: bool) -> Path:
     """Compile the host extension module (no device code) against torch's headers."""
     obj = OBJ_DIR / (HOST_SRC.stem + ".o")
-    newest = max(HOST_SRC.stat().st_mtime, _headers_mtime())
+    newest = max(*(f.stat().st_mtime for f in HOST_SRC.parent.iterdir()), _headers_mtime())
     if not force and obj.exists() and obj.stat().st_mtime >= newest:
         return obj
     from torch.utils.cpp_extension import include_paths

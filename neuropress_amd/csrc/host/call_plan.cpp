@@ -882,7 +882,19 @@ PyObject* tracked_tensor(PyObject*, PyObject* xo) {
   return translated([&] { return PyBool_FromLong(tracked(THPVariable_Unpack(xo))); });
 }
 
+}  // namespace
+
+#include "feed_forward.hpp"
+
+namespace {
+
+PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
+
 PyMethodDef module_methods[] = {
+    {"layer_norm", fast(layer_norm), METH_FASTCALL, "layer_norm(x, weight, bias, eps, stats): the output (with the rows' statistics), or None"},
+    {"layer_norm_backward", fast(layer_norm_backward), METH_FASTCALL, "layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight, dbias): the gradients, or None"},
+    {"dense_linear_act", fast(dense_linear_act), METH_FASTCALL, "dense_linear_act(x, w, bias, activation, residual): the output, or None"},
+    {"moe_layer", fast(moe_layer), METH_FASTCALL, "moe_layer(x, 7 tensors, 6 numbers, renormalize): the output, or None"},
     {"tracked", tracked_tensor, METH_O, "tracked(x): whether torch follows what is done to x, so that no plan issues the call"},
     {"row_distance", row_distance, METH_O, "row_distance(x): elements between the rows a plan would read, or None"},
     {"set_module_class", set_module_class, METH_VARARGS, "set_module_class(torch.nn.Module, its call in Python)"},

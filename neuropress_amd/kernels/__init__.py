@@ -1119,6 +1119,13 @@ def _on_device(t: torch.Tensor):
     return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def _rows_of(what: str, x: torch.Tensor, width: int) -> int:
+    rows = x.numel() // width
+    if max(rows, width) > 2**31 - 1:
+        raise RuntimeError(f"{what}: at most 2**31 - 1 rows and columns, got {rows} x {width}")
+    return rows
+
+
 def _lead2d(t: torch.Tensor, rows: int, width: int) -> torch.Tensor:
     """*t* ``[..., width]`` as *rows* rows for a kernel: a view where they lie at one distance, else a copy."""
     return _rows(t if t.dim() == 2 else t.reshape(rows, width))
@@ -1142,8 +1149,10 @@ def _norm_args(what: str, x: torch.Tensor, *params: torch.Tensor | None) -> int:
 
 
 def _layer_norm(what, x, weight, bias, eps, stats):
+    if stats and (out := _lib.host().layer_norm(x, weight, bias, eps, True)) is not None:
+        return out
     h = _norm_args(what, x, weight, bias)
-    m = x.numel() // h
+    m = _rows_of(what, x, h)
     x2 = _lead2d(x, m, h)
     weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
     out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
@@ -1176,6 +1185,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     Where a gradient of x, weight or bias is recorded, the backward pass is :func:`layer_norm_backward`'s kernels (first derivatives).  Calls that torch follows in
     other ways (forward mode, ``torch.func``, traces, autocast to another type) go through ``torch.nn.functional.layer_norm``.
     """
+    out = _lib.host().layer_norm(x, weight, bias, eps, False)
+    if out is not None:
+        return out
     followed = [t for t in (x, weight, bias) if t is not None and tracked(t)]
     if not followed:
         return _layer_norm("layer_norm", x, weight, bias, eps, False)[0]
@@ -1204,12 +1216,15 @@ def layer_norm_backward(
 ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
     """Gradients of x, weight and bias (``npamd_layer_norm_backward``), in x's dtype; None where *needs* says no.  *mean*, *rstd*: of
     :func:`layer_norm_stats`.  The same bits from run to run."""
+    out = _lib.host().layer_norm_backward(dy, x, weight, mean, rstd, *needs)
+    if out is not None:
+        return out
     what = "layer_norm_backward"
     h = _norm_args(what, x, weight)
     _check_device(what, x, dy, mean, rstd)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise RuntimeError(f"{what}: dy must have x's shape and dtype")
-    m = x.numel() // h
+    m = _rows_of(what, x, h)
     x2, dy2 = _lead2d(x, m, h), _lead2d(dy, m, h)
     for t in (mean, rstd):
         if t.dtype != torch.float32 or t.numel() != m:
@@ -1249,11 +1264,15 @@ def dense_linear_act(
     *activation*: None, ``"relu"``, ``"gelu"`` (with erf), ``"gelu_tanh"`` or ``"silu"``; *bias* ``[N]`` in float32 or x's dtype; *residual* ``[..., N]`` in x's
     dtype.  Any sizes.  Calls that torch follows (:func:`tracked`) go through torch's own operations, which round in between.
     """
+    code = ACTIVATIONS.get(activation)
+    y = None if code is None else _lib.host().dense_linear_act(x, w, bias, code, residual)
+    if y is not None:
+        return y
     what = "dense_linear_act"
     _check_device(what, x, w, bias, residual)
     if x.dtype not in (torch.float16, torch.bfloat16) or w.dtype != x.dtype or w.dim() != 2 or x.dim() < 1 or w.shape[1] != x.shape[-1]:
         raise RuntimeError(f"{what}: x and w must be float16 or bfloat16 [..., K] and [N, K]")
-    if activation not in ACTIVATIONS:
+    if code is None:
         raise RuntimeError(f"{what}: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     n, k = w.shape
     if k < 1:
@@ -1265,7 +1284,8 @@ def dense_linear_act(
         raise RuntimeError(f"{what}: residual must be {list(shape)} in x's dtype")
     if any(t is not None and tracked(t) for t in (x, w, bias, residual)):
         return _torch_linear_act(x, w, bias, activation, residual)
-    m = x.numel() // k
+    m = _rows_of(what, x, k)
+    _rows_of(what, w, k)
     x2, w = _lead2d(x, m, k), _rows(w)
     if m > _lib.GEMV_MAX_M:  # the tiles read 16 bytes at a time: rows of whole pieces
         if k % 8:
@@ -1279,7 +1299,7 @@ def dense_linear_act(
     ws = torch.empty(need // 4, device=x.device, dtype=torch.float32) if need > 0 else None
     with _on_device(x):
         _lib.call("npamd_dense_gemm_act", x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _ptr(bias), _lib.F32 if bias is None else _DT[bias.dtype],
-                  ACTIVATIONS[activation], _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), n, m, n, k, _DT[x.dtype], _ptr(ws), need, _stream(x))  # fmt: skip
+                  code, _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), n, m, n, k, _DT[x.dtype], _ptr(ws), need, _stream(x))  # fmt: skip
     return y
 
 
@@ -1343,6 +1363,10 @@ def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: boo
     """A whole mixture-of-experts layer for up to 32 tokens *x* ``[..., H]`` (``npamd_moe_layer``): softmax router over all experts, the *top_k* largest (ties: the
     lower index; divided by their sum with *renormalize*), ``down(silu(gate(x)) * up(x))`` of each, weighted sum.  For inference: calls that torch follows
     (:func:`tracked`) are refused."""
+    y = _lib.host().moe_layer(x, experts.router, experts.gate_up, experts.gate_up_scale, experts.gate_up_zero, experts.down, experts.down_scale, experts.down_zero,
+                              experts.experts, top_k, experts.hidden, experts.inter, experts.nbits, experts.group_size, renormalize)  # fmt: skip
+    if y is not None:
+        return y
     what = "moe_layer"
     _check_device(what, x, experts.router)
     h = experts.hidden
@@ -1350,7 +1374,7 @@ def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: boo
         raise RuntimeError(f"{what}: x must be {experts.router.dtype} [..., {h}], got {x.dtype} {list(x.shape)}")
     if tracked(x):
         raise RuntimeError(f"{what}: for inference only: no gradient, trace or transform of torch can follow it")
-    m, e, i = x.numel() // h, experts.experts, experts.inter
+    m, e, i = _rows_of(what, x, h), experts.experts, experts.inter
     x2 = _lead2d(x, m, h)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     need = int(_lib.load().npamd_moe_workspace_bytes(m, e, int(top_k), h, i))

@@ -147,3 +147,45 @@ def test_the_feed_forward_half_of_a_block(gpu, tokens, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
+
+
+class _Declining:
+    """The native call path as it answers a call that it does not take."""
+
+    def __init__(self, host):
+        self._host, self.asked = host, []
+
+    def __getattr__(self, name):
+        if name not in ("layer_norm", "layer_norm_backward", "dense_linear_act", "moe_layer"):
+            return getattr(self._host, name)
+        return lambda *args: self.asked.append(name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m", [1, 2, 9, 32])
+def test_native_and_python_route_agree(gpu, monkeypatch, dtype, m):
+    from neuropress_amd import _lib, kernels
+
+    g = torch.Generator().manual_seed(5 + m)
+    rand = lambda *s: torch.randn(*s, generator=g).to(dtype).to("cuda")
+    x, dy, w, b, res = rand(m, 192), rand(m, 192), rand(192), rand(192), rand(m, 200)
+    xs = rand(2, 16, 256)[:, : (m + 1) // 2, :192]  # rows that no single distance joins
+    lin, experts = rand(200, 192), kernels.MoEExperts(rand(6, 192), rand(6, 128, 192) / 14, rand(6, 192, 64) / 8)
+
+    def calls():
+        y, mean, rstd = kernels.layer_norm_stats(x, w, b, 1e-5)
+        out = [y, mean, rstd, kernels.layer_norm(x, w, b), kernels.layer_norm(xs, None, b, 0), kernels.layer_norm(x[:0], w, b)]
+        out += kernels.layer_norm_backward(dy, x, w, mean, rstd) + kernels.layer_norm_backward(dy.T.contiguous().T, x, None, mean, rstd, needs=(1, 0, 1))
+        for args in [(x, lin), (x, lin, b.new_ones(200).float(), "silu"), (x, lin[:, ::2].repeat(1, 2), b.new_ones(200), "gelu", res), (xs, lin, None, "relu")]:
+            out.append(kernels.dense_linear_act(*args))
+        return out + [kernels.moe_layer(x, experts, 2), kernels.moe_layer(x, experts, 3, 0)] + ([kernels.moe_layer(xs, experts, 3, 1)] if xs.numel() <= 32 * 192 else [])
+
+    with torch.no_grad():
+        native = calls()
+        host = _Declining(_lib.host())
+        monkeypatch.setattr(_lib, "host", lambda: host)
+        python = calls()
+    assert set(host.asked) == {"layer_norm", "layer_norm_backward", "dense_linear_act", "moe_layer"}
+    for a, c in zip(native, python, strict=True):
+        assert (a is None) == (c is None) and (a is None or (a.dtype == c.dtype and torch.equal(a, c)))
