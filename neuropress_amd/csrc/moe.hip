@@ -37,6 +37,7 @@ struct MoeArgs {
   float* logits;   // [M][E]
   uint16_t* ids;   // [M][top_k]
   float* share;    // [M][top_k]
+  uint32_t* entries;  // [M * top_k], and how many there are
   uint32_t* done;  // [H / 32] blocks of the down kernel that have left their part
   float* parts;    // [part][H / 32][M * 32]
   uint16_t* xs;    // [M][H], rows as the up kernel reads them
@@ -70,6 +71,7 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a) {
     for (int t = 0; t < TB; ++t) {
       const u32x4 xv = *reinterpret_cast<const u32x4_any*>(x + min(m0 + t, a.M - 1) * a.ldx + 8 * k);
       v[t] = add_dot8<ACT>(xv, r, v[t]);
+      if ((m0 + t) % a.E == e && m0 + t < a.M) reinterpret_cast<u32x4*>(a.xs)[(int64_t)(m0 + t) * octets + k] = NIBBLES ? octet_order(xv) : xv;
     }
   }
 #pragma unroll
@@ -77,11 +79,6 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a) {
     const float s = wave_sum_last(v[t]);
     if (lane == 63) part[wave][t] = s;
   }
-  for (int m = m0 + e; m < min(m0 + TB, a.M); m += a.E)
-    for (int k = threadIdx.x; k < octets; k += 256) {
-      const u32x4 xv = *reinterpret_cast<const u32x4_any*>(x + m * a.ldx + 8 * k);
-      reinterpret_cast<u32x4*>(a.xs)[(int64_t)m * octets + k] = NIBBLES ? octet_order(xv) : xv;
-    }
   __syncthreads();
   const int t = threadIdx.x;
   if (t < TB && m0 + t < a.M) a.logits[(m0 + t) * a.E + e] = part[0][t] + part[1][t] + part[2][t] + part[3][t];
@@ -435,6 +432,10 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) m
   for (int m = wave; m < a.M; m += waves) pick_experts(a, m, lane, route, blockIdx.x == 0);
   __syncthreads();
   list_entries(a, route, cap);
+  if (blockIdx.x == 0) {  // for the down kernel
+    for (int p = threadIdx.x; p < *route.n_entries; p += blockDim.x) a.entries[p] = route.entries[p];
+    if (threadIdx.x == 0) a.entries[a.M * a.top_k] = *route.n_entries;
+  }
 
   const int groups = TOGETHER ? waves : 1, tiles = a.I / 16 / groups, items = __builtin_amdgcn_readfirstlane(*route.n_entries) * tiles, steps = (a.H + S::kColumns - 1) / S::kColumns;
   const int first = TOGETHER ? 0 : steps * wave / waves, last = TOGETHER ? steps : steps * (wave + 1) / waves;  // this wave's steps of an item: one at least
@@ -530,10 +531,10 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const Mo
   uint8_t* const tokens = lds + waves * 2 * Walk::kPlace;
   Walk walk(lds + wave * 2 * Walk::kPlace, tokens + wave * 2 * x_bytes, S::x_loads(cap), a.I, a.shift, 0, 1);
   float* const sums = reinterpret_cast<float*>(tokens + waves * 2 * x_bytes);  // [wave][M][32]
-  for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) route.ids[p] = a.ids[p];
+  for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) route.ids[p] = a.ids[p], route.entries[p] = a.entries[p];  // those behind the last: never looked at
+  if (threadIdx.x == 0) *route.n_entries = (int)a.entries[a.M * a.top_k];
   for (int o = threadIdx.x; o < waves * a.M * 32; o += blockDim.x) sums[o] = 0.f;
   __syncthreads();
-  list_entries(a, route, cap);
 
   const int n0 = blockIdx.x * 32, steps = (a.I + S::kColumns - 1) / S::kColumns, all = __builtin_amdgcn_readfirstlane(*route.n_entries) * steps;
   const int shares = waves * gridDim.y, of = blockIdx.y * waves + wave;
@@ -613,7 +614,7 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const Mo
 }
 
 struct MoeSpace {
-  int64_t logits, ids, share, xs, h, done, parts, bytes;
+  int64_t logits, ids, share, entries, xs, h, done, parts, bytes;
   MoeSpace(int M, int E, int top_k, int H, int I) {
     int64_t at = 0;
     auto take = [&](int64_t n) {
@@ -624,6 +625,7 @@ struct MoeSpace {
     logits = take((int64_t)M * E * 4);
     ids = take((int64_t)M * top_k * 2);
     share = take((int64_t)M * top_k * 4);
+    entries = take(((int64_t)M * top_k + 1) * 4);
     xs = take((int64_t)M * H * 2);
     h = take((int64_t)M * top_k * I * 2);
     done = take((int64_t)H / 32 * 4);
@@ -643,7 +645,9 @@ int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   using S = MoeStep<FMT, ASYM>;
   constexpr int kRoom = 160 * 1024;
   const bool together = a.M >= kMoeTogether;
-  const int cap = std::min(a.M, 16), pairs = a.M * a.top_k, x_bytes = 2 * S::x_loads(cap) * 1024;
+  // Pairs of an entry: all that an MFMA takes, or half as many where an expert has four at the mean; their places in LDS keep blocks out (us with 16 / eight: 16 tokens
+  // int4 through two of eight 190 / 183, through eight of 64 88 / 70), an expert that has more is read again (32 tokens through two of eight 199 / 231).
+  const int pairs = a.M * a.top_k, cap = std::min(a.M, pairs <= 4 * a.E ? 8 : 16), x_bytes = 2 * S::x_loads(cap) * 1024;
   auto up_own = [&](int waves) { return waves * 4 * S::kItem + (together ? x_bytes : waves * (x_bytes + cap * kMoeRedRow * 4)); };
   auto down_own = [&](int waves) { return waves * (x_bytes + 4 * S::kItem + a.M * 32 * 4); };
   const int up_waves = together ? kMoeUpWaves : std::min(kMoeUpWaves, (a.H + S::kColumns - 1) / S::kColumns);
@@ -722,6 +726,6 @@ extern "C" int npamd_moe_layer(const void* x, int64_t ldx, const void* router, c
   while (codes && (32 << shift) < group_size) ++shift;
   const MoeArgs a{x, router, (const uint8_t*)gate_up, (const uint8_t*)down, half(gate_up_scale_f16), half(gate_up_zero_f16), half(down_scale_f16),
                   half(down_zero_f16), y, ldx, ldy, M, E, top_k, H, I, shift, renormalize, (float*)(at + space.logits), (uint16_t*)(at + space.ids),
-                  (float*)(at + space.share), (uint32_t*)(at + space.done), (float*)(at + space.parts), (uint16_t*)(at + space.xs), (uint16_t*)(at + space.h)};
+                  (float*)(at + space.share), (uint32_t*)(at + space.entries), (uint32_t*)(at + space.done), (float*)(at + space.parts), (uint16_t*)(at + space.xs), (uint16_t*)(at + space.h)};
   return act_dtype == NPAMD_BF16 ? launch_moe<NPAMD_BF16>(a, nbits, (hipStream_t)stream) : launch_moe<NPAMD_F16>(a, nbits, (hipStream_t)stream);
 }

@@ -246,3 +246,15 @@ def test_refusals(gpu):
     dense, _ = _layer(1, 4, 96, 128, torch.float16, 16)
     with pytest.raises(RuntimeError, match="multiples of 64"):
         kernels.moe_layer(x[:, :96], _experts(dense), 2)
+
+
+@pytest.mark.parametrize("m,experts,top_k", [(9, 9, 4), (10, 9, 4), (16, 8, 2), (17, 8, 2), (32, 32, 4), (32, 31, 4)])
+def test_all_tokens_meet_in_the_same_experts(gpu, m, experts, top_k):
+    """More tokens at an expert than one pass over its weights takes, on both sides of the number of pairs from which a pass takes more."""
+    from neuropress_amd import kernels
+
+    layer, dense = _layer(m + experts, experts, 128, 192, torch.float16, 8, 64, True)
+    x = torch.randn(m, 128, generator=cases.gen(m)).abs().half()  # positive, so the first experts' positive rows are far ahead
+    layer["router"][:top_k] = layer["router"][:top_k].abs() + 0.05 * torch.arange(1, top_k + 1)[:, None]
+    assert ((x.double() @ layer["router"].double().T).topk(top_k).indices < top_k).all()
+    _check(kernels.moe_layer(x.to(gpu), _experts(layer), top_k), *_reference(x, layer, dense, top_k, True), torch.float16)
