@@ -636,7 +636,7 @@ struct MoeSpace {
 
 // Four waves to a block of the up kernel (us of the layer with two / four / eight: int4 4096 x 14336, one token 54 / 50 / 56; dense 2048 x 2048, four tokens 67 / 65 / 66)
 // and eight of the down kernel (four / eight / 16: 54 / 50 / 52, 65 / 65 / 66), whose blocks split the columns where there are fewer row tiles than compute units (one part /
-// two: 57 / 50; hidden size 2048, seven tokens int8 one / four: 103 / 73).  From five tokens on the up kernel's waves share them: 16 tokens int4 271 / 219, one token 54 / 57.
+// two: 57 / 50; hidden size 2048, seven tokens int8 one / four: 103 / 73).  From entries of five pairs on the up kernel's waves share them: 16 tokens int4 271 / 219, one token 54 / 57.
 constexpr int kMoeUpWaves = 4, kMoeDownWaves = 8, kMoeTogether = 5, kMoeBlocks = 256, kMoeBlocksPerCu = 4;
 
 template <int ACT, int FMT, bool ASYM, int GROUP>
@@ -644,10 +644,11 @@ int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   const char* what = "npamd_moe_layer";
   using S = MoeStep<FMT, ASYM>;
   constexpr int kRoom = 160 * 1024;
-  const bool together = a.M >= kMoeTogether;
-  // Pairs of an entry: all that an MFMA takes, or half as many where an expert has four at the mean; their places in LDS keep blocks out (us with 16 / eight: 16 tokens
-  // int4 through two of eight 190 / 183, through eight of 64 88 / 70), an expert that has more is read again (32 tokens through two of eight 199 / 231).
-  const int pairs = a.M * a.top_k, cap = std::min(a.M, pairs <= 4 * a.E ? 8 : 16), x_bytes = 2 * S::x_loads(cap) * 1024;
+  // Pairs of an entry: their places in LDS keep blocks out, an expert that has more pairs is read again.  All that an MFMA takes; eight where an expert has four at the mean
+  // (us with 16 / eight: 16 tokens int4 through two of eight 190 / 183, through eight of 64 88 / 70, 32 tokens through two of eight 199 / 231); four where it has one, of int8,
+  // whose steps are the largest, two (eight of 64 experts, hidden size 2048, with eight / four / two: eight tokens dense 129 / 112 / 112, seven int8 70 / 73 / 65).
+  const int pairs = a.M * a.top_k, cap = std::min(a.M, pairs <= a.E ? (FMT == 8 ? 2 : 4) : pairs <= 4 * a.E ? 8 : 16), x_bytes = 2 * S::x_loads(cap) * 1024;
+  const bool together = cap >= kMoeTogether;
   auto up_own = [&](int waves) { return waves * 4 * S::kItem + (together ? x_bytes : waves * (x_bytes + cap * kMoeRedRow * 4)); };
   auto down_own = [&](int waves) { return waves * (x_bytes + 4 * S::kItem + a.M * 32 * 4); };
   const int up_waves = together ? kMoeUpWaves : std::min(kMoeUpWaves, (a.H + S::kColumns - 1) / S::kColumns);

@@ -248,12 +248,13 @@ def test_refusals(gpu):
         kernels.moe_layer(x[:, :96], _experts(dense), 2)
 
 
-@pytest.mark.parametrize("m,experts,top_k", [(9, 9, 4), (10, 9, 4), (16, 8, 2), (17, 8, 2), (32, 32, 4), (32, 31, 4)])
-def test_all_tokens_meet_in_the_same_experts(gpu, m, experts, top_k):
+@pytest.mark.parametrize("m,experts,top_k", [(9, 9, 4), (10, 9, 4), (16, 8, 2), (17, 8, 2), (32, 32, 4), (32, 31, 4), (5, 20, 4), (5, 19, 4), (32, 128, 4)])
+@pytest.mark.parametrize("nbits", [4, 8, 16])
+def test_all_tokens_meet_in_the_same_experts(gpu, nbits, m, experts, top_k):
     """More tokens at an expert than one pass over its weights takes, on both sides of the number of pairs from which a pass takes more."""
     from neuropress_amd import kernels
 
-    layer, dense = _layer(m + experts, experts, 128, 192, torch.float16, 8, 64, True)
+    layer, dense = _layer(m + experts, experts, 128, 192, torch.float16, nbits, 64, nbits == 8)
     x = torch.randn(m, 128, generator=cases.gen(m)).abs().half()  # positive, so the first experts' positive rows are far ahead
     layer["router"][:top_k] = layer["router"][:top_k].abs() + 0.05 * torch.arange(1, top_k + 1)[:, None]
     assert ((x.double() @ layer["router"].double().T).topk(top_k).indices < top_k).all()
