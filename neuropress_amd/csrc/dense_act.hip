@@ -275,6 +275,7 @@ extern "C" int npamd_dense_gemm_act(const void* x, int64_t ldx, const void* w, i
                                     int64_t workspace_bytes, void* stream) {
   const char* what = "npamd_dense_gemm_act";
   NPAMD_REQUIRE(M >= 0 && N >= 0 && K >= 1, "%s: bad shape M=%d N=%d K=%d", what, M, N, K);
+  if (N > 1 << 25 || K > 1 << 30) return fail(NPAMD_ERR_UNSUPPORTED, "%s: N=%d and K=%d have to be at most 2^25 and 2^30", what, N, K);
   NPAMD_REQUIRE(act_dtype == NPAMD_F16 || act_dtype == NPAMD_BF16, "%s: f16 or bf16 only", what);
   NPAMD_REQUIRE(!bias || bias_dtype == NPAMD_F32 || bias_dtype == act_dtype, "%s: the bias is f32 or of x's dtype", what);
   NPAMD_REQUIRE(activation >= NPAMD_ACT_NONE && activation <= NPAMD_ACT_SILU, "%s: unknown activation %d", what, activation);

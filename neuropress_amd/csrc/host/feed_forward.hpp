@@ -135,10 +135,6 @@ PyObject* dense_linear_act(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!rows_argument(args[0], device, &x) || !rows_argument(args[1], device, &w) || !PyLong_Check(args[3])) Py_RETURN_NONE;
     if (x.code == NPAMD_F32 || w.code != x.code || w.t->dim() != 2 || w.width != x.width) Py_RETURN_NONE;
     const at::ScalarType type = x.t->scalar_type();
-    // Past the GEMV's tokens the tiles take it, for which the Python function makes rows of whole pieces at aligned addresses.
-    if (x.m > NPAMD_GEMV_MAX_M && (x.width % 8 || x.ld % 8 || w.ld % 8 || x.ld >= NPAMD_TILE_MAX_STRIDE || w.ld >= NPAMD_TILE_MAX_STRIDE ||
-                                   (((uintptr_t)x.t->const_data_ptr() | (uintptr_t)w.t->const_data_ptr()) & 15)))
-      Py_RETURN_NONE;
     c10::SmallVector<int64_t, 6> sizes(x.t->sizes().begin(), x.t->sizes().end());
     sizes.back() = w.m;
     const void* bias;
@@ -146,12 +142,26 @@ PyObject* dense_linear_act(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (wide && !vector_of(args[2], device, at::kFloat, w.m, &bias)) Py_RETURN_NONE;
     if (!is_none(args[4]) && (!rows_argument(args[4], device, &res) || res.code != x.code || res.t->sizes() != at::IntArrayRef(sizes))) Py_RETURN_NONE;
     const long activation = PyLong_AsLong(args[3]);
-    const int64_t bytes = npamd_dense_gemm_act_workspace_bytes((int)x.m, (int)w.m, (int)x.width);
+    const hipStream_t st = current_stream(device);
+    // Past the GEMV's tokens the tiles take it, which read rows of whole pieces at aligned addresses.
+    const int64_t k = x.m > NPAMD_GEMV_MAX_M ? (x.width + 7) / 8 * 8 : x.width;
+    const void *xp = x.t->const_data_ptr(), *wp = w.t->const_data_ptr();
+    at::Tensor xc, wc;
+    auto whole_pieces = [&](Rows& r, const void*& p, at::Tensor& copy) {
+      if (x.m <= NPAMD_GEMV_MAX_M || (r.width == k && r.ld % 8 == 0 && r.ld < NPAMD_TILE_MAX_STRIDE && ((uintptr_t)p & 15) == 0)) return true;
+      copy = empty({r.m, k}, type, device);
+      const bool ok = npamd_gather_columns(p, r.ld, nullptr, copy.data_ptr(), k, (int)r.m, (int)r.width, st) == NPAMD_OK;
+      p = copy.const_data_ptr();
+      r.ld = k;
+      return ok;
+    };
+    if (!whole_pieces(x, xp, xc) || !whole_pieces(w, wp, wc)) Py_RETURN_NONE;
+    const int64_t bytes = npamd_dense_gemm_act_workspace_bytes((int)x.m, (int)w.m, (int)k);
     at::Tensor scratch, y = empty(sizes, type, device);
     if (bytes > 0) scratch = floats(bytes, device);
-    if (npamd_dense_gemm_act(x.t->const_data_ptr(), x.ld, w.t->const_data_ptr(), w.ld, bias, wide ? NPAMD_F32 : x.code, (int)activation,
-                             res.t ? res.t->const_data_ptr() : nullptr, res.ld, y.data_ptr(), w.m, (int)x.m, (int)w.m, (int)x.width, x.code,
-                             bytes > 0 ? scratch.data_ptr() : nullptr, bytes, current_stream(device)) != NPAMD_OK)
+    if (npamd_dense_gemm_act(xp, x.ld, wp, w.ld, bias, wide ? NPAMD_F32 : x.code, (int)activation,
+                             res.t ? res.t->const_data_ptr() : nullptr, res.ld, y.data_ptr(), w.m, (int)x.m, (int)w.m, (int)k, x.code,
+                             bytes > 0 ? scratch.data_ptr() : nullptr, bytes, st) != NPAMD_OK)
       Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(y));
   });

@@ -12,6 +12,9 @@ using namespace npamd;
 
 namespace {
 
+// Rows of a launch that gives each a block of 256 threads: a launch has fewer than 2^32 threads.
+constexpr int64_t kRowsAtOnce = 1 << 23;
+
 // Below so many waves a row gets more of them: 1100 x 4096 7.3 -> 6.7 us, 300 x 2048 4.0 -> 2.8.
 constexpr int kFewWaves = 4096;
 
@@ -31,7 +34,7 @@ struct Pieces {
   // Value `at` of a row, which is the same for all lanes.
   static __device__ __forceinline__ u32x4 load(const uint8_t* row, int at) { return *reinterpret_cast<const u32x4_any*>(row + (uint32_t)at * kBytes); }
   static __device__ __forceinline__ void store(uint8_t* row, int at, const u32x4& v) { *reinterpret_cast<u32x4_any*>(row + (uint32_t)at * kBytes) = v; }
-  static __device__ __forceinline__ const uint8_t* row_of(const void* p, int64_t row, int64_t ld) { return (const uint8_t*)p + row * ld * kBytes; }
+  static __host__ __device__ __forceinline__ const uint8_t* row_of(const void* p, int64_t row, int64_t ld) { return (const uint8_t*)p + row * ld * kBytes; }
   // What is made of a piece from here on is made anew: kept since it was made before, it would take two to four times the registers.
   static __device__ __forceinline__ void forget(u32x4& v) {
     if constexpr (DT != NPAMD_F32) asm volatile("" : "+v"(v));
@@ -233,12 +236,14 @@ layer_norm_back_columns_kernel(const LayerNormBack a, float* __restrict__ partia
     partials[((int64_t)blockIdx.y * 2 + wave) * a.H + col] = sums[0][wave][lane] + sums[1][wave][lane] + sums[2][wave][lane] + sums[3][wave][lane];
 }
 
+constexpr int kManyGroups = 8;
+
 // All of it in one pass over x and dy, 8192 x 4096 bf16 41.7 us in all, 4.8 TB/s, as fast as a copy (with masks for every value and pieces unpacked twice, 48: the vector
 // instructions were the limit): RW waves to a row, G rows to a block at a time, a lane has NV pieces of every row that its group meets, the weight's at hand, and adds up
 // its columns' part of the weight's and bias's gradients in registers.  The next rows are requested before the two sums of these meet in LDS (one barrier a turn).
 template <int DT, int NV>
 __global__ void __launch_bounds__(1024)
-layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, int RW, int G) {
+layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, void* __restrict__ dw_out, void* __restrict__ db_out, int RW, int G) {
   using P = Pieces<DT>;
   constexpr int V = P::V;
   extern __shared__ __attribute__((aligned(16))) float back_lds[];
@@ -348,8 +353,37 @@ layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, int 
       P::store(to, min(p * V, a.H - V), P::pack(g[i]));
     }
   }
-  if (!partials) return;
-  // The groups' sums meet in the first group, in their order.
+  if (!partials && !dw_out && !db_out) return;
+  // The groups' sums meet in LDS and are added in their order: by the first group, or by all threads where there are many (8 x 320 4.2 -> 2.9 us, 64 x 768
+  // 7.9 -> 7.1; but 64 x 2048, four groups, 7.7 -> 8.3).  Rows of whole pieces: a row's last piece lies behind those before, whole.
+  const int width = pieces * V;
+  float* const to = partials + (int64_t)blockIdx.x * 2 * width;
+  if (G >= kManyGroups) {
+    float* const mine = back_lds + (int64_t)group * 2 * width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = lane + lanes * i;
+      if (p >= pieces) continue;
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        *reinterpret_cast<f32x4*>(mine + p * V + e) = f32x4{dw[i][e], dw[i][e + 1], dw[i][e + 2], dw[i][e + 3]};
+        *reinterpret_cast<f32x4*>(mine + width + p * V + e) = f32x4{db[i][e], db[i][e + 1], db[i][e + 2], db[i][e + 3]};
+      }
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < 2 * width; o += blockDim.x) {
+      float v = 0.f;
+      for (int g = 0; g < G; ++g) v += back_lds[g * 2 * width + o];
+      if (partials) {
+        to[o] = v;
+        continue;
+      }
+      void* const out = o < width ? dw_out : db_out;
+      const int at = o < width ? o : o - width, whole = a.H / V * V, column = at < whole ? at : at + a.H - width;
+      if (out && (at < whole || column >= whole)) store_from_f32<DT>(out, column, v);
+    }
+    return;
+  }
   float* const mine = back_lds + (int64_t)(group - 1) * 2 * NV * V * lanes + lane;
   if (group > 0) {
 #pragma unroll
@@ -366,8 +400,21 @@ layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, int 
 #pragma unroll
       for (int e = 0; e < V; ++e) dw[i][e] += theirs[(2 * (i * V + e)) * lanes], db[i][e] += theirs[(2 * (i * V + e) + 1) * lanes];
   }
-  // Rows of whole pieces, as the lanes have them.
-  float* const to = partials + (int64_t)blockIdx.x * 2 * pieces * V;
+  if (!partials) {  // the only block: its sums are all there is
+    auto leave = [&](void* out, const float (&sum)[NV][V]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int p = lane + lanes * i, at = min(p * V, a.H - V);
+        if (p >= pieces) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (at + e >= p * V) store_from_f32<DT>(out, at + e, sum[i][e]);  // the others are the piece's before
+      }
+    };
+    if (dw_out) leave(dw_out, dw);
+    if (db_out) leave(db_out, db);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int p = lane + lanes * i;
@@ -375,7 +422,7 @@ layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, int 
 #pragma unroll
     for (int e = 0; e < V; e += 4) {
       *reinterpret_cast<f32x4*>(to + p * V + e) = f32x4{dw[i][e], dw[i][e + 1], dw[i][e + 2], dw[i][e + 3]};
-      *reinterpret_cast<f32x4*>(to + (pieces + p) * V + e) = f32x4{db[i][e], db[i][e + 1], db[i][e + 2], db[i][e + 3]};
+      *reinterpret_cast<f32x4*>(to + width + p * V + e) = f32x4{db[i][e], db[i][e + 1], db[i][e + 2], db[i][e + 3]};
     }
   }
 }
@@ -410,23 +457,25 @@ constexpr int kTurns = 2;
 // Which kernel the backward pass takes.  parts: sums over rows that it leaves to be added.
 struct BackPlan {
   int nv = 0, row_waves = 0, groups = 0, parts = 0;  // nv 0: rows that do not fit the registers
+  // Bytes of LDS where the groups' sums meet: 64 KiB at most (rows of two pieces to a lane have one group).
+  int lds(int pieces, int V) const { return (groups >= kManyGroups ? groups * pieces : (groups - 1) * nv * 64 * row_waves) * 2 * V * 4; }
   BackPlan(int M, int H, int dtype) {
     const int V = dtype == NPAMD_F32 ? 4 : 8, pieces = (H + V - 1) / V;
     if (H < V || pieces > 64 * 16 * 2) {
-      parts = std::min(64, (M + 63) / 64);
+      parts = (int)std::min<int64_t>(64, ((int64_t)M + 63) / 64);
       return;
     }
     nv = pieces <= 1024 ? 1 : 2;
     row_waves = 1;
     while (row_waves * 64 * nv < pieces) row_waves *= 2;
-    groups = 16 / row_waves;
-    parts = std::min(256, (M + groups * kTurns - 1) / (groups * kTurns));
+    groups = std::min(16 / row_waves, std::max(1, M));
+    parts = (int)std::min<int64_t>(256, ((int64_t)M + groups * kTurns - 1) / (groups * kTurns));
   }
 };
 
 template <int DT>
-int launch_forward(const void* x, int64_t ldx, const void* w, const void* b, void* out, int64_t ldo, float* mean, float* rstd, int M, int H, float eps,
-                   hipStream_t st) {
+int launch_forward_rows(const void* x, int64_t ldx, const void* w, const void* b, void* out, int64_t ldo, float* mean, float* rstd, int M, int H, float eps,
+                        hipStream_t st) {
   constexpr int V = Pieces<DT>::V;
   const int pieces = (H + V - 1) / V;
   if (H < V || pieces > 256 * 16) {
@@ -457,17 +506,43 @@ int launch_forward(const void* x, int64_t ldx, const void* w, const void* b, voi
 }
 
 template <int DT>
+int launch_forward(const void* x, int64_t ldx, const void* w, const void* b, void* out, int64_t ldo, float* mean, float* rstd, int M, int H, float eps,
+                   hipStream_t st) {
+  using P = Pieces<DT>;
+  for (int64_t at = 0; at < M; at += kRowsAtOnce) {
+    const int rc = launch_forward_rows<DT>(P::row_of(x, at, ldx), ldx, w, b, const_cast<uint8_t*>(P::row_of(out, at, ldo)), ldo, mean ? mean + at : nullptr,
+                                           rstd ? rstd + at : nullptr, (int)std::min<int64_t>(kRowsAtOnce, M - at), H, eps, st);
+    if (rc != NPAMD_OK) return rc;
+  }
+  return NPAMD_OK;
+}
+
+template <int DT>
 int launch_backward(const LayerNormBack& a, void* dw, void* db, float* partials, hipStream_t st) {
   const char* what = "npamd_layer_norm_backward";
   const bool sums = dw || db;
   const BackPlan p(a.M, a.H, DT);
   const unsigned columns = (unsigned)(a.H + 63) / 64;
   if (a.M && p.nv) {
-    const int lds = sums ? (p.groups - 1) * 2 * p.nv * Pieces<DT>::V * 64 * p.row_waves * 4 : 0;
+    constexpr int V = Pieces<DT>::V;
+    const int lds = sums ? p.lds((a.H + V - 1) / V, V) : 0;
     const auto kernel = p.nv == 1 ? layer_norm_back_kernel<DT, 1> : layer_norm_back_kernel<DT, 2>;
-    if (sums || a.dx) launch(kernel, p.parts, 1024, lds, st, a, sums ? partials : nullptr, p.row_waves, p.groups);
+    static LdsLatch latch[2];
+    const hipError_t e = enable_dynamic_lds(latch[p.nv - 1], reinterpret_cast<const void*>(kernel), lds);
+    if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
+    const bool alone = p.parts == 1;
+    if (sums || a.dx)
+      launch(kernel, p.parts, 64 * p.row_waves * p.groups, lds, st, a, sums && !alone ? partials : nullptr, alone ? dw : nullptr, alone ? db : nullptr, p.row_waves, p.groups);
+    if (alone) return check_launch(what);
   } else if (a.M) {
-    if (a.dx) launch(layer_norm_back_block_kernel<DT>, a.M, 256, 0, st, a);
+    if (a.dx) {
+      LayerNormBack part = a;
+      for (int64_t at = 0; at < a.M; at += kRowsAtOnce) {
+        part.dy = Pieces<DT>::row_of(a.dy, at, a.lddy), part.x = Pieces<DT>::row_of(a.x, at, a.ldx);
+        part.dx = const_cast<uint8_t*>(Pieces<DT>::row_of(a.dx, at, a.lddx)), part.mean = a.mean + at, part.rstd = a.rstd + at;
+        launch(layer_norm_back_block_kernel<DT>, (unsigned)std::min<int64_t>(kRowsAtOnce, a.M - at), 256, 0, st, part);
+      }
+    }
     if (sums) launch(layer_norm_back_columns_kernel<DT>, dim3(columns, p.parts), 256, 0, st, a, partials, p.parts);
   }
   constexpr int V = Pieces<DT>::V;
@@ -481,7 +556,7 @@ int launch_backward(const LayerNormBack& a, void* dw, void* db, float* partials,
 extern "C" int npamd_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, void* out, int64_t ldo, float* mean, float* rstd,
                                 int M, int H, float eps, int dtype, void* stream) {
   const char* what = "npamd_layer_norm";
-  NPAMD_REQUIRE(M >= 0 && H >= 1, "%s: bad shape M=%d H=%d", what, M, H);
+  NPAMD_REQUIRE(M >= 0 && H >= 1 && H <= 1 << 30, "%s: bad shape M=%d H=%d", what, M, H);
   NPAMD_REQUIRE(dtype == NPAMD_F16 || dtype == NPAMD_BF16 || dtype == NPAMD_F32, "%s: bad dtype %d", what, dtype);
   NPAMD_REQUIRE(ldx >= H && ldo >= H, "%s: bad row stride", what);
   if (M == 0) return NPAMD_OK;
@@ -493,7 +568,7 @@ extern "C" int npamd_layer_norm(const void* x, int64_t ldx, const void* weight, 
 }
 
 extern "C" int64_t npamd_layer_norm_workspace_bytes(int M, int H) {
-  if (M < 1 || H < 1) return 0;
+  if (M < 1 || H < 1 || H > 1 << 30) return 0;
   return (int64_t)std::max(BackPlan(M, H, NPAMD_F16).parts, BackPlan(M, H, NPAMD_F32).parts) * 2 * ((H + 7) / 8 * 8) * 4;
 }
 
@@ -501,7 +576,7 @@ extern "C" int npamd_layer_norm_backward(const void* dy, int64_t lddy, const voi
                                          const float* rstd, void* dx, int64_t lddx, void* dweight, void* dbias, int M, int H, int dtype,
                                          void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "npamd_layer_norm_backward";
-  NPAMD_REQUIRE(M >= 0 && H >= 1, "%s: bad shape M=%d H=%d", what, M, H);
+  NPAMD_REQUIRE(M >= 0 && H >= 1 && H <= 1 << 30, "%s: bad shape M=%d H=%d", what, M, H);
   NPAMD_REQUIRE(dtype == NPAMD_F16 || dtype == NPAMD_BF16 || dtype == NPAMD_F32, "%s: bad dtype %d", what, dtype);
   NPAMD_REQUIRE(lddy >= H && ldx >= H && (!dx || lddx >= H), "%s: bad row stride", what);
   NPAMD_REQUIRE(M == 0 || (dy && x && mean && rstd), "%s: null pointer", what);

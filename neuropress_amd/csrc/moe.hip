@@ -689,7 +689,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 }  // namespace
 
 extern "C" int64_t npamd_moe_workspace_bytes(int M, int E, int top_k, int H, int I) {
-  if (M < 1 || E < 1 || top_k < 1 || H < 1 || I < 1) return 0;
+  if (M < 1 || E < 1 || top_k < 1 || H < 1 || I < 1 || M > kMoeMaxTokens || E > kMoeMaxExperts || top_k > std::min(E, kMoeMaxTopK)) return 0;  // refused without any
   return MoeSpace(M, E, top_k, H, I).bytes;
 }
 

@@ -325,3 +325,66 @@ def test_module_and_lowering(gpu):
             assert torch.allclose(g, want[n], rtol=1e-3, atol=max(1e-3 * want[n].abs().max().item(), 6e-5)), n
     unlower_model(model)
     assert model.norm is norm and model.again is norm and not is_lowered(model)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h", [8, 64, 321, 777, 2052, 4099, 8200])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17, 31, 32, 33, 65])
+def test_backward_of_few_rows(gpu, dtype, m, h):
+    """As many rows as a block takes at once or in a second turn, one more and one less: its sums meet in other ways, or are all there is."""
+    from neuropress_amd import kernels
+
+    x, w, _, dy = _inputs(m, h, dtype, seed=3)
+    _, mean, rstd = kernels.layer_norm_stats(x.to(gpu), None, None, EPS)
+    got = kernels.layer_norm_backward(dy.to(gpu), x.to(gpu), w.to(gpu), mean, rstd)
+    for t, (ref, slack), what in zip(got, _reference_back(dy, x, w, mean.cpu(), rstd.cpu()), ("dx", "dw", "db")):
+        _check(t, ref, slack, dtype, what)
+
+
+@pytest.mark.parametrize("h", [2, 8])
+def test_more_rows_than_a_launch_has_blocks(gpu, h):
+    from neuropress_amd import kernels
+
+    m = (1 << 24) + 5
+    g = torch.Generator(device=gpu).manual_seed(h)
+    x, dy = (torch.randn(m, h, generator=g, device=gpu).to(torch.float16) for _ in range(2))
+    y, mean, rstd = kernels.layer_norm_stats(x, None, None, EPS)
+    dx, _, _ = kernels.layer_norm_backward(dy, x, None, mean, rstd, needs=(True, False, False))
+    for first in (0, (1 << 23) - 3, (1 << 24) - 3):
+        rows = slice(first, first + 8)
+        xs, dys = x[rows].cpu(), dy[rows].cpu()
+        ref, _, _, slack = _reference(xs, None, None)
+        _check(y[rows], ref, slack, torch.float16, "y")
+        _check(dx[rows], *_reference_back(dys, xs, None, mean[rows].cpu(), rstd[rows].cpu())[0], torch.float16, "dx")
+    assert torch.equal(y, kernels.layer_norm(x, None, None, EPS)) and bool(torch.isfinite(dx).all())
+
+
+def test_captured_training_step(gpu):
+    """Forward and backward through autograd, recorded after a step on the same side stream whose graph is gone."""
+    from neuropress_amd import kernels
+
+    x, w, b, dy = (t.to(gpu) for t in _inputs(70, 640, torch.bfloat16))
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+
+    def step():
+        for t in leaves:
+            t.grad = None
+        kernels.layer_norm(*leaves, EPS).backward(dy)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for seed in range(3):
+        nx, _, _, ndy = (t.to(gpu) for t in _inputs(70, 640, torch.bfloat16, seed=seed))
+        with torch.no_grad():
+            leaves[0].copy_(nx)
+        dy.copy_(ndy)
+        graph.replay()
+        torch.cuda.synchronize()
+        _, mean, rstd = kernels.layer_norm_stats(nx, w, b, EPS)
+        assert all(torch.equal(t.grad, c) for t, c in zip(leaves, kernels.layer_norm_backward(ndy, nx, w, mean, rstd)))
