@@ -1,6 +1,6 @@
 // Dense product with an epilogue: y = act(x @ W^T + bias) + residual, f32 up to the one rounding at the store.
 //
-// For few tokens W is all that counts.  One and two: every wave streams whole rows of it into registers.  Up to 16 or 32: whole lines into LDS, MFMAs.  More: the tiles of the
+// For few tokens W is all that counts.  One and two: every wave streams whole rows of it into registers.  Up to 16, 32 or 64: whole lines into LDS, MFMAs.  More: the tiles of the
 // dense product, with an epilogue of their own (wide_gemm.hpp, dense_gemm.hip).
 #include <algorithm>
 #include <type_traits>
@@ -224,10 +224,11 @@ int launch_some_tile(const FewArgs& a, int waves, hipStream_t st, const char* wh
 // Row tiles of a block and its waves, us at eight tokens: 8192 x 2048 with one / two 11.3 / 9.5, 4096 x 4096 9.5 / 12.3; with four waves 4096 x 4096 11.1.
 template <int ACT>
 int launch_some(const FewArgs& a, hipStream_t st, const char* what) {
-  const int steps = (a.K / 8 + 15) / 16, mt = a.M <= 16 ? 1 : 2, r = a.N >= 8192 ? 2 : 1;
+  const int steps = (a.K / 8 + 15) / 16, mt = (a.M + 15) / 16, r = a.N >= 8192 && mt <= 2 ? 2 : 1;
   const int waves = std::min(std::min(8, steps), 160 * 1024 / ((mt + r) * 8192));
   if (mt == 1) return r == 1 ? launch_some_tile<ACT, 1, 1>(a, waves, st, what) : launch_some_tile<ACT, 1, 2>(a, waves, st, what);
-  return r == 1 ? launch_some_tile<ACT, 2, 1>(a, waves, st, what) : launch_some_tile<ACT, 2, 2>(a, waves, st, what);
+  if (mt == 2) return r == 1 ? launch_some_tile<ACT, 2, 1>(a, waves, st, what) : launch_some_tile<ACT, 2, 2>(a, waves, st, what);
+  return mt == 3 ? launch_some_tile<ACT, 3, 1>(a, waves, st, what) : launch_some_tile<ACT, 4, 1>(a, waves, st, what);
 }
 
 // Rows of a wave: two from two tokens on, which then share a read of x.  Four waves to a row where there are few rows (1024 x 4096, one token, one wave / four 3.9 / 3.5 us).
@@ -252,12 +253,14 @@ int launch_few(const FewArgs& a, hipStream_t st, const char* what) {
 
 // Which kernel takes a call; aligned: rows that the tiles can read.  Us with dense_few_kernel / dense_some_kernel / the tiles, silu and a residual: two tokens 4096 x 4096 10.2 /
 // 9.3 / 13.9, 640 x 2048 3.3 / 3.9 / 8.9; eight 4096 x 4096 - / 9.5 / 13.9, 4096 x 14336 - / 23.7 / 28.1, 1024 x 4096 - / 5.3 / 9.5; 32 tokens 8192 x 2048 - / 14.0 / 14.7,
-// 4096 x 4096 - / 14.0 / 19.7, 4096 x 14336 - / 35 / 29.
+// 4096 x 4096 - / 14.0 / 19.7, 4096 x 14336 - / 35 / 29.  Past 32 tokens a block has few waves and reads many tokens: it needs a compute unit of its own and K no longer
+// than that lasts: 64 tokens 4096 x 4096 16.0 / 18.0, 2048 x 2048 8.4 / 9.1, 3003 x 2184 11.7 / 15.8; but 8192 x 2048 19.9 / 13.6, 1024 x 4096 11.6 / 9.9, 2048 x 8192 24 / 15.
 enum Path { kFew, kSome, kTiles };
 Path path_of(int M, int N, int K, bool aligned) {
   if (M <= 2) return kFew;
   if (!aligned) return M <= NPAMD_GEMV_MAX_M ? kFew : kTiles;
-  return M <= 16 || (M <= 32 && (int64_t)N * K <= (int64_t)1 << 24) ? kSome : kTiles;
+  if (M <= 16 || (M <= 32 && (int64_t)N * K <= 1 << 24)) return kSome;
+  return M <= 64 && N <= 4096 && K <= std::max(N, 2560) ? kSome : kTiles;
 }
 
 bool tiles_take(const void* x, int64_t ldx, const void* w, int64_t ldw, int K) {

@@ -11,7 +11,7 @@ from neuropress_amd import build
 
 
 @pytest.mark.parametrize("source, kernel, count, transfers",
-                         [("dense_act.hip", "dense_some_kernel", 2 * 2 * 2, True), ("dense_act.hip", "dense_few_kernel", 2 * 3 * 2, False),
+                         [("dense_act.hip", "dense_some_kernel", 2 * (2 * 2 + 2), True), ("dense_act.hip", "dense_few_kernel", 2 * 3 * 2, False),
                           ("wide_gemm_epilogue.hip", "wide_gemm_kernel", 2 * 13, True)])  # fmt: skip
 def test_m0_is_the_transfers_own_and_nothing_spills(tmp_path, source, kernel, count, transfers):
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"

@@ -204,8 +204,8 @@ def test_the_residual_in_its_own_place(gpu):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m", [2, 3, 15, 16, 17, 31, 32, 33])
-@pytest.mark.parametrize("n,k", [(1, 8), (16, 120), (17, 128), (100, 1032), (8191, 136), (8192, 136), (8209, 1160)])
+@pytest.mark.parametrize("m", [2, 3, 15, 16, 17, 31, 32, 33, 48, 49, 64, 65])
+@pytest.mark.parametrize("n,k", [(1, 8), (16, 120), (17, 128), (100, 1032), (40, 2560), (40, 2568), (4096, 264), (4100, 264), (8191, 136), (8192, 136), (8209, 1160)])
 def test_where_one_kernel_takes_over_from_another(gpu, dtype, m, n, k):
     """Tokens and rows on both sides of where the kernel changes; columns that end inside a step, or before every wave has one."""
     x, w, b, r = _inputs(m, n, k, dtype)
@@ -213,7 +213,7 @@ def test_where_one_kernel_takes_over_from_another(gpu, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("n", [4096, 4112])  # 2^24 weights of 4096 columns, and some more
-@pytest.mark.parametrize("m", [16, 17, 32])
+@pytest.mark.parametrize("m", [16, 17, 32, 50])
 def test_weights_on_both_sides_of_the_line(gpu, m, n):
     x, w, b, r = _inputs(m, n, 4096, torch.bfloat16)
     _check(_run(x, w, b, "gelu", r), x, w, b, "gelu", r)
