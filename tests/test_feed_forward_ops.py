@@ -150,15 +150,6 @@ def test_the_feed_forward_half_of_a_block(gpu, tokens, dtype):
             want[m] += p[m, t] / p[m, :2].sum() * (dense["down"][ids[m, t]] @ (f.silu(gate) * u))
     clear = p[:, 1] - p[:, 2] > 0.02 * p[:, 1]  # where the rounded norm picks the same experts
     assert bool(clear.any()) and (y.double().cpu() - want)[clear].abs().max() < 24 * eps * max(1.0, want.abs().max().item())
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        out = block(*on)
-    for k in range(3):
-        on[0].copy_(torch.randn(tokens, h, generator=cases.gen(k)))
-        again = block(*on)
-        graph.replay()
-        torch.cuda.synchronize()
-        assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
 
 
 class _Declining:

@@ -233,32 +233,6 @@ def test_calls_that_torch_follows_otherwise(gpu):
         dx.sum().backward()
 
 
-def test_captured_forward_and_backward(gpu):
-    from neuropress_amd import kernels
-
-    x, w, b, dy = (t.to(gpu) for t in _inputs(300, 1000, torch.bfloat16))
-
-    def step():
-        y, mean, rstd = kernels.layer_norm_stats(x, w, b, EPS)
-        return (y, *kernels.layer_norm_backward(dy, x, w, mean, rstd))
-
-    stream = torch.cuda.Stream()
-    with torch.cuda.stream(stream):
-        step()
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph, stream=stream):
-        out = step()
-    for seed in range(4):
-        nx, _, _, ndy = _inputs(300, 1000, torch.bfloat16, seed=seed)
-        x.copy_(nx)
-        dy.copy_(ndy)
-        want = step()
-        graph.replay()
-        torch.cuda.synchronize()
-        assert all(torch.equal(a, c) for a, c in zip(out, want))
-
-
 def test_in_place_and_rows_behind_the_last(gpu):
     """Through the C entry: out may be x, dx may be dy, and nothing behind the rows is written."""
     from neuropress_amd import _lib, kernels
@@ -357,34 +331,3 @@ def test_more_rows_than_a_launch_has_blocks(gpu, h):
         _check(y[rows], ref, slack, torch.float16, "y")
         _check(dx[rows], *_reference_back(dys, xs, None, mean[rows].cpu(), rstd[rows].cpu())[0], torch.float16, "dx")
     assert torch.equal(y, kernels.layer_norm(x, None, None, EPS)) and bool(torch.isfinite(dx).all())
-
-
-def test_captured_training_step(gpu):
-    """Forward and backward through autograd, recorded after a step on the same side stream whose graph is gone."""
-    from neuropress_amd import kernels
-
-    x, w, b, dy = (t.to(gpu) for t in _inputs(70, 640, torch.bfloat16))
-    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
-
-    def step():
-        for t in leaves:
-            t.grad = None
-        kernels.layer_norm(*leaves, EPS).backward(dy)
-
-    stream = torch.cuda.Stream()
-    stream.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(stream):
-        step()
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph, stream=stream):
-        step()
-    for seed in range(3):
-        nx, _, _, ndy = (t.to(gpu) for t in _inputs(70, 640, torch.bfloat16, seed=seed))
-        with torch.no_grad():
-            leaves[0].copy_(nx)
-        dy.copy_(ndy)
-        graph.replay()
-        torch.cuda.synchronize()
-        _, mean, rstd = kernels.layer_norm_stats(nx, w, b, EPS)
-        assert all(torch.equal(t.grad, c) for t, c in zip(leaves, kernels.layer_norm_backward(ndy, nx, w, mean, rstd)))

@@ -191,32 +191,6 @@ def test_shapes_strides_and_no_tokens(gpu):
     assert torch.equal(kernels.moe_layer(x, kernels.MoEExperts(**{k: shifted(v) for k, v in layer.items()}), 2), y)
 
 
-def test_captured_twice_and_on_two_streams(gpu):
-    """Two captured calls and eager ones, replayed in turn and side by side: each has scratch of its own."""
-    from neuropress_amd import kernels
-
-    layer, _ = _layer(9, 16, 256, 512, torch.float16, 4)
-    experts = _experts(layer)
-    xs = [torch.randn(m, 256, generator=cases.gen(m)).half().to(gpu) for m in (3, 12)]
-    for x in xs:
-        kernels.moe_layer(x, experts, 4)
-    torch.cuda.synchronize()
-    streams, graphs, outs = [torch.cuda.Stream() for _ in xs], [torch.cuda.CUDAGraph() for _ in xs], []
-    for x, st, graph in zip(xs, streams, graphs):
-        with torch.cuda.graph(graph, stream=st):
-            outs.append(kernels.moe_layer(x, experts, 4))
-    for seed in range(5):
-        for x in xs:
-            x.copy_(torch.randn(x.shape, generator=cases.gen(seed)).half())
-        want = [kernels.moe_layer(x, experts, 4) for x in xs]
-        torch.cuda.synchronize()
-        for st, graph in zip(streams, graphs):
-            with torch.cuda.stream(st):
-                graph.replay()
-        torch.cuda.synchronize()
-        assert all(torch.equal(a, b) for a, b in zip(outs, want))
-
-
 def test_refusals(gpu):
     from neuropress_amd import kernels
 
