@@ -8,18 +8,18 @@ namespace npamd {
 
 __device__ __forceinline__ float silu_f32(float v) { return v * __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
-// v Phi(v), Phi by erfc: exp(z^2) erfc(z), z >= 0, is a polynomial in t = 1 / (1 + 0.51 z) without a constant term, to 9e-7 relative (fitted up to z = 10, past which
-// exp(-z^2) is zero).
+// v Phi(v), Phi by erfc: exp(z^2) erfc(z) / 2, z = |v| / sqrt(2), is a polynomial in t = 1 / (1 + 0.51 z) without a constant term, to 9e-7 relative (fitted up to z = 10,
+// past which exp(-z^2) is zero).
 __device__ __forceinline__ float gelu_f32(float v) {
-  const float z = fabsf(v) * 0.70710678f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.51f, z, 1.f));
-  float q = 0.09450017660856247f;
-  q = __builtin_fmaf(q, t, -0.35913553833961487f);
-  q = __builtin_fmaf(q, t, 0.35844647884368896f);
-  q = __builtin_fmaf(q, t, 0.05505234748125076f);
-  q = __builtin_fmaf(q, t, 0.2790662944316864f);
-  q = __builtin_fmaf(q, t, 0.2841522991657257f);
-  q = __builtin_fmaf(q, t, 0.28791749477386475f);
-  const float half = 0.5f * q * t * __expf(-z * z);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.51f * 0.70710678f, fabsf(v), 1.f));
+  float q = 0.047250088304281235f;
+  q = __builtin_fmaf(q, t, -0.17956776916980743f);
+  q = __builtin_fmaf(q, t, 0.17922323942184448f);
+  q = __builtin_fmaf(q, t, 0.02752617374062538f);
+  q = __builtin_fmaf(q, t, 0.1395331472158432f);
+  q = __builtin_fmaf(q, t, 0.14207614958286285f);
+  q = __builtin_fmaf(q, t, 0.14395874738693237f);
+  const float half = q * t * __builtin_amdgcn_exp2f(v * v * -0.72134752f);  // exp(-v^2 / 2)
   return v * (v < 0.f ? half : 1.f - half);
 }
 
