@@ -498,7 +498,7 @@ int npamd_dense_gemm_preferred(int M, int N, int K);
 /*
  * Layer norm over the last dimension: out[m, i] = round((x[m, i] - mean) * rstd * weight[i] + bias[i]), f32 arithmetic, the variance
  * (over H, not H - 1) taken around the mean.  x, weight, bias, out share `dtype` (NPAMD_F16 / NPAMD_BF16 / NPAMD_F32); weight and bias
- * may be NULL; any H >= 1 and any alignment.  mean, rstd: NULL, or f32 [M] each, what the backward pass reads.  out may be x.
+ * may be NULL; any H from 1 to 2^27 and any alignment.  mean, rstd: NULL, or f32 [M] each, what the backward pass reads.  out may be x.
  */
 int npamd_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, void* out, int64_t ldo,
                      float* mean, float* rstd, int M, int H, float eps, int dtype, void* stream);
@@ -520,7 +520,7 @@ int64_t npamd_layer_norm_workspace_bytes(int M, int H);
  * Dense product with an epilogue: y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n], f32 up to one rounding.
  * x, w, residual, y: act_dtype (NPAMD_F16 or NPAMD_BF16); bias: NULL, or bias_dtype NPAMD_F32 or act_dtype; residual: NULL, or
  * [M, N] with row stride ldr, and may be y itself (same row distance).  activation: one of NPAMD_ACT_*; GELU is v * (1 + erf(v / sqrt 2)) / 2, GELU_TANH
- * its form with tanh, SILU v / (1 + exp(-v)).  Any shape and alignment up to NPAMD_GEMV_MAX_M tokens; past that K has to be a multiple of 8, x and w 16-byte
+ * its form with tanh, SILU v / (1 + exp(-v)).  N up to 2^25, K up to 2^30; any alignment up to NPAMD_GEMV_MAX_M tokens; past that K has to be a multiple of 8, x and w 16-byte
  * aligned, ldx and ldw multiples of 8 and below NPAMD_TILE_MAX_STRIDE.
  * workspace: optional, npamd_dense_gemm_act_workspace_bytes of them, 16-byte aligned, contents irrelevant; with less, K is not
  * split over blocks.  Calls that overlap must not share one.

@@ -251,6 +251,8 @@ int launch_few(const FewArgs& a, hipStream_t st, const char* what) {
   return check_launch(what);
 }
 
+constexpr int kMaxRows = 1 << 25, kMaxColumns = 1 << 30;  // of W: a launch has fewer than 2^32 threads
+
 // Which kernel takes a call; aligned: rows that the tiles can read.  Us with dense_few_kernel / dense_some_kernel / the tiles, silu and a residual: two tokens 4096 x 4096 10.2 /
 // 9.3 / 13.9, 640 x 2048 3.3 / 3.9 / 8.9; eight 4096 x 4096 - / 9.5 / 13.9, 4096 x 14336 - / 23.7 / 28.1, 1024 x 4096 - / 5.3 / 9.5; 32 tokens 8192 x 2048 - / 14.0 / 14.7,
 // 4096 x 4096 - / 14.0 / 19.7, 4096 x 14336 - / 35 / 29.  Past 32 tokens a block has few waves and reads many tokens: it needs a compute unit of its own and K no longer
@@ -270,7 +272,7 @@ bool tiles_take(const void* x, int64_t ldx, const void* w, int64_t ldw, int K) {
 }  // namespace
 
 extern "C" int64_t npamd_dense_gemm_act_workspace_bytes(int M, int N, int K) {
-  return M < 1 || N < 1 || K < 1 || path_of(M, N, K, true) != kTiles ? 0 : npamd_dense_gemm_workspace_bytes(M, N, (K + 63) / 64 * 64);
+  return M < 1 || N < 1 || K < 1 || N > kMaxRows || K > kMaxColumns || path_of(M, N, K, true) != kTiles ? 0 : npamd_dense_gemm_workspace_bytes(M, N, (K + 63) / 64 * 64);
 }
 
 extern "C" int npamd_dense_gemm_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int activation,
@@ -278,7 +280,7 @@ extern "C" int npamd_dense_gemm_act(const void* x, int64_t ldx, const void* w, i
                                     int64_t workspace_bytes, void* stream) {
   const char* what = "npamd_dense_gemm_act";
   NPAMD_REQUIRE(M >= 0 && N >= 0 && K >= 1, "%s: bad shape M=%d N=%d K=%d", what, M, N, K);
-  if (N > 1 << 25 || K > 1 << 30) return fail(NPAMD_ERR_UNSUPPORTED, "%s: N=%d and K=%d have to be at most 2^25 and 2^30", what, N, K);
+  if (N > kMaxRows || K > kMaxColumns) return fail(NPAMD_ERR_UNSUPPORTED, "%s: N=%d and K=%d have to be at most 2^25 and 2^30", what, N, K);
   NPAMD_REQUIRE(act_dtype == NPAMD_F16 || act_dtype == NPAMD_BF16, "%s: f16 or bf16 only", what);
   NPAMD_REQUIRE(!bias || bias_dtype == NPAMD_F32 || bias_dtype == act_dtype, "%s: the bias is f32 or of x's dtype", what);
   NPAMD_REQUIRE(activation >= NPAMD_ACT_NONE && activation <= NPAMD_ACT_SILU, "%s: unknown activation %d", what, activation);

@@ -43,7 +43,7 @@ bool rows_argument(PyObject* o, int device, Rows* r) {
   if (!r->t || r->t->dim() < 1) return false;
   r->code = dtype_code(r->t->scalar_type());
   r->width = r->t->size(-1);
-  if (r->code < 0 || r->code == 3 || r->width < 1 || r->width > INT32_MAX) return false;
+  if (r->code < 0 || r->code == 3 || r->width < 1 || r->width > 1 << 30) return false;
   r->m = r->t->numel() / r->width;
   return r->m >= 1 && r->m <= INT32_MAX && rows_of(*r->t, &r->ld);
 }

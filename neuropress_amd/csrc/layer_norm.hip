@@ -14,6 +14,7 @@ namespace {
 
 // Rows of a launch that gives each a block of 256 threads: a launch has fewer than 2^32 threads.
 constexpr int64_t kRowsAtOnce = 1 << 23;
+constexpr int kMaxWidth = 1 << 27;
 
 // Below so many waves a row gets more of them: 1100 x 4096 7.3 -> 6.7 us, 300 x 2048 4.0 -> 2.8.
 constexpr int kFewWaves = 4096;
@@ -535,6 +536,8 @@ int launch_backward(const LayerNormBack& a, void* dw, void* db, float* partials,
       launch(kernel, p.parts, 64 * p.row_waves * p.groups, lds, st, a, sums && !alone ? partials : nullptr, alone ? dw : nullptr, alone ? db : nullptr, p.row_waves, p.groups);
     if (alone) return check_launch(what);
   } else if (a.M) {
+    // The columns' sums first: dx may take the place of dy or x.
+    if (sums) launch(layer_norm_back_columns_kernel<DT>, dim3(columns, p.parts), 256, 0, st, a, partials, p.parts);
     if (a.dx) {
       LayerNormBack part = a;
       for (int64_t at = 0; at < a.M; at += kRowsAtOnce) {
@@ -543,7 +546,6 @@ int launch_backward(const LayerNormBack& a, void* dw, void* db, float* partials,
         launch(layer_norm_back_block_kernel<DT>, (unsigned)std::min<int64_t>(kRowsAtOnce, a.M - at), 256, 0, st, part);
       }
     }
-    if (sums) launch(layer_norm_back_columns_kernel<DT>, dim3(columns, p.parts), 256, 0, st, a, partials, p.parts);
   }
   constexpr int V = Pieces<DT>::V;
   const int width = p.nv ? (a.H + V - 1) / V * V : a.H, last = p.nv ? a.H / V * V : a.H;
@@ -556,7 +558,7 @@ int launch_backward(const LayerNormBack& a, void* dw, void* db, float* partials,
 extern "C" int npamd_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, void* out, int64_t ldo, float* mean, float* rstd,
                                 int M, int H, float eps, int dtype, void* stream) {
   const char* what = "npamd_layer_norm";
-  NPAMD_REQUIRE(M >= 0 && H >= 1 && H <= 1 << 30, "%s: bad shape M=%d H=%d", what, M, H);
+  NPAMD_REQUIRE(M >= 0 && H >= 1 && H <= kMaxWidth, "%s: bad shape M=%d H=%d", what, M, H);
   NPAMD_REQUIRE(dtype == NPAMD_F16 || dtype == NPAMD_BF16 || dtype == NPAMD_F32, "%s: bad dtype %d", what, dtype);
   NPAMD_REQUIRE(ldx >= H && ldo >= H, "%s: bad row stride", what);
   if (M == 0) return NPAMD_OK;
@@ -568,7 +570,7 @@ extern "C" int npamd_layer_norm(const void* x, int64_t ldx, const void* weight, 
 }
 
 extern "C" int64_t npamd_layer_norm_workspace_bytes(int M, int H) {
-  if (M < 1 || H < 1 || H > 1 << 30) return 0;
+  if (M < 1 || H < 1 || H > kMaxWidth) return 0;
   return (int64_t)std::max(BackPlan(M, H, NPAMD_F16).parts, BackPlan(M, H, NPAMD_F32).parts) * 2 * ((H + 7) / 8 * 8) * 4;
 }
 
@@ -576,7 +578,7 @@ extern "C" int npamd_layer_norm_backward(const void* dy, int64_t lddy, const voi
                                          const float* rstd, void* dx, int64_t lddx, void* dweight, void* dbias, int M, int H, int dtype,
                                          void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "npamd_layer_norm_backward";
-  NPAMD_REQUIRE(M >= 0 && H >= 1 && H <= 1 << 30, "%s: bad shape M=%d H=%d", what, M, H);
+  NPAMD_REQUIRE(M >= 0 && H >= 1 && H <= kMaxWidth, "%s: bad shape M=%d H=%d", what, M, H);
   NPAMD_REQUIRE(dtype == NPAMD_F16 || dtype == NPAMD_BF16 || dtype == NPAMD_F32, "%s: bad dtype %d", what, dtype);
   NPAMD_REQUIRE(lddy >= H && ldx >= H && (!dx || lddx >= H), "%s: bad row stride", what);
   NPAMD_REQUIRE(M == 0 || (dy && x && mean && rstd), "%s: null pointer", what);

@@ -1,4 +1,4 @@
-"""NPLayerNorm: layer norm as one HIP kernel, its backward pass as three, and the pass that installs it.
+"""NPLayerNorm: layer norm as one HIP kernel, its backward pass as one or two, and the pass that installs it.
 
 A neighbour of :mod:`.np_rms_norm` for models that norm with mean and variance.  It replaces ``nn.LayerNorm`` over the last dimension on a GPU; the
 parameters stay the module's own objects, so optimizers and ``state_dict`` keys go on as before.  ``AutoKernelLowering`` runs the pass with

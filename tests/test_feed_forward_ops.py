@@ -61,8 +61,8 @@ def test_moe_layer_refuses():
 @no_gpu
 def test_sizes_past_the_kernels_are_refused():
     far = 1 << 31
-    _refused("npamd_layer_norm", P, far, P, P, P, far, None, None, 2, far // 2 + 1, 1e-5, 1, None, match="bad shape")
-    _refused("npamd_layer_norm_backward", P, far, P, far, P, P, P, P, far, None, None, 2, far // 2 + 1, 1, None, 0, None, match="bad shape")
+    _refused("npamd_layer_norm", P, far, P, P, P, far, None, None, 2, 2**27 + 1, 1e-5, 1, None, match="bad shape")
+    _refused("npamd_layer_norm_backward", P, far, P, far, P, P, P, P, far, None, None, 2, 2**27 + 1, 1, None, 0, None, match="bad shape")
     for n, k in ((2**25 + 1, 64), (32, 2**30 + 1)):
         _refused("npamd_dense_gemm_act", P, far, P, far, None, 2, 0, None, 0, P, far, 40, n, k, 0, None, 0, None, match="at most", code=-2)
     lib = _lib.load()

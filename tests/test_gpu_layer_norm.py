@@ -254,6 +254,24 @@ def test_in_place_and_rows_behind_the_last(gpu):
         assert torch.equal(room[:m, :h], dx) and bool((room[m] == 7).all()) and bool((room[:, h:] == 7).all())
 
 
+@pytest.mark.parametrize("over", ["dy", "x"])
+@pytest.mark.parametrize("m,h", [(5, 4096), (40, 321), (70, 640), (300, 5), (130, 17000)])
+def test_gradient_in_the_place_of_an_input(gpu, over, m, h):
+    """Through the C entry, with the gradients of weight and bias, which are sums over what dx replaces."""
+    from neuropress_amd import _lib, kernels
+
+    x, w, _, dy = (None if t is None else t.to(gpu) for t in _inputs(m, h, torch.float16))
+    _, mean, rstd = kernels.layer_norm_stats(x, None, None, EPS)
+    want = kernels.layer_norm_backward(dy, x, w, mean, rstd)
+    dw, db = torch.empty_like(w), torch.empty_like(w)
+    need = _lib.load().npamd_layer_norm_workspace_bytes(m, h)
+    ws = torch.empty(need // 4, device=gpu)
+    place = dy if over == "dy" else x
+    _lib.call("npamd_layer_norm_backward", dy.data_ptr(), h, x.data_ptr(), h, w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), place.data_ptr(), h, dw.data_ptr(),
+              db.data_ptr(), m, h, 0, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)  # fmt: skip
+    assert all(torch.equal(a, c) for a, c in zip((place, dw, db), want))
+
+
 def test_module_and_lowering(gpu):
     from neuropress_amd import AutoKernelLowering, is_lowered, unlower_model
     from neuropress_amd.nn import NPLayerNorm
