@@ -31,6 +31,8 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -892,6 +894,7 @@ PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) { retu
 
 PyMethodDef module_methods[] = {
     {"layer_norm", fast(layer_norm), METH_FASTCALL, "layer_norm(x, weight, bias, eps, stats): the output (with the rows' statistics), or None"},
+    {"layer_norm_recorded", fast(layer_norm_recorded), METH_FASTCALL, "layer_norm_recorded(x, weight, bias, eps): the output, with its node in the graph of gradients"},
     {"layer_norm_backward", fast(layer_norm_backward), METH_FASTCALL, "layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight, dbias): the gradients, or None"},
     {"dense_linear_act", fast(dense_linear_act), METH_FASTCALL, "dense_linear_act(x, w, bias, activation, residual): the output, or None"},
     {"moe_layer", fast(moe_layer), METH_FASTCALL, "moe_layer(x, 7 tensors, 6 numbers, renormalize): the output, or None"},

@@ -123,6 +123,74 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// Rows for a kernel: t where they lie at one distance, else a copy.
+at::Tensor as_rows(const at::Tensor& t, int64_t* ld) { return rows_of(t, ld) ? t : (*ld = t.size(-1), t.contiguous()); }
+
+const void* data_or_null(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+// Layer norm in a recorded graph; arguments that Python has checked.  First derivatives only: what a backward pass that is itself recorded gives refuses to be differentiated.
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
+                            double eps) {
+    const c10::DeviceGuard guard(x.device());
+    const int device = x.get_device(), h = (int)x.size(-1), m = (int)(x.numel() / h);
+    int64_t ld;
+    const at::Tensor rows = as_rows(x, &ld), w = weight ? weight->contiguous() : at::Tensor(), b = bias ? bias->contiguous() : at::Tensor();
+    const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+    at::Tensor y = empty(x.sizes(), x.scalar_type(), device), mean = empty(lead, at::kFloat, device), rstd = empty(lead, at::kFloat, device);
+    TORCH_CHECK(npamd_layer_norm(rows.const_data_ptr(), ld, data_or_null(w), data_or_null(b), y.data_ptr(), h, mean.data_ptr<float>(), rstd.data_ptr<float>(), m, h,
+                                 (float)eps, dtype_code(x.scalar_type()), current_stream(device)) == NPAMD_OK, npamd_last_error());
+    ctx->save_for_backward({x, weight ? *weight : at::Tensor(), mean, rstd});
+    ctx->saved_data["has"] = (int64_t)((weight ? 1 : 0) | (bias ? 2 : 0));
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
+    const bool recorded = c10::GradMode::is_enabled();
+    torch::autograd::variable_list out(4);
+    const at::Tensor &x = saved[0], &mean = saved[2], &rstd = saved[3];
+    const c10::DeviceGuard guard(x.device());
+    {
+      const c10::AutoGradMode off(false);
+      const int64_t has = ctx->saved_data["has"].toInt();
+      const bool need[3] = {ctx->needs_input_grad(0), (has & 1) && ctx->needs_input_grad(1), (has & 2) && ctx->needs_input_grad(has & 1 ? 2 : 1)};
+      const int device = x.get_device(), h = (int)x.size(-1), m = (int)(x.numel() / h);
+      int64_t ldx, lddy;
+      const at::Tensor rows = as_rows(x, &ldx), dy = as_rows(grads[0], &lddy), w = saved[1].defined() ? saved[1].contiguous() : at::Tensor();
+      if (need[0]) out[0] = empty(x.sizes(), x.scalar_type(), device);
+      for (int i = 1; i < 3; ++i)
+        if (need[i]) out[i] = empty({h}, x.scalar_type(), device);
+      const int64_t bytes = need[1] || need[2] ? npamd_layer_norm_workspace_bytes(m, h) : 0;
+      at::Tensor scratch;
+      if (bytes > 0) scratch = floats(bytes, device);
+      auto at = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      TORCH_CHECK(npamd_layer_norm_backward(dy.const_data_ptr(), lddy, rows.const_data_ptr(), ldx, data_or_null(w), mean.const_data_ptr<float>(),
+                                            rstd.const_data_ptr<float>(), at(out[0]), h, at(out[1]), at(out[2]), m, h, dtype_code(x.scalar_type()), at(scratch), bytes,
+                                            current_stream(device)) == NPAMD_OK, npamd_last_error());
+    }
+    if (recorded) {
+      for (at::Tensor& t : out)
+        if (t.defined())
+          t = torch::autograd::DelayedError("layer_norm: its backward pass cannot be differentiated", 1).apply(torch::autograd::variable_list{t.requires_grad_(true)})[0];
+    }
+    return out;
+  }
+};
+
+// layer_norm_recorded(x, weight, bias, eps): tensors (or None) that Python has checked, on one device and of one type
+PyObject* layer_norm_recorded(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4 || !THPVariable_Check(args[0]) || !PyFloat_Check(args[3])) {
+    PyErr_SetString(PyExc_TypeError, "layer_norm_recorded(x, weight, bias, eps)");
+    return nullptr;
+  }
+  return translated([&]() -> PyObject* {
+    auto maybe = [](PyObject* o) { return THPVariable_Check(o) ? std::optional<at::Tensor>(THPVariable_Unpack(o)) : std::nullopt; };
+    const at::Tensor x = THPVariable_Unpack(args[0]);
+    const double eps = PyFloat_AS_DOUBLE(args[3]);
+    return THPVariable_Wrap(LayerNormNode::apply(x, maybe(args[1]), maybe(args[2]), eps));
+  });
+}
+
 // dense_linear_act(x, w, bias, activation's number, residual)
 PyObject* dense_linear_act(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 5) {

@@ -67,7 +67,7 @@ struct Pieces {
 // pieces to a lane 15.4: too few waves for the registers), 8192 x 2048 14.1 (12.9); by the launch and one round trip below that: 300 x 2048 2.8, one row 2.2.
 template <int DT, int NV, int RW>
 __global__ void __launch_bounds__(256)
-layer_norm_row_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* __restrict__ out, int64_t ldo,
+layer_norm_row_kernel(const void* x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* out, int64_t ldo,
                       float* __restrict__ mean_out, float* __restrict__ rstd_out, int M, int H, float eps) {
   using P = Pieces<DT>;
   constexpr int V = P::V, kLanes = 64 * RW;
@@ -162,7 +162,7 @@ layer_norm_row_kernel(const void* __restrict__ x, int64_t ldx, const void* __res
 // Rows too short for a piece or too long for the registers: a block per row, which it reads three times.
 template <int DT>
 __global__ void __launch_bounds__(256)
-layer_norm_block_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* __restrict__ out,
+layer_norm_block_kernel(const void* x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* out,
                         int64_t ldo, float* __restrict__ mean_out, float* __restrict__ rstd_out, int H, float eps) {
   __shared__ float part[2][4];
   const int64_t row = blockIdx.x;

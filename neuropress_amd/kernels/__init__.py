@@ -1165,20 +1165,6 @@ def _layer_norm(what, x, weight, bias, eps, stats):
     return out, mean, rstd
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        out, mean, rstd = _layer_norm("layer_norm", x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        return *layer_norm_backward(dy, x, weight, mean, rstd, needs=ctx.needs_input_grad[:3]), None
-
-
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dimension of *x* ``[..., H]`` (``npamd_layer_norm``): *weight* and *bias* ``[H]`` of its dtype or None; the result has x's dtype.
 
@@ -1196,7 +1182,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         otherwise = any(tracked(t) for t in followed)
     if otherwise:
         return torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps)
-    return _LayerNorm.apply(x, weight, bias, eps)
+    _rows_of("layer_norm", x, x.shape[-1])
+    return _lib.host().layer_norm_recorded(x, weight, bias, float(eps))
 
 
 def layer_norm_stats(

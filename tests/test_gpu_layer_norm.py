@@ -349,3 +349,35 @@ def test_more_rows_than_a_launch_has_blocks(gpu, h):
         _check(y[rows], ref, slack, torch.float16, "y")
         _check(dx[rows], *_reference_back(dys, xs, None, mean[rows].cpu(), rstd[rows].cpu())[0], torch.float16, "dx")
     assert torch.equal(y, kernels.layer_norm(x, None, None, EPS)) and bool(torch.isfinite(dx).all())
+
+
+def test_what_autograd_hands_to_the_backward_pass(gpu):
+    """Gradients that are expanded, transposed or missing, inputs without rows or at no single distance, an input changed in between, one backward pass after another."""
+    from neuropress_amd import kernels
+
+    x, w, b, dy = (t.to(gpu) for t in _inputs(24, 160, torch.float32))
+    xs = torch.randn(4, 6, 400, device=gpu)[:, ::2, 30:190].requires_grad_()
+    w.requires_grad_(), b.requires_grad_()
+    f = lambda t: torch.nn.functional.layer_norm(t, (160,), w, b, EPS)
+    for t in (xs, x.view(2, 12, 160).transpose(0, 1).detach().requires_grad_()):
+        for loss in (lambda y: y.sum(), lambda y: (y.transpose(0, 1) * 0.5).contiguous().square().sum(), lambda y: y[:, :2].mean()):
+            got, want = torch.autograd.grad(loss(kernels.layer_norm(t, w, b, EPS)), [t, w, b]), torch.autograd.grad(loss(f(t)), [t, w, b])
+            # both are f32 sums of up to 72 x 160 terms of about one
+            assert all(torch.allclose(a, c, rtol=1e-4, atol=1e-4) for a, c in zip(got, want))
+    none = x[:0].detach().requires_grad_()
+    got = torch.autograd.grad(kernels.layer_norm(none, w, b, EPS).sum(), [none, w, b])
+    assert got[0].shape == none.shape and not got[1].any() and not got[2].any()
+    y = kernels.layer_norm(xs, w, b, EPS)
+    y.sum().backward(retain_graph=True)
+    first = w.grad.clone()
+    y.sum().backward()
+    assert torch.equal(w.grad, 2 * first)
+    moved = x.clone()
+    y = kernels.layer_norm(moved, w, b, EPS)
+    moved.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = kernels.layer_norm(x, w, b, EPS)
+    with pytest.raises(RuntimeError, match="at most 2\\*\\*31"):
+        kernels.layer_norm(x[:1].expand(1 << 31, 160), w, b, EPS)
+    del y
