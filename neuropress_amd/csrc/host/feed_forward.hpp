@@ -140,20 +140,33 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     at::Tensor y = empty(x.sizes(), x.scalar_type(), device), mean = empty(lead, at::kFloat, device), rstd = empty(lead, at::kFloat, device);
     TORCH_CHECK(npamd_layer_norm(rows.const_data_ptr(), ld, data_or_null(w), data_or_null(b), y.data_ptr(), h, mean.data_ptr<float>(), rstd.data_ptr<float>(), m, h,
                                  (float)eps, dtype_code(x.scalar_type()), current_stream(device)) == NPAMD_OK, npamd_last_error());
-    ctx->save_for_backward({x, weight ? *weight : at::Tensor(), mean, rstd});
-    ctx->saved_data["has"] = (int64_t)((weight ? 1 : 0) | (bias ? 2 : 0));
+    ctx->save_for_backward({x, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), mean, rstd});
     return y;
+  }
+  // Inside a capture torch would go on to leaves whose nodes another graph that is still alive has made on another stream: waiting for that stream there ends the process.
+  static void refuse_foreign_leaves(const torch::autograd::variable_list& inputs) {
+    const auto stream = c10::hip::getCurrentHIPStream();
+    hipStreamCaptureStatus status;
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) return (void)hipGetLastError();
+    if (status == hipStreamCaptureStatusNone) return;
+    for (int i = 0; i < 3; ++i) {
+      if (!inputs[i].defined() || !inputs[i].is_leaf() || !inputs[i].requires_grad()) continue;
+      const auto leaf = torch::autograd::impl::try_get_grad_accumulator(inputs[i]);
+      TORCH_CHECK(!leaf || !leaf->stream() || leaf->stream()->id() == stream.id(),
+                  "layer_norm: a backward pass cannot be captured while a graph of the same leaves from another stream is alive: free it, or make it on the stream of the capture");
+    }
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const torch::autograd::variable_list saved = ctx->get_saved_variables();
     const bool recorded = c10::GradMode::is_enabled();
     torch::autograd::variable_list out(4);
-    const at::Tensor &x = saved[0], &mean = saved[2], &rstd = saved[3];
+    const at::Tensor &x = saved[0], &mean = saved[3], &rstd = saved[4];
     const c10::DeviceGuard guard(x.device());
+    refuse_foreign_leaves(saved);
     {
       const c10::AutoGradMode off(false);
-      const int64_t has = ctx->saved_data["has"].toInt();
-      const bool need[3] = {ctx->needs_input_grad(0), (has & 1) && ctx->needs_input_grad(1), (has & 2) && ctx->needs_input_grad(has & 1 ? 2 : 1)};
+      const bool with_w = saved[1].defined(), with_b = saved[2].defined();
+      const bool need[3] = {ctx->needs_input_grad(0), with_w && ctx->needs_input_grad(1), with_b && ctx->needs_input_grad(with_w ? 2 : 1)};
       const int device = x.get_device(), h = (int)x.size(-1), m = (int)(x.numel() / h);
       int64_t ldx, lddy;
       const at::Tensor rows = as_rows(x, &ldx), dy = as_rows(grads[0], &lddy), w = saved[1].defined() ? saved[1].contiguous() : at::Tensor();

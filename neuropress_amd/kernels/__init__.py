@@ -1168,8 +1168,8 @@ def _layer_norm(what, x, weight, bias, eps, stats):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dimension of *x* ``[..., H]`` (``npamd_layer_norm``): *weight* and *bias* ``[H]`` of its dtype or None; the result has x's dtype.
 
-    Where a gradient of x, weight or bias is recorded, the backward pass is :func:`layer_norm_backward`'s kernels (first derivatives).  Calls that torch follows in
-    other ways (forward mode, ``torch.func``, traces, autocast to another type) go through ``torch.nn.functional.layer_norm``.
+    Where a gradient of x, weight or bias is recorded, the backward pass is :func:`layer_norm_backward`'s kernels (first derivatives).  Captured into a graph it is refused
+    while another graph of the same leaves, made on another stream, is alive (torch would end the process).  Calls that torch follows in other ways (forward mode, ``torch.func``, traces, autocast to another type) go through ``torch.nn.functional.layer_norm``.
     """
     out = _lib.host().layer_norm(x, weight, bias, eps, False)
     if out is not None:

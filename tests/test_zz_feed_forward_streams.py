@@ -145,3 +145,27 @@ def test_captured_feed_forward_half_of_a_block(gpu, tokens, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(out, again))
+
+
+def test_capture_beside_an_eager_graph_of_the_same_leaves(gpu):
+    """Refused in the backward pass, before torch waits for the other graph's stream inside the capture; once that graph is gone the same step is captured."""
+    from neuropress_amd import kernels
+
+    x, w, b, dy = (t.to(gpu) for t in norm_inputs(20, 320, torch.bfloat16))
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    alive = kernels.layer_norm(*leaves, EPS)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            kernels.layer_norm(*leaves, EPS).backward(dy)
+    torch.cuda.synchronize()
+    assert torch.equal(alive, kernels.layer_norm(*leaves, EPS)) and all(t.grad is None for t in leaves)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        kernels.layer_norm(*leaves, EPS).backward(dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    _, mean, rstd = kernels.layer_norm_stats(x, w, b, EPS)
+    assert all(torch.equal(t.grad, c) for t, c in zip(leaves, kernels.layer_norm_backward(dy, x, w, mean, rstd)))
