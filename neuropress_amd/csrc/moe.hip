@@ -25,7 +25,7 @@ using namespace npamd;
 namespace {
 
 constexpr int kMoeMaxTokens = NPAMD_GEMV_MAX_M, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
-constexpr int kMoeMaxWaves = 8, kMoeMaxParts = 8;  // of a block
+constexpr int kMoeMaxWaves = 8;  // of a block
 
 struct MoeArgs {
   const void *x, *router;
@@ -116,6 +116,25 @@ __device__ __forceinline__ void pick_experts(const MoeArgs& a, int m, int lane, 
     v[i] = lane + 64 * i < a.E ? a.logits[m * a.E + lane + 64 * i] : -INFINITY;
     const uint32_t bits = __builtin_bit_cast(uint32_t, v[i] + 0.f);  // minus zero is zero
     if (lane + 64 * i < a.E) key[i] = v[i] != v[i] ? 0xFFFFFFFFu : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+  }
+  // A lane's expert is as many places behind the first as there are larger keys: three instructions for each, where a turn below waits for some 20 one after the other.
+  if (a.E <= 64 && a.E <= 16 * a.top_k) {
+    int place = 0;
+    for (int e = 0; e < a.E; ++e) {
+      const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)key[0], e);
+      place += other > key[0] || (other == key[0] && e < lane);
+    }
+    const bool picked = lane < a.E && place < a.top_k;
+    if (picked) route.ids[m * a.top_k + place] = (uint16_t)lane;
+    if (!first) return;
+    const uint32_t top = wave_max(key[0]);
+    const float most = top == 0xFFFFFFFFu ? NAN : __builtin_bit_cast(float, top & 0x80000000u ? top & 0x7FFFFFFFu : ~top);
+    const float power = lane < a.E ? __expf(v[0] - most) : 0.f, p = power / wave_sum(power), total = wave_sum(picked ? p : 0.f);
+    if (picked) {
+      a.ids[m * a.top_k + place] = (uint16_t)lane;
+      a.share[m * a.top_k + place] = a.renormalize ? p / total : p;
+    }
+    return;
   }
   float most = 0.f, sum = 0.f, mine = 0.f, total = 0.f;
   int id = 0;
@@ -613,6 +632,10 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const Mo
   }
 }
 
+// The down kernel's blocks, a row tile's parts times its row tiles: no more than compute units.
+constexpr int kMoeBlocks = 256;
+int moe_max_parts(int H) { return std::max(1, kMoeBlocks / std::max(1, H / 32)); }
+
 struct MoeSpace {
   int64_t logits, ids, share, entries, xs, h, done, parts, bytes;
   MoeSpace(int M, int E, int top_k, int H, int I) {
@@ -629,15 +652,17 @@ struct MoeSpace {
     xs = take((int64_t)M * H * 2);
     h = take((int64_t)M * top_k * I * 2);
     done = take((int64_t)H / 32 * 4);
-    parts = take((int64_t)kMoeMaxParts * M * H * 4);
+    parts = take((int64_t)moe_max_parts(H) * M * H * 4);
     bytes = at;
   }
 };
 
-// Four waves to a block of the up kernel (us of the layer with two / four / eight: int4 4096 x 14336, one token 54 / 50 / 56; dense 2048 x 2048, four tokens 67 / 65 / 66)
-// and eight of the down kernel (four / eight / 16: 54 / 50 / 52, 65 / 65 / 66), whose blocks split the columns where there are fewer row tiles than compute units (one part /
-// two: 57 / 50; hidden size 2048, seven tokens int8 one / four: 103 / 73).  From entries of five pairs on the up kernel's waves share them: 16 tokens int4 271 / 219, one token 54 / 57.
-constexpr int kMoeUpWaves = 4, kMoeDownWaves = 8, kMoeTogether = 5, kMoeBlocks = 256, kMoeBlocksPerCu = 4;
+// Four waves to a block of the up kernel (us of the layer with two / four / eight: int4 4096 x 14336, one token 54 / 50 / 56; dense 2048 x 2048, four tokens 67 / 65 / 66), three
+// where that many divide an item's steps better (nine steps, hidden size 2304: 59.7 / 58.2), and eight of the down kernel (four / eight / 16: 54 / 50 / 52, 65 / 65 / 66), whose
+// blocks split the columns (one part / two: int4 one token 57 / 50; hidden size 256, inner 13440, 14 experts, one / eight / 16 / 32 parts 186 / 51 / 43 / 44; 384 and 1152, 12
+// experts 30 / 24 / 26 / 28).  From entries of five pairs on the up kernel's waves share them: 16 tokens int4 271 / 219, one token 54 / 57; unless that leaves compute units
+// without a block (19 tokens through four of four, 3840 x 768 42 / 35).
+constexpr int kMoeUpWaves = 4, kMoeDownWaves = 8, kMoeTogether = 5, kMoeWavesPerCu = 16;
 
 template <int ACT, int FMT, bool ASYM, int GROUP>
 int launch_moe_format(const MoeArgs& a, hipStream_t st) {
@@ -648,10 +673,13 @@ int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   // (us with 16 / eight: 16 tokens int4 through two of eight 190 / 183, through eight of 64 88 / 70, 32 tokens through two of eight 199 / 231); four where it has one, of int8,
   // whose steps are the largest, two (eight of 64 experts, hidden size 2048, with eight / four / two: eight tokens dense 129 / 112 / 112, seven int8 70 / 73 / 65).
   const int pairs = a.M * a.top_k, cap = std::min(a.M, pairs <= a.E ? (FMT == 8 ? 2 : 4) : pairs <= 4 * a.E ? 8 : 16), x_bytes = 2 * S::x_loads(cap) * 1024;
-  const bool together = cap >= kMoeTogether;
+  const int most_entries = std::min(pairs, a.E + pairs / cap);
+  const bool together = cap >= kMoeTogether && (int64_t)most_entries * (a.I / 16 / kMoeUpWaves) >= kMoeBlocks;
   auto up_own = [&](int waves) { return waves * 4 * S::kItem + (together ? x_bytes : waves * (x_bytes + cap * kMoeRedRow * 4)); };
   auto down_own = [&](int waves) { return waves * (x_bytes + 4 * S::kItem + a.M * 32 * 4); };
-  const int up_waves = together ? kMoeUpWaves : std::min(kMoeUpWaves, (a.H + S::kColumns - 1) / S::kColumns);
+  const int up_steps = (a.H + S::kColumns - 1) / S::kColumns;
+  auto idle = [&](int waves) { return (float)((up_steps + waves - 1) / waves * waves) / (float)up_steps; };
+  const int up_waves = together ? kMoeUpWaves : up_steps < kMoeUpWaves ? up_steps : idle(3) * 1.1f < idle(kMoeUpWaves) ? 3 : kMoeUpWaves;
   int down_waves = kMoeDownWaves;
   while (down_own(down_waves) + MoeRoute::bytes(pairs, down_waves) > kRoom) --down_waves;
   const int up_lds = up_own(up_waves) + MoeRoute::bytes(pairs, up_waves), down_lds = down_own(down_waves) + MoeRoute::bytes(pairs, down_waves);
@@ -663,10 +691,15 @@ int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve LDS: %s", what, hipGetErrorString(e));
   if (a.M == 1) launch(moe_logits_kernel<ACT, 1, FMT == 4>, a.E, 256, 0, st, a);
   else launch(moe_logits_kernel<ACT, 4, FMT == 4>, dim3(a.E, (a.M + 3) / 4), 256, 0, st, a);
-  const int64_t items = (int64_t)std::min(pairs, a.E + pairs / cap) * (a.I / 16 / (together ? up_waves : 1));  // no more than that
-  const int per_cu = std::max(1, std::min(kMoeBlocksPerCu, kRoom / up_lds));
+  const int64_t items = (int64_t)most_entries * (a.I / 16 / (together ? up_waves : 1));  // no more than that
+  const int per_cu = std::max(1, std::min(kMoeWavesPerCu / up_waves, kRoom / up_lds));
   launch(up, (unsigned)std::min<int64_t>(items, kMoeBlocks * per_cu), 64 * up_waves, up_lds, st, a, cap, up_own(up_waves));
-  const int parts = std::max(1, std::min(kMoeMaxParts, kMoeBlocks / (a.H / 32)));
+  // Parts of the columns: a wave's steps, 2 us each, against 0.4 us for each part that meets the others.
+  const int down_steps = std::min(pairs, a.E) * ((a.I + S::kColumns - 1) / S::kColumns);  // if every expert that can be met is
+  auto down_cost = [&](int n) { return 5 * ((down_steps + n * down_waves - 1) / (n * down_waves)) + n; };
+  int parts = 1;
+  for (int n = 2; n <= moe_max_parts(a.H); ++n)
+    if (down_cost(n) < down_cost(parts)) parts = n;
   launch(down, dim3(a.H / 32, parts), 64 * down_waves, down_lds, st, a, cap, down_own(down_waves));
   return check_launch(what);
 }

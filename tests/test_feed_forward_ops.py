@@ -68,6 +68,7 @@ def test_sizes_past_the_kernels_are_refused():
     lib = _lib.load()
     assert lib.npamd_layer_norm_workspace_bytes(2, far - 1) == 0 == lib.npamd_moe_workspace_bytes(33, 8, 2, 128, 192)
     assert lib.npamd_moe_workspace_bytes(4, 8, 9, 128, 192) == 0 == lib.npamd_moe_workspace_bytes(4, 600, 2, 128, 192)
+    assert lib.npamd_moe_workspace_bytes(1, 1, 1, 1, 1) > 0  # refused by the call, not here
 
 
 def test_wrappers_refuse_what_is_not_on_a_gpu():

@@ -233,3 +233,55 @@ def test_all_tokens_meet_in_the_same_experts(gpu, nbits, m, experts, top_k):
     layer["router"][:top_k] = layer["router"][:top_k].abs() + 0.05 * torch.arange(1, top_k + 1)[:, None]
     assert ((x.double() @ layer["router"].double().T).topk(top_k).indices < top_k).all()
     _check(kernels.moe_layer(x.to(gpu), _experts(layer), top_k), *_reference(x, layer, dense, top_k, True), torch.float16)
+
+
+@pytest.mark.parametrize("nbits,group,zero", [(4, 64, True), (8, 64, True), (8, 128, False), (16, 32, False)])
+@pytest.mark.parametrize("e,top_k,h,i,m", [(2, 2, 256, 4480, 2), (14, 7, 128, 2688, 2), (4, 4, 640, 192, 19), (4, 4, 128, 128, 32), (6, 2, 2304, 128, 3), (6, 2, 1152, 128, 1),
+                                           (8, 8, 64, 1024, 32)])  # fmt: skip
+def test_few_row_tiles_many_columns_and_the_other_way_round(gpu, nbits, group, zero, e, top_k, h, i, m):
+    """Columns in many parts, blocks of three waves, entries of sixteen pairs whose items are too few to share tokens."""
+    from neuropress_amd import kernels
+
+    if nbits != 16 and (h % group or i % group):
+        group = 64
+    layer, dense = _layer(e + m, e, h, i, torch.float16, nbits, group, zero)
+    x = torch.randn(m, h, generator=cases.gen(m)).half()
+    _check(kernels.moe_layer(x.to(gpu), _experts(layer), top_k), *_reference(x, layer, dense, top_k, True), torch.float16)
+
+
+@pytest.mark.parametrize("e,top_k", [(1, 1), (2, 1), (16, 1), (17, 1), (32, 2), (33, 2), (63, 4), (64, 4), (64, 3), (65, 5), (64, 16), (128, 8)])
+def test_routing(gpu, e, top_k):
+    """Equal logits go to the lower index, NaN above all, infinities in their order; shares against the softmax in 64 bits.  Expert k answers in column k % 64,
+    so y tells which experts were met, at which share."""
+    from neuropress_amd import kernels
+
+    h = i = 64
+    g = cases.gen(e + top_k)
+    router = torch.zeros(e, h).half()
+    router[:, :4] = torch.randint(-2, 3, (e, 4), generator=g).half()  # sums of small whole numbers: many equal logits
+    gate_up, down = torch.zeros(e, 2 * i, h).half(), torch.zeros(e, h, i).half()
+    gate_up[:, 0, 4], gate_up[:, i, 4] = 4.0, 1.0
+    down[:, torch.arange(64), 0] = 0
+    down[torch.arange(e), torch.arange(e) % 64, 0] = 1.0
+    x = torch.zeros(7, h).half()
+    x[:, :4] = torch.randint(-1, 2, (7, 4), generator=g).half()
+    x[:, 4] = 1.0
+    layer = kernels.MoEExperts(router.to(gpu), gate_up.to(gpu), down.to(gpu))
+    logits = x.double() @ router.double().T
+    p = torch.softmax(logits, -1)
+    ids = torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    answer = float(torch.nn.functional.silu(torch.tensor(4.0, dtype=torch.float64)))
+    for renormalize in (True, False):
+        share = p.gather(1, ids)
+        share = share / share.sum(-1, keepdim=True) if renormalize else share
+        want = torch.zeros(7, h, dtype=torch.float64)
+        for m in range(7):
+            for t in range(top_k):
+                want[m, ids[m, t] % 64] += share[m, t] * answer
+        y = kernels.moe_layer(x.to(gpu), layer, top_k, renormalize).double().cpu()
+        # silu(4) and y are rounded to half a step each, 2^-11, f32 far less
+        assert bool(((y - want).abs() <= 2.0**-9.9 * want + 2.0**-24).all())
+    bad = router.clone()
+    bad[e - 1, 5] = float("nan")  # this expert's logit is NaN whatever x holds: it is met first and every share is NaN
+    y = kernels.moe_layer(x.to(gpu), kernels.MoEExperts(bad.to(gpu), gate_up.to(gpu), down.to(gpu)), top_k)
+    assert bool(y.isnan().all(0)[(e - 1) % 64])
