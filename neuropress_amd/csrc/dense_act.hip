@@ -33,7 +33,7 @@ __device__ __forceinline__ void finish(const FewArgs& a, int m, int n, float v) 
 
 // R rows of W and TB tokens to a wave, KS of a block's four waves to a row, U pieces of each row on their way; tokens past TB in further blocks.  Any K and any
 // addresses: a row that does not end with a piece of eight has its last one end with the row, and the values that the piece before has too are zeroed in x.  x comes from
-// the L1.  4096 x 14336, one token: 22.9 us, 5.1 TB/s, the rate of a large copy; 640 x 2048 2.9 us.
+// the L1.  4096 x 14336, one token: 22.1 us, 5.3 TB/s, the rate of reads; 640 x 2048 2.9 us.
 template <int ACT, int R, int TB, int KS, int U>
 __global__ void __launch_bounds__(256) dense_few_kernel(const FewArgs a) {
   __shared__ float sums[4][R * TB];
@@ -231,12 +231,13 @@ int launch_some(const FewArgs& a, hipStream_t st, const char* what) {
   return mt == 3 ? launch_some_tile<ACT, 3, 1>(a, waves, st, what) : launch_some_tile<ACT, 4, 1>(a, waves, st, what);
 }
 
-// Rows of a wave: two from two tokens on, which then share a read of x.  Four waves to a row where there are few rows (1024 x 4096, one token, one wave / four 3.9 / 3.5 us).
+// Rows of a wave: two from two tokens on, which then share a read of x.  Four waves to a row where there are few rows and each wave has
+// columns to read (one token, one wave / four 1024 x 4096 4.1 / 3.7 us, 2048 x 8192 8.3 / 8.4, two tokens 10.5 / 8.9; but 4096 x 2048 5.4 / 6.1, 5488 x 311 3.7 / 5.9).
 template <int ACT>
 int launch_few(const FewArgs& a, hipStream_t st, const char* what) {
 #define NPAMD_FEW(R, TB, KS)                                                                                                 \
   launch(dense_few_kernel<ACT, R, TB, KS, 4>, dim3((unsigned)((a.N + R * (4 / KS) - 1) / (R * (4 / KS))), (unsigned)((a.M + TB - 1) / TB)), 256, 0, st, a)
-  const bool together = a.N < 8192;
+  const bool together = a.N <= 2048 && a.K > 1024;
   if (a.M == 1) {
     if (together) NPAMD_FEW(1, 1, 4);
     else NPAMD_FEW(1, 1, 1);
@@ -253,7 +254,7 @@ int launch_few(const FewArgs& a, hipStream_t st, const char* what) {
 
 constexpr int kMaxRows = 1 << 25, kMaxColumns = 1 << 30;  // of W: a launch has fewer than 2^32 threads
 
-// Which kernel takes a call; aligned: rows that the tiles can read.  Us with dense_few_kernel / dense_some_kernel / the tiles, silu and a residual: two tokens 4096 x 4096 10.2 /
+// Which kernel takes a call; aligned: rows that the tiles can read.  Us with dense_few_kernel / dense_some_kernel / the tiles, silu and a residual: two tokens 4096 x 4096 9.1 /
 // 9.3 / 13.9, 640 x 2048 3.3 / 3.9 / 8.9; eight 4096 x 4096 - / 9.5 / 13.9, 4096 x 14336 - / 23.7 / 28.1, 1024 x 4096 - / 5.3 / 9.5; 32 tokens 8192 x 2048 - / 14.0 / 14.7,
 // 4096 x 4096 - / 14.0 / 19.7, 4096 x 14336 - / 35 / 29.  Past 32 tokens a block has few waves and reads many tokens: it needs a compute unit of its own and K no longer
 // than that lasts: 64 tokens 4096 x 4096 16.0 / 18.0, 2048 x 2048 8.4 / 9.1, 3003 x 2184 11.7 / 15.8; but 8192 x 2048 19.9 / 13.6, 1024 x 4096 11.6 / 9.9, 2048 x 8192 24 / 15.

@@ -184,7 +184,7 @@ def test_the_residual_in_its_own_place(gpu):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m", [2, 3, 15, 16, 17, 31, 32, 33, 48, 49, 64, 65])
-@pytest.mark.parametrize("n,k", [(1, 8), (16, 120), (17, 128), (100, 1032), (40, 2560), (40, 2568), (4096, 264), (4100, 264), (8191, 136), (8192, 136), (8209, 1160)])
+@pytest.mark.parametrize("n,k", [(1, 8), (16, 120), (17, 128), (100, 1032), (40, 2560), (40, 2568), (4096, 264), (4100, 264), (8191, 136), (8192, 136), (8209, 1160), (2048, 1032), (2049, 1032), (2048, 1021)])
 def test_where_one_kernel_takes_over_from_another(gpu, dtype, m, n, k):
     """Tokens and rows on both sides of where the kernel changes; columns that end inside a step, or before every wave has one."""
     x, w, b, r = _inputs(m, n, k, dtype)
