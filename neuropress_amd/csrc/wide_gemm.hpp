@@ -19,6 +19,7 @@
 #include "dense_gemm.hpp"
 #include "gemm_tile.hpp"
 #include "lds_transfer.hpp"
+#include "wave_ops.hpp"
 
 namespace npamd {
 
@@ -224,8 +225,7 @@ wide_gemm_kernel(const DenseShape s) {
       const int at = min(wn0 + n + e, s.N - 1);
       if (s.ep.bias) bias[e] = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, at) : ((const float*)s.ep.bias)[at];
     }
-    const bool whole = s.N % 8 == 0 && s.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(s.y) & 15) == 0 &&
-                       (!s.ep.residual || (s.ep.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(s.ep.residual) & 15) == 0));
+    const bool whole = n + 8 <= cols;  // at whatever address
     uint16_t* const to = reinterpret_cast<uint16_t*>(s.y) + (int64_t)wm0 * s.ldy + wn0;
     const uint16_t* const from = reinterpret_cast<const uint16_t*>(s.ep.residual) + (int64_t)wm0 * s.ep.ldr + wn0;
     constexpr int kTurns = (16 + kRowsAtOnce - 1) / kRowsAtOnce;
@@ -243,7 +243,7 @@ wide_gemm_kernel(const DenseShape s) {
         if (row < 0) continue;
         const uint16_t* const at = from + (int64_t)(16 * a + row) * s.ep.ldr + n;
         if (whole) {
-          res[set][i] = *reinterpret_cast<const u32x4*>(at);
+          res[set][i] = *reinterpret_cast<const u32x4_any*>(at);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -287,7 +287,7 @@ wide_gemm_kernel(const DenseShape s) {
         if (row >= 0) {
           uint16_t* const at = to + (int64_t)(16 * a + row) * s.ldy + n;
           if (whole) {
-            *reinterpret_cast<u32x4*>(at) = u32x4{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16), bits[4] | (bits[5] << 16), bits[6] | (bits[7] << 16)};
+            *reinterpret_cast<u32x4_any*>(at) = u32x4{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16), bits[4] | (bits[5] << 16), bits[6] | (bits[7] << 16)};
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
