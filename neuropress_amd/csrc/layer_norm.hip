@@ -452,9 +452,10 @@ layer_norm_back_sum_kernel(const float* __restrict__ partials, int parts, int H,
   store_from_f32<DT>(out, col, v);
 }
 
-// Turns of a block at least, where rows are few: every block leaves sums of two rows' bytes in f32, and a turn takes 1.3 us (509 x 3003 with one / two / three turns
-// 11.7 / 9.9 / 12.2 us, 64 x 4096 7.0 / 7.9 / 9.3); and no more blocks than compute units (8192 x 4096 with 192 / 256 / 512 55 / 48 / 54 us).
-constexpr int kTurns = 2;
+// A block's turns, where rows are few: a turn takes 1.3 us, but every block leaves sums of two rows' bytes in f32, so two where those would be more than kMaxSums bytes (one /
+// two / four turns 509 x 3003, 6 MB with one, 11.7 / 10.0 / 12.8 us, 512 x 2048, 2 MB, 7.9 / 9.2 / 10.9, 104 x 176 5.4 / 6.4 / 7.9) or where one block then takes all rows,
+// without a second launch (16 x 768 5.9 / 5.1); and no more blocks than compute units (8192 x 4096 with 192 / 256 / 512 55 / 48 / 54 us).
+constexpr int64_t kMaxSums = 4 << 20;
 // Which kernel the backward pass takes.  parts: sums over rows that it leaves to be added.
 struct BackPlan {
   int nv = 0, row_waves = 0, groups = 0, parts = 0;  // nv 0: rows that do not fit the registers
@@ -470,7 +471,8 @@ struct BackPlan {
     row_waves = 1;
     while (row_waves * 64 * nv < pieces) row_waves *= 2;
     groups = std::min(16 / row_waves, std::max(1, M));
-    parts = (int)std::min<int64_t>(256, ((int64_t)M + groups * kTurns - 1) / (groups * kTurns));
+    auto blocks = [&](int turns) { return std::min<int64_t>(256, ((int64_t)M + groups * turns - 1) / (groups * turns)); };
+    parts = (int)blocks(blocks(2) > 1 && blocks(1) * H * 8 <= kMaxSums ? 1 : 2);
   }
 };
 
