@@ -6,7 +6,8 @@
 //
 // Three launches: the logits (a block per expert), up (every block first picks each token's experts from the logits, then walks (expert, 16 gate rows and their
 // 16 up rows)), down (a block per 16 rows of y, all its experts one behind the other).  The experts' weights are all that counts: each byte is read once, an expert's
-// tokens share it as the 16 columns of an MFMA.
+// tokens share it as the 16 columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 4.8, 29.7 and 19.4 us by
+// themselves, 49 in a row, 4.0 TB/s of 198 MB; 16 tokens fp16 with zero points 173-183 us, 4.1 TB/s.  Bound by HBM inside the walks, by round trips in front of and behind them.
 //
 // Codes: an MFMA 16x16x32 sees 32 columns of one scale group, so a group's scale multiplies the f32 sum behind it, four multiply-adds for 512 weights, instead of the
 // weights in front of it; nothing is rounded to 16 bits that way.  The codes become operands as they are, their bits under an exponent: q + 128, + 1024 or + 64
