@@ -5,8 +5,8 @@
 // silu(gate) * up, the operand of the second product: sums and p stay in f32 up to the store of y.
 //
 // Three launches: the logits (a block per expert), up (every block first picks each token's experts from the logits, then walks (expert, 16 gate rows and their
-// 16 up rows)), down (a block per 16 rows of y, all its experts one behind the other).  The experts' weights are all that counts: each byte is read once, an expert's
-// tokens share it as the 16 columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 4.8, 29.7 and 19.4 us by
+// 16 up rows)), down (a block per 32 rows of y and part of all their experts' columns).  The experts' weights are all that counts: each byte is read once for up to 16
+// of an expert's tokens, which share it as the columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 4.8, 29.7 and 19.4 us by
 // themselves, 49 in a row, 4.0 TB/s of 198 MB; 16 tokens fp16 with zero points 173-183 us, 4.1 TB/s.  Bound by HBM inside the walks, by round trips in front of and behind them.
 //
 // Codes: an MFMA 16x16x32 sees 32 columns of one scale group, so a group's scale multiplies the f32 sum behind it, four multiply-adds for 512 weights, instead of the
