@@ -1362,6 +1362,8 @@ def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: boo
     if tracked(x):
         raise RuntimeError(f"{what}: for inference only: no gradient, trace or transform of torch can follow it")
     m, e, i = _rows_of(what, x, h), experts.experts, experts.inter
+    if not 1 <= int(top_k) <= e:
+        raise RuntimeError(f"{what}: bad shape: top_k must lie between 1 and the {e} experts, got {top_k}")
     x2 = _lead2d(x, m, h)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     need = int(_lib.load().npamd_moe_workspace_bytes(m, e, int(top_k), h, i))

@@ -199,7 +199,7 @@ def test_refusals(gpu):
     x = torch.randn(2, 128, device=gpu).half()
     with pytest.raises(RuntimeError, match="at most 32 tokens"):
         kernels.moe_layer(x[:1].expand(33, 128), experts, 2)
-    for top_k in (0, 5):
+    for top_k in (0, 5, -1, (1 << 32) + 2):
         with pytest.raises(RuntimeError, match="bad shape"):
             kernels.moe_layer(x, experts, top_k)
     with pytest.raises(RuntimeError, match="x must be"):
