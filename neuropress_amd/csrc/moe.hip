@@ -1,13 +1,13 @@
 // A mixture-of-experts layer for a few tokens:
 //   logits = x router^T,  p = softmax(logits) over all experts,  the top_k largest (ties to the lower index), divided by their sum on request
 //   y = sum over them of p_e down_e(silu(gate_e(x)) * up_e(x))
-// Expert weights are dense or group-quantized codes, w = (q - zero) scale, which is not rounded.  What is rounded to the activation type on the way is
-// silu(gate) * up, the operand of the second product: sums and p stay in f32 up to the store of y.
+// Expert weights are dense or group-quantized codes, w = (q - zero) scale, which is not rounded.  Sums and p stay in f32 up to the store of y.  silu(gate) * up, the operand
+// of the second product, is kept as the sum of two bf16: to 2^-17, in the range of f32 whatever the activations' type (in fp16 it would be infinite past 65504).
 //
 // Three launches: the logits (a block per expert), up (every block first picks each token's experts from the logits, then walks (expert, 16 gate rows and their
 // 16 up rows)), down (a block per 32 rows of y and part of all their experts' columns).  The experts' weights are all that counts: each byte is read once for up to 16
 // of an expert's tokens, which share it as the columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 4.8, 29.7 and 19.4 us by
-// themselves, 49 in a row, 4.0 TB/s of 198 MB; 16 tokens fp16 with zero points 173-183 us, 4.1 TB/s.  Bound by HBM inside the walks, by round trips in front of and behind them.
+// themselves, 49 in a row, 4.0 TB/s of 198 MB; 16 tokens fp16 with zero points 181-183 us, 4.0 TB/s.  Bound by HBM inside the walks, by round trips in front of and behind them.
 //
 // Codes: an MFMA 16x16x32 sees 32 columns of one scale group, so a group's scale multiplies the f32 sum behind it, four multiply-adds for 512 weights, instead of the
 // weights in front of it; nothing is rounded to 16 bits that way.  The codes become operands as they are, their bits under an exponent: q + 128, + 1024 or + 64
@@ -42,7 +42,7 @@ struct MoeArgs {
   uint32_t* done;  // [H / 32] blocks of the down kernel that have left their part
   float* parts;    // [part][H / 32][M * 32]
   uint16_t* xs;    // [M][H], rows as the up kernel reads them
-  uint16_t* h;     // [M][top_k][I]
+  uint16_t* h;     // [M][top_k][2][I], bf16: silu(gate) * up, and what its rounding leaves
 };
 
 // int4 operands hold the columns of an octet in the order 0 4 1 5 2 6 3 7 (the nibbles 4 i and 4 i + 16 of a dword are a pair): where column k of it lies.
@@ -239,8 +239,8 @@ __device__ __forceinline__ uint32_t masked_or(uint32_t v) {
   return (v & mask) | bits;
 }
 
-// GROUP: MFMAs that see one scale group, one after the other into one sum.
-template <int ACT, int FMT, bool ASYM, int R, int GROUP>
+// ACT: the type of the tokens and so of the operands; DENSE: of dense weights.  GROUP: MFMAs that see one scale group, one after the other into one sum.
+template <int ACT, int FMT, bool ASYM, int R, int GROUP, int DENSE>
 struct MoeWalk {
   using S = MoeStep<FMT, ASYM>;
   static constexpr int kXLoads = S::x_loads(16), kPlace = R * S::kItem;
@@ -277,14 +277,15 @@ struct MoeWalk {
     if constexpr (FMT != 16) scale[r] = uniform_ptr((const uint8_t*)(scales + row * groups));
     if constexpr (ASYM) zero[r] = uniform_ptr((const uint8_t*)(zeros + row * groups));
   }
-  // The tokens: rows list[j] / divide of x.
-  __device__ __forceinline__ void tokens(const uint16_t* rows_of_x, const uint16_t* list, int n, int divide) {
+  // The n tokens: rows row_of(j) of rows_of_x.
+  template <class Row>
+  __device__ __forceinline__ void tokens(const uint16_t* rows_of_x, int n, Row&& row_of) {
     x = reinterpret_cast<const uint8_t*>(rows_of_x);
     x_loads = __builtin_amdgcn_readfirstlane(S::x_loads(n));
 #pragma unroll
     for (int i = 0; i < kXLoads; ++i) {
       const int j = min(i * S::kTokensPerLoad + lane / S::kXSlots, n - 1);
-      x_row[i] = (uint32_t)((int)list[j] / divide) * (uint32_t)(K * 2);
+      x_row[i] = (uint32_t)row_of(j) * (uint32_t)(K * 2);
     }
   }
   __device__ __forceinline__ void load(int step, int place) {
@@ -361,9 +362,21 @@ struct MoeWalk {
     }
   }
   static __device__ __forceinline__ u32x4 ones() { return ACT == NPAMD_F16 ? constant(0x3C003C00u, 0x3C003C00u) : constant(0x3F803F80u, 0x3F803F80u); }
-
-
-
+  // Dense fp16 weights as sums of two bf16, exactly: eight and three bits.  An infinite one's second part is finite.
+  static __device__ __forceinline__ void split_f16(const uint32_t (&v)[S::kWords], u32x4* first, u32x4* second) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t part[2], rest[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float w = f16_bits_to_f32((v[i] >> (16 * e)) & 0xFFFFu), finite = __builtin_amdgcn_fmed3f(w, -65504.f, 65504.f);
+        part[e] = __builtin_bit_cast(uint32_t, w);
+        rest[e] = __builtin_bit_cast(uint32_t, finite - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, finite) & 0xFFFF0000u));
+      }
+      (*first)[i] = __builtin_amdgcn_perm(part[1], part[0], 0x07060302u);
+      (*second)[i] = __builtin_amdgcn_perm(rest[1], rest[0], 0x07060302u);
+    }
+  }
 
   // The step in `place`, with `n` tokens.
   __device__ __forceinline__ void multiply(int step, int place, int n) {
@@ -402,8 +415,15 @@ struct MoeWalk {
 #pragma unroll
             for (int e = 0; e < 4; ++e) raw[e] = v[e];
           }
-          if constexpr (FMT == 16) acc[r] = mfma16<ACT>(xa[i], operand(raw), acc[r]);
-          else d[r] = mfma16<ACT>(xa[i], operand(raw), d[r]);
+          if constexpr (FMT != 16) {
+            d[r] = mfma16<ACT>(xa[i], operand(raw), d[r]);
+          } else if constexpr (DENSE == ACT) {
+            acc[r] = mfma16<ACT>(xa[i], operand(raw), acc[r]);
+          } else {
+            u32x4 first, second;
+            split_f16(raw, &first, &second);
+            acc[r] = mfma16<ACT>(xa[i], first, mfma16<ACT>(xa[i], second, acc[r]));
+          }
         }
       }
       if constexpr (FMT != 16) {
@@ -443,18 +463,19 @@ constexpr int kMoeRedRow = 36;  // floats of a token's row where the waves' sums
 // tokens, a barrier per step; else they share the columns of one pair of row tiles, each with tokens of its own, and their sums meet at the item's end.  Tokens
 // take LDS and come from the L2 once per wave or per block: few of them are best brought by each wave, many are not.
 template <int ACT, int FMT, bool ASYM, int GROUP, bool TOGETHER>
-__global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) moe_up_kernel(const MoeArgs a, int cap, int own_lds) {
-  using Walk = MoeWalk<ACT, FMT, ASYM, 2, GROUP>;
+__global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) moe_up_kernel(const MoeArgs a, int cap, int down_cap, int own_lds) {
+  using Walk = MoeWalk<ACT, FMT, ASYM, 2, GROUP, ACT>;
   using S = typename Walk::S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const MoeRoute route(lds + own_lds, a.M * a.top_k, waves, lds);
   for (int m = wave; m < a.M; m += waves) pick_experts(a, m, lane, route, blockIdx.x == 0);
   __syncthreads();
-  list_entries(a, route, cap);
+  list_entries(a, route, blockIdx.x == 0 ? down_cap : cap);
   if (blockIdx.x == 0) {  // for the down kernel
     for (int p = threadIdx.x; p < *route.n_entries; p += blockDim.x) a.entries[p] = route.entries[p];
     if (threadIdx.x == 0) a.entries[a.M * a.top_k] = *route.n_entries;
+    if (down_cap != cap) list_entries(a, route, cap);  // those are read before its first barrier
   }
 
   const int groups = TOGETHER ? waves : 1, tiles = a.I / 16 / groups, items = __builtin_amdgcn_readfirstlane(*route.n_entries) * tiles, steps = (a.H + S::kColumns - 1) / S::kColumns;
@@ -477,7 +498,7 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) m
         uint16_t* const list = route.lists + (wave * 2 + ahead_slot) * 16;
         const int n = list_pairs(a, route, entry, cap, lane, list);
         if (lane == 0) route.counts[wave * 2 + ahead_slot] = n;
-        walk.tokens(a.xs, list, n, a.top_k);
+        walk.tokens(a.xs, n, [&](int j) { return (int)list[j] / a.top_k; });
       }
       const int64_t row = (int64_t)(entry & 0xFFFF) * 2 * a.I + (ahead % tiles * groups + (TOGETHER ? wave : 0)) * 16;
       walk.rows(0, a.gate_up, a.gate_up_scale, a.gate_up_zero, row);
@@ -507,7 +528,12 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) m
     const int tile = item % tiles;
     auto store = [&](int j, int k, float gate, float up) __attribute__((always_inline)) {
       const int to = FMT == 4 ? (k & ~7) | octet_place(k & 7) : k;
-      store_from_f32<ACT>(a.h, (int64_t)list[j] * a.I + to, silu_f32(gate) * up);
+      const float v = silu_f32(gate) * up;
+      const uint32_t bits = f32_to_bf16_bits(v);
+      const float rounded = bf16_bits_to_f32(bits);
+      uint16_t* const at = a.h + (int64_t)list[j] * 2 * a.I + to;
+      at[0] = (uint16_t)bits;
+      at[a.I] = (uint16_t)f32_to_bf16_bits(fabsf(rounded) < INFINITY ? v - rounded : 0.f);
     };
     if constexpr (TOGETHER) {
 #pragma unroll
@@ -538,18 +564,19 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) m
   }
 }
 
-// A block per 32 rows of y and part of the columns of all entries, laid one behind the other; its waves share those.  Parts leave their sums in the workspace, past the
+// A block per 32 rows of y and part of the columns of all entries, laid one behind the other; its waves share those.  A pair is two of an MFMA's 16 tokens, the two parts of
+// its hidden values: as many MFMAs as with one part, for up to kMoeDownPairs pairs.  Codes are exact in bf16, dense fp16 weights are taken apart.  Parts leave their sums in the workspace, past the
 // L2 (agent scope), and the last of a row tile's blocks to do so adds them in their order.
 template <int ACT, int FMT, bool ASYM, int GROUP>
 __global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const MoeArgs a, int cap, int own_lds) {
-  using Walk = MoeWalk<ACT, FMT, ASYM, 2, GROUP>;
+  using Walk = MoeWalk<NPAMD_BF16, FMT, ASYM, 2, GROUP, ACT>;
   using S = typename Walk::S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int x_bytes = S::x_loads(cap) * 1024;
+  const int x_loads = S::x_loads(2 * cap), x_bytes = x_loads * 1024;
   const MoeRoute route(lds + own_lds, a.M * a.top_k, waves, lds);
   uint8_t* const tokens = lds + waves * 2 * Walk::kPlace;
-  Walk walk(lds + wave * 2 * Walk::kPlace, tokens + wave * 2 * x_bytes, S::x_loads(cap), a.I, a.shift, 0, 1);
+  Walk walk(lds + wave * 2 * Walk::kPlace, tokens + wave * 2 * x_bytes, x_loads, a.I, a.shift, 0, 1);
   float* const sums = reinterpret_cast<float*>(tokens + waves * 2 * x_bytes);  // [wave][M][32]
   for (int p = threadIdx.x; p < a.M * a.top_k; p += blockDim.x) route.ids[p] = a.ids[p], route.entries[p] = a.entries[p];  // those behind the last: never looked at
   if (threadIdx.x == 0) *route.n_entries = (int)a.entries[a.M * a.top_k];
@@ -574,7 +601,7 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const Mo
       const int64_t row = (int64_t)(entry & 0xFFFF) * a.H + n0;
       walk.rows(0, a.down, a.down_scale, a.down_zero, row);
       walk.rows(1, a.down, a.down_scale, a.down_zero, row + 16);
-      walk.tokens(a.h, list, n, 1);
+      walk.tokens(a.h, 2 * n, [&](int j) { return (int)list[j >> 1] * 2 + (j & 1); });
     }
     walk.load(ahead_step, place);
     if (++ahead_step == steps) {
@@ -590,20 +617,20 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const Mo
     const int count = __builtin_amdgcn_readfirstlane(route.counts[wave * 2 + slot]);
     Walk::arrived();
     request(place ^ 1);
-    walk.multiply(step, place, count);
+    walk.multiply(step, place, 2 * count);
     place ^= 1;
     if (++step != steps && i != last - 1) continue;
     // the entry's tokens, each times its share: a token's place is written by one lane
     step = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = 4 * (lane >> 4) + e;
+    for (int e = 0; e < 2; ++e) {
+      const int j = 2 * (lane >> 4) + e;
       if (j < count) {
         const int pair = route.lists[(wave * 2 + slot) * 16 + j];
         const float share = a.share[pair];
         float* const to = mine + pair / a.top_k * 32 + (lane & 15);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) to[16 * r] = __builtin_fmaf(share, walk.acc[r][e], to[16 * r]);
+        for (int r = 0; r < 2; ++r) to[16 * r] = __builtin_fmaf(share, walk.acc[r][2 * e] + walk.acc[r][2 * e + 1], to[16 * r]);
       }
     }
     slot ^= 1;
@@ -651,7 +678,7 @@ struct MoeSpace {
     share = take((int64_t)M * top_k * 4);
     entries = take(((int64_t)M * top_k + 1) * 4);
     xs = take((int64_t)M * H * 2);
-    h = take((int64_t)M * top_k * I * 2);
+    h = take((int64_t)M * top_k * 2 * I * 2);
     done = take((int64_t)H / 32 * 4);
     parts = take((int64_t)moe_max_parts(H) * M * H * 4);
     bytes = at;
@@ -663,7 +690,7 @@ struct MoeSpace {
 // blocks split the columns (one part / two: int4 one token 57 / 50; hidden size 256, inner 13440, 14 experts, one / eight / 16 / 32 parts 186 / 51 / 43 / 44; 384 and 1152, 12
 // experts 30 / 24 / 26 / 28).  From entries of five pairs on the up kernel's waves share them: 16 tokens int4 271 / 219, one token 54 / 57; unless that leaves compute units
 // without a block (19 tokens through four of four, 3840 x 768 42 / 35).
-constexpr int kMoeUpWaves = 4, kMoeDownWaves = 8, kMoeTogether = 5, kMoeWavesPerCu = 16;
+constexpr int kMoeUpWaves = 4, kMoeDownWaves = 8, kMoeTogether = 5, kMoeWavesPerCu = 16, kMoeDownPairs = 8;
 
 template <int ACT, int FMT, bool ASYM, int GROUP>
 int launch_moe_format(const MoeArgs& a, hipStream_t st) {
@@ -674,10 +701,11 @@ int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   // (us with 16 / eight: 16 tokens int4 through two of eight 190 / 183, through eight of 64 88 / 70, 32 tokens through two of eight 199 / 231); four where it has one, of int8,
   // whose steps are the largest, two (eight of 64 experts, hidden size 2048, with eight / four / two: eight tokens dense 129 / 112 / 112, seven int8 70 / 73 / 65).
   const int pairs = a.M * a.top_k, cap = std::min(a.M, pairs <= a.E ? (FMT == 8 ? 2 : 4) : pairs <= 4 * a.E ? 8 : 16), x_bytes = 2 * S::x_loads(cap) * 1024;
+  const int down_cap = std::min(cap, kMoeDownPairs), down_x_bytes = 2 * S::x_loads(2 * down_cap) * 1024;
   const int most_entries = std::min(pairs, a.E + pairs / cap);
   const bool together = cap >= kMoeTogether && (int64_t)most_entries * (a.I / 16 / kMoeUpWaves) >= kMoeBlocks;
   auto up_own = [&](int waves) { return waves * 4 * S::kItem + (together ? x_bytes : waves * (x_bytes + cap * kMoeRedRow * 4)); };
-  auto down_own = [&](int waves) { return waves * (x_bytes + 4 * S::kItem + a.M * 32 * 4); };
+  auto down_own = [&](int waves) { return waves * (down_x_bytes + 4 * S::kItem + a.M * 32 * 4); };
   const int up_steps = (a.H + S::kColumns - 1) / S::kColumns;
   auto idle = [&](int waves) { return (float)((up_steps + waves - 1) / waves * waves) / (float)up_steps; };
   const int up_waves = together ? kMoeUpWaves : up_steps < kMoeUpWaves ? up_steps : idle(3) * 1.1f < idle(kMoeUpWaves) ? 3 : kMoeUpWaves;
@@ -694,14 +722,14 @@ int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   else launch(moe_logits_kernel<ACT, 4, FMT == 4>, dim3(a.E, (a.M + 3) / 4), 256, 0, st, a);
   const int64_t items = (int64_t)most_entries * (a.I / 16 / (together ? up_waves : 1));  // no more than that
   const int per_cu = std::max(1, std::min(kMoeWavesPerCu / up_waves, kRoom / up_lds));
-  launch(up, (unsigned)std::min<int64_t>(items, kMoeBlocks * per_cu), 64 * up_waves, up_lds, st, a, cap, up_own(up_waves));
+  launch(up, (unsigned)std::min<int64_t>(items, kMoeBlocks * per_cu), 64 * up_waves, up_lds, st, a, cap, down_cap, up_own(up_waves));
   // Parts of the columns: a wave's steps, 2 us each, against 0.4 us for each part that meets the others.
   const int down_steps = std::min(pairs, a.E) * ((a.I + S::kColumns - 1) / S::kColumns);  // if every expert that can be met is
   auto down_cost = [&](int n) { return 5 * ((down_steps + n * down_waves - 1) / (n * down_waves)) + n; };
   int parts = 1;
   for (int n = 2; n <= moe_max_parts(a.H); ++n)
     if (down_cost(n) < down_cost(parts)) parts = n;
-  launch(down, dim3(a.H / 32, parts), 64 * down_waves, down_lds, st, a, cap, down_own(down_waves));
+  launch(down, dim3(a.H / 32, parts), 64 * down_waves, down_lds, st, a, down_cap, down_own(down_waves));
   return check_launch(what);
 }
 

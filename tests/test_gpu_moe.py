@@ -285,3 +285,62 @@ def test_routing(gpu, e, top_k):
     bad[e - 1, 5] = float("nan")  # this expert's logit is NaN whatever x holds: it is met first and every share is NaN
     y = kernels.moe_layer(x.to(gpu), kernels.MoEExperts(bad.to(gpu), gate_up.to(gpu), down.to(gpu)), top_k)
     assert bool(y.isnan().all(0)[(e - 1) % 64])
+
+
+def _single_products(m, e, dtype, nbits, zero):
+    """One expert takes all tokens; token t has one value that is not zero, in column t, and row t of the expert's gate and up rows meets nothing else: y[t, n] is one
+    product of a weight and silu(gate) * up."""
+    h = i = 64
+    g = cases.gen(m + nbits + e)
+    rand = lambda *s: torch.rand(*s, generator=g)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g) * 2 - 1
+    x = torch.zeros(m, h, dtype=dtype)
+    x[torch.arange(m), torch.arange(m)] = ((rand(m) + 0.5) * sign(m)).to(dtype)
+    layer, dense = {"router": torch.zeros(e, h, dtype=dtype), "nbits": nbits, "group_size": 32}, {}
+    for name, rows, cols in (("gate_up", 2 * i, h), ("down", h, i)):
+        full = torch.ones(e, rows, cols, dtype=torch.bool) if name == "down" else (torch.arange(rows)[:, None] % i == torch.arange(cols)).expand(e, rows, cols)
+        if nbits == 16:
+            layer[name] = (torch.where(full, (rand(e, rows, cols) + 0.5) * sign(e, rows, cols), 0.0)).to(dtype)
+            dense[name] = layer[name].double()
+            continue
+        half = 1 << (nbits - 1)
+        codes = torch.where(full, half + sign(e, rows, cols) * torch.randint(half // 2, half, (e, rows, cols), generator=g), half).to(torch.uint8)
+        layer[name] = BitPacking(nbits).compress(codes.reshape(e * rows, cols)).reshape(e, rows, -1)
+        s = layer[name + "_scale"] = ((rand(e, rows, cols // 32) + 0.5) / half).half()
+        if zero:
+            layer[name + "_zero"] = torch.full_like(s, half)
+        dense[name] = (codes.double() - half) * s.double().repeat_interleave(32, -1)
+    return x, layer, dense
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nbits,zero", [(16, False), (4, False), (4, True), (8, False), (8, True)])
+@pytest.mark.parametrize("m,e", [(1, 1), (3, 8), (5, 1), (9, 2), (32, 1), (32, 8)])
+def test_the_hidden_values_are_not_rounded_to_sixteen_bits(gpu, dtype, nbits, zero, m, e):
+    """y is rounded once.  What else there is: 2^-17 of the hidden values' two parts, 2^-20 of SiLU, and f32 sums of codes with an offset of up to 1032 on values of at
+    least four, 2^-24 1032 / 4 = 2^-16 each for gate, up and down: 2^-13 is more than all of it."""
+    from neuropress_amd import kernels
+
+    x, layer, dense = _single_products(m, e, dtype, nbits, zero)
+    both = x.double() @ dense["gate_up"][0].T
+    ref = (torch.nn.functional.silu(both[:, :64]) * both[:, 64:]) @ dense["down"][0].T
+    y = kernels.moe_layer(x.to(gpu), _experts(layer), 1).double().cpu()
+    assert bool(((y - ref).abs() <= ref.abs() * (torch.finfo(dtype).eps / 2 * 1.0001 + 2.0**-13) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all())
+
+
+@pytest.mark.parametrize("nbits,group,zero", FORMATS)
+@pytest.mark.parametrize("m,e,top_k", [(1, 8, 2), (7, 8, 3), (32, 4, 2)])
+def test_hidden_values_past_the_range_of_fp16(gpu, nbits, group, zero, m, e, top_k):
+    """silu(gate) * up past 65504 where y is not."""
+    from neuropress_amd import kernels
+
+    layer, dense = _layer(m + nbits, e, 256, 384, torch.float16, nbits, group, zero)
+    layer["gate_up" if nbits == 16 else "gate_up_scale"] *= 128  # exact
+    dense["gate_up"] = dense["gate_up"] * 128
+    x = torch.randn(m, 256, generator=cases.gen(m)).half()
+    both = torch.einsum("erc,mc->emr", dense["gate_up"], x.double())
+    assert (torch.nn.functional.silu(both[..., :384]) * both[..., 384:]).abs().max() > 65504
+    ref, tol = _reference(x, layer, dense, top_k, True)
+    y, inside = kernels.moe_layer(x.to(gpu), _experts(layer), top_k).cpu(), ref.abs() + tol < 65504  # a few results are past it themselves
+    assert inside.double().mean() > 0.99 and not y.isnan().any()
+    _check(y[inside], ref[inside], tol[inside], torch.float16)
