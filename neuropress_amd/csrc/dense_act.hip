@@ -32,8 +32,8 @@ __device__ __forceinline__ void finish(const FewArgs& a, int m, int n, float v) 
 }
 
 // R rows of W and TB tokens to a wave, KS of a block's four waves to a row, U pieces of each row on their way; tokens past TB in further blocks.  Any K and any
-// addresses: a row that does not end with a piece of eight has its last one end with the row, and the values that the piece before has too are zeroed in x.  x comes from
-// the L1.  4096 x 14336, one token: 22.1 us, 5.3 TB/s, the rate of reads; 640 x 2048 2.9 us.
+// addresses: a row that does not end with a piece of eight has its last one end with the row, and the values that the piece before has too are zeroed in both
+// (an infinite one times zero would be NaN).  x comes from the L1.  4096 x 14336, one token: 22.1 us, 5.3 TB/s, the rate of reads; 640 x 2048 2.9 us.
 template <int ACT, int R, int TB, int KS, int U>
 __global__ void __launch_bounds__(256) dense_few_kernel(const FewArgs a) {
   __shared__ float sums[4][R * TB];
@@ -53,15 +53,21 @@ __global__ void __launch_bounds__(256) dense_few_kernel(const FewArgs a) {
   // pieces [first, last) of the part, whole turns of 64 of them dealt out
   const int turns = (pieces + 63) / 64, first = turns * part / KS * 64, last = min(turns * (part + 1) / KS * 64, pieces);
   auto at = [&](int p) { return min(p * 8, a.K - 8); };
-  auto tile = [&](int p, const u32x4 (&wv)[R]) __attribute__((always_inline)) {
+  auto blank = [&](u32x4& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < tail) v[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+  };
+  auto tile = [&](int p, u32x4 (&wv)[R]) __attribute__((always_inline)) {
+    const bool ends = p == pieces - 1 && tail;
+    if (ends) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) blank(wv[r]);
+    }
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
       u32x4 xv = *reinterpret_cast<const u32x4_any*>(xr[t] + at(p));
-      if (p == pieces - 1 && tail) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < tail) xv[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-      }
+      if (ends) blank(xv);
 #pragma unroll
       for (int r = 0; r < R; ++r) acc[r][t] = add_dot8<ACT>(wv[r], xv, acc[r][t]);
     }

@@ -206,3 +206,17 @@ def test_nothing_of_other_rows_reaches_a_result(gpu):
         xs[:m, :200], ws[:n, :200] = x[:m], w[:n]
         xs, ws = xs.to("cuda")[:m, :200], ws.to("cuda")[:n, :200]
         _check(_run(xs, ws, b[:n], "relu", r[:m, :n]), xs, ws, b[:n], "relu", r[:m, :n])
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 17, 32, 40])
+@pytest.mark.parametrize("k", [9, 11, 15, 523])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_values_in_the_columns_that_two_pieces_share(gpu, dtype, m, k):
+    """A row's last piece of eight starts inside the one before; what it has of that counts once, also where it is not finite."""
+    x, w, b, r = _inputs(m, 21, k, dtype)
+    x = x.abs() + 0.5
+    w[3, k // 8 * 8 - 8 + k % 8], w[4, k - 8], w[5, k // 8 * 8 - 1], w[6, k - 1] = float("-inf"), float("inf"), float("-inf"), float("inf")
+    for act in ACTS:
+        y = _run(x, w, b, act, r).cpu()
+        ref = _act(act, x.double() @ w.double().T + b.double()) + r.double()
+        assert torch.equal(y.isnan(), ref.isnan()) and torch.equal(y == float("inf"), ref == float("inf")) and torch.equal(y == float("-inf"), ref == float("-inf")), act
