@@ -70,8 +70,9 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!PyFloat_Check(args[3]) || !PyBool_Check(args[4]) || !rows_argument(args[0], device, &x)) Py_RETURN_NONE;
     const at::ScalarType type = x.t->scalar_type();
     if (!vector_of(args[1], device, type, x.width, &weight) || !vector_of(args[2], device, type, x.width, &bias)) Py_RETURN_NONE;
-    at::Tensor y = empty(x.t->sizes(), type, device), mean, rstd;
     const bool stats = args[4] == Py_True;
+    if (!stats && at::isReducedFloatingType(type) && at::autocast::is_autocast_enabled(at::kCUDA)) Py_RETURN_NONE;  // torch norms in f32 there
+    at::Tensor y = empty(x.t->sizes(), type, device), mean, rstd;
     if (stats) {
       const at::IntArrayRef rows = x.t->sizes().slice(0, x.t->dim() - 1);
       mean = empty(rows, at::kFloat, device);

@@ -1166,20 +1166,22 @@ def _layer_norm(what, x, weight, bias, eps, stats):
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
-    """Layer norm over the last dimension of *x* ``[..., H]`` (``npamd_layer_norm``): *weight* and *bias* ``[H]`` of its dtype or None; the result has x's dtype.
+    """Layer norm over the last dimension of *x* ``[..., H]`` (``npamd_layer_norm``): *weight* and *bias* ``[H]`` of its dtype or None; the result has x's dtype, under autocast
+    float32, as torch's own has.
 
     Where a gradient of x, weight or bias is recorded, the backward pass is :func:`layer_norm_backward`'s kernels (first derivatives).  Captured into a graph it is refused
-    while another graph of the same leaves, made on another stream, is alive (torch would end the process).  Calls that torch follows in other ways (forward mode, ``torch.func``, traces, autocast to another type) go through ``torch.nn.functional.layer_norm``.
+    while another graph of the same leaves, made on another stream, is alive (torch would end the process).  Calls that torch follows in other ways (forward mode, ``torch.func``, traces, 16-bit types under autocast) go through ``torch.nn.functional.layer_norm``.
     """
     out = _lib.host().layer_norm(x, weight, bias, eps, False)
     if out is not None:
         return out
     followed = [t for t in (x, weight, bias) if t is not None and tracked(t)]
-    if not followed:
+    widened = x.dtype in (torch.float16, torch.bfloat16) and torch.is_autocast_enabled("cuda")
+    if not followed and not widened:
         return _layer_norm("layer_norm", x, weight, bias, eps, False)[0]
     _norm_args("layer_norm", x, weight, bias)
     with torch.no_grad():  # what is left of it when no gradient is recorded
-        otherwise = any(tracked(t) for t in followed)
+        otherwise = widened or any(tracked(t) for t in followed)
     if otherwise:
         return torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps)
     _rows_of("layer_norm", x, x.shape[-1])

@@ -381,3 +381,18 @@ def test_what_autograd_hands_to_the_backward_pass(gpu):
     with pytest.raises(RuntimeError, match="at most 2\\*\\*31"):
         kernels.layer_norm(x[:1].expand(1 << 31, 160), w, b, EPS)
     del y
+
+
+@pytest.mark.parametrize("auto", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_autocast_norms_in_float32(gpu, dtype, auto):
+    """Whether its type is the inputs' or not; with and without a recorded gradient.  Two f32 norms of the same values: off by n 2^-24 of a few units each."""
+    from neuropress_amd import kernels
+
+    x, w, b, dy = (t.to(gpu) for t in _inputs(5, 64, dtype))
+    with torch.autocast("cuda", auto):
+        want = torch.nn.functional.layer_norm(x, (64,), w, b, EPS)
+        got = kernels.layer_norm(x, w, b, EPS)
+        recorded = kernels.layer_norm(x.requires_grad_(), w, b, EPS)
+    assert got.dtype == recorded.dtype == want.dtype == torch.float32 and recorded.grad_fn is not None
+    assert torch.allclose(got, want, rtol=1e-5, atol=1e-5) and torch.allclose(recorded, want, rtol=1e-5, atol=1e-5)
