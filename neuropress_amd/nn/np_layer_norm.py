@@ -18,7 +18,8 @@ log = logging.getLogger(__name__)
 
 
 class NPLayerNorm(nn.Module):
-    """``(x - mean) * rstd * weight + bias`` over the last dimension in f32 arithmetic, rounded once to x's dtype; differentiable."""
+    """``(x - mean) * rstd * weight + bias`` over the last dimension in f32 arithmetic, rounded once to x's dtype; differentiable.  Types, and what autocast makes of
+    them, are those of ``nn.LayerNorm``."""
 
     def __init__(self, weight: nn.Parameter | None, bias: nn.Parameter | None, width: int, eps: float = 1e-5, source: nn.Module | None = None) -> None:
         super().__init__()
@@ -37,8 +38,10 @@ class NPLayerNorm(nn.Module):
         return source
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        w, b = (p if p is None or p.dtype == x.dtype else p.to(x.dtype) for p in (self.weight, self.bias))
-        if x.is_cuda:
+        w, b = self.weight, self.bias
+        # Parameters of another type are torch's to decide on, as they were the replaced module's: under autocast it norms in float32 with the
+        # parameters as they are, without it refuses.
+        if x.is_cuda and all(p is None or p.dtype == x.dtype for p in (w, b)):
             from .. import kernels
 
             if x.shape[-1:] != (self.width,):

@@ -396,3 +396,50 @@ def test_autocast_norms_in_float32(gpu, dtype, auto):
         recorded = kernels.layer_norm(x.requires_grad_(), w, b, EPS)
     assert got.dtype == recorded.dtype == want.dtype == torch.float32 and recorded.grad_fn is not None
     assert torch.allclose(got, want, rtol=1e-5, atol=1e-5) and torch.allclose(recorded, want, rtol=1e-5, atol=1e-5)
+
+
+def _lowered(width, dtype):
+    """A module with one norm, and its lowered copy."""
+    import copy
+
+    from neuropress_amd import AutoKernelLowering
+    from neuropress_amd.nn import NPLayerNorm
+
+    torch.manual_seed(1)
+    plain = torch.nn.Sequential(torch.nn.LayerNorm(width))
+    for p in plain.parameters():
+        torch.nn.init.normal_(p)
+    plain = plain.to("cuda", dtype)
+    lowered = copy.deepcopy(plain)
+    AutoKernelLowering(norm_backend="all").apply(lowered)
+    assert type(lowered[0]) is NPLayerNorm
+    return plain, lowered
+
+
+@pytest.mark.parametrize("auto", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_module_under_autocast(gpu, dtype, auto):
+    """Mixed-precision training: float32 parameters, x of any type.  Results, their types and gradients are the replaced module's; both sides norm in f32."""
+    x = _inputs(7, 96, dtype)[0].to(gpu)
+    results = []
+    for model in _lowered(96, torch.float32):
+        leaf = x.clone().requires_grad_()
+        with torch.autocast("cuda", auto):
+            y = model(leaf)
+            with torch.no_grad():
+                silent = model(x)
+        y.float().square().sum().backward()
+        results.append((y, silent, leaf.grad, *(p.grad for p in model.parameters())))
+    for want, got in zip(*results, strict=True):
+        assert got.dtype == want.dtype
+        # gradients in x's type: the same f32 values to a few 2^-24, so another rounding at most
+        eps = torch.finfo(want.dtype).eps
+        assert torch.allclose(got.float(), want.float(), rtol=max(eps, 1e-5), atol=1e-4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_module_refuses_mixed_types_as_the_one_it_replaced(gpu, dtype):
+    x = torch.randn(7, 96, device=gpu).to(dtype)
+    for model in _lowered(96, torch.float32):
+        with pytest.raises(RuntimeError):
+            model(x)
