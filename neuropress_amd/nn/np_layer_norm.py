@@ -16,6 +16,8 @@ __all__ = ["NPLayerNorm", "linearize_layer_norms"]
 
 log = logging.getLogger(__name__)
 
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)  # of the kernels
+
 
 class NPLayerNorm(nn.Module):
     """``(x - mean) * rstd * weight + bias`` over the last dimension in f32 arithmetic, rounded once to x's dtype; differentiable.  Types, and what autocast makes of
@@ -39,9 +41,9 @@ class NPLayerNorm(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         w, b = self.weight, self.bias
-        # Parameters of another type are torch's to decide on, as they were the replaced module's: under autocast it norms in float32 with the
+        # Types that the kernels do not have, and parameters of another type, are torch's to decide on, as they were the replaced module's: under autocast it norms in float32 with the
         # parameters as they are, without it refuses.
-        if x.is_cuda and all(p is None or p.dtype == x.dtype for p in (w, b)):
+        if x.is_cuda and x.dtype in _DTYPES and all(p is None or p.dtype == x.dtype for p in (w, b)):
             from .. import kernels
 
             if x.shape[-1:] != (self.width,):
@@ -53,13 +55,15 @@ class NPLayerNorm(nn.Module):
         return f"H={self.width}, eps={self.eps}, weight={self.weight is not None}, bias={self.bias is not None}"
 
 
-def _on_gpu(module: nn.Module) -> bool:
-    return module.weight is not None and module.weight.device.type == "cuda"
+def _fits(module: nn.Module) -> bool:
+    """Whether the kernels can norm what *module* norms: one dimension, with a weight on a GPU, of a type that they have."""
+    w = module.weight
+    return len(module.normalized_shape) == 1 and w is not None and w.device.type == "cuda" and w.dtype in _DTYPES
 
 
 def linearize_layer_norms(model: nn.Module) -> int:
-    """Replace every ``nn.LayerNorm`` inside *model* that has a weight on a GPU and norms one dimension; returns how many.  Subclasses are left alone: what
-    they override is theirs."""
+    """Replace every ``nn.LayerNorm`` inside *model* that has a weight on a GPU, of a type that the kernels have, and norms one dimension; returns how many.
+    Subclasses are left alone: what they override is theirs."""
     from .backends import is_hip_backend_available
 
     if not is_hip_backend_available():
@@ -67,7 +71,7 @@ def linearize_layer_norms(model: nn.Module) -> int:
         return 0
     fused: dict[int, NPLayerNorm] = {}  # a module that stands in several places is replaced by one
     for name, mod in list(model.named_modules(remove_duplicate=False)):
-        if not name or type(mod) is not nn.LayerNorm or len(mod.normalized_shape) != 1 or not _on_gpu(mod):
+        if not name or type(mod) is not nn.LayerNorm or not _fits(mod):
             continue
         if id(mod) not in fused:
             fused[id(mod)] = NPLayerNorm(mod.weight, mod.bias, mod.normalized_shape[0], mod.eps, source=mod).train(mod.training)

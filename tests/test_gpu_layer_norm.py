@@ -443,3 +443,21 @@ def test_module_refuses_mixed_types_as_the_one_it_replaced(gpu, dtype):
     for model in _lowered(96, torch.float32):
         with pytest.raises(RuntimeError):
             model(x)
+
+
+def test_float64_norms_stay_torchs(gpu):
+    """Left alone by the lowering, and computed as before by a module that is moved to float64 afterwards."""
+    from neuropress_amd import AutoKernelLowering
+
+    x = torch.randn(7, 96, dtype=torch.float64, device=gpu)
+    model = torch.nn.Sequential(torch.nn.LayerNorm(96)).to("cuda", torch.float64)
+    want = model(x)
+    AutoKernelLowering(norm_backend="all").apply(model)
+    assert type(model[0]) is torch.nn.LayerNorm and torch.equal(model(x), want)
+    plain, lowered = _lowered(96, torch.float32)
+    plain.double(), lowered.double()
+    leaves = [x.clone().requires_grad_() for _ in range(2)]
+    ys = [net(leaf) for net, leaf in zip((plain, lowered), leaves)]
+    for y in ys:
+        y.square().sum().backward()
+    assert torch.equal(*ys) and torch.equal(leaves[0].grad, leaves[1].grad)
