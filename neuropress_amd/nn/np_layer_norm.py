@@ -16,6 +16,8 @@ __all__ = ["NPLayerNorm", "linearize_layer_norms"]
 
 log = logging.getLogger(__name__)
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks", "_state_dict_hooks", "_state_dict_pre_hooks",
+          "_load_state_dict_pre_hooks", "_load_state_dict_post_hooks")  # fmt: skip
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)  # of the kernels
 
 
@@ -61,9 +63,15 @@ def _fits(module: nn.Module) -> bool:
     return len(module.normalized_shape) == 1 and w is not None and w.device.type == "cuda" and w.dtype in _DTYPES
 
 
+def _as_made(module: nn.Module) -> bool:
+    """Whether nothing was hung on *module* that its replacement would not have: a hook, a forward of its own, another parameter, buffer or child."""
+    own = vars(module)
+    return not any(own.get(name) for name in _HOOKS) and "forward" not in own and set(own["_parameters"]) <= {"weight", "bias"} and not own["_buffers"] and not own["_modules"]
+
+
 def linearize_layer_norms(model: nn.Module) -> int:
     """Replace every ``nn.LayerNorm`` inside *model* that has a weight on a GPU, of a type that the kernels have, and norms one dimension; returns how many.
-    Subclasses are left alone: what they override is theirs."""
+    Subclasses are left alone: what they override is theirs; so are modules with hooks, which would be lost."""
     from .backends import is_hip_backend_available
 
     if not is_hip_backend_available():
@@ -71,7 +79,7 @@ def linearize_layer_norms(model: nn.Module) -> int:
         return 0
     fused: dict[int, NPLayerNorm] = {}  # a module that stands in several places is replaced by one
     for name, mod in list(model.named_modules(remove_duplicate=False)):
-        if not name or type(mod) is not nn.LayerNorm or not _fits(mod):
+        if not name or type(mod) is not nn.LayerNorm or not _fits(mod) or not _as_made(mod):
             continue
         if id(mod) not in fused:
             fused[id(mod)] = NPLayerNorm(mod.weight, mod.bias, mod.normalized_shape[0], mod.eps, source=mod).train(mod.training)

@@ -461,3 +461,22 @@ def test_float64_norms_stay_torchs(gpu):
     for y in ys:
         y.square().sum().backward()
     assert torch.equal(*ys) and torch.equal(leaves[0].grad, leaves[1].grad)
+
+
+@pytest.mark.parametrize("kind", ["forward_hook", "forward_pre_hook", "full_backward_hook", "full_backward_pre_hook", "state_dict_post_hook", "load_state_dict_post_hook", "forward"])
+def test_norms_with_hooks_are_left_alone(gpu, kind):
+    from neuropress_amd import AutoKernelLowering
+    from neuropress_amd.nn import NPLayerNorm
+
+    model = torch.nn.Sequential(torch.nn.LayerNorm(64), torch.nn.LayerNorm(64)).to(gpu)
+    seen = []
+    if kind == "forward":
+        forward = model[0].forward
+        model[0].forward = lambda x: seen.append(kind) or forward(x)
+    else:
+        getattr(model[0], "register_" + kind)(lambda *args: seen.append(kind))
+    AutoKernelLowering(norm_backend="all").apply(model)
+    assert type(model[0]) is torch.nn.LayerNorm and type(model[1]) is NPLayerNorm
+    model(torch.randn(3, 64, device=gpu, requires_grad=True)).sum().backward()
+    model.load_state_dict(model.state_dict())
+    assert seen
