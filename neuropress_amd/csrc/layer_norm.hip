@@ -290,7 +290,6 @@ layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, void
 #pragma unroll
     for (int i = 0; i < NV; ++i) xc[i] = xv[i], dc[i] = dv[i];
     request(row + step);
-    const float shift = -mean * rstd;  // (x - mean) rstd, rounded once: it is off by 2^-24 mean rstd, as it is by the mean's own rounding
     float s1 = 0.f, s2 = 0.f, xh[NV][V], g[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -308,7 +307,7 @@ layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, void
       };
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        xh[i][e] = __builtin_fmaf(xh[i][e], rstd, shift);
+        xh[i][e] = (xh[i][e] - mean) * rstd;
         g[i][e] = a.w ? d[e] * wf[e] : d[e];
       }
       if (p * V + V <= a.H) {
@@ -345,7 +344,7 @@ layer_norm_back_kernel(const LayerNormBack a, float* __restrict__ partials, void
         P::unpack(wv[i], wf);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          xh[i][e] = __builtin_fmaf(xh[i][e], rstd, shift);
+          xh[i][e] = (xh[i][e] - mean) * rstd;
           if (a.w) g[i][e] *= wf[e];
         }
       }

@@ -480,3 +480,19 @@ def test_norms_with_hooks_are_left_alone(gpu, kind):
     model(torch.randn(3, 64, device=gpu, requires_grad=True)).sum().backward()
     model.load_state_dict(model.state_dict())
     assert seen
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,h", [(5, 64), (40, 1000), (3, 8192), (300, 512), (5, 12288), (2, 5), (3, 40000)])
+def test_gradients_of_constant_rows(gpu, dtype, m, h):
+    """x - mean is exactly zero there, whatever kernel takes the row: the weight's gradient is zero, and that of x is what the mean of dy * weight leaves."""
+    from neuropress_amd import kernels
+
+    x = (torch.arange(m) * 7 + 99.0)[:, None].expand(m, h).to(dtype)
+    _, w, _, dy = _inputs(m, h, dtype)
+    mean, rstd = x[:, 0].float(), torch.full((m,), EPS).rsqrt()
+    dx, dw, db = kernels.layer_norm_backward(dy.to(gpu), x.to(gpu), w.to(gpu), mean.to(gpu), rstd.to(gpu))
+    assert not dw.any()
+    refs = _reference_back(dy, x, w, mean, rstd)
+    for got, (ref, slack), what in zip((dx, db), (refs[0], refs[2]), ("dx", "db")):
+        _check(got, ref, slack, dtype, what)
