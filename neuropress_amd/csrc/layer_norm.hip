@@ -216,25 +216,26 @@ layer_norm_back_block_kernel(const LayerNormBack a) {
   }
 }
 
-// And sums over strips of rows for the gradients of weight and bias: partials [parts][2][H], a lane per column.
+// And sums over strips of rows for the gradients of weight and bias: partials [parts][2][H], a lane per column.  A strip may have any number of rows: in f64, so that
+// the error does not grow with them.
 template <int DT>
 __global__ void __launch_bounds__(256)
 layer_norm_back_columns_kernel(const LayerNormBack a, float* __restrict__ partials, int parts) {
-  __shared__ float sums[4][2][64];
+  __shared__ double sums[4][2][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
   const int first = (int)((int64_t)a.M * blockIdx.y / parts), last = (int)((int64_t)a.M * (blockIdx.y + 1) / parts);
-  float dw = 0.f, db = 0.f;
+  double dw = 0., db = 0.;
   if (col < a.H)
     for (int64_t row = first + wave; row < last; row += 4) {
       const float d = load_as_f32<DT>(a.dy, row * a.lddy + col);
-      dw = __builtin_fmaf(d, (load_as_f32<DT>(a.x, row * a.ldx + col) - a.mean[row]) * a.rstd[row], dw);
-      db += d;
+      dw = __builtin_fma((double)d, (double)((load_as_f32<DT>(a.x, row * a.ldx + col) - a.mean[row]) * a.rstd[row]), dw);
+      db += (double)d;
     }
   sums[wave][0][lane] = dw;
   sums[wave][1][lane] = db;
   __syncthreads();
   if (wave < 2 && col < a.H)
-    partials[((int64_t)blockIdx.y * 2 + wave) * a.H + col] = sums[0][wave][lane] + sums[1][wave][lane] + sums[2][wave][lane] + sums[3][wave][lane];
+    partials[((int64_t)blockIdx.y * 2 + wave) * a.H + col] = (float)(sums[0][wave][lane] + sums[1][wave][lane] + sums[2][wave][lane] + sums[3][wave][lane]);
 }
 
 constexpr int kManyGroups = 8;
@@ -463,7 +464,8 @@ struct BackPlan {
   BackPlan(int M, int H, int dtype) {
     const int V = dtype == NPAMD_F32 ? 4 : 8, pieces = (H + V - 1) / V;
     if (H < V || pieces > 64 * 16 * 2) {
-      parts = (int)std::min<int64_t>(64, ((int64_t)M + 63) / 64);
+      // strips of 64 rows, 1024 of them where their sums are small (64 / 1024: 2^20 x 2 f32 1336 / 726 us, 100000 x 5 fp16 146 / 89, dx among them)
+      parts = (int)std::min<int64_t>(std::clamp<int64_t>(kMaxSums / (8 * (int64_t)H), 64, 1024), ((int64_t)M + 63) / 64);
       return;
     }
     nv = pieces <= 1024 ? 1 : 2;

@@ -496,3 +496,20 @@ def test_gradients_of_constant_rows(gpu, dtype, m, h):
     refs = _reference_back(dy, x, w, mean, rstd)
     for got, (ref, slack), what in zip((dx, db), (refs[0], refs[2]), ("dx", "db")):
         _check(got, ref, slack, dtype, what)
+
+
+@pytest.mark.parametrize("h", [2, 3, 8])
+def test_sums_over_very_many_rows(gpu, h):
+    """Equal addends, whose roundings in a long f32 chain all go the same way.  Short rows: strips in f64, rounded once, then up to 64 + 16 of them in f32.  Others: a chain
+    of M / 4096 rows for each of 256 blocks' 16 groups."""
+    from neuropress_amd import kernels
+
+    m = (1 << 24) + 5
+    x = torch.zeros(m, h, device=gpu)
+    x[:, ::2] = 1.0
+    dy = torch.full((m, h), 1.001, device=gpu)
+    mean, rstd = torch.full((m,), 0.5, device=gpu), torch.full((m,), 2.0, device=gpu)  # (x - mean) * rstd is 1 and -1
+    _, dw, db = kernels.layer_norm_backward(dy, x, None, mean, rstd, needs=(False, True, True))
+    want = m * dy[0, 0].double()
+    off = EPS32 * (100 + (m / 4096 if h >= 4 else 0)) * want
+    assert bool(((db.double() - want).abs() <= off).all()) and bool(((dw[::2].double() - want).abs() <= off).all()) and bool(((dw[1::2].double() + want).abs() <= off).all())
