@@ -1321,6 +1321,8 @@ class MoEExperts:
             raise RuntimeError(f"{what}: router must be float16 or bfloat16 [E, H], gate_up [E, 2 I, H] and down [E, H, I]")
         e, h = router.shape
         i = gate_up.shape[1] // 2
+        if min(e, h, i) < 1:
+            raise RuntimeError(f"{what}: at least one expert, column and row, got E={e}, H={h}, I={i}")
         if nbits != 16 and group_size < 1:
             raise RuntimeError(f"{what}: group_size must be positive, got {group_size}")
         dtype = router.dtype if nbits == 16 else torch.uint8

@@ -344,3 +344,11 @@ def test_hidden_values_past_the_range_of_fp16(gpu, nbits, group, zero, m, e, top
     y, inside = kernels.moe_layer(x.to(gpu), _experts(layer), top_k).cpu(), ref.abs() + tol < 65504  # a few results are past it themselves
     assert inside.double().mean() > 0.99 and not y.isnan().any()
     _check(y[inside], ref[inside], tol[inside], torch.float16)
+
+
+@pytest.mark.parametrize("e,h,i", [(0, 64, 64), (2, 0, 64), (2, 64, 0)])
+def test_experts_of_no_size_are_refused(gpu, e, h, i):
+    from neuropress_amd import kernels
+
+    with pytest.raises(RuntimeError, match="at least one expert"):
+        kernels.MoEExperts(*(torch.zeros(*s, device=gpu).half() for s in ((e, h), (e, 2 * i, h), (e, h, i))))
