@@ -6,7 +6,7 @@
 //
 // Three launches: the logits (a block per expert), up (every block first picks each token's experts from the logits, then walks (expert, 16 gate rows and their
 // 16 up rows)), down (a block per 32 rows of y and part of all their experts' columns).  The experts' weights are all that counts: each byte is read once for up to 16
-// of an expert's tokens, which share it as the columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 4.8, 29.7 and 19.4 us by
+// of an expert's tokens (eight in the down kernel), which share it as the columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 4.8, 29.7 and 19.4 us by
 // themselves, 49 in a row, 4.0 TB/s of 198 MB; 16 tokens fp16 with zero points 181-183 us, 4.0 TB/s.  Bound by HBM inside the walks, by round trips in front of and behind them.
 //
 // Codes: an MFMA 16x16x32 sees 32 columns of one scale group, so a group's scale multiplies the f32 sum behind it, four multiply-adds for 512 weights, instead of the
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, 4) moe_down_kernel(const Mo
   }
 }
 
-// The down kernel's blocks, a row tile's parts times its row tiles: no more than compute units.
+// The down kernel's blocks: the columns are parted while all row tiles' parts are no more than compute units (row tiles alone may be).
 constexpr int kMoeBlocks = 256;
 int moe_max_parts(int H) { return std::max(1, kMoeBlocks / std::max(1, H / 32)); }
 
@@ -699,9 +699,14 @@ int launch_moe_format(const MoeArgs& a, hipStream_t st) {
   constexpr int kRoom = 160 * 1024;
   // Pairs of an entry: their places in LDS keep blocks out, an expert that has more pairs is read again.  All that an MFMA takes; eight where an expert has four at the mean
   // (us with 16 / eight: 16 tokens int4 through two of eight 190 / 183, through eight of 64 88 / 70, 32 tokens through two of eight 199 / 231); four where it has one, of int8,
-  // whose steps are the largest, two (eight of 64 experts, hidden size 2048, with eight / four / two: eight tokens dense 129 / 112 / 112, seven int8 70 / 73 / 65).
+  // whose steps are the largest, two (with eight / four / two / one: eight tokens dense through eight of 64 129 / 112 / 112 / -; int8 through eight of 64, seven 67 / 71 / 64 / 73,
+  // four 54 / 54 / 46 / 49; eight of 128, 12 tokens 92 / 100 / 87 / 98; four of 60, ten 73 / 74 / 67 / 73; one of 32, 32 tokens 138 / 121 / 114 / 140; two of eight 4096 x 14336, four
+  // 201 / 201 / 203 / 230; with zero points eight of 128, 16 tokens 127 / 127 / 130 / 159).
   const int pairs = a.M * a.top_k, cap = std::min(a.M, pairs <= a.E ? (FMT == 8 ? 2 : 4) : pairs <= 4 * a.E ? 8 : 16), x_bytes = 2 * S::x_loads(cap) * 1024;
-  const int down_cap = std::min(cap, kMoeDownPairs), down_x_bytes = 2 * S::x_loads(2 * down_cap) * 1024;
+  // The down kernel's, whose pairs are two tokens each: eight, four up to a mean of two (us with four / eight: 16 tokens int4 through eight of 64 65 / 71, 24 through four of 60
+  // 80 / 86, 20 through three of 32 106 / 112; 16 int8 through eight of 64 95 / 94, eight dense through four of 16 89 / 90; but at four 16 tokens int4 through two of
+  // eight 197 / 186, 32 int8 through eight of 64 135 / 126, 32 dense through four of 16 137 / 117).
+  const int down_cap = std::min(cap, pairs <= 2 * a.E ? 4 : kMoeDownPairs), down_x_bytes = 2 * S::x_loads(2 * down_cap) * 1024;
   const int most_entries = std::min(pairs, a.E + pairs / cap);
   const bool together = cap >= kMoeTogether && (int64_t)most_entries * (a.I / 16 / kMoeUpWaves) >= kMoeBlocks;
   auto up_own = [&](int waves) { return waves * 4 * S::kItem + (together ? x_bytes : waves * (x_bytes + cap * kMoeRedRow * 4)); };
