@@ -1,5 +1,5 @@
-// Activations of the epilogues, in f32: to 2^-20 of their argument.  None is infinite or NaN where its limit is not; those of minus infinity are NaN, as a product of
-// it and zero.
+// Activations of the epilogues, in f32: to 2^-20 of their argument.  None is infinite or NaN at a finite argument whose activation is not; those of minus infinity but
+// ReLU's are NaN, as a product of it and zero.
 #pragma once
 
 #include "common.hpp"
@@ -9,7 +9,8 @@ namespace npamd {
 __device__ __forceinline__ float silu_f32(float v) { return v * __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 // v Phi(v), Phi by erfc: exp(z^2) erfc(z) / 2, z = |v| / sqrt(2), is a polynomial in t = 1 / (1 + 0.51 z) without a constant term, to 9e-7 relative (fitted up to z = 10,
-// past which exp(-z^2) is zero).
+// past which exp(-z^2) is zero).  GELU itself is off by up to 7e-6 relative where it is small, far below zero (5e-6 from
+// -9 on, 2e-6 from -6): the exponent is rounded, 2^-24 of some v^2.
 __device__ __forceinline__ float gelu_f32(float v) {
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.51f * 0.70710678f, fabsf(v), 1.f));
   float q = 0.047250088304281235f;
