@@ -542,7 +542,7 @@ int64_t npamd_dense_gemm_act_workspace_bytes(int M, int N, int K);
  * x, router [E, H], y: act_dtype (NPAMD_F16 or NPAMD_BF16).  gate_up: [E, 2 I, H], an expert's I gate rows before its I up rows;
  * down: [E, H, I].  nbits 16: dense, act_dtype.  nbits 4 / 8: codes packed as for npamd_q_gemv, w = (q - zero) * scale, scale f16
  * [E, rows, K / group_size], zero f16 of the same shape or NULL (2^(nbits - 1)).  f32 accumulate; w is not rounded, silu(gate) * up is
- * held to 2^-17 in the range of f32, y is rounded once.
+ * held to 2^-16 in the range of f32 (past it codes make the token's row NaN), y is rounded once.
  * H and I multiples of 64, at most 2^20, group_size a power of two from 32 on that divides both, E <= 512, top_k <= 16, 16-byte aligned
  * router and weights, 4-byte aligned scales and zero points; others are NPAMD_ERR_UNSUPPORTED or NPAMD_ERR_INVALID.
  * workspace: npamd_moe_workspace_bytes bytes of 16-byte aligned device memory, contents irrelevant before and after; calls that

@@ -2,7 +2,7 @@
 //   logits = x router^T,  p = softmax(logits) over all experts,  the top_k largest (ties to the lower index), divided by their sum on request
 //   y = sum over them of p_e down_e(silu(gate_e(x)) * up_e(x))
 // Expert weights are dense or group-quantized codes, w = (q - zero) scale, which is not rounded.  Sums and p stay in f32 up to the store of y.  silu(gate) * up, the operand
-// of the second product, is kept as the sum of two bf16: to 2^-17, in the range of f32 whatever the activations' type (in fp16 it would be infinite past 65504).
+// of the second product, is kept as the sum of two bf16: to 2^-16, in the range of f32 whatever the activations' type (in fp16 it would be infinite past 65504).
 //
 // Three launches: the logits (a block per expert), up (every block first picks each token's experts from the logits, then walks (expert, 16 gate rows and their
 // 16 up rows)), down (a block per 32 rows of y and part of all their experts' columns).  The experts' weights are all that counts: each byte is read once for up to 16
@@ -42,7 +42,7 @@ struct MoeArgs {
   uint32_t* done;  // [H / 32] blocks of the down kernel that have left their part
   float* parts;    // [part][H / 32][M * 32]
   uint16_t* xs;    // [M][H], rows as the up kernel reads them
-  uint16_t* h;     // [M][top_k][2][I], bf16: silu(gate) * up, and what its rounding leaves
+  uint16_t* h;     // [M][top_k][2][I], bf16: silu(gate) * up, and what is left of it
 };
 
 // int4 operands hold the columns of an octet in the order 0 4 1 5 2 6 3 7 (the nibbles 4 i and 4 i + 16 of a dword are a pair): where column k of it lies.
@@ -362,7 +362,8 @@ struct MoeWalk {
     }
   }
   static __device__ __forceinline__ u32x4 ones() { return ACT == NPAMD_F16 ? constant(0x3C003C00u, 0x3C003C00u) : constant(0x3F803F80u, 0x3F803F80u); }
-  // Dense fp16 weights as sums of two bf16, exactly: eight and three bits.  An infinite one's second part is finite.
+  // Dense fp16 weights as sums of two bf16, exactly: eight and three bits.  Both parts have the weight's sign and neither is zero where it is not (2^-100 of it is lost in any
+  // other second part), so that what meets an infinite hidden value is not NaN; an infinite weight's second part is finite.
   static __device__ __forceinline__ void split_f16(const uint32_t (&v)[S::kWords], u32x4* first, u32x4* second) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -371,7 +372,7 @@ struct MoeWalk {
       for (int e = 0; e < 2; ++e) {
         const float w = f16_bits_to_f32((v[i] >> (16 * e)) & 0xFFFFu), finite = __builtin_amdgcn_fmed3f(w, -65504.f, 65504.f);
         part[e] = __builtin_bit_cast(uint32_t, w);
-        rest[e] = __builtin_bit_cast(uint32_t, finite - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, finite) & 0xFFFF0000u));
+        rest[e] = __builtin_bit_cast(uint32_t, __builtin_fmaf(finite, 0x1p-100f, finite - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, finite) & 0xFFFF0000u)));
       }
       (*first)[i] = __builtin_amdgcn_perm(part[1], part[0], 0x07060302u);
       (*second)[i] = __builtin_amdgcn_perm(rest[1], rest[0], 0x07060302u);
@@ -528,12 +529,13 @@ __global__ void __launch_bounds__(64 * kMoeMaxWaves, FMT == 8 && ASYM ? 3 : 4) m
     const int tile = item % tiles;
     auto store = [&](int j, int k, float gate, float up) __attribute__((always_inline)) {
       const int to = FMT == 4 ? (k & ~7) | octet_place(k & 7) : k;
+      // Cut, not rounded: both parts have the value's sign, and neither is zero where it is not, so that an infinite weight makes no NaN of them.
       const float v = silu_f32(gate) * up;
-      const uint32_t bits = f32_to_bf16_bits(v);
-      const float rounded = bf16_bits_to_f32(bits);
+      const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+      const float rest = fabsf(v) < INFINITY ? v - __builtin_bit_cast(float, bits & 0xFFFF0000u) : 0.f;
       uint16_t* const at = a.h + (int64_t)list[j] * 2 * a.I + to;
-      at[0] = (uint16_t)bits;
-      at[a.I] = (uint16_t)f32_to_bf16_bits(fabsf(rounded) < INFINITY ? v - rounded : 0.f);
+      at[0] = (uint16_t)(bits >> 16);
+      at[a.I] = (uint16_t)f32_to_bf16_bits(v != 0.f ? copysignf(fmaxf(fabsf(rest), 0x1p-126f), v) : 0.f);
     };
     if constexpr (TOGETHER) {
 #pragma unroll

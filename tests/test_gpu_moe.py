@@ -317,7 +317,7 @@ def _single_products(m, e, dtype, nbits, zero):
 @pytest.mark.parametrize("nbits,zero", [(16, False), (4, False), (4, True), (8, False), (8, True)])
 @pytest.mark.parametrize("m,e", [(1, 1), (3, 8), (5, 1), (9, 2), (32, 1), (32, 8)])
 def test_the_hidden_values_are_not_rounded_to_sixteen_bits(gpu, dtype, nbits, zero, m, e):
-    """y is rounded once.  What else there is: 2^-17 of the hidden values' two parts, 2^-20 of SiLU, and f32 sums of codes with an offset of up to 1032 on values of at
+    """y is rounded once.  What else there is: 2^-16 of the hidden values' two parts, 2^-20 of SiLU, and f32 sums of codes with an offset of up to 1032 on values of at
     least four, 2^-24 1032 / 4 = 2^-16 each for gate, up and down: 2^-13 is more than all of it."""
     from neuropress_amd import kernels
 
@@ -352,3 +352,32 @@ def test_experts_of_no_size_are_refused(gpu, e, h, i):
 
     with pytest.raises(RuntimeError, match="at least one expert"):
         kernels.MoEExperts(*(torch.zeros(*s, device=gpu).half() for s in ((e, h), (e, 2 * i, h), (e, h, i))))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["weight", "hidden"])
+@pytest.mark.parametrize("m,top_k", [(1, 1), (5, 2), (32, 3)])
+def test_infinite_weights_and_hidden_values(gpu, dtype, kind, m, top_k):
+    """Dense experts: an infinite weight of the down-projection leaves an infinity of the product's sign, and so do weights that meet an infinite hidden value."""
+    from neuropress_amd import kernels
+
+    layer, _ = _layer(17, 4, 128, 128, dtype, 16)
+    x = torch.randn(m, 128, generator=cases.gen(m)).to(dtype)
+    x[:, 0] = 1.0
+    down, gate_up = layer["down"], layer["gate_up"]
+    down[down == 0] = 1.0
+    if kind == "weight":
+        down[:, 3, 5], down[:, 7, 9], down[:, 64:, 11] = float("inf"), float("-inf"), float("inf")
+    else:
+        gate_up[:, 20] = 0
+        gate_up[:, 20, 0] = float("inf")
+    logits = x.double() @ layer["router"].double().T
+    order = torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    p = torch.softmax(logits, -1).gather(1, order)
+    ref = torch.zeros(m, 128, dtype=torch.float64)
+    for t in range(m):
+        for e, share in zip(order[t], p[t]):
+            gate, up = (gate_up[e].double() @ x[t].double()).chunk(2)
+            ref[t] += share * (down[e].double() @ (torch.nn.functional.silu(gate) * up))
+    y = kernels.moe_layer(x.to(gpu), _experts(layer), top_k, False).double().cpu()
+    assert ref.isinf().any() and torch.equal(y.isnan(), ref.isnan()) and torch.equal(y == float("inf"), ref == float("inf")) and torch.equal(y == float("-inf"), ref == float("-inf"))
