@@ -2,7 +2,7 @@
 //   mean = sum(x) / H,  rstd = 1 / sqrt(sum((x - mean)^2) / H + eps),  xh = (x - mean) rstd
 //   y = xh w + b
 //   backward, g = dy w:  dx = rstd (g - sum(g) / H - xh sum(g xh) / H),  dw = sum over rows of dy xh,  db = sum over rows of dy
-// All arithmetic in f32, one rounding at the store; the variance is taken around the mean, in a second pass over the row.
+// All arithmetic in f32 (but f64 in the sums over rows that do not fit the registers), one rounding at the store; the variance is taken around the mean, in a second pass over the row.
 #include <algorithm>
 
 #include "common.hpp"
@@ -453,8 +453,8 @@ layer_norm_back_sum_kernel(const float* __restrict__ partials, int parts, int H,
 }
 
 // A block's turns, where rows are few: a turn takes 1.3 us, but every block leaves sums of two rows' bytes in f32, so two where those would be more than kMaxSums bytes (one /
-// two / four turns 509 x 3003, 6 MB with one, 11.7 / 10.0 / 12.8 us, 512 x 2048, 2 MB, 7.9 / 9.2 / 10.9, 104 x 176 5.4 / 6.4 / 7.9) or where one block then takes all rows,
-// without a second launch (16 x 768 5.9 / 5.1); and no more blocks than compute units (8192 x 4096 with 192 / 256 / 512 55 / 48 / 54 us).
+// two / four turns 509 x 3003, 6 MB with one, 12.3 / 10.5 / 13.8 us, 512 x 2048, 2 MB, 8.2 / 9.6 / 11.3, 104 x 176 5.5 / 6.7 / 8.5) or where one block then takes all rows,
+// without a second launch (16 x 768 6.0 / 5.2); and no more blocks than compute units (8192 x 4096 with 192 / 256 / 512 55 / 48 / 54 us).
 constexpr int64_t kMaxSums = 4 << 20;
 // Which kernel the backward pass takes.  parts: sums over rows that it leaves to be added.
 struct BackPlan {

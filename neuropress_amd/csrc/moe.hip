@@ -6,8 +6,8 @@
 //
 // Three launches: the logits (a block per expert), up (every block first picks each token's experts from the logits, then walks (expert, 16 gate rows and their
 // 16 up rows)), down (a block per 32 rows of y and part of all their experts' columns).  The experts' weights are all that counts: each byte is read once for up to 16
-// of an expert's tokens (eight in the down kernel), which share it as the columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 4.8, 29.7 and 19.4 us by
-// themselves, 49 in a row, 4.0 TB/s of 198 MB; 16 tokens fp16 with zero points 181-183 us, 4.0 TB/s.  Bound by HBM inside the walks, by round trips in front of and behind them.
+// of an expert's tokens (eight in the down kernel), which share it as the columns of an MFMA.  One token through two of eight int4 experts of 4096 x 14336: 5.0, 31.4 and 20.6 us by
+// themselves, 50 in a row, 4.0 TB/s of 198 MB; 16 tokens fp16 with zero points 181-186 us, 4.0 TB/s.  Bound by HBM inside the walks, by round trips in front of and behind them.
 //
 // Codes: an MFMA 16x16x32 sees 32 columns of one scale group, so a group's scale multiplies the f32 sum behind it, four multiply-adds for 512 weights, instead of the
 // weights in front of it; nothing is rounded to 16 bits that way.  The codes become operands as they are, their bits under an exponent: q + 128, + 1024 or + 64
@@ -687,11 +687,12 @@ struct MoeSpace {
   }
 };
 
-// Four waves to a block of the up kernel (us of the layer with two / four / eight: int4 4096 x 14336, one token 54 / 50 / 56; dense 2048 x 2048, four tokens 67 / 65 / 66), three
-// where that many divide an item's steps better (nine steps, hidden size 2304: 59.7 / 58.2), and eight of the down kernel (four / eight / 16: 54 / 50 / 52, 65 / 65 / 66), whose
-// blocks split the columns (one part / two: int4 one token 57 / 50; hidden size 256, inner 13440, 14 experts, one / eight / 16 / 32 parts 186 / 51 / 43 / 44; 384 and 1152, 12
-// experts 30 / 24 / 26 / 28).  From entries of five pairs on the up kernel's waves share them: 16 tokens int4 271 / 219, one token 54 / 57; unless that leaves compute units
-// without a block (19 tokens through four of four, 3840 x 768 42 / 35).
+// Four waves to a block of the up kernel (us of the layer with two / four / eight: int4 4096 x 14336, one token 54 / 50 / 56; dense 2048 x 2048, four tokens 58 / 55 / 56), three
+// where that many divide an item's steps better (nine steps, hidden size 2304, with four / three: int4 one token 31.2 / 30.9, four tokens 64.1 / 62.3, int8 39.2 / 39.5), and
+// eight of the down kernel (four / eight: 54 / 50, 55.7 / 55.4), whose blocks split the columns (one part / two: int4 one token 57 / 50; hidden size 256, inner 13440, 14
+// experts, one / eight / 16 / 32 parts 130 / 47 / 42 / 45; 384 and 1152, 12 experts 22 / 19 / 21 / 23).  From entries of five pairs on the up kernel's waves share them (each for
+// itself / shared: 16 tokens int4 197 / 187, one token 50 / 53); unless that leaves compute units without a block (19 tokens through four of four, 3840 x 768, shared / each
+// for itself 46 / 37).
 constexpr int kMoeUpWaves = 4, kMoeDownWaves = 8, kMoeTogether = 5, kMoeWavesPerCu = 16, kMoeDownPairs = 8;
 
 template <int ACT, int FMT, bool ASYM, int GROUP>
