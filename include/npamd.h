@@ -554,6 +554,32 @@ int npamd_moe_layer(const void* x, int64_t ldx, const void* router, const void* 
                     int act_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t npamd_moe_workspace_bytes(int M, int E, int top_k, int H, int I);
 
+/* ------------------------------------- between the halves of a block ---- */
+/*
+ * Residual add between an RMS norm behind a half of a block and the one in front of the next, f32 arithmetic, each output rounded once:
+ *   b = y * rsqrt(mean_i(y^2) + eps) * post_weight (y itself with post_weight NULL),
+ *   stream_out = x + scale * gate * b (gate NULL: 1),  normed = r * rsqrt(mean_i(r^2) + eps) * weight with r = stream_out before it is rounded.
+ * x, y, weight, post_weight, gate, stream_out, normed: `dtype` (NPAMD_F16 / NPAMD_BF16 / NPAMD_F32), row strides in elements, any alignment, any H from 1 to 2^27.
+ * Row m takes row m / gate_every of the gate, rows ldg apart: gate_every = 1 for a gate of every row's own, M for one that all share.
+ * post_rstd, rstd: NULL, or f32 [M], what the backward pass reads.  stream_out may be x and normed may be y (with the same row distance).
+ */
+int npamd_residual_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, const void* weight, const void* post_weight, const void* gate, int64_t ldg,
+                        int gate_every, float scale, void* stream_out, int64_t lds, void* normed, int64_t ldn, float* post_rstd, float* rstd, int M, int H,
+                        float eps, int dtype, void* stream);
+
+/*
+ * Its backward pass, from the gradients of both outputs (one of dstream and dnormed may be NULL: zero), y, stream_out as it was rounded, and the statistics; formulas at the
+ * kernels (residual_norm.hip).  M at least 1.  dx, dy, dweight, dpost_weight [H] and dgate (a row of H for every row of the gate, one behind the other) may be NULL: not asked for.
+ * dx may be dstream, dy may be y or dnormed (with the same row distance).  The sums over rows are added in a fixed order: the same from run to run.
+ * workspace: npamd_residual_norm_workspace_bytes(M, H, gate_every, dtype) bytes (gate_every 0 without a gate) of 16-byte aligned device memory, contents irrelevant; calls
+ * that overlap must not share one.
+ */
+int npamd_residual_norm_backward(const void* dstream, int64_t ldds, const void* dnormed, int64_t lddz, const void* y, int64_t ldy, const void* stream_in, int64_t ldr,
+                                 const void* weight, const void* post_weight, const void* gate, int64_t ldg, int gate_every, float scale,
+                                 const float* post_rstd, const float* rstd, void* dx, int64_t lddx, void* dy, int64_t lddy, void* dweight, void* dpost_weight,
+                                 void* dgate, int M, int H, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t npamd_residual_norm_workspace_bytes(int M, int H, int gate_every, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,7 +37,9 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
+#include <array>
 #include <deque>
+#include <optional>
 #include <unordered_map>
 #include <vector>
 
@@ -887,6 +889,7 @@ PyObject* tracked_tensor(PyObject*, PyObject* xo) {
 }  // namespace
 
 #include "feed_forward.hpp"
+#include "block_joints.hpp"
 
 namespace {
 
@@ -898,6 +901,9 @@ PyMethodDef module_methods[] = {
     {"layer_norm_backward", fast(layer_norm_backward), METH_FASTCALL, "layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight, dbias): the gradients, or None"},
     {"dense_linear_act", fast(dense_linear_act), METH_FASTCALL, "dense_linear_act(x, w, bias, activation, residual): the output, or None"},
     {"moe_layer", fast(moe_layer), METH_FASTCALL, "moe_layer(x, 7 tensors, 6 numbers, renormalize): the output, or None"},
+    {"residual_norm", fast(residual_norm), METH_FASTCALL, "residual_norm(x, y, weight, post_weight, gate, scale, eps, stats): the outputs, or None"},
+    {"residual_norm_recorded", fast(residual_norm_recorded), METH_FASTCALL, "residual_norm_recorded(x, y, weight, post_weight, gate, scale, eps): the outputs, with their node"},
+    {"residual_norm_backward", fast(residual_norm_backward), METH_FASTCALL, "residual_norm_backward(10 arguments, 5 booleans): the gradients, or None"},
     {"tracked", tracked_tensor, METH_O, "tracked(x): whether torch follows what is done to x, so that no plan issues the call"},
     {"row_distance", row_distance, METH_O, "row_distance(x): elements between the rows a plan would read, or None"},
     {"set_module_class", set_module_class, METH_VARARGS, "set_module_class(torch.nn.Module, its call in Python)"},

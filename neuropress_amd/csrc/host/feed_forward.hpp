@@ -129,6 +129,20 @@ at::Tensor as_rows(const at::Tensor& t, int64_t* ld) { return rows_of(t, ld) ? t
 
 const void* data_or_null(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
+// Inside a capture torch would go on to leaves whose nodes another graph that is still alive has made on another stream: waiting for that stream there ends the process.
+void refuse_foreign_leaves(const char* what, std::initializer_list<at::Tensor> inputs) {
+  const auto stream = c10::hip::getCurrentHIPStream();
+  hipStreamCaptureStatus status;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) return (void)hipGetLastError();
+  if (status == hipStreamCaptureStatusNone) return;
+  for (const at::Tensor& t : inputs) {
+    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) continue;
+    const auto leaf = torch::autograd::impl::try_get_grad_accumulator(t);
+    TORCH_CHECK(!leaf || !leaf->stream() || leaf->stream()->id() == stream.id(), what,
+                ": a backward pass cannot be captured while a graph of the same leaves from another stream is alive: free it, or make it on the stream of the capture");
+  }
+}
+
 // Layer norm in a recorded graph; arguments that Python has checked.  First derivatives only: what a backward pass that is itself recorded gives refuses to be differentiated.
 struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
@@ -144,26 +158,13 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     ctx->save_for_backward({x, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), mean, rstd});
     return y;
   }
-  // Inside a capture torch would go on to leaves whose nodes another graph that is still alive has made on another stream: waiting for that stream there ends the process.
-  static void refuse_foreign_leaves(const torch::autograd::variable_list& inputs) {
-    const auto stream = c10::hip::getCurrentHIPStream();
-    hipStreamCaptureStatus status;
-    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) return (void)hipGetLastError();
-    if (status == hipStreamCaptureStatusNone) return;
-    for (int i = 0; i < 3; ++i) {
-      if (!inputs[i].defined() || !inputs[i].is_leaf() || !inputs[i].requires_grad()) continue;
-      const auto leaf = torch::autograd::impl::try_get_grad_accumulator(inputs[i]);
-      TORCH_CHECK(!leaf || !leaf->stream() || leaf->stream()->id() == stream.id(),
-                  "layer_norm: a backward pass cannot be captured while a graph of the same leaves from another stream is alive: free it, or make it on the stream of the capture");
-    }
-  }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const torch::autograd::variable_list saved = ctx->get_saved_variables();
     const bool recorded = c10::GradMode::is_enabled();
     torch::autograd::variable_list out(4);
     const at::Tensor &x = saved[0], &mean = saved[3], &rstd = saved[4];
     const c10::DeviceGuard guard(x.device());
-    refuse_foreign_leaves(saved);
+    refuse_foreign_leaves("layer_norm", {saved[0], saved[1], saved[2]});
     {
       const c10::AutoGradMode off(false);
       const bool with_w = saved[1].defined(), with_b = saved[2].defined();
