@@ -580,6 +580,29 @@ int npamd_residual_norm_backward(const void* dstream, int64_t ldds, const void* 
                                  void* dgate, int M, int H, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t npamd_residual_norm_workspace_bytes(int M, int H, int gate_every, int dtype);
 
+/*
+ * The gated product of a feed-forward block: y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) * (sum_k x[m, k] w[N + n, k] + bias[N + n]), f32 up to one rounding, with w = gate_up:
+ * [2 N, K], N gate rows before N up rows.  x, gate_up, y, pre: act_dtype (NPAMD_F16 or NPAMD_BF16); bias: NULL, or [2 N] of bias_dtype NPAMD_F32 or act_dtype; activation: one of
+ * NPAMD_ACT_*.  pre: NULL, or [M, 2 N], rows ldp apart: the two sums (bias among them), rounded, for the backward pass.  Addresses, alignment and workspace as for
+ * npamd_dense_gemm_act, N up to 2^24; past NPAMD_GEMV_MAX_M tokens ldy and ldp below NPAMD_TILE_MAX_STRIDE.
+ */
+int npamd_gated_linear(const void* x, int64_t ldx, const void* gate_up, int64_t ldw, const void* bias, int bias_dtype, int activation, void* y, int64_t ldy,
+                       void* pre, int64_t ldp, int M, int N, int K, int act_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t npamd_gated_linear_workspace_bytes(int M, int N, int K);
+
+/*
+ * Its backward pass from dh [M, N], x, gate_up and pre: with g and u the halves of pre, dg = dh u act'(g) and du = dh act(g) (f32, rounded to act_dtype as operands),
+ *   dx = [dg du] gate_up,  dgate_up = [dg du]^T x,  dbias = sums over rows of the unrounded [dg du] (of bias_dtype), f32 sums, each rounded once.
+ * dx [M, K], dgate_up [2 N, K], dbias [2 N] may be NULL: not asked for; then what only they need may be, too.  M at least 1.  dh and pre lie at any address; x and gate_up at 16-byte
+ * addresses with row distances that are multiples of 8, and their rows are readable up to a multiple of eight columns (the last one too); row distances below
+ * NPAMD_TILE_MAX_STRIDE.  The same from run to run.  workspace: npamd_gated_linear_backward_workspace_bytes bytes of 16-byte aligned device memory (its last three arguments say which
+ * gradients are asked for), contents irrelevant; calls that overlap must not share one.
+ */
+int npamd_gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* gate_up, int64_t ldw, const void* pre, int64_t ldp, int activation,
+                                void* dx, int64_t lddx, void* dgate_up, int64_t lddw, void* dbias, int bias_dtype, int M, int N, int K, int act_dtype,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+int64_t npamd_gated_linear_backward_workspace_bytes(int M, int N, int K, int dx, int dgate_up, int dbias);
+
 #ifdef __cplusplus
 }
 #endif

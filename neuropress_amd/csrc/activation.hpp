@@ -11,7 +11,7 @@ __device__ __forceinline__ float silu_f32(float v) { return v * __builtin_amdgcn
 // v Phi(v), Phi by erfc: exp(z^2) erfc(z) / 2, z = |v| / sqrt(2), is a polynomial in t = 1 / (1 + 0.51 z) without a constant term, to 9e-7 relative (fitted up to z = 10,
 // past which exp(-z^2) is zero).  GELU itself is off by up to 7e-6 relative where it is small, far below zero (5e-6 from
 // -9 on, 2e-6 from -6): the exponent is rounded, 2^-24 of some v^2.
-__device__ __forceinline__ float gelu_f32(float v) {
+__device__ __forceinline__ float gelu_cdf_f32(float v) {
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.51f * 0.70710678f, fabsf(v), 1.f));
   float q = 0.047250088304281235f;
   q = __builtin_fmaf(q, t, -0.17956776916980743f);
@@ -21,8 +21,9 @@ __device__ __forceinline__ float gelu_f32(float v) {
   q = __builtin_fmaf(q, t, 0.14207614958286285f);
   q = __builtin_fmaf(q, t, 0.14395874738693237f);
   const float half = q * t * __builtin_amdgcn_exp2f(v * v * -0.72134752f);  // exp(-v^2 / 2)
-  return v * (v < 0.f ? half : 1.f - half);
+  return v < 0.f ? half : 1.f - half;
 }
+__device__ __forceinline__ float gelu_f32(float v) { return v * gelu_cdf_f32(v); }
 
 // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2 u))
 __device__ __forceinline__ float gelu_tanh_f32(float v) {

@@ -406,8 +406,11 @@ void count_tiles(int M, int N, int64_t* tiles, std::index_sequence<I...>) {
 // Every call of the band is planned, one at a new token count three times: sizes are divided by constants, and the parts of a tile are looked at only while what they cannot go
 // below (their bytes, their share of the walk and the sum) is less than the best so far.  us on the host, all tiles and parts in turn / so: 384 x 4096 x 4096
 // 0.61 / 0.17, 77 x 3003 x 2176 0.83 / 0.16, 64 x 1024 x 4096 0.87 / 0.32, 528 x 336 x 13440 0.94 / 0.56.
-DensePlan plan_dense(int M, int N, int K, int forced_tile, int max_splits, bool wide = true) {
+//
+// `tiles_there`: bit i for tile i of the list, of the forms that not every tile has; 64 x 128 in two groups and the kernel above are in no such list.
+DensePlan plan_dense(int M, int N, int K, int forced_tile, int max_splits, bool wide = true, unsigned tiles_there = ~0u) {
   DensePlan best{0, 1, 1e30f};
+  if (forced_tile > 0 && forced_tile <= kDenseTiles && !(tiles_there >> (forced_tile - 1) & 1)) forced_tile = 0;
   const int steps = K / 64;
   const int forced = tuning().dense_splits, most = max_splits < steps ? max_splits : steps;
   const int forced_splits = forced < most ? forced : most;
@@ -418,6 +421,7 @@ DensePlan plan_dense(int M, int N, int K, int forced_tile, int max_splits, bool 
   const bool two_groups = only >= 0 || (M >= N && steps >= 64);
   auto load = [&](int i) { return (float)tiles[i] * steps * (kDenseCost[i].bm + kDenseCost[i].bn) * 128e-6f * kDenseCost[i].per_mb; };
   auto look = [&](int i, int splits, int part, float bytes, float sum) {
+    if (!(tiles_there >> i & 1)) return;
     const DenseCost& c = kDenseCost[i];
     const int64_t rounds = ((tiles[i] * splits + 7) / 8 + 31) / 32;
     if (i == kDenseTwoGroups && only < 0 && (splits == 1 || rounds > 1 || !two_groups)) return;
@@ -501,6 +505,121 @@ int npamd::dense_gemm_epilogue(const char* what, const DenseShape& shape, int K,
   s.pieces = K / 8;
   return act == NPAMD_BF16 ? launch_dense_epilogue<NPAMD_BF16>(s, p.tile, st, what) : launch_dense_epilogue<NPAMD_F16>(s, p.tile, st, what);
 }
+
+namespace npamd {
+namespace {
+
+// The sums of the parts of the gated product and what becomes of them: four columns of y to a thread, the parts' loads of the gate's and the up projection's columns in batches.
+template <int ACT>
+__global__ void __launch_bounds__(64) splitk_reduce_gated_kernel(const DenseShape s) {
+  const int n = ((int)blockIdx.x * 64 + (int)threadIdx.x) * 4, last = min(3, s.N - 1 - n);  // columns past N: the last one again, not stored
+  if (n >= s.N) return;
+  const bool vec = s.N % 4 == 0 && (reinterpret_cast<uintptr_t>(s.partials) & 15) == 0;
+  float bias[2][4] = {};
+  if (s.ep.bias) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = u * s.N + n + min(j, last);
+        bias[u][j] = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, at) : ((const float*)s.ep.bias)[at];
+      }
+  }
+  for (int m = blockIdx.y; m < s.M; m += gridDim.y) {
+    const float* const p = s.partials + (size_t)m * 2 * s.N + n;
+    float sum[2][4] = {};
+    for (int z0 = 0; z0 < s.splits; z0 += kReduceBatch) {
+      float v[kReduceBatch][2][4];
+#pragma unroll
+      for (int i = 0; i < kReduceBatch; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float* const q = p + (size_t)min(z0 + i, s.splits - 1) * s.M * 2 * s.N + (size_t)u * s.N;
+          if (vec) {
+            const f32x4 t = *reinterpret_cast<const f32x4*>(q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][u][j] = t[j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][u][j] = q[min(j, last)];
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < kReduceBatch; ++i)
+        if (z0 + i < s.splits) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[u][j] += v[i][u][j];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sum[u][j] += bias[u][j];
+        if (s.ep.pre && j <= last) store_from_f32<ACT>(s.ep.pre, (int64_t)m * s.ep.ldp + (int64_t)u * s.N + n + j, sum[u][j]);
+      }
+    activate_all(s.ep.act, [&](auto f) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[0][j] = f(sum[0][j]);
+    });
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j <= last) store_from_f32<ACT>(s.y, (int64_t)m * s.ldy + n + j, sum[0][j] * sum[1][j]);
+  }
+}
+
+constexpr unsigned kGatedTiles = 1u << 1 | 1u << 2 | 1u << 3 | 1u << 5 | 1u << 6 | 1u << 7 | 1u << 8 | 1u << 9 | 1u << 11;
+constexpr unsigned kTurnedTiles = 1u << 1 | 1u << 2 | 1u << 3 | 1u << 5 | 1u << 11;
+
+DensePlan plan_gated(int M, int N, int K, int max_splits) { return plan_dense(M, 2 * N, K, tuning().dense_tile, max_splits, true, kGatedTiles); }
+DensePlan plan_turned(int M, int N, int K, int max_splits) { return plan_dense(M, N, K, tuning().dense_tile, max_splits, true, kTurnedTiles); }
+
+int whole_steps(int K) { return (K + 63) / 64 * 64; }
+
+}  // namespace
+
+int64_t dense_gemm_gated_workspace_bytes(int M, int N, int K) {
+  const DensePlan p = plan_gated(M, N, whole_steps(K), kDenseMaxSplits);
+  return p.splits > 1 ? (int64_t)p.splits * M * 2 * N * 4 : 0;
+}
+
+int dense_gemm_gated(const char* what, const DenseShape& shape, int K, int act, int64_t workspace_bytes, hipStream_t st) {
+  DenseShape s = shape;
+  DensePlan p = plan_gated(s.M, s.N, whole_steps(K), kDenseMaxSplits);
+  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * 2 * s.N * 4) < p.splits)) p = plan_gated(s.M, s.N, whole_steps(K), 1);
+  s.steps = whole_steps(K) / 64;
+  s.splits = p.splits;
+  s.pieces = K / 8;
+  const int rc = launch_wide_gated(s, act, p.tile, st);
+  if (rc != NPAMD_OK || s.splits == 1) return rc;
+  const dim3 grid((unsigned)(((s.N + 3) / 4 + 63) / 64), (unsigned)(s.M < 65535 ? s.M : 65535));
+  if (act == NPAMD_BF16) launch(splitk_reduce_gated_kernel<NPAMD_BF16>, grid, 64, 0, st, s);
+  else launch(splitk_reduce_gated_kernel<NPAMD_F16>, grid, 64, 0, st, s);
+  return check_launch(what);
+}
+
+int64_t dense_gemm_turned_workspace_bytes(int M, int N, int K, bool) {
+  const DensePlan p = plan_turned(M, N, whole_steps(K), kDenseMaxSplits);
+  return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
+}
+
+int dense_gemm_turned(const char* what, const DenseShape& shape, int K, bool x_too, int act, int64_t workspace_bytes, hipStream_t st) {
+  DenseShape s = shape;
+  DensePlan p = plan_turned(s.M, s.N, whole_steps(K), kDenseMaxSplits);
+  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * s.N * 4) < p.splits)) p = plan_turned(s.M, s.N, whole_steps(K), 1);
+  s.steps = whole_steps(K) / 64;
+  s.splits = p.splits;
+  s.K = K;
+  const int rc = launch_wide_turned(s, act, p.tile, x_too, st);
+  if (rc != NPAMD_OK || s.splits == 1) return rc;
+  if (act == NPAMD_BF16) launch_splitk_reduce<NPAMD_BF16>(s.partials, s.splits, s.M, s.N, nullptr, s.y, s.ldy, st);
+  else launch_splitk_reduce<NPAMD_F16>(s.partials, s.splits, s.M, s.N, nullptr, s.y, s.ldy, st);
+  return check_launch(what);
+}
+
+}  // namespace npamd
 
 // Rows of x and w that end inside a 64-k step, K a multiple of 8: neither is copied to whole steps first.
 extern "C" int npamd_dense_gemm_ragged(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, void* y, int64_t ldy,

@@ -12,6 +12,9 @@ struct DenseEpilogue {
   const void* residual;  // [M][N] of the activations' type, rows ldr apart
   int64_t ldr;
   int act, bias_16;
+  // Of the gated product act(gate sum) * up sum, N columns of each, gate rows of w before up rows: null, or where the two sums go, [M][2 N], rows ldp apart.
+  void* pre;
+  int64_t ldp;
 };
 
 struct DenseShape {
@@ -26,6 +29,7 @@ struct DenseShape {
   int pieces;        // 16-byte pieces of a row: K / 8
   int group;         // row tiles of a group (wide tiles)
   DenseEpilogue ep;  // of the kernels that have one
+  int K;             // of the kernels with an operand whose rows are the contracted ones
 };
 
 // The product on wide tile `tile` of the plan's list; splits > 1: its parts, without their sum.
@@ -34,5 +38,17 @@ int launch_wide_epilogue(const DenseShape& s, int act, int tile, hipStream_t st)
 
 // The product with an epilogue, on the tile and parts of K that are planned for the shape without one: x and w 16-byte aligned, K and rows' distances multiples of 8.
 int dense_gemm_epilogue(const char* what, const DenseShape& s, int K, int act, int64_t workspace_bytes, hipStream_t st);
+
+// The gated product (s.N: columns of y), x and w as above; its bytes of workspace.
+int dense_gemm_gated(const char* what, const DenseShape& s, int K, int act, int64_t workspace_bytes, hipStream_t st);
+int64_t dense_gemm_gated_workspace_bytes(int M, int N, int K);
+
+// y[m][n] = sum over k of x w with w as [K][N] and, with x_too, x as [K][M]: rows 16-byte aligned, their distances multiples of 8, readable up to a multiple of eight columns; x
+// as [M][K] up to a multiple of eight k.  Any K: what lies past it counts for nothing.
+int dense_gemm_turned(const char* what, const DenseShape& s, int K, bool x_too, int act, int64_t workspace_bytes, hipStream_t st);
+int64_t dense_gemm_turned_workspace_bytes(int M, int N, int K, bool x_too);
+
+int launch_wide_gated(const DenseShape& s, int act, int tile, hipStream_t st);
+int launch_wide_turned(const DenseShape& s, int act, int tile, bool x_too, hipStream_t st);
 
 }  // namespace npamd

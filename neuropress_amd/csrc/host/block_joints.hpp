@@ -1,4 +1,4 @@
-// The functions between a decoder block's halves (residual norm and its backward pass), issued from native code.
+// The functions that join a decoder block's halves (residual norm, gated product, their backward passes), issued from native code.
 //
 // As in feed_forward.hpp the functions that Python tries first return None for what is not as the kernels want it; Python then checks, reports, copies, and calls them again.
 // What the library refuses is an error at once.
@@ -214,6 +214,145 @@ PyObject* residual_norm_recorded(PyObject*, PyObject* const* args, Py_ssize_t n)
     auto out = ResidualNormNode::apply(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2]), maybe_tensor(args[3]), maybe_tensor(args[4]),
                                        PyFloat_AS_DOUBLE(args[5]), PyFloat_AS_DOUBLE(args[6]));
     return wrap_all({out[0], out[1]});
+  });
+}
+
+// Rows that the tiles can read, of whole 16-byte pieces: t where it lies so, else a copy, its rows padded with zeros.
+at::Tensor whole_pieces(const at::Tensor& t, int64_t* ld) {
+  const at::Tensor rows = as_rows(t, ld);
+  const int64_t k = t.size(-1), m = t.numel() / k, padded = (k + 7) / 8 * 8;
+  const void* const p = rows.const_data_ptr();
+  if (k == padded && *ld % 8 == 0 && *ld < NPAMD_TILE_MAX_STRIDE && ((uintptr_t)p & 15) == 0) return rows;
+  at::Tensor copy = empty({m, padded}, t.scalar_type(), t.get_device());
+  TORCH_CHECK(npamd_gather_columns(p, *ld, nullptr, copy.data_ptr(), padded, (int)m, (int)k, current_stream(t.get_device())) == NPAMD_OK, npamd_last_error());
+  *ld = padded;
+  return copy;
+}
+
+at::Tensor last_dimension(const at::Tensor& t, int64_t n) {
+  c10::SmallVector<int64_t, 6> sizes(t.sizes().begin(), t.sizes().end());
+  sizes.back() = n;
+  return empty(sizes, t.scalar_type(), t.get_device());
+}
+
+// h and, with keep, pre; of tensors that have been checked.
+std::array<at::Tensor, 2> gated_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, int activation, bool keep) {
+  const int k = (int)x.size(-1), m = (int)(x.numel() / k), n = (int)(w.size(0) / 2), code = dtype_code(x.scalar_type()), device = x.get_device();
+  const bool tiles = m > NPAMD_GEMV_MAX_M;
+  int64_t ldx, ldw;
+  const at::Tensor xr = tiles ? whole_pieces(x, &ldx) : as_rows(x, &ldx), wr = tiles ? whole_pieces(w, &ldw) : as_rows(w, &ldw);
+  const at::Tensor b = bias.defined() ? bias.contiguous() : at::Tensor();
+  const int columns = tiles ? (k + 7) / 8 * 8 : k;
+  std::array<at::Tensor, 2> out{last_dimension(x, n), keep ? last_dimension(x, 2 * (int64_t)n) : at::Tensor()};
+  const int64_t bytes = npamd_gated_linear_workspace_bytes(m, n, columns);
+  at::Tensor scratch;
+  if (bytes > 0) scratch = floats(bytes, device);
+  TORCH_CHECK(npamd_gated_linear(xr.const_data_ptr(), ldx, wr.const_data_ptr(), ldw, data_or_null(b), b.defined() ? dtype_code(b.scalar_type()) : NPAMD_F32, activation,
+                                 out[0].data_ptr(), n, out_or_null(out[1]), 2 * (int64_t)n, m, n, columns, code, out_or_null(scratch), bytes, current_stream(device)) == NPAMD_OK,
+              npamd_last_error());
+  return out;
+}
+
+// The gradients of x, gate_up and bias that are needed, the last in `bias_type`.
+std::array<at::Tensor, 3> gated_backward(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& w, const at::Tensor& pre, int activation, at::ScalarType bias_type,
+                                         const bool (&need)[3]) {
+  const int k = (int)x.size(-1), m = (int)(x.numel() / k), n = (int)(w.size(0) / 2), code = dtype_code(x.scalar_type()), device = x.get_device();
+  int64_t lddh, ldp, ldx = 0, ldw = 0;
+  const at::Tensor dhr = as_rows(dh, &lddh), pr = as_rows(pre, &ldp);
+  const at::Tensor wr = need[0] ? whole_pieces(w, &ldw) : at::Tensor(), xr = need[1] ? whole_pieces(x, &ldx) : at::Tensor();
+  std::array<at::Tensor, 3> out;
+  if (need[0]) out[0] = empty(x.sizes(), x.scalar_type(), device);
+  if (need[1]) out[1] = empty(w.sizes(), x.scalar_type(), device);
+  if (need[2]) out[2] = empty({2 * (int64_t)n}, bias_type, device);
+  if (!need[0] && !need[1] && !need[2]) return out;
+  const int64_t bytes = npamd_gated_linear_backward_workspace_bytes(m, n, k, need[0], need[1], need[2]);
+  const at::Tensor scratch = floats((bytes + 3) / 4 * 4, device);
+  TORCH_CHECK(npamd_gated_linear_backward(dhr.const_data_ptr(), lddh, data_or_null(xr), ldx, data_or_null(wr), ldw, pr.const_data_ptr(), ldp, activation, out_or_null(out[0]), k,
+                                          out_or_null(out[1]), k, out_or_null(out[2]), dtype_code(bias_type), m, n, k, code, scratch.data_ptr(), bytes,
+                                          current_stream(device)) == NPAMD_OK, npamd_last_error());
+  return out;
+}
+
+// gate_up [2 N, K] for x's rows.
+bool gated_weight(PyObject* o, const Rows& x, int device, Rows* w) {
+  return x.code != NPAMD_F32 && rows_argument(o, device, w) && w->code == x.code && w->t->dim() == 2 && w->width == x.width && w->m % 2 == 0;
+}
+
+int activation_of(PyObject* o) { return PyLong_Check(o) ? (int)PyLong_AsLong(o) : -1; }
+
+// gated_linear(x, gate_up, bias, activation's number, pre?): h, with pre (h, pre), or None
+PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "gated_linear(x, gate_up, bias, activation, pre)");
+    return nullptr;
+  }
+  return translated([&]() -> PyObject* {
+    const int device = device_of(args[0]);
+    Rows x, w;
+    if (!PyBool_Check(args[4]) || activation_of(args[3]) < 0 || !rows_argument(args[0], device, &x) || !gated_weight(args[1], x, device, &w)) Py_RETURN_NONE;
+    const void* p;
+    if (!vector_of(args[2], device, x.t->scalar_type(), w.m, &p) && !vector_of(args[2], device, at::kFloat, w.m, &p)) Py_RETURN_NONE;
+    const bool keep = args[4] == Py_True;
+    auto out = gated_forward(*x.t, *w.t, is_none(args[2]) ? at::Tensor() : THPVariable_Unpack(args[2]), activation_of(args[3]), keep);
+    return keep ? wrap_all({out[0], out[1]}) : THPVariable_Wrap(std::move(out[0]));
+  });
+}
+
+// gated_linear_backward(dh, x, gate_up, pre, activation's number, bias in float32?, dx?, dgate_up?, dbias?): the gradients, or None
+PyObject* gated_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9) {
+    PyErr_SetString(PyExc_TypeError, "gated_linear_backward(dh, x, gate_up, pre, activation, 4 booleans)");
+    return nullptr;
+  }
+  return translated([&]() -> PyObject* {
+    const int device = device_of(args[1]);
+    Rows dh, x, w, pre;
+    if (activation_of(args[4]) < 0 || !rows_argument(args[1], device, &x) || !gated_weight(args[2], x, device, &w)) Py_RETURN_NONE;
+    if (!rows_argument(args[0], device, &dh) || !rows_argument(args[3], device, &pre) || dh.code != x.code || pre.code != x.code) Py_RETURN_NONE;
+    if (dh.m != x.m || pre.m != x.m || 2 * dh.width != w.m || pre.width != w.m) Py_RETURN_NONE;
+    for (int i = 5; i < 9; ++i)
+      if (!PyBool_Check(args[i])) Py_RETURN_NONE;
+    const bool need[3] = {args[6] == Py_True, args[7] == Py_True, args[8] == Py_True};
+    auto out = gated_backward(*dh.t, *x.t, *w.t, *pre.t, activation_of(args[4]), args[5] == Py_True ? at::kFloat : x.t->scalar_type(), need);
+    return wrap_all({out[0], out[1], out[2]});
+  });
+}
+
+// The gated product in a recorded graph; arguments that Python has checked.  First derivatives only.
+struct GatedLinearNode : torch::autograd::Function<GatedLinearNode> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation) {
+    const c10::DeviceGuard guard(x.device());
+    const auto out = gated_forward(x, w, bias.value_or(at::Tensor()), (int)activation, true);
+    ctx->save_for_backward({x, w, bias.value_or(at::Tensor()), out[1]});
+    ctx->saved_data["activation"] = activation;
+    return out[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
+    const bool recorded = c10::GradMode::is_enabled();
+    const at::Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &pre = saved[3];
+    const c10::DeviceGuard guard(x.device());
+    refuse_foreign_leaves("gated_linear", {x, w, bias});
+    torch::autograd::variable_list result(4);
+    std::array<at::Tensor, 3> out;
+    {
+      const c10::AutoGradMode off(false);
+      const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), bias.defined() && ctx->needs_input_grad(2)};
+      out = gated_backward(grads[0], x, w, pre, (int)ctx->saved_data["activation"].toInt(), bias.defined() ? bias.scalar_type() : at::kFloat, need);
+    }
+    for (int i = 0; i < 3; ++i) result[i] = recorded ? final_gradient("gated_linear: its backward pass cannot be differentiated", out[i]) : out[i];
+    return result;
+  }
+};
+
+// gated_linear_recorded(x, gate_up, bias, activation's number): tensors (or None) that Python has checked, on one device
+PyObject* gated_linear_recorded(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || activation_of(args[3]) < 0) {
+    PyErr_SetString(PyExc_TypeError, "gated_linear_recorded(x, gate_up, bias, activation)");
+    return nullptr;
+  }
+  return translated([&]() -> PyObject* {
+    return THPVariable_Wrap(GatedLinearNode::apply(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), maybe_tensor(args[2]), (int64_t)activation_of(args[3])));
   });
 }
 

@@ -904,6 +904,9 @@ PyMethodDef module_methods[] = {
     {"residual_norm", fast(residual_norm), METH_FASTCALL, "residual_norm(x, y, weight, post_weight, gate, scale, eps, stats): the outputs, or None"},
     {"residual_norm_recorded", fast(residual_norm_recorded), METH_FASTCALL, "residual_norm_recorded(x, y, weight, post_weight, gate, scale, eps): the outputs, with their node"},
     {"residual_norm_backward", fast(residual_norm_backward), METH_FASTCALL, "residual_norm_backward(10 arguments, 5 booleans): the gradients, or None"},
+    {"gated_linear", fast(gated_linear), METH_FASTCALL, "gated_linear(x, gate_up, bias, activation, pre): the output (with the sums), or None"},
+    {"gated_linear_recorded", fast(gated_linear_recorded), METH_FASTCALL, "gated_linear_recorded(x, gate_up, bias, activation): the output, with its node"},
+    {"gated_linear_backward", fast(gated_linear_backward), METH_FASTCALL, "gated_linear_backward(dh, x, gate_up, pre, activation, 4 booleans): the gradients, or None"},
     {"tracked", tracked_tensor, METH_O, "tracked(x): whether torch follows what is done to x, so that no plan issues the call"},
     {"row_distance", row_distance, METH_O, "row_distance(x): elements between the rows a plan would read, or None"},
     {"set_module_class", set_module_class, METH_VARARGS, "set_module_class(torch.nn.Module, its call in Python)"},

@@ -4,7 +4,7 @@
 namespace npamd {
 
 int launch_wide(const DenseShape& s, int act, int tile, hipStream_t st) {
-  return act == NPAMD_BF16 ? launch_wide_on<NPAMD_BF16, false>(s, tile, st) : launch_wide_on<NPAMD_F16, false>(s, tile, st);
+  return act == NPAMD_BF16 ? launch_wide_on<NPAMD_BF16, kWidePlain>(s, tile, st) : launch_wide_on<NPAMD_F16, kWidePlain>(s, tile, st);
 }
 
 }  // namespace npamd

@@ -43,11 +43,60 @@ struct WideTile {
   static_assert(kLds <= kLdsPerBlockMax && SPAN <= 2 * kMfmas && (ST - 1) * kLoads < 64);
 };
 
-// EPILOGUE: s.ep is applied to the sums, which leave through LDS in f32, 16 rows of a wave at a time.
-template <int ACT, class T, bool EPILOGUE = false>
+// What becomes of the sums.  Epilogue: s.ep is applied to them, and they leave through LDS in f32, 16 rows of a wave at a time.  Gated: the first half of a wave's column
+// groups are gate rows of W, the others the up rows of the same columns of y, so that a lane has both sums of each of its values.
+enum WideForm { kWidePlain, kWideEpilogue, kWideGated };
+
+// An operand that lies in memory with the contracted index as its row ("turned"), 64 rows of B columns to a step, lies so in LDS as well, 2 B bytes to a row: a load brings 1024 bytes of
+// them one behind the other.  An MFMA's operand, eight k of a column to a lane, is then two transposing reads, each four rows of 16 columns to 16 lanes: 32 bytes of a row side by
+// side.  The 32-byte pieces of row k lie in the places p ^ turned_place(k), so that the eight rows of 32 lanes are in different banks.
+template <int B>
+__device__ __forceinline__ constexpr int turned_place(int k) {
+  return (k & 3) | (B >= 128 ? ((k >> 3) & 1) << 2 : 0);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// The rows of a wave's tile, 16 MT of 16 NC columns, from its part of LDS (rows of 32 NC + 16 bytes) to memory.
+template <int MT, int NC>
+__device__ __forceinline__ void store_rows(const uint8_t* ep, int lane, void* y, int64_t ldy64, int wm0, int wn0, int rows, int cols, bool whole_rows) {
+  constexpr uint32_t kBuffer = 0x80000000u, kNowhere = kBuffer;  // bytes: what lies outside the result is stored past the end of the buffer, which the hardware drops
+  constexpr int kRaw = 0x00020000, kRow = 32 * NC + 16;
+  uint16_t* const to = reinterpret_cast<uint16_t*>(y) + (int64_t)wm0 * ldy64 + wn0;
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)kBuffer, kRaw);
+  const uint32_t ldy = (uint32_t)ldy64;
+  if (whole_rows) {
+    constexpr int kPerRow = 2 * NC, kRowsAtOnce = 64 / kPerRow;  // 16-byte pieces; NC = 3, 7: a few lanes idle
+    const int r = lane / kPerRow, p = lane % kPerRow;
+#pragma unroll 8
+    for (int i = 0; i < (16 * MT + kRowsAtOnce - 1) / kRowsAtOnce; ++i) {
+      const int m = i * kRowsAtOnce + r;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(ep + min(m, 16 * MT - 1) * kRow + p * 16);
+      const bool in = r < kRowsAtOnce && m < min(rows, 16 * MT) && p * 8 < cols;
+      __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, in ? ((uint32_t)m * ldy + (uint32_t)p * 8u) * 2u : kNowhere, 0, 0);
+    }
+    return;
+  }
+  // Rows at odd addresses: a value at a time, a row's side by side.
+#pragma unroll 8
+  for (int m = 0; m < 16 * MT; ++m) {
+#pragma unroll
+    for (int n0 = 0; n0 < 16 * NC; n0 += 64) {
+      const int n = n0 + lane;
+      const uint16_t v = *reinterpret_cast<const uint16_t*>(ep + m * kRow + min(n, 16 * NC - 1) * 2);
+      __builtin_amdgcn_raw_buffer_store_b16(v, rsrc, m < rows && n < 16 * NC && n < cols ? ((uint32_t)m * ldy + (uint32_t)n) * 2u : kNowhere, 0, 0);
+    }
+  }
+}
+
+template <int ACT, class T, int FORM = kWidePlain, bool XK = false, bool WK = false>
 __global__ void __launch_bounds__(T::kThreads, T::kThreads == 256 ? 2 : 1)
 wide_gemm_kernel(const DenseShape s) {
   constexpr int MT = T::MT, NT = T::NT, ST = T::ST, L = T::kLoads, kM = T::kMfmas, SPAN = T::SPAN;
+  constexpr bool EPILOGUE = FORM == kWideEpilogue, GATED = FORM == kWideGated, TURNED = XK || WK;
+  static_assert(!GATED || (NT % 2 == 0 && !TURNED));
+  static_assert(!(XK && (MT & (MT - 1) || (T::kBM != 64 && T::kBM != 128 && T::kBM != 256))), "places of a turned row");
+  static_assert(!(WK && (NT & (NT - 1) || (T::kBN != 64 && T::kBN != 128 && T::kBN != 256))), "places of a turned row");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   // blockIdx.x % 8 names the die; a die takes an eighth of the units, counted down the columns of a group of row tiles (launch_wide_tile).
   const int unit = (blockIdx.x & 7) * s.units_per_die + (blockIdx.x >> 3), columns = s.col_tiles * s.splits;
@@ -55,7 +104,7 @@ wide_gemm_kernel(const DenseShape s) {
   const int group = unit / (s.group * columns), in = unit - group * (s.group * columns), group_rows = min(s.group, s.row_tiles - group * s.group);
   const int column = in / group_rows, rt = group * s.group + in - column * group_rows;
   const int ct = s.splits > 1 ? column / s.splits : column, part = column - ct * s.splits;
-  const int m0 = rt * T::kBM, n0 = ct * T::kBN;
+  const int m0 = rt * T::kBM, n0 = ct * (GATED ? T::kBN / 2 : T::kBN);
   const int step0 = (int)((int64_t)s.steps * part / s.splits);
   const int steps = (int)((int64_t)s.steps * (part + 1) / s.splits) - step0;  // of this part
 
@@ -68,13 +117,36 @@ wide_gemm_kernel(const DenseShape s) {
   auto piece_of = [&](int i) NPAMD_INLINE { return min(wave * L + i, T::kPieces - 2 + ((wave * L + i) & 1)); };
   // Piece p of row r lies in place p ^ ((r >> 1) & 7): a lane's differs between even and odd i only.
   auto piece_in_row = [&](int i) NPAMD_INLINE { return (lane & 7) ^ ((((wave * L + i) & 1) * 4 + (lane >> 4)) & 7); };
+  // Where what a lane brings of piece q of a turned operand comes from.
+  struct TurnedPlace {
+    int row, column;
+  };
+  auto turned_at = [&](int q) NPAMD_INLINE {
+    const bool is_x = q < T::kPiecesX;
+    const int B = is_x ? T::kBM : T::kBN, at = (is_x ? q : q - T::kPiecesX) * 1024 + lane * 16, row = at / (2 * B), p = at % (2 * B) / 16;
+    const int place = is_x ? turned_place<T::kBM>(row) : turned_place<T::kBN>(row);
+    return TurnedPlace{row, ((p >> 1) ^ place) * 16 + (p & 1) * 8};
+  };
+  auto advance = [&](bool is_x) NPAMD_INLINE { return (is_x ? XK : WK) ? (is_x ? s.ldx : s.ldw) * 128 : (int64_t)128; };  // bytes from a step to the next
   uint32_t voff[L];
   const uint8_t* from[L];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     const int q = piece_of(i);
     const bool is_x = q < T::kPiecesX;
+    if (is_x ? XK : WK) {
+      const TurnedPlace at = turned_at(q);
+      voff[i] = (uint32_t)(at.row * (is_x ? s.ldx : s.ldw) * 2) + (uint32_t)(min(at.column, ((is_x ? s.M - m0 : s.N - n0) - 1) & ~7) * 2);
+      from[i] = uniform_ptr((is_x ? reinterpret_cast<const uint8_t*>(s.x) + (int64_t)m0 * 2 : reinterpret_cast<const uint8_t*>(s.w) + (int64_t)n0 * 2) + step0 * advance(is_x));
+      continue;
+    }
     const int r = (is_x ? q : q - T::kPiecesX) * 8 + (lane >> 3);
+    if (GATED && !is_x) {
+      const int b = r / 16 % NT, row = min(r / (16 * NT) * 8 * NT + b % (NT / 2) * 16 + r % 16, s.N - 1 - n0);
+      voff[i] = (uint32_t)((int64_t)row * s.ldw * 2) + (uint32_t)(piece_in_row(i) * 16);
+      from[i] = uniform_ptr(reinterpret_cast<const uint8_t*>(s.w) + ((int64_t)(n0 + (q - T::kPiecesX) / 2 % NT / (NT / 2) * s.N) * s.ldw + (int64_t)step0 * 64) * 2);
+      continue;
+    }
     const int row = is_x ? min(r, s.M - 1 - m0) : min(r, s.N - 1 - n0);  // rows past the end: a valid row nobody stores
     voff[i] = (uint32_t)((int64_t)row * (is_x ? s.ldx : s.ldw) * 2) + (uint32_t)(piece_in_row(i) * 16);
     from[i] = uniform_ptr(is_x ? reinterpret_cast<const uint8_t*>(s.x) + ((int64_t)m0 * s.ldx + (int64_t)step0 * 64) * 2
@@ -82,14 +154,22 @@ wide_gemm_kernel(const DenseShape s) {
   }
   const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   auto load = [&](int i, int slot, int step) NPAMD_INLINE {
-    lds_load16(ring + (uint32_t)(slot * T::kStageBytes + piece_of(i) * 1024), voff[i], from[i] + (int64_t)step * 128);
+    lds_load16(ring + (uint32_t)(slot * T::kStageBytes + piece_of(i) * 1024), voff[i], from[i] + step * advance(piece_of(i) < T::kPiecesX));
   };
   // Rows that end inside the last step: its loads bring the last piece again for those past the end, and the operands there are zeroed.
-  const int there = s.pieces - (step0 + steps - 1) * 8;  // pieces of this part's last step
+  // Turned operands end with any k; a row of x as it lies next to a turned W is read to the end of its last piece.
+  const int there_k = s.K - (step0 + steps - 1) * 64;
+  const int there = TURNED ? (there_k + 7) / 8 : s.pieces - (step0 + steps - 1) * 8;  // pieces of this part's last step
+  const bool short_end = TURNED ? there_k < 64 : there < 8;
   auto end_rows = [&](int first, int last) NPAMD_INLINE {
 #pragma unroll
     for (int i = 0; i < L; ++i)
-      if (i >= first && i < last) voff[i] -= (uint32_t)(max(piece_in_row(i) - (there - 1), 0) * 16);
+      if (i >= first && i < last) {
+        const int q = piece_of(i);
+        const bool is_x = q < T::kPiecesX;
+        if (is_x ? XK : WK) voff[i] -= (uint32_t)(max(turned_at(q).row - (there_k - 1), 0) * (int)(is_x ? s.ldx : s.ldw) * 2);
+        else voff[i] -= (uint32_t)(max(piece_in_row(i) - (there - 1), 0) * 16);
+      }
   };
 
   f32x4 acc[MT][NT];
@@ -101,11 +181,34 @@ wide_gemm_kernel(const DenseShape s) {
   u32x4 xo[2][MT], wo[2][NT];
   const uint32_t x_off = (uint32_t)((wm * 16 * MT + c) * 128), w_off = (uint32_t)((T::kBM + wn * 16 * NT + c) * 128);
   const uint32_t place[2] = {(uint32_t)((h ^ ((c >> 1) & 7)) << 4), (uint32_t)(((4 | h) ^ ((c >> 1) & 7)) << 4)};
+  // Of a turned operand: the lane's row and columns of the first four k of its eight; column group i is i places further, by exclusive or.
+  const int tk = 8 * h + ((lane & 15) >> 2);
+  const uint32_t x_turned = XK ? (uint32_t)(tk * 2 * T::kBM + ((wm * MT) ^ turned_place<T::kBM>(tk)) * 32 + (lane & 3) * 8) : 0u;
+  const uint32_t w_turned = WK ? (uint32_t)(tk * 2 * T::kBN + ((wn * NT) ^ turned_place<T::kBN>(tk)) * 32 + (lane & 3) * 8) : 0u;
+  auto read_turned = [&](const uint8_t* at, int rows4) NPAMD_INLINE {
+    typedef __attribute__((address_space(3))) s16x4* Place;
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Place)(__attribute__((address_space(3))) uint8_t*)at));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Place)(__attribute__((address_space(3))) uint8_t*)(at + rows4)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
   auto read_one = [&](int j, const uint8_t* stage, int i) NPAMD_INLINE {
-    if (i < NT) wo[j][i] = *reinterpret_cast<const u32x4*>(stage + w_off + i * 2048 + place[j]);
+    if (i < NT && WK) wo[j][i] = read_turned(stage + T::kBM * 128 + j * 64 * T::kBN + (w_turned ^ (uint32_t)(i * 32)), 8 * T::kBN);
+    else if (i >= NT && XK) xo[j][i - NT] = read_turned(stage + j * 64 * T::kBM + (x_turned ^ (uint32_t)((i - NT) * 32)), 8 * T::kBM);
+    else if (i < NT) wo[j][i] = *reinterpret_cast<const u32x4*>(stage + w_off + i * 2048 + place[j]);
     else xo[j][i - NT] = *reinterpret_cast<const u32x4*>(stage + x_off + (i - NT) * 2048 + place[j]);
   };
   auto blank = [&](int j) NPAMD_INLINE {
+    if constexpr (TURNED) {
+      const int live = there_k - (32 * j + 8 * h);  // of the lane's eight k
+      u32x4 keep;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keep[e] = live >= 2 * e + 2 ? 0xFFFFFFFFu : live == 2 * e + 1 ? 0xFFFFu : 0u;
+#pragma unroll
+      for (int b = 0; b < NT; ++b) wo[j][b] &= keep;
+#pragma unroll
+      for (int a = 0; a < MT; ++a) xo[j][a] &= keep;
+      return;
+    }
     const bool dead = 4 * j + h >= there;
 #pragma unroll
     for (int b = 0; b < NT; ++b) wo[j][b] = dead ? u32x4{0, 0, 0, 0} : wo[j][b];
@@ -130,7 +233,7 @@ wide_gemm_kernel(const DenseShape s) {
     const uint8_t* const stage = lds + slot * T::kStageBytes;
     const int behind = slot == ST - 1 ? 0 : slot + 1, before = slot == 0 ? ST - 1 : slot - 1;
     const uint8_t* const next = lds + behind * T::kStageBytes;
-    const bool ends = MODE == 0 && it == steps - 1 && there < 8;
+    const bool ends = MODE == 0 && it == steps - 1 && short_end;
     if (ends) blank(0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -164,7 +267,7 @@ wide_gemm_kernel(const DenseShape s) {
   for (int p = 0; p < ST; ++p) {
     if (p < steps) {
       const int loads = p < ST - 1 ? L : kFirstLoads;
-      if (p == steps - 1 && there < 8) end_rows(0, loads);
+      if (p == steps - 1 && short_end) end_rows(0, loads);
 #pragma unroll
       for (int i = 0; i < loads; ++i) load(i, p, p);
     }
@@ -175,12 +278,12 @@ wide_gemm_kernel(const DenseShape s) {
 #pragma unroll
   for (int i = 0; i < MT + NT; ++i) read_one(0, lds, i);
   int it = 0;
-  for (const int ragged = there < 8 ? steps - 1 - ST : -1; it < steps - ST; ++it) {
+  for (const int ragged = short_end ? steps - 1 - ST : -1; it < steps - ST; ++it) {
     if (it == ragged) end_rows(0, kFirstLoads);
     step(std::integral_constant<int, 2>{}, it);
   }
   if (SPAN > kM && it == steps - ST) {
-    if (there < 8) end_rows(kFirstLoads, L);
+    if (short_end) end_rows(kFirstLoads, L);
     step(std::integral_constant<int, 1>{}, it);
     ++it;
   }
@@ -189,18 +292,20 @@ wide_gemm_kernel(const DenseShape s) {
   // What lies outside the result is stored past the end of the buffer, which the hardware drops: no branches.
   constexpr uint32_t kBuffer = 0x80000000u, kNowhere = kBuffer;  // bytes
   constexpr int kRaw = 0x00020000;                               // of a buffer descriptor: bytes as they lie
-  const int wm0 = m0 + wm * 16 * MT, wn0 = n0 + wn * 16 * NT, rows = s.M - wm0, cols = s.N - wn0;  // of the wave's tile
-  // A lane has the columns 16 b + 4 h .. + 3 of row 16 a + c.
+  const int wm0 = m0 + wm * 16 * MT, wn0 = n0 + wn * (GATED ? 8 : 16) * NT, rows = s.M - wm0, cols = s.N - wn0;  // of the wave's tile
+  // A lane has the columns 16 b + 4 h .. + 3 of row 16 a + c.  Gated: those of the gate and, NT / 2 column groups later, of the up projection.
   if (s.splits > 1) {
-    float* const to = s.partials + ((int64_t)part * s.M + wm0) * s.N + wn0;
+    const int row_values = GATED ? 2 * s.N : s.N;
+    float* const to = s.partials + ((int64_t)part * s.M + wm0) * row_values + wn0;
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)kBuffer, kRaw);
     const bool whole = s.N % 4 == 0 && (reinterpret_cast<uintptr_t>(s.partials) & 15) == 0;
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
       for (int b = 0; b < NT; ++b) {
-        const int m = 16 * a + c, n = 16 * b + 4 * h;
-        const uint32_t off = (uint32_t)(m * s.N + n) * 4u;
+        const bool up = GATED && b >= NT / 2;
+        const int m = 16 * a + c, n = 16 * (up ? b - NT / 2 : b) + 4 * h;
+        const uint32_t off = (uint32_t)(m * row_values + n + (up ? s.N : 0)) * 4u;
         if (whole) {
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[a][b]), rsrc, m < rows && n < cols ? off : kNowhere, 0, 0);
         } else {
@@ -211,6 +316,62 @@ wide_gemm_kernel(const DenseShape s) {
           }
         }
       }
+    return;
+  }
+  if constexpr (GATED) {
+    constexpr int HN = NT / 2;
+    uint8_t* const ep = lds + wave * 16 * MT * (32 * HN + 16);
+    float bias[NT][4];
+#pragma unroll
+    for (int b = 0; b < NT; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[b][e] = 0.f;
+    if (s.ep.bias) {
+#pragma unroll
+      for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = min(wn0 + 16 * (b % HN) + 4 * h + e, s.N - 1) + (b >= HN ? s.N : 0);
+          bias[b][e] = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, at) : ((const float*)s.ep.bias)[at];
+        }
+    }
+    // The four values that of(a, b, v) makes of each of HN column groups leave through LDS, each wave in a part of its own: rows then leave whole.
+    auto leave = [&](auto of, void* to, int64_t ld, int first) NPAMD_INLINE {
+#pragma unroll
+      for (int b = 0; b < HN; ++b)
+#pragma unroll
+        for (int a = 0; a < MT; ++a) {
+          float v[4];
+          of(a, b, v);
+          uint32_t bits[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bits[e] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(v[e]) : f32_to_f16_bits(v[e]);
+          *reinterpret_cast<u32x2*>(ep + (16 * a + c) * (32 * HN + 16) + 32 * b + 8 * h) = u32x2{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16)};
+        }
+      uint16_t* const at = reinterpret_cast<uint16_t*>(to) + first;
+      store_rows<MT, HN>(ep, lane, at, ld, wm0, wn0, rows, cols, ld % 8 == 0 && s.N % 8 == 0 && (reinterpret_cast<uintptr_t>(at) & 15) == 0);
+    };
+    auto sums = [&](int a, int b, float (&v)[4]) NPAMD_INLINE {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[a][b][e] + bias[b][e];
+    };
+    if (s.ep.pre) {
+      leave([&](int a, int b, float (&v)[4]) NPAMD_INLINE { sums(a, b, v); }, s.ep.pre, s.ep.ldp, 0);
+      leave([&](int a, int b, float (&v)[4]) NPAMD_INLINE { sums(a, HN + b, v); }, s.ep.pre, s.ep.ldp, s.N);
+    }
+    leave(
+        [&](int a, int b, float (&v)[4]) NPAMD_INLINE {
+          float up[4];
+          sums(a, b, v);
+          sums(a, HN + b, up);
+          activate_all(s.ep.act, [&](auto f) NPAMD_INLINE {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = f(v[e]);
+          });
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= up[e];
+        },
+        s.y, s.ldy, 0);
     return;
   }
   if constexpr (EPILOGUE) {
@@ -319,37 +480,14 @@ wide_gemm_kernel(const DenseShape s) {
       *reinterpret_cast<u32x2*>(ep + (16 * a + c) * T::kEpRow + 32 * b + 8 * h) = u32x2{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16)};
     }
   }
-  uint16_t* const to = reinterpret_cast<uint16_t*>(s.y) + (int64_t)wm0 * s.ldy + wn0;
-  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)kBuffer, kRaw);
-  const uint32_t ldy = (uint32_t)s.ldy;
-  if (s.ldy % 8 == 0 && s.N % 8 == 0 && (reinterpret_cast<uintptr_t>(s.y) & 15) == 0) {
-    constexpr int kPerRow = 2 * NT, kRowsAtOnce = 64 / kPerRow;  // 16-byte pieces; NT = 3, 7: a few lanes idle
-    const int r = lane / kPerRow, p = lane % kPerRow;
-#pragma unroll 8
-    for (int i = 0; i < (16 * MT + kRowsAtOnce - 1) / kRowsAtOnce; ++i) {
-      const int m = i * kRowsAtOnce + r;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(ep + min(m, 16 * MT - 1) * T::kEpRow + p * 16);
-      const bool in = r < kRowsAtOnce && m < min(rows, 16 * MT) && p * 8 < cols;
-      __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, in ? ((uint32_t)m * ldy + (uint32_t)p * 8u) * 2u : kNowhere, 0, 0);
-    }
-    return;
-  }
-  // Rows at odd addresses: a value at a time, a row's side by side.
-#pragma unroll 8
-  for (int m = 0; m < 16 * MT; ++m) {
-#pragma unroll
-    for (int n0 = 0; n0 < 16 * NT; n0 += 64) {
-      const int n = n0 + lane;
-      const uint16_t v = *reinterpret_cast<const uint16_t*>(ep + m * T::kEpRow + min(n, 16 * NT - 1) * 2);
-      __builtin_amdgcn_raw_buffer_store_b16(v, rsrc, m < rows && n < 16 * NT && n < cols ? ((uint32_t)m * ldy + (uint32_t)n) * 2u : kNowhere, 0, 0);
-    }
-  }
+  store_rows<MT, NT>(ep, lane, s.y, s.ldy, wm0, wn0, rows, cols, s.ldy % 8 == 0 && s.N % 8 == 0 && (reinterpret_cast<uintptr_t>(s.y) & 15) == 0);
 }
 
-template <int ACT, class T, bool EPILOGUE = false>
+template <int ACT, class T, int FORM = kWidePlain, bool XK = false, bool WK = false>
 int launch_wide_tile(DenseShape s, hipStream_t st) {
+  constexpr int kColumns = FORM == kWideGated ? T::kBN / 2 : T::kBN;  // of y
   s.row_tiles = (s.M + T::kBM - 1) / T::kBM;
-  s.col_tiles = (s.N + T::kBN - 1) / T::kBN;
+  s.col_tiles = (s.N + kColumns - 1) / kColumns;
   const int64_t units = (int64_t)s.col_tiles * s.row_tiles * s.splits, blocks = (units + 7) / 8 * 8;
   if (blocks > 0x7FFFFFFF) return fail(NPAMD_ERR_UNSUPPORTED, "npamd_dense_gemm: too many tiles");
   s.units_per_die = (int)(blocks / 8);
@@ -357,9 +495,9 @@ int launch_wide_tile(DenseShape s, hipStream_t st) {
   // 2048 rows, x does not come into the L2s again for every column tile; where x is the longer side, down four row tiles, as then it is what each die would
   // bring whole.  Decode + product of int4 layers with groups of 4 tiles / of 2048 rows, us: 656 x 1452 x 4608 27.2 / 22.7, 304 x 3690 x 2048 22.9 / 18.1, 1104 x 2714
   // x 1024 19.2 / 15.3; 1440 x 970 x 8832 53.4 / 59.2, 1956 x 1532 x 11008 102.2 / 108.5, 3575 x 703 x 1536 17.3 / 20.3.
-  s.group = s.M > 1.2f * s.N ? 4 : 2048 / T::kBM;
+  s.group = s.M > 1.2f * s.N * (FORM == kWideGated ? 2 : 1) ? 4 : 2048 / T::kBM;
   static LdsLatch latch;
-  const auto kernel = wide_gemm_kernel<ACT, T, EPILOGUE>;
+  const auto kernel = wide_gemm_kernel<ACT, T, FORM, XK, WK>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), T::kLds);
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "npamd_dense_gemm: cannot reserve %d bytes of LDS: %s", T::kLds, hipGetErrorString(e));
   launch(kernel, (unsigned)blocks, T::kThreads, T::kLds, st, s);
@@ -367,22 +505,22 @@ int launch_wide_tile(DenseShape s, hipStream_t st) {
 }
 
 // Which number of the plan's list (dense_gemm.hip) is which tile.
-template <int ACT, bool EPILOGUE>
+template <int ACT, int FORM>
 int launch_wide_on(const DenseShape& s, int tile, hipStream_t st) {
   switch (tile) {
-    case 1: return launch_wide_tile<ACT, WideTile<2, 2, 2, 2, 6, 4>, EPILOGUE>(s, st);    // 64 x 64
-    case 2: return launch_wide_tile<ACT, WideTile<2, 2, 2, 4, 5, 12>, EPILOGUE>(s, st);   // 64 x 128
-    case 3: return launch_wide_tile<ACT, WideTile<2, 2, 4, 4, 4, 24>, EPILOGUE>(s, st);   // 128 x 128
-    case 4: return launch_wide_tile<ACT, WideTile<2, 2, 5, 4, 4, 24>, EPILOGUE>(s, st);   // 160 x 128
-    case 5: return launch_wide_tile<ACT, WideTile<4, 2, 4, 4, 3, 24>, EPILOGUE>(s, st);   // 256 x 128
-    case 6: return launch_wide_tile<ACT, WideTile<4, 2, 3, 4, 3, 20>, EPILOGUE>(s, st);   // 192 x 128
-    case 7: return launch_wide_tile<ACT, WideTile<2, 2, 3, 4, 4, 20>, EPILOGUE>(s, st);   // 96 x 128
-    case 8: return launch_wide_tile<ACT, WideTile<2, 4, 5, 4, 3, 24>, EPILOGUE>(s, st);   // 160 x 256
-    case 9: return launch_wide_tile<ACT, WideTile<2, 4, 6, 4, 2, 20>, EPILOGUE>(s, st);   // 192 x 256
-    case 10: return launch_wide_tile<ACT, WideTile<4, 2, 4, 7, 2, 24>, EPILOGUE>(s, st);  // 256 x 224
-    case 11: return launch_wide_tile<ACT, WideTile<2, 4, 8, 4, 2, 24>, EPILOGUE>(s, st);  // 256 x 256
-    case 12: return launch_wide_tile<ACT, WideTile<2, 2, 3, 2, 6, 6>, EPILOGUE>(s, st);   // 96 x 64
-    default: return launch_wide_tile<ACT, WideTile<2, 4, 6, 3, 3, 24>, EPILOGUE>(s, st);  // 192 x 192
+    case 1: return launch_wide_tile<ACT, WideTile<2, 2, 2, 2, 6, 4>, FORM>(s, st);    // 64 x 64
+    case 2: return launch_wide_tile<ACT, WideTile<2, 2, 2, 4, 5, 12>, FORM>(s, st);   // 64 x 128
+    case 3: return launch_wide_tile<ACT, WideTile<2, 2, 4, 4, 4, 24>, FORM>(s, st);   // 128 x 128
+    case 4: return launch_wide_tile<ACT, WideTile<2, 2, 5, 4, 4, 24>, FORM>(s, st);   // 160 x 128
+    case 5: return launch_wide_tile<ACT, WideTile<4, 2, 4, 4, 3, 24>, FORM>(s, st);   // 256 x 128
+    case 6: return launch_wide_tile<ACT, WideTile<4, 2, 3, 4, 3, 20>, FORM>(s, st);   // 192 x 128
+    case 7: return launch_wide_tile<ACT, WideTile<2, 2, 3, 4, 4, 20>, FORM>(s, st);   // 96 x 128
+    case 8: return launch_wide_tile<ACT, WideTile<2, 4, 5, 4, 3, 24>, FORM>(s, st);   // 160 x 256
+    case 9: return launch_wide_tile<ACT, WideTile<2, 4, 6, 4, 2, 20>, FORM>(s, st);   // 192 x 256
+    case 10: return launch_wide_tile<ACT, WideTile<4, 2, 4, 7, 2, 24>, FORM>(s, st);  // 256 x 224
+    case 11: return launch_wide_tile<ACT, WideTile<2, 4, 8, 4, 2, 24>, FORM>(s, st);  // 256 x 256
+    case 12: return launch_wide_tile<ACT, WideTile<2, 2, 3, 2, 6, 6>, FORM>(s, st);   // 96 x 64
+    default: return launch_wide_tile<ACT, WideTile<2, 4, 6, 3, 3, 24>, FORM>(s, st);  // 192 x 192
   }
 }
 

@@ -1379,7 +1379,14 @@ def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: boo
     return y
 
 
-from .block_joints import residual_norm, residual_norm_backward, residual_norm_stats  # noqa: E402, F401  (they use what stands above)
+from .block_joints import (  # noqa: E402, F401  (they use what stands above)
+    gated_linear,
+    gated_linear_backward,
+    gated_linear_pre,
+    residual_norm,
+    residual_norm_backward,
+    residual_norm_stats,
+)
 
 # The functions a lowered module's call plan stands in for.  Replacing one (instrumentation, a test's spy) makes the
 # plans step aside, so that the replacement is called.

@@ -1,4 +1,4 @@
-"""Between the halves of a decoder block: the residual add with the norms around it.
+"""What joins the halves of a decoder block: the residual add with the norms around it, and the gated product of a feed-forward half.
 
 Operators of the framework's own, next to ``layer_norm``, ``rms_norm`` and ``dense_linear_act``, whose rules they follow: torch's current stream, outputs of torch's
 allocator, ``RuntimeError`` for what the kernels do not take.
@@ -9,9 +9,9 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from . import _check_device, _dt, _on_device, _rows_of, tracked
+from . import ACTIVATIONS, _check_device, _dt, _on_device, _rows_of, tracked
 
-__all__ = ["residual_norm", "residual_norm_stats", "residual_norm_backward"]
+__all__ = ["residual_norm", "residual_norm_stats", "residual_norm_backward", "gated_linear", "gated_linear_pre", "gated_linear_backward"]
 
 
 def _residual_args(what, x, y, weight, post_weight, gate) -> int:
@@ -139,6 +139,107 @@ def residual_norm_backward(
     with torch.no_grad(), _on_device(y):
         tensors = [None if t is None else t.detach().contiguous() for t in (dstream, dnormed, y, stream, weight, post_weight, gate, post_rstd if post_weight is not None else None, rstd)]
         out = _lib.host().residual_norm_backward(*tensors[:7], float(scale), *tensors[7:], *(bool(n) for n in needs))
+    if out is None:
+        raise RuntimeError(f"{what}: no kernel for these tensors")
+    return out
+
+
+def _gated_args(what, x, gate_up, bias, activation) -> tuple[int, int]:
+    """Checks the arguments that the forward and the backward pass share; returns the number of rows and of columns of the output."""
+    _check_device(what, x, gate_up, bias)
+    if x.dtype not in (torch.float16, torch.bfloat16) or gate_up.dtype != x.dtype or gate_up.dim() != 2 or x.dim() < 1 or gate_up.shape[1] != x.shape[-1] or gate_up.shape[0] % 2:
+        raise RuntimeError(f"{what}: x and gate_up must be float16 or bfloat16 [..., K] and [2 N, K]")
+    if activation not in ACTIVATIONS:
+        raise RuntimeError(f"{what}: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    if x.shape[-1] < 1:
+        raise RuntimeError(f"{what}: K must be at least 1")
+    if bias is not None and (bias.dtype not in (torch.float32, x.dtype) or bias.shape != gate_up.shape[:1]):
+        raise RuntimeError(f"{what}: bias must be [2 N] in float32 or x's dtype")
+    _rows_of(what, gate_up, x.shape[-1])
+    return _rows_of(what, x, x.shape[-1]), gate_up.shape[0] // 2
+
+
+def _torch_gated_linear(x, gate_up, bias, activation):
+    f = torch.nn.functional
+    gate, up = f.linear(x, gate_up, None if bias is None else bias.to(gate_up.dtype)).chunk(2, -1)
+    if activation is not None:
+        gate = f.gelu(gate, approximate="tanh") if activation == "gelu_tanh" else getattr(f, activation)(gate)
+    return gate * up
+
+
+def _gated_linear(what, x, gate_up, bias, activation, pre):
+    rows, n = _gated_args(what, x, gate_up, bias, activation)
+    if rows == 0 or n == 0:
+        out = x.new_empty((*x.shape[:-1], n))
+        return (out, x.new_empty((*x.shape[:-1], 2 * n))) if pre else out
+    with torch.no_grad(), _on_device(x):
+        x, gate_up, bias = (None if t is None else t.detach().contiguous() for t in (x, gate_up, bias))
+        out = _lib.host().gated_linear(x, gate_up, bias, ACTIVATIONS[activation], pre)
+    if out is None:
+        raise RuntimeError(f"{what}: no kernel for these tensors")
+    return out
+
+
+def gated_linear(x: torch.Tensor, gate_up: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = "silu") -> torch.Tensor:
+    """``act(x @ gate.T + bias) * (x @ up.T + bias)`` of an fp16 / bf16 *x* ``[..., K]`` and *gate_up* ``[2 N, K]`` of its dtype, N gate rows before N up rows (as
+    :class:`MoEExperts` has them), rounded once (``npamd_gated_linear``): the first half of a gated feed-forward block in one kernel.
+
+    *activation*: as for :func:`dense_linear_act`; *bias* ``[2 N]`` in float32 or x's dtype.  Any sizes.  Where a gradient is recorded both sums are kept, rounded to x's dtype, and the
+    backward pass is :func:`gated_linear_backward`'s kernels (first derivatives; captured under the terms of :func:`layer_norm`).  Calls that torch follows in other ways go through torch's
+    own operations, which round in between.
+    """
+    code = ACTIVATIONS.get(activation)
+    out = None if code is None else _lib.host().gated_linear(x, gate_up, bias, code, False)
+    if out is not None:
+        return out
+    what = "gated_linear"
+    tensors = [t for t in (x, gate_up, bias) if t is not None]
+    if not any(tracked(t) for t in tensors):
+        return _gated_linear(what, x, gate_up, bias, activation, False)
+    rows, n = _gated_args(what, x, gate_up, bias, activation)
+    with torch.no_grad():  # what is left of it when no gradient is recorded
+        otherwise = any(tracked(t) for t in tensors)
+    if otherwise or rows == 0 or n == 0:
+        return _torch_gated_linear(x, gate_up, bias, activation)
+    return _lib.host().gated_linear_recorded(x, gate_up, bias, code)
+
+
+def gated_linear_pre(x: torch.Tensor, gate_up: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = "silu") -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`gated_linear` without a recorded gradient, and both sums ``[..., 2 N]`` in x's dtype, which :func:`gated_linear_backward` takes."""
+    code = ACTIVATIONS.get(activation)
+    out = None if code is None else _lib.host().gated_linear(x, gate_up, bias, code, True)
+    return out if out is not None else _gated_linear("gated_linear_pre", x, gate_up, bias, activation, True)
+
+
+def gated_linear_backward(
+    dh: torch.Tensor,
+    x: torch.Tensor,
+    gate_up: torch.Tensor,
+    pre: torch.Tensor,
+    activation: str | None = "silu",
+    needs: tuple[bool, bool, bool] = (True, True, True),
+    bias_dtype: torch.dtype | None = None,
+) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of x, gate_up and the bias (``npamd_gated_linear_backward``) from that of the output, in x's dtype (the bias's in *bias_dtype*, float32 or x's); None where *needs* says
+    no.  *pre*: of :func:`gated_linear_pre`.  What goes into the products is rounded to x's dtype, the products' sums are float32.  The same bits from run to run."""
+    what = "gated_linear_backward"
+    code = ACTIVATIONS.get(activation)
+    wide = bias_dtype == torch.float32
+    if bias_dtype not in (None, torch.float32, x.dtype):
+        raise RuntimeError(f"{what}: bias_dtype must be float32 or x's dtype, got {bias_dtype}")
+    out = None if code is None else _lib.host().gated_linear_backward(dh, x, gate_up, pre, code, wide, *needs)
+    if out is not None:
+        return out
+    rows, n = _gated_args(what, x, gate_up, None, activation)
+    _check_device(what, x, dh, pre)
+    if dh.dtype != x.dtype or pre.dtype != x.dtype or dh.shape != (*x.shape[:-1], n) or pre.shape != (*x.shape[:-1], 2 * n):
+        raise RuntimeError(f"{what}: dh and pre must be [..., N] and [..., 2 N] in x's dtype")
+    if rows == 0 or n == 0:
+        made = (lambda: torch.zeros_like(x), lambda: torch.zeros_like(gate_up), lambda: torch.zeros(2 * n, device=x.device, dtype=bias_dtype or x.dtype))
+        return tuple(make() if need else None for make, need in zip(made, needs))
+    with torch.no_grad(), _on_device(x):
+        dh, x, gate_up, pre = (t.detach().contiguous() for t in (dh, x, gate_up, pre))
+        out = _lib.host().gated_linear_backward(dh, x, gate_up, pre, code, wide, *(bool(need) for need in needs))
     if out is None:
         raise RuntimeError(f"{what}: no kernel for these tensors")
     return out

@@ -44,10 +44,43 @@ def test_workspace_of_the_residual_norm_grows_with_neither_rows_nor_sequences():
         assert size(2**31 - 1, 64, 2, dtype) <= 3 * 256 * 64 * 4
 
 
+@no_gpu
+def test_gated_linear_refuses():
+    far = 1 << 31
+    ok = dict(x=P, ldx=64, w=P, ldw=64, b=P, bdt=2, act=4, y=P, ldy=32, pre=P, ldp=64, m=70, n=32, k=64, dtype=0, ws=None, wsn=0, st=None)
+    for change, match in [(dict(k=0), "bad shape"), (dict(m=-1), "bad shape"), (dict(n=-1), "bad shape"), (dict(dtype=2), "f16 or bf16"), (dict(bdt=1), "bias"), (dict(act=5), "activation"),
+                          (dict(act=-1), "activation"), (dict(ldx=63), "stride"), (dict(ldw=63), "stride"), (dict(ldp=63), "stride"), (dict(ldy=31), "stride"), (dict(x=None), "null"),
+                          (dict(w=None), "null"), (dict(y=None), "null"), (dict(x=P + 2), "16-byte"), (dict(ldw=65), "16-byte"), (dict(k=63), "16-byte"), (dict(ldx=1 << 22), "16-byte"),
+                          (dict(ws=P + 4), "16-byte")]:  # fmt: skip
+        _refused("npamd_gated_linear", *{**ok, **change}.values(), match=match)
+    for change, match in [(dict(n=2**24 + 1, ldy=far, ldp=far), "at most"), (dict(k=2**30 + 1, ldx=far, ldw=far), "at most"), (dict(ldy=1 << 22), "less than"), (dict(ldp=1 << 22), "less than")]:
+        _refused("npamd_gated_linear", *{**ok, **change}.values(), match=match, code=-2)
+    for m, n in ((0, 32), (70, 0)):
+        assert _lib.load().npamd_gated_linear(*{**ok, "m": m, "n": n, "x": None}.values()) == 0
+    size = _lib.load().npamd_gated_linear_workspace_bytes
+    assert size(0, 32, 64) == 0 == size(70, 2**24 + 1, 64) == size(1, 32, 64) and size(70, 64, 8192) > 0
+
+
+@no_gpu
+def test_gated_linear_backward_refuses():
+    size = _lib.load().npamd_gated_linear_backward_workspace_bytes
+    need = size(70, 32, 64, 1, 1, 1)
+    assert need > 0 and size(0, 32, 64, 1, 1, 1) == 0
+    ok = dict(dh=P, lddh=32, x=P, ldx=64, w=P, ldw=64, pre=P, ldp=64, act=4, dx=P, lddx=64, dw=P, lddw=64, db=P, bdt=2, m=70, n=32, k=64, dtype=0, ws=P, wsn=need, st=None)
+    for change, match in [(dict(m=0), "bad shape"), (dict(n=0), "bad shape"), (dict(k=0), "bad shape"), (dict(dtype=2), "f16 or bf16"), (dict(bdt=1), "bias"), (dict(act=5), "activation"),
+                          (dict(lddh=31), "stride"), (dict(ldp=63), "stride"), (dict(ldx=63), "stride"), (dict(ldw=63), "stride"), (dict(lddx=63), "stride"), (dict(lddw=63), "stride"),
+                          (dict(dh=None), "null"), (dict(pre=None), "null"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(x=P + 2), "16-byte"), (dict(w=P + 8), "16-byte"),
+                          (dict(ldx=66), "16-byte"), (dict(ldw=1 << 22), "16-byte"), (dict(ws=None), "workspace"), (dict(ws=P + 8), "workspace"), (dict(wsn=need - 1), "workspace")]:  # fmt: skip
+        _refused("npamd_gated_linear_backward", *{**ok, **change}.values(), match=match)
+    for change in (dict(lddx=1 << 22), dict(lddw=1 << 22)):
+        _refused("npamd_gated_linear_backward", *{**ok, **change}.values(), match="less than", code=-2)
+
+
 def test_wrappers_refuse_what_is_not_on_a_gpu():
     from neuropress_amd import kernels
 
     x, w = torch.randn(2, 64).half(), torch.randn(64).half()
-    for call in (lambda: kernels.residual_norm(x, x, w), lambda: kernels.residual_norm_stats(x, x, w), lambda: kernels.residual_norm_backward(x, x, x, x, w, None, None, 1.0, None, w)):
+    for call in (lambda: kernels.residual_norm(x, x, w), lambda: kernels.residual_norm_stats(x, x, w), lambda: kernels.residual_norm_backward(x, x, x, x, w, None, None, 1.0, None, w),
+                 lambda: kernels.gated_linear(x, x), lambda: kernels.gated_linear_pre(x, x), lambda: kernels.gated_linear_backward(x[:, :1], x, x, x[:, :2])):  # fmt: skip
         with pytest.raises(RuntimeError, match="GPU"):
             call()
