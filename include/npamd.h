@@ -603,6 +603,17 @@ int npamd_gated_linear_backward(const void* dh, int64_t lddh, const void* x, int
                                 void* workspace, int64_t workspace_bytes, void* stream);
 int64_t npamd_gated_linear_backward_workspace_bytes(int M, int N, int K, int dx, int dgate_up, int dbias);
 
+/*
+ * Low-rank adapters of many requests beside a projection that they share: y[m] = base[m] + scale[i] * (x[m] A_i^T) B_i^T with i = ids[m]; y[m] = base[m], bit for bit, where ids[m] is not in
+ * 0 .. adapters - 1.  x [M, K], base (NULL: zero), y [M, N], a [adapters, rank, K], b: act_dtype (NPAMD_F16 or NPAMD_BF16); ids [M]: integers of ids_bits 32 or 64; scale: NULL (1), or f32
+ * [adapters].  b: [adapters, N, rank rounded up to a multiple of eight], zeros past the rank, at a 16-byte address.  f32 sums; x A^T is held to 2^-16 (bf16) or 2^-21 (f16); y is rounded
+ * once.  y may be base (with the same row distance).  K at least 8, rank at most 256, at most 8192 adapters, 2^22 tokens, 2^24 columns of y; any alignment but b's.
+ * workspace: npamd_adapter_linear_workspace_bytes bytes of 16-byte aligned device memory, contents irrelevant; calls that overlap must not share one.
+ */
+int npamd_adapter_linear(const void* x, int64_t ldx, const void* ids, int ids_bits, const void* a, const void* b, const float* scale, const void* base, int64_t ldbase,
+                         void* y, int64_t ldy, int M, int N, int K, int rank, int adapters, int act_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t npamd_adapter_linear_workspace_bytes(int M, int N, int K, int rank, int adapters);
+
 #ifdef __cplusplus
 }
 #endif

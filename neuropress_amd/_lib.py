@@ -86,6 +86,8 @@ SIGNATURES: dict[str, list] = {
     "npamd_gated_linear_workspace_bytes": [_int] * 3,
     "npamd_gated_linear_backward": [_vp, _i64] * 4 + [_int, _vp, _i64, _vp, _i64, _vp, _int, _int, _int, _int, _int, _vp, _i64, _vp],
     "npamd_gated_linear_backward_workspace_bytes": [_int] * 6,
+    "npamd_adapter_linear": [_vp, _i64, _vp, _int, _vp, _vp, _vp, _vp, _i64, _vp, _i64] + [_int] * 6 + [_vp, _i64, _vp],
+    "npamd_adapter_linear_workspace_bytes": [_int] * 5,
     "npamd_dense_gemm_preferred": [_int, _int, _int],
     "npamd_gemv_blocks_preferred": [_int] * 7,
     "npamd_gather_columns": [_vp, _i64, _vp, _vp, _i64, _int, _int, _vp],
@@ -103,6 +105,7 @@ _RESTYPES = {"npamd_vq_sliced_workspace_bytes": _i64, "npamd_gemm_tile_workspace
              "npamd_vq_slice_workspace_bytes": _i64, "npamd_layer_norm_workspace_bytes": _i64, "npamd_dense_gemm_act_workspace_bytes": _i64,
              "npamd_moe_workspace_bytes": _i64, "npamd_residual_norm_workspace_bytes": _i64,
              "npamd_gated_linear_workspace_bytes": _i64, "npamd_gated_linear_backward_workspace_bytes": _i64,
+             "npamd_adapter_linear_workspace_bytes": _i64,
              "npamd_diag_reload_tuning": None}
 SLICED_HEADER_BYTES = 128
 SLICED_STATIC_WORKSPACE_BYTES = 4 * 1024 * 1024

@@ -1,4 +1,4 @@
-// The functions that join a decoder block's halves (residual norm, gated product, their backward passes), issued from native code.
+// The functions that join a decoder block's halves (residual norm, gated product, their backward passes, low-rank adapters), issued from native code.
 //
 // As in feed_forward.hpp the functions that Python tries first return None for what is not as the kernels want it; Python then checks, reports, copies, and calls them again.
 // What the library refuses is an error at once.
@@ -353,6 +353,37 @@ PyObject* gated_linear_recorded(PyObject*, PyObject* const* args, Py_ssize_t n) 
   }
   return translated([&]() -> PyObject* {
     return THPVariable_Wrap(GatedLinearNode::apply(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), maybe_tensor(args[2]), (int64_t)activation_of(args[3])));
+  });
+}
+
+// adapter_linear(x, ids, a, b, scale, base, columns of y): y, or None; a, b and scale are those of LowRankAdapters, which has checked them
+PyObject* adapter_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "adapter_linear(x, ids, a, b, scale, base, columns)");
+    return nullptr;
+  }
+  return translated([&]() -> PyObject* {
+    const int device = device_of(args[0]);
+    Rows x, base{nullptr, 0, 0, 0, 0};
+    if (!rows_argument(args[0], device, &x) || !PyLong_Check(args[6])) Py_RETURN_NONE;
+    const at::Tensor *ids = readable(args[1], device), *a = readable(args[2], device), *b = readable(args[3], device);
+    if (!ids || !a || !b || !ids->is_contiguous() || ids->sizes() != x.t->sizes().slice(0, x.t->dim() - 1) ||
+        (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong)) Py_RETURN_NONE;
+    if (a->scalar_type() != x.t->scalar_type() || a->size(2) != x.width) Py_RETURN_NONE;
+    const void* scale;
+    if (!vector_of(args[4], device, at::kFloat, a->size(0), &scale)) Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 6> sizes(x.t->sizes().begin(), x.t->sizes().end());
+    sizes.back() = PyLong_AsLong(args[6]);
+    if (sizes.back() < 1 || sizes.back() > INT32_MAX) Py_RETURN_NONE;
+    if (!is_none(args[5]) && (!rows_argument(args[5], device, &base) || base.code != x.code || base.t->sizes() != at::IntArrayRef(sizes))) Py_RETURN_NONE;
+    const int m = (int)x.m, cols = (int)sizes.back(), k = (int)x.width, rank = (int)a->size(1), adapters = (int)a->size(0);
+    const int64_t bytes = npamd_adapter_linear_workspace_bytes(m, cols, k, rank, adapters);
+    at::Tensor scratch, y = empty(sizes, x.t->scalar_type(), device);
+    if (bytes > 0) scratch = floats(bytes, device);
+    TORCH_CHECK(npamd_adapter_linear(x.t->const_data_ptr(), x.ld, ids->const_data_ptr(), ids->scalar_type() == at::kInt ? 32 : 64, a->const_data_ptr(), b->const_data_ptr(),
+                                     (const float*)scale, base.t ? base.t->const_data_ptr() : nullptr, base.ld, y.data_ptr(), cols, m, cols, k, rank, adapters, x.code,
+                                     out_or_null(scratch), bytes, current_stream(device)) == NPAMD_OK, npamd_last_error());
+    return THPVariable_Wrap(std::move(y));
   });
 }
 

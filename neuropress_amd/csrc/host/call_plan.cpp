@@ -907,6 +907,7 @@ PyMethodDef module_methods[] = {
     {"gated_linear", fast(gated_linear), METH_FASTCALL, "gated_linear(x, gate_up, bias, activation, pre): the output (with the sums), or None"},
     {"gated_linear_recorded", fast(gated_linear_recorded), METH_FASTCALL, "gated_linear_recorded(x, gate_up, bias, activation): the output, with its node"},
     {"gated_linear_backward", fast(gated_linear_backward), METH_FASTCALL, "gated_linear_backward(dh, x, gate_up, pre, activation, 4 booleans): the gradients, or None"},
+    {"adapter_linear", fast(adapter_linear), METH_FASTCALL, "adapter_linear(x, ids, a, b, scale, base, columns): the output, or None"},
     {"tracked", tracked_tensor, METH_O, "tracked(x): whether torch follows what is done to x, so that no plan issues the call"},
     {"row_distance", row_distance, METH_O, "row_distance(x): elements between the rows a plan would read, or None"},
     {"set_module_class", set_module_class, METH_VARARGS, "set_module_class(torch.nn.Module, its call in Python)"},

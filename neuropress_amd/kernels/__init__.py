@@ -1380,6 +1380,8 @@ def moe_layer(x: torch.Tensor, experts: MoEExperts, top_k: int, renormalize: boo
 
 
 from .block_joints import (  # noqa: E402, F401  (they use what stands above)
+    LowRankAdapters,
+    adapter_linear,
     gated_linear,
     gated_linear_backward,
     gated_linear_pre,

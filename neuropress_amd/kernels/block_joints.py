@@ -1,4 +1,5 @@
-"""What joins the halves of a decoder block: the residual add with the norms around it, and the gated product of a feed-forward half.
+"""What joins the halves of a decoder block: the residual add with the norms around it, the gated product of a feed-forward half, and
+low-rank adapters beside a projection.
 
 Operators of the framework's own, next to ``layer_norm``, ``rms_norm`` and ``dense_linear_act``, whose rules they follow: torch's current stream, outputs of torch's
 allocator, ``RuntimeError`` for what the kernels do not take.
@@ -9,9 +10,10 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from . import ACTIVATIONS, _check_device, _dt, _on_device, _rows_of, tracked
+from . import ACTIVATIONS, _check_device, _dt, _on_device, _rows_of, gather_columns, tracked
 
-__all__ = ["residual_norm", "residual_norm_stats", "residual_norm_backward", "gated_linear", "gated_linear_pre", "gated_linear_backward"]
+__all__ = ["residual_norm", "residual_norm_stats", "residual_norm_backward", "gated_linear", "gated_linear_pre", "gated_linear_backward", "LowRankAdapters",
+           "adapter_linear"]  # fmt: skip
 
 
 def _residual_args(what, x, y, weight, post_weight, gate) -> int:
@@ -243,3 +245,72 @@ def gated_linear_backward(
     if out is None:
         raise RuntimeError(f"{what}: no kernel for these tensors")
     return out
+
+
+class LowRankAdapters:
+    """The adapters of one projection, checked and laid out once, for :func:`adapter_linear`.
+
+    *a* ``[L, r, K]`` and *b* ``[L, N, r]`` in float16 or bfloat16, *scale* float32 ``[L]`` or None (1): adapter i adds ``scale[i] * (x @ a[i].T) @ b[i].T``.  Ranks up to 256, up to
+    8192 adapters.  Ranks that are no multiple of eight are padded (a copy of *b*); otherwise the tensors are kept as they are.
+    """
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor | None = None):
+        what = "LowRankAdapters"
+        _check_device(what, a, b, scale)
+        if a.dtype not in (torch.float16, torch.bfloat16) or b.dtype != a.dtype or a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise RuntimeError(f"{what}: a and b must be float16 or bfloat16 [L, r, K] and [L, N, r]")
+        if min(*a.shape, *b.shape) < 1:
+            raise RuntimeError(f"{what}: at least one adapter, rank, column and row, got {list(a.shape)} and {list(b.shape)}")
+        if scale is not None and (scale.dtype != torch.float32 or scale.shape != a.shape[:1]):
+            raise RuntimeError(f"{what}: scale must be float32 [L]")
+        self.adapters, self.rank, self.in_features = a.shape
+        self.out_features = b.shape[1]
+        if self.rank > 256 or self.adapters > 8192:
+            raise RuntimeError(f"{what}: ranks up to 256 and up to 8192 adapters, got {self.rank} and {self.adapters}")
+        a, b = a.detach(), b.detach()
+        if self.rank % 8:
+            b = torch.nn.functional.pad(b, (0, -self.rank % 8))
+        if self.in_features < 8:  # the kernels read pieces of eight columns
+            a = torch.nn.functional.pad(a, (0, 8 - self.in_features))
+        b = b.contiguous()
+        self.a, self.b = a.contiguous(), b if b.data_ptr() % 16 == 0 else b.clone()
+        self.scale = None if scale is None else scale.detach().contiguous()
+
+
+def adapter_linear(x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor, base: torch.Tensor | None = None) -> torch.Tensor:
+    """``base + scale[i] * (x @ a[i].T) @ b[i].T`` with i each token's adapter (``npamd_adapter_linear``): the adapters of many requests at once, next to a projection of *x*
+    ``[..., K]`` that they share, whose output is *base* ``[..., N]`` (None: zero).
+
+    *ids*: int32 or int64, one for each token (x's dimensions but the last) or for each of the first of x's dimensions (``[B]`` for x ``[B, T, K]``); a number that is no adapter's, such as
+    -1, leaves its tokens' base as it is.  Tokens may come in any order; each adapter's weights are read once for up to 16 tokens of a decode step or 128 of a prompt.  For inference: calls that torch
+    follows (:func:`tracked`) are refused.
+    """
+    y = None
+    if adapters.in_features >= 8:
+        y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, base, adapters.out_features)
+    if y is not None:
+        return y
+    what = "adapter_linear"
+    _check_device(what, x, ids, base, adapters.a)
+    k, n = adapters.in_features, adapters.out_features
+    if x.dtype != adapters.a.dtype or x.dim() < 1 or x.shape[-1] != k:
+        raise RuntimeError(f"{what}: x must be {adapters.a.dtype} [..., {k}], got {x.dtype} {list(x.shape)}")
+    lead = x.shape[:-1]
+    if ids.dtype not in (torch.int32, torch.int64) or ids.shape != lead[: ids.dim()]:
+        raise RuntimeError(f"{what}: ids must be int32 or int64, one for each token or for each of the first of x's dimensions, got {ids.dtype} {list(ids.shape)}")
+    if base is not None and (base.dtype != x.dtype or base.shape != (*lead, n)):
+        raise RuntimeError(f"{what}: base must be {[*lead, n]} in x's dtype")
+    if tracked(x) or (base is not None and tracked(base)):
+        raise RuntimeError(f"{what}: for inference only: no gradient, trace or transform of torch can follow it")
+    rows = _rows_of(what, x, k)
+    if rows > 1 << 22 or n > 1 << 24:
+        raise RuntimeError(f"{what}: at most 2**22 tokens and 2**24 columns, got {rows} and {n}")
+    if rows == 0:
+        return x.new_empty((*lead, n))
+    with torch.no_grad(), _on_device(x):
+        ids = ids.reshape(*ids.shape, *[1] * (len(lead) - ids.dim())).expand(lead).contiguous()
+        x = x.detach().contiguous() if k >= 8 else gather_columns(x.detach().reshape(rows, k), None, 8).view(*lead, 8)
+        y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, None if base is None else base.detach().contiguous(), n)
+    if y is None:
+        raise RuntimeError(f"{what}: no kernel for these tensors")
+    return y

@@ -35,6 +35,24 @@ def test_residual_norm_refuses():
         _refused("npamd_residual_norm_backward", *{**ok, **change}.values(), match=match)
 
 
+@no_gpu
+def test_adapter_linear_refuses():
+    size = _lib.load().npamd_adapter_linear_workspace_bytes
+    for m in (1, 64, 65, 5000):
+        need = size(m, 72, 64, 12, 4)
+        ok = dict(x=P, ldx=64, ids=P, bits=32, a=P, b=P, scale=P, base=P, ldb=72, y=P, ldy=72, m=m, n=72, k=64, r=12, l=4, dtype=0, ws=P, wsn=need, st=None)
+        for change, match in [(dict(m=-1), "bad shape"), (dict(n=-1), "bad shape"), (dict(k=0), "bad shape"), (dict(r=0), "bad shape"), (dict(l=0), "bad shape"), (dict(dtype=2), "f16 or bf16"),
+                              (dict(bits=16), "32 or 64"), (dict(ldx=63), "stride"), (dict(ldy=71), "stride"), (dict(ldb=71), "stride"), (dict(x=None), "null"), (dict(ids=None), "null"),
+                              (dict(a=None), "null"), (dict(b=None), "null"), (dict(y=None), "null"), (dict(b=P + 8), "16-byte"), (dict(ws=None), "workspace"), (dict(ws=P + 4), "workspace"),
+                              (dict(wsn=need - 1), "workspace")]:  # fmt: skip
+            _refused("npamd_adapter_linear", *{**ok, **change}.values(), match=match)
+        for change in (dict(k=7), dict(r=257), dict(l=8193), dict(m=2**22 + 1), dict(n=2**24 + 1, ldy=1 << 25, ldb=1 << 25)):
+            _refused("npamd_adapter_linear", *{**ok, **change}.values(), match="at most", code=-2)
+        for change in (dict(m=0), dict(n=0)):
+            assert _lib.load().npamd_adapter_linear(*{**ok, **change, "x": None, "ws": None}.values()) == 0
+    assert size(0, 72, 64, 12, 4) == 0 == size(4, 72, 64, 257, 4) == size(4, 72, 64, 12, 8193)
+
+
 def test_workspace_of_the_residual_norm_grows_with_neither_rows_nor_sequences():
     size = _lib.load().npamd_residual_norm_workspace_bytes
     for dtype in (0, 1, 2):
@@ -80,7 +98,23 @@ def test_wrappers_refuse_what_is_not_on_a_gpu():
     from neuropress_amd import kernels
 
     x, w = torch.randn(2, 64).half(), torch.randn(64).half()
+    with pytest.raises(RuntimeError, match="GPU"):
+        kernels.LowRankAdapters(x[None], x[None])
     for call in (lambda: kernels.residual_norm(x, x, w), lambda: kernels.residual_norm_stats(x, x, w), lambda: kernels.residual_norm_backward(x, x, x, x, w, None, None, 1.0, None, w),
                  lambda: kernels.gated_linear(x, x), lambda: kernels.gated_linear_pre(x, x), lambda: kernels.gated_linear_backward(x[:, :1], x, x, x[:, :2])):  # fmt: skip
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+def test_attaching_adapters_to_what_is_not_there():
+    from neuropress_amd.nn import NPAdapterLinear, attach_adapters, set_adapter_ids
+
+    model = torch.nn.Sequential(torch.nn.Linear(4, 4))
+    for name in ("1", "0.weight", "a.b", ""):
+        with pytest.raises(RuntimeError, match="no module|itself"):
+            attach_adapters(model, {"0": None, name: None})
+        assert isinstance(model[0], torch.nn.Linear)
+    layer = NPAdapterLinear(model[0], None)  # without ids it is the projection
+    set_adapter_ids(torch.nn.Sequential(layer), None)
+    x = torch.randn(3, 4)
+    assert torch.equal(layer(x), model[0](x)) and set(layer.state_dict()) == {"base.weight", "base.bias"}
