@@ -3,13 +3,18 @@
 // Two products whose weights depend on the token.  Tokens of one adapter meet its weights as the columns of MFMAs (16x16x32), so both kernels work on entries: an adapter and some of its
 // tokens.  Up to 64 tokens every wave finds its entry's tokens by itself from the ids (one comparison of all of them and a count of bits), so a call is two launches; past that a
 // block of one launch more sorts tokens by adapter and lists the entries.
-//   down: t = x A^T, f32.  A block takes an entry's tokens, 16 to 64 ranks and (where rows are long) a part of K, which its waves share; their sums meet in LDS.
-//   up:   y = base + scale t B^T.  A wave takes 64 columns: B's rows are dealt to the MFMAs' rows so that a lane ends up with 16 neighbouring columns of one token, whose base it reads and whose y
-//         it writes as they lie.  t is not rounded to 16 bits: it is two parts of B's type (2^-16 of it left with bf16; fp16, scaled by a power of two to the row's largest, 2^-21), an MFMA each.
+//   down: t = x A^T, f32.  Few tokens: a wave (or a block's four) streams a row of A into registers, as the dense product of one or two tokens does.  More: a block takes 32 tokens of an entry,
+//         up to 64 ranks and a part of K, x and A come into LDS in whole lines, each wave with steps of its own; the waves' sums meet in LDS.
+//   up:   y = base + scale t B^T.  A block brings its entry's t into LDS once, as two parts of B's type, for an MFMA each (t is not rounded to 16 bits: 2^-16 of it is left with bf16; fp16, scaled
+//         by a power of two to the row's largest, 2^-21), and its waves take 64 or 128 columns each.  Column 8 c + b of a wave is row c of MFMA b, so that a lane ends up with eight neighbouring columns
+//         of four tokens and 16 lanes with 256 bytes of a row of base and y, side by side.  (With four tokens' rows in every quarter of the lanes instead, as the MFMAs' own layout
+//         has them, a load touches 64 places: 64 to 86 us in the place of XX for 4096 tokens through 14336 columns.)
 // Bound by the latency of two dependent launches for a decode step, by the bytes of base and y for prompts.
 #include <algorithm>
 
 #include "common.hpp"
+#include "gemm_tile.hpp"
+#include "lds_transfer.hpp"
 #include "wave_ops.hpp"
 
 using namespace npamd;
@@ -28,7 +33,7 @@ struct AdapterArgs {
   const void *x, *ids, *a, *b, *base;
   const float* scale;
   void* y;
-  int64_t ldx, ldbase, ldy;
+  int64_t ldx, lda, ldbase, ldy;
   int M, N, K, rank, rank8, adapters, ids_64, parts;
   float* t;              // [parts][M][rank8]
   const int* order;      // listed entries
@@ -43,10 +48,10 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int m) {
   return id >= 0 && id < a.adapters ? (int)id : -1;
 }
 
-// An entry as a wave holds it: lane c of each 16 lanes knows tokens c, 16 + c, ... of it.
+// An entry as a wave holds it.
 struct Tokens {
   int adapter, first, count;  // count 0: no entry
-  int mine;                   // ballot: the lane's token, valid below count
+  int mine;                   // of up to 64 tokens: the entry's token number lane % 16, valid below count
 };
 
 // Block `e` of up to 64 tokens has an entry if token e is the first, 17th, 33rd ... of its adapter.
@@ -69,97 +74,175 @@ __device__ __forceinline__ Tokens listed_entry(const AdapterArgs& a, int e) {
   return {__builtin_amdgcn_readfirstlane(v.adapter), __builtin_amdgcn_readfirstlane(v.first), __builtin_amdgcn_readfirstlane(v.count), 0};
 }
 
-// TG groups of 16 tokens, RG of 16 ranks; blockIdx.x: entry (and its part of 32 tokens), .y: ranks, .z: part of K.  Any K of at least eight and any address: a row that does not end with a
-// piece of eight has its last one end with the row, and the values that the piece before has too are zeroed in both operands.
-template <int ACT, int TG, int RG, bool LISTED>
-__global__ void __launch_bounds__(1024) adapter_down_kernel(const AdapterArgs a) {
-  extern __shared__ __attribute__((aligned(16))) float down_sums[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, c = lane & 15, h = lane >> 4;
-  Tokens e;
-  if constexpr (LISTED) {
-    const int pieces = a.entry_tokens / kDownTokens, part = blockIdx.x % pieces;
-    e = listed_entry(a, blockIdx.x / pieces);
-    e.first += part * kDownTokens;
-    e.count = min(e.count - part * kDownTokens, kDownTokens);
-  } else {
-    e = ballot_entry(a, blockIdx.x);
+// Few tokens: KS of a block's four waves to a row of A, TB tokens at a time.  Any K of at least eight and any address of x: a row that does not end with a piece of eight has its last one end
+// with the row, and the values that the piece before has too are zeroed in both operands.  blockIdx.x: entry, .y: ranks, those that only fill B's rows up among them.
+template <int ACT, int TB>
+__device__ __forceinline__ void few_sums(const uint16_t* ar, const uint16_t* const (&xr)[TB], int K, int first, int last, float (&acc)[TB]) {
+  constexpr int U = TB == 1 ? 8 : 4;  // pieces on their way
+  const int lane = threadIdx.x & 63, pieces = (K + 7) / 8, tail = pieces * 8 - K;
+  auto at = [&](int p) { return min(p * 8, K - 8); };
+  auto blank = [&](u32x4& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < tail) v[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+  };
+#pragma unroll
+  for (int t = 0; t < TB; ++t) acc[t] = 0.f;
+  for (int p0 = first; p0 < last; p0 += U * 64) {
+    u32x4 av[U], xv[U][TB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int p = p0 + u * 64 + lane;
+      av[u] = u32x4{0, 0, 0, 0};
+      if (p < last) av[u] = *reinterpret_cast<const u32x4_any*>(ar + at(p));
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        xv[u][t] = u32x4{0, 0, 0, 0};
+        if (p < last) xv[u][t] = *reinterpret_cast<const u32x4_any*>(xr[t] + at(p));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool ends = tail && p0 + u * 64 + lane == pieces - 1;
+      if (ends) blank(av[u]);
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        if (ends) blank(xv[u][t]);
+        acc[t] = add_dot8<ACT>(av[u], xv[u][t], acc[t]);
+      }
+    }
   }
+}
+
+template <int ACT, int KS>
+__global__ void __launch_bounds__(256) adapter_few_kernel(const AdapterArgs a) {
+  __shared__ float sums[4][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS;
+  const Tokens e = ballot_entry(a, blockIdx.x);
   if (e.count <= 0 || e.adapter < 0) return;
-  int token[TG];
+  const int r = blockIdx.y * (4 / KS) + wave / KS;
+  const uint16_t* const ar = (const uint16_t*)a.a + ((int64_t)e.adapter * a.rank + min(r, a.rank - 1)) * a.lda;
+  const int pieces = (a.K + 7) / 8, turns = (pieces + 63) / 64, first = turns * part / KS * 64, last = min(turns * (part + 1) / KS * 64, pieces);
+  for (int j = 0; j < e.count; j += 4) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint16_t* xr[4];
 #pragma unroll
-  for (int g = 0; g < TG; ++g) {  // past the entry's end: its last token, not stored
-    const int at = min(16 * g + c, e.count - 1);
-    token[g] = LISTED ? a.order[e.first + at] : __builtin_amdgcn_ds_bpermute(at * 4, e.mine);
+    for (int t = 0; t < 4; ++t) xr[t] = (const uint16_t*)a.x + __builtin_amdgcn_readlane(e.mine, min(j + t, e.count - 1)) * a.ldx;
+    if (e.count - j == 1) {
+      const uint16_t* const one[1] = {xr[0]};
+      float sum[1];
+      few_sums<ACT, 1>(ar, one, a.K, first, last, sum);
+      acc[0] = sum[0];
+    } else {
+      few_sums<ACT, 4>(ar, xr, a.K, first, last, acc);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const float v = wave_sum_last(acc[t]);
+      if (lane == 63) sums[wave][t] = v;
+    }
+    __syncthreads();
+    const int token = __builtin_amdgcn_ds_bpermute(min(j + lane, e.count - 1) * 4, e.mine);  // of all lanes: those that give have to take part
+    if (part == 0 && lane < 4 && j + lane < e.count && r < a.rank8) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) v += sums[wave + i][lane];
+      a.t[(int64_t)token * a.rank8 + r] = r < a.rank ? v : 0.f;
+    }
+    __syncthreads();
   }
-  const int r0 = blockIdx.y * 16 * RG;
-  const uint16_t *xr[TG], *ar[RG];
-#pragma unroll
-  for (int g = 0; g < TG; ++g) xr[g] = (const uint16_t*)a.x + token[g] * a.ldx;
-#pragma unroll
-  for (int q = 0; q < RG; ++q) ar[q] = (const uint16_t*)a.a + ((int64_t)e.adapter * a.rank + min(r0 + 16 * q + c, a.rank - 1)) * a.K;
-  const int pieces = (a.K + 7) / 8, tail = pieces * 8 - a.K, steps = (pieces + 3) / 4;
+}
+
+// Listed entries: RG groups of 16 ranks of 32 tokens; blockIdx.x: entry and its part of 32 tokens, .y: ranks, .z: part of K.  A wave takes every so manieth 64-k step of the part, in two places of its
+// own in LDS: rows of 128 bytes, 16-byte piece p of row r in place p ^ ((r >> 1) & 7).  Tokens' rows come from wherever they are.
+template <int RG>
+struct DownTile {
+  static constexpr int kRows = kDownTokens + 16 * RG, kPlace = kRows * 128, kSums = 2 * RG * 1024;
+  static constexpr int kWaves = kLdsPerBlockMax / (2 * kPlace) < 8 ? kLdsPerBlockMax / (2 * kPlace) : 8;
+  static constexpr int lds(int waves) { return waves * 2 * kPlace; }
+  static_assert(2 * kPlace >= kSums);
+};
+
+template <int ACT, int RG>
+__global__ void __launch_bounds__(512) adapter_down_kernel(const AdapterArgs a) {
+  using T = DownTile<RG>;
+  constexpr int TG = kDownTokens / 16, L = T::kRows / 8;
+  extern __shared__ __attribute__((aligned(16))) uint8_t down_lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, c = lane & 15, h = lane >> 4;
+  const int parts_of_entry = a.entry_tokens / kDownTokens, part = blockIdx.x % parts_of_entry;
+  Tokens e = listed_entry(a, blockIdx.x / parts_of_entry);
+  e.first += part * kDownTokens;
+  e.count = min(e.count - part * kDownTokens, kDownTokens);
+  if (e.count <= 0 || e.adapter < 0) return;
+  const int r0 = blockIdx.y * 16 * RG, pieces = a.K / 8, steps = (pieces + 7) / 8;
   const int from = (int)((int64_t)steps * blockIdx.z / a.parts), till = (int)((int64_t)steps * (blockIdx.z + 1) / a.parts);
-  const int first = from + (till - from) * wave / waves, last = from + (till - from) * (wave + 1) / waves;
+  // Load i brings rows 8 i .. 8 i + 7: tokens (past the entry's end: its last one), then ranks (past the last: it again; neither is stored).
+  const int row8 = lane >> 3;
+  const uint8_t* row[L];
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const int r = 8 * i + row8;
+    if (8 * i < kDownTokens) row[i] = (const uint8_t*)a.x + (int64_t)a.order[e.first + min(r, e.count - 1)] * a.ldx * 2;
+    else row[i] = (const uint8_t*)a.a + ((int64_t)e.adapter * a.rank + min(r0 + r - kDownTokens, a.rank - 1)) * a.lda * 2;
+  }
+  uint8_t* const mine = down_lds + wave * 2 * T::kPlace;
+  const uint32_t mine_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
+  auto load = [&](int step, int place) __attribute__((always_inline)) {
+    const int end = pieces - step * 8 - 1;  // pieces past the rows' end: the last one again
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int p = min((lane & 7) ^ (((8 * i + row8) >> 1) & 7), end);
+      lds_load16_from(mine_at + (uint32_t)(place * T::kPlace + i * 1024), row[i] + (int64_t)step * 128 + p * 16);
+    }
+  };
   f32x4 acc[TG][RG];
 #pragma unroll
   for (int g = 0; g < TG; ++g)
 #pragma unroll
     for (int q = 0; q < RG; ++q) acc[g][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int U = TG * RG > 4 ? 2 : 4;  // steps on their way
-  auto get = [&](const uint16_t* row, int step) __attribute__((always_inline)) {
-    const int p = step * 4 + h;
-    u32x4 v{0, 0, 0, 0};
-    if (p < pieces && step < last) v = *reinterpret_cast<const u32x4_any*>(row + min(p * 8, a.K - 8));
-    return v;
-  };
-  for (int step = first; step < last; step += U) {
-    u32x4 xo[U][TG], ao[U][RG];
+  int place = 0;
+  if (from + wave < till) load(from + wave, 0);
+  for (int step = from + wave; step < till; step += waves, place ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (step + waves < till) load(step + waves, place ^ 1);
+    const uint8_t* const at = mine + place * T::kPlace;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int j = 0; j < 2; ++j) {
+      u32x4 xo[TG], ao[RG];
+      const int spot = ((4 * j + h) ^ ((c >> 1) & 7)) << 4;
 #pragma unroll
-      for (int g = 0; g < TG; ++g) xo[u][g] = get(xr[g], step + u);
+      for (int g = 0; g < TG; ++g) xo[g] = *reinterpret_cast<const u32x4*>(at + (16 * g + c) * 128 + spot);
 #pragma unroll
-      for (int q = 0; q < RG; ++q) ao[u][q] = get(ar[q], step + u);
-    }
-    if (tail && step + U >= steps) {  // the last piece's first values are the piece's before
+      for (int q = 0; q < RG; ++q) ao[q] = *reinterpret_cast<const u32x4*>(at + (kDownTokens + 16 * q + c) * 128 + spot);
+      if (step * 8 + 4 * j + h >= pieces) {  // past the rows' end: counts for nothing, whatever it is
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool ends = (step + u) * 4 + h == pieces - 1;
-        auto blank = [&](u32x4& v) __attribute__((always_inline)) {
+        for (int g = 0; g < TG; ++g) xo[g] = u32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (ends && i < tail) v[i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-        };
-#pragma unroll
-        for (int g = 0; g < TG; ++g) blank(xo[u][g]);
-#pragma unroll
-        for (int q = 0; q < RG; ++q) blank(ao[u][q]);
+        for (int q = 0; q < RG; ++q) ao[q] = u32x4{0, 0, 0, 0};
       }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int g = 0; g < TG; ++g)
 #pragma unroll
-        for (int q = 0; q < RG; ++q) acc[g][q] = mfma16<ACT>(ao[u][q], xo[u][g], acc[g][q]);
+        for (int q = 0; q < RG; ++q) acc[g][q] = mfma16<ACT>(ao[q], xo[g], acc[g][q]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the place may be loaded again
   }
   // A lane has the ranks 16 q + 4 h .. + 3 of token 16 g + c.
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(down_lds);
 #pragma unroll
   for (int g = 0; g < TG; ++g)
 #pragma unroll
-    for (int q = 0; q < RG; ++q) *reinterpret_cast<f32x4*>(down_sums + (((wave * TG + g) * RG + q) * 64 + lane) * 4) = acc[g][q];
+    for (int q = 0; q < RG; ++q) *reinterpret_cast<f32x4*>(sums + (((wave * TG + g) * RG + q) * 64 + lane) * 4) = acc[g][q];
   __syncthreads();
   for (int o = wave; o < TG * RG; o += waves) {
     const int g = o / RG, q = o % RG, r = r0 + 16 * q + 4 * h;
     f32x4 v{0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(down_sums + ((w * TG * RG + o) * 64 + lane) * 4);
+    for (int w = 0; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(sums + ((w * TG * RG + o) * 64 + lane) * 4);
     if (16 * g + c >= e.count || r >= a.rank8) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = r + i < a.rank ? v[i] : 0.f;  // what only fills B's rows up
-    int m = token[0];
-#pragma unroll
-    for (int i = 1; i < TG; ++i) m = g == i ? token[i] : m;
-    *reinterpret_cast<f32x4*>(a.t + ((int64_t)blockIdx.z * a.M + m) * a.rank8 + r) = v;
+    *reinterpret_cast<f32x4*>(a.t + ((int64_t)blockIdx.z * a.M + a.order[e.first + 16 * g + c]) * a.rank8 + r) = v;
   }
 }
 
@@ -177,8 +260,8 @@ __device__ __forceinline__ void two_parts(const float (&v)[8], u32x4& hi, u32x4&
     if constexpr (ACT == NPAMD_BF16) first = __builtin_bit_cast(float, bits & 0xFFFF0000u);
     else first = (float)__builtin_amdgcn_cvt_pkrtz(v[i], 0.f)[0];
     float left = fabsf(v[i]) == __builtin_inff() ? 0.f : v[i] - first;
-    first = (v[i] != 0.f) & (fabsf(first) < kTiny) ? tiny : first;
-    left = (v[i] != 0.f) & (fabsf(left) < kTiny) ? tiny : left;
+    first = (v[i] != 0.f && fabsf(first) < kTiny) ? tiny : first;
+    left = (v[i] != 0.f && fabsf(left) < kTiny) ? tiny : left;
     h16[i] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(first) : f32_to_f16_bits(first);
     l16[i] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(left) : f32_to_f16_bits(left);
   }
@@ -186,62 +269,32 @@ __device__ __forceinline__ void two_parts(const float (&v)[8], u32x4& hi, u32x4&
   for (int i = 0; i < 4; ++i) hi[i] = h16[2 * i] | (h16[2 * i + 1] << 16), lo[i] = l16[2 * i] | (l16[2 * i + 1] << 16);
 }
 
-// RC chunks of 32 ranks; blockIdx.x: 64 columns to each of the block's waves, .y: entry.
+// RC chunks of 32 ranks, CT columns to a lane; blockIdx.x: 16 CT columns to each of the block's waves, .y: entry.  LDS: t's two parts, rows of 64 RC + 16 bytes, then what each token's sums are
+// multiplied with, and the tokens.
+template <int RC>
+struct UpTile {
+  static constexpr int kRow = 64 * RC + 16, kCT = RC <= 2 ? 8 : 4;
+  static constexpr int kTokens = RC <= 2 ? 128 : 256 / RC;  // of an entry, at most
+  static constexpr int lds(int tokens) { return tokens * (2 * kRow + 8); }
+};
+
 template <int ACT, int RC, bool LISTED>
 __global__ void __launch_bounds__(256) adapter_up_kernel(const AdapterArgs a) {
+  using T = UpTile<RC>;
+  constexpr int CT = T::kCT, kPieces = 4 * RC;  // of a row of t, eight values each
+  typedef uint32_t Columns __attribute__((ext_vector_type(CT / 2)));
+  typedef uint32_t ColumnsAny __attribute__((ext_vector_type(CT / 2), aligned(2)));
+  extern __shared__ __attribute__((aligned(16))) uint8_t up_lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
-  const int64_t col0 = ((int64_t)blockIdx.x * (blockDim.x >> 6) + wave) * 64;
-  if (col0 >= a.N) return;
   const Tokens e = LISTED ? listed_entry(a, blockIdx.y) : ballot_entry(a, blockIdx.y);
   if (e.count <= 0) return;
   const int groups = (e.count + 15) / 16;
-  const int64_t n0 = col0 + 16 * h;  // the lane's 16 columns
-  struct Row {
-    int m;
-    u32x4 base[2];
-    f32x4 t[RC][2];
-  };
-  // Pieces of eight columns: whole ones as they lie, a row's last values one by one.
-  auto piece = [&](const uint16_t* row, int64_t n) __attribute__((always_inline)) {
-    u32x4 v{0, 0, 0, 0};
-    if (n + 8 <= a.N) return (u32x4) * reinterpret_cast<const u32x4_any*>(row + n);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (n + i < a.N) v[i >> 1] |= (uint32_t)row[n + i] << (16 * (i & 1));
-    return v;
-  };
-  auto request = [&](int g) __attribute__((always_inline)) {
-    Row row;
-    const int at = min(16 * g + c, e.count - 1);  // past the entry's end: its last token, not stored
-    row.m = LISTED ? a.order[e.first + at] : __builtin_amdgcn_ds_bpermute(at * 4, e.mine);
-    row.base[0] = row.base[1] = u32x4{0, 0, 0, 0};
-    if (a.base) {
-      const uint16_t* const from = (const uint16_t*)a.base + row.m * a.ldbase;
-      row.base[0] = piece(from, n0);
-      row.base[1] = piece(from, n0 + 8);
-    }
-#pragma unroll
-    for (int q = 0; q < RC; ++q) {
-      row.t[q][0] = row.t[q][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int r = 32 * q + 8 * h;
-      if (e.adapter < 0 || r >= a.rank8) continue;
-      for (int z = 0; z < a.parts; ++z) {
-        const f32x4* const from = reinterpret_cast<const f32x4*>(a.t + ((int64_t)z * a.M + row.m) * a.rank8 + r);
-        row.t[q][0] += from[0];
-        row.t[q][1] += from[1];
-      }
-    }
-    return row;
-  };
-  u32x4 bo[RC][4];
-  float scale = 0.f;
+  const int64_t col0 = ((int64_t)blockIdx.x * (blockDim.x >> 6) + wave) * 16 * CT, n0 = col0 + CT * c;
+  u32x4 bo[RC][CT];
   if (e.adapter >= 0) {
-    scale = a.scale ? a.scale[e.adapter] : 1.f;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      // Row 4 h' + i of MFMA b is column 16 h' + 4 b + i.
-      const int64_t n = min(col0 + 16 * (c >> 2) + 4 * b + (c & 3), (int64_t)a.N - 1);
-      const uint16_t* const row = (const uint16_t*)a.b + ((int64_t)e.adapter * a.N + n) * a.rank8;
+    for (int b = 0; b < CT; ++b) {
+      const uint16_t* const row = (const uint16_t*)a.b + ((int64_t)e.adapter * a.N + min(n0 + b, (int64_t)a.N - 1)) * a.rank8;
 #pragma unroll
       for (int q = 0; q < RC; ++q) {
         const int r = 32 * q + 8 * h;
@@ -250,70 +303,122 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const AdapterArgs a) {
       }
     }
   }
-  Row next = request(0);
-  for (int g = 0; g < groups; ++g) {
-    Row row = next;
-    if (g + 1 < groups) next = request(g + 1);
-    float v[16];
+  // Columns of a row: as they lie, a row's last ones one by one.
+  auto base_of = [&](int m) __attribute__((always_inline)) {
+    Columns v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[2 * i] = act_bits_to_f32<ACT>(row.base[i >> 2][i & 3] & 0xFFFFu);
-      v[2 * i + 1] = act_bits_to_f32<ACT>(row.base[i >> 2][i & 3] >> 16);
-    }
-    if (e.adapter >= 0) {
-      float up = 1.f, down = 1.f;  // powers of two
-      if constexpr (ACT == NPAMD_F16) {
-        // The row's largest finite value to 2^14 .. 2^15.
-        int top = 0;
+    for (int i = 0; i < CT / 2; ++i) v[i] = 0;
+    if (!a.base || n0 >= a.N) return v;
+    const uint16_t* const row = (const uint16_t*)a.base + m * a.ldbase;
+    if (n0 + CT <= a.N) return (Columns) * reinterpret_cast<const ColumnsAny*>(row + n0);
 #pragma unroll
-        for (int q = 0; q < RC; ++q)
+    for (int i = 0; i < CT; ++i)
+      if (n0 + i < a.N) v[i >> 1] |= (uint32_t)row[n0 + i] << (16 * (i & 1));
+    return v;
+  };
+  int next_m[4];
+  Columns next[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float value = row.t[q][i >> 2][i & 3];  // a copy: the cast of an element itself takes the first one's bits
-            const int x = __builtin_bit_cast(int, value) >> 23 & 255;
-            top = max(top, x == 255 ? 0 : x);
-          }
-        top = max(top, __shfl_xor(top, 16, 64));
-        top = max(max(top, __shfl_xor(top, 32, 64)), 15);
-        up = __builtin_bit_cast(float, (268 - top) << 23);
-        down = __builtin_bit_cast(float, (top - 14) << 23);
+  for (int i = 0; i < 4; ++i) {  // the first group's, on their way while t comes
+    const int at = min(4 * h + i, e.count - 1);
+    next_m[i] = LISTED ? a.order[e.first + at] : __builtin_amdgcn_ds_bpermute(at * 4, e.mine);
+    next[i] = base_of(next_m[i]);
+  }
+  uint8_t* const first_part = up_lds;
+  uint8_t* const second_part = up_lds + groups * 16 * T::kRow;
+  float* const factors = reinterpret_cast<float*>(second_part + groups * 16 * T::kRow);
+  int* const tokens = reinterpret_cast<int*>(factors + groups * 16);
+  const float scale = e.adapter < 0 ? 0.f : a.scale ? a.scale[e.adapter] : 1.f;
+  for (int o = threadIdx.x; o < groups * 16 * kPieces; o += blockDim.x) {
+    const int at = o / kPieces, r = o % kPieces * 8;
+    const int m = LISTED ? a.order[e.first + min(at, e.count - 1)] : __builtin_amdgcn_ds_bpermute(min(at, e.count - 1) * 4, e.mine);
+    if (r == 0) tokens[at] = m;
+    if (e.adapter < 0) continue;
+    f32x4 sum[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    if (at < e.count && r < a.rank8) {
+      for (int z = 0; z < a.parts; ++z) {
+        const f32x4* const from = reinterpret_cast<const f32x4*>(a.t + ((int64_t)z * a.M + m) * a.rank8 + r);
+        sum[0] += from[0];
+        sum[1] += from[1];
       }
-      f32x4 acc[4];
+    }
+    float v[8], back = 1.f;  // a power of two
 #pragma unroll
-      for (int b = 0; b < 4; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 8; ++i) v[i] = sum[i >> 2][i & 3];
+    if constexpr (ACT == NPAMD_F16) {
+      // The row's largest finite value to 2^14 .. 2^15.
+      int top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int x = __builtin_bit_cast(int, v[i]) >> 23 & 255;
+        top = max(top, x == 255 ? 0 : x);
+      }
+#pragma unroll
+      for (int far = 1; far < kPieces; far *= 2) top = max(top, __shfl_xor(top, far, 64));
+      top = max(top, 15);
+      const float up = __builtin_bit_cast(float, (268 - top) << 23);
+      back = __builtin_bit_cast(float, (top - 14) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= up;
+    }
+    u32x4 hi, lo;
+    two_parts<ACT>(v, hi, lo);
+    *reinterpret_cast<u32x4*>(first_part + at * T::kRow + r * 2) = hi;
+    *reinterpret_cast<u32x4*>(second_part + at * T::kRow + r * 2) = lo;
+    if (r == 0) factors[at] = scale * back;
+  }
+  __syncthreads();
+  if (col0 >= a.N) return;
+  for (int g = 0; g < groups; ++g) {
+    int m[4];
+    Columns base[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = next_m[i], base[i] = next[i];
+    if (g + 1 < groups) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        next_m[i] = tokens[16 * (g + 1) + 4 * h + i];
+        next[i] = base_of(next_m[i]);
+      }
+    }
+    f32x4 acc[CT];  // token 16 g + 4 h + i, column n0 + b
+    float factor[4];
+    if (e.adapter >= 0) {
+#pragma unroll
+      for (int b = 0; b < CT; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < RC; ++q) {
-        float t[8];
+        const uint32_t at = (16 * g + c) * T::kRow + q * 64 + h * 16;
+        const u32x4 hi = *reinterpret_cast<const u32x4*>(first_part + at), lo = *reinterpret_cast<const u32x4*>(second_part + at);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = row.t[q][i >> 2][i & 3] * up;
-        u32x4 hi, lo;
-        two_parts<ACT>(t, hi, lo);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) acc[b] = mfma16<ACT>(bo[q][b], hi, mfma16<ACT>(bo[q][b], lo, acc[b]));
+        for (int b = 0; b < CT; ++b) acc[b] = mfma16<ACT>(hi, bo[q][b], mfma16<ACT>(lo, bo[q][b], acc[b]));
       }
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * b + i] = __builtin_fmaf(scale, acc[b][i] * down, v[4 * b + i]);
+      for (int i = 0; i < 4; ++i) factor[i] = factors[16 * g + 4 * h + i];
     }
-    if (16 * g + c >= e.count) continue;
-    uint32_t bits[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) bits[i] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(v[i]) : f32_to_f16_bits(v[i]);
-    uint16_t* const to = (uint16_t*)a.y + row.m * a.ldy;
+    for (int i = 0; i < 4; ++i) {
+      if (16 * g + 4 * h + i >= e.count) continue;
+      Columns out = base[i];  // without an adapter: as it is, whatever it is
+      if (e.adapter >= 0) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int64_t n = n0 + 8 * p;
-      u32x4 out;
+        for (int k = 0; k < CT / 2; ++k) {
+          uint32_t bits[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out[i] = bits[8 * p + 2 * i] | (bits[8 * p + 2 * i + 1] << 16);
-      if (e.adapter < 0) out = row.base[p];  // as it is, whatever it is
-      if (n + 8 <= a.N) {
-        *reinterpret_cast<u32x4_any*>(to + n) = out;
+          for (int u = 0; u < 2; ++u) {
+            const float v = __builtin_fmaf(factor[i], acc[2 * k + u][i], act_bits_to_f32<ACT>(u ? base[i][k] >> 16 : base[i][k] & 0xFFFFu));
+            bits[u] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+          }
+          out[k] = bits[0] | (bits[1] << 16);
+        }
+      }
+      uint16_t* const to = (uint16_t*)a.y + m[i] * a.ldy;
+      if (n0 + CT <= a.N) {
+        *reinterpret_cast<ColumnsAny*>(to + n0) = out;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (n + i < a.N) to[n + i] = (uint16_t)(out[i >> 1] >> (16 * (i & 1)));
+        for (int k = 0; k < CT; ++k)
+          if (n0 + k < a.N) to[n0 + k] = (uint16_t)(out[k >> 1] >> (16 * (k & 1)));
       }
     }
   }
@@ -323,20 +428,33 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const AdapterArgs a) {
 // side by side with one atomic addition, so that a prompt's stay together.  A token's results do not depend on its place.
 __global__ void __launch_bounds__(1024) adapter_list_kernel(const AdapterArgs a, int* __restrict__ order, Entry* __restrict__ entries, int* __restrict__ count) {
   extern __shared__ int places[];  // [adapters + 1]
-  __shared__ int sums[2][17];
+  __shared__ int sums[2][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, buckets = a.adapters + 1;
   for (int i = threadIdx.x; i < buckets; i += 1024) places[i] = 0;
   __syncthreads();
-  // f(bucket of the lane's token, its place among the wave's of that bucket, how many those are, first lane?) for every token, once.
+  // f(a bucket, the wave's lanes whose token is in it, whether the lane's is, its token) for all buckets of every 64 tokens.  The first turns' ids are read once, all at a time.
+  constexpr int kKept = 8;
+  int kept[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    const int m = i * 1024 + (int)threadIdx.x;
+    kept[i] = m < a.M ? adapter_of(a, m) : -2;
+  }
   auto each = [&](auto&& f) __attribute__((always_inline)) {
-    for (int64_t at = 0; at < a.M; at += 1024) {
-      const int64_t m = at + threadIdx.x;
-      const int id = m < a.M ? adapter_of(a, (int)m) : -2;
+    for (int turn = 0; turn * 1024 < a.M; ++turn) {
+      const int m = turn * 1024 + (int)threadIdx.x;
+      int id = -2;
+      if (turn < kKept) {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) id = turn == i ? kept[i] : id;
+      } else if (m < a.M) {
+        id = adapter_of(a, m);
+      }
       uint64_t open = __ballot(id != -2);
       while (open) {
         const int chosen = __builtin_amdgcn_readlane(id, __ffsll((unsigned long long)open) - 1);
         const uint64_t same = __ballot(id == chosen);
-        f(chosen < 0 ? a.adapters : chosen, same, id == chosen, (int)m);
+        f(chosen < 0 ? a.adapters : chosen, same, id == chosen, m);
         open &= ~same;
       }
     }
@@ -362,24 +480,20 @@ __global__ void __launch_bounds__(1024) adapter_list_kernel(const AdapterArgs a,
     if (lane == 63) sums[k][wave] = before[k];
   }
   __syncthreads();
-  if (threadIdx.x < 2) {
-    int v = 0;
-    for (int w = 0; w < 16; ++w) {
-      const int next = sums[threadIdx.x][w];
-      sums[threadIdx.x][w] = v;
-      v += next;
-    }
-    sums[threadIdx.x][16] = v;
+  int token = before[0] - tokens, entry = before[1] - parts, all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    token += w < wave ? sums[0][w] : 0;
+    entry += w < wave ? sums[1][w] : 0;
+    all += sums[1][w];
   }
-  __syncthreads();
-  int token = sums[0][wave] + before[0] - tokens, entry = sums[1][wave] + before[1] - parts;
   for (int i = first; i < last; ++i) {
     const int n = places[i];
     places[i] = token;
     for (int at = 0; at < n; at += a.entry_tokens) entries[entry++] = Entry{i < a.adapters ? i : -1, token + at, min(a.entry_tokens, n - at), 0};
     token += n;
   }
-  if (threadIdx.x == 0) *count = sums[1][16];
+  if (threadIdx.x == 0) *count = all;
   __syncthreads();
   each([&](int bucket, uint64_t same, bool mine, int m) __attribute__((always_inline)) {
     int at = 0;
@@ -390,9 +504,10 @@ __global__ void __launch_bounds__(1024) adapter_list_kernel(const AdapterArgs a,
 }
 
 // Tokens of a listed entry: as many as leave two rounds of the up kernel's blocks, B being read once for each.
-int entry_tokens_of(int M, int N) {
-  const int64_t columns = ((int64_t)N + 255) / 256;
-  int tokens = 128;
+int entry_tokens_of(int M, int N, int rank8) {
+  const int most = rank8 <= 64 ? 128 : rank8 <= 128 ? 64 : 32;
+  const int64_t columns = ((int64_t)N + 511) / 512;
+  int tokens = most;
   while (tokens > kDownTokens && columns * ((M + tokens - 1) / tokens) < 512) tokens /= 2;
   return tokens;
 }
@@ -404,9 +519,11 @@ struct AdapterSpace {
   AdapterSpace(int M, int N, int K, int rank, int adapters) {
     listed = M > kBallotTokens;
     rank8 = (rank + 7) / 8 * 8;
-    parts = listed ? 1 : std::clamp((K + 4095) / 4096, 1, 16);
-    tokens = listed ? entry_tokens_of(M, N) : 16;
+    tokens = listed ? entry_tokens_of(M, N, rank8) : 16;
     most = listed ? (int)std::min<int64_t>(M, ((int64_t)M + tokens - 1) / tokens + adapters + 1) : M;
+    // Parts of K of the down kernel, so that there are as many blocks as compute units.
+    const int blocks = (M + kDownTokens - 1) / kDownTokens * ((rank8 + 63) / 64);
+    parts = listed ? std::clamp(std::min(256 / blocks, K / 1024), 1, 8) : 1;
     t = (int64_t)parts * M * rank8 * 4;
     entries = listed ? 16 + (int64_t)most * sizeof(Entry) : 0;
     order = listed ? ((int64_t)M * 4 + 15) / 16 * 16 : 0;
@@ -414,36 +531,48 @@ struct AdapterSpace {
   }
 };
 
-template <int ACT, int TG, int RG, bool LISTED>
+template <int ACT, int RG>
 int launch_down(const AdapterArgs& a, unsigned blocks, hipStream_t st, const char* what) {
-  const int steps = ((a.K + 7) / 8 + 3) / 4, waves = std::clamp((steps + a.parts - 1) / a.parts, 1, 16), lds = waves * TG * RG * 1024;
+  using T = DownTile<RG>;
+  const int steps = (a.K + 63) / 64, waves = std::clamp((steps + a.parts - 1) / a.parts, 1, T::kWaves), lds = T::lds(waves);
   static LdsLatch latch;
-  const auto kernel = adapter_down_kernel<ACT, TG, RG, LISTED>;
+  const auto kernel = adapter_down_kernel<ACT, RG>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), lds);
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
   launch(kernel, dim3(blocks, (unsigned)((a.rank8 + 16 * RG - 1) / (16 * RG)), (unsigned)a.parts), 64 * waves, lds, st, a);
   return check_launch(what);
 }
 
+template <int ACT, int RC, bool LISTED>
+int launch_up_tile(const AdapterArgs& a, unsigned entries, hipStream_t st, const char* what) {
+  using T = UpTile<RC>;
+  // A wave to a block where columns and entries are few.
+  const int64_t strips = ((int64_t)a.N + 16 * T::kCT - 1) / (16 * T::kCT);
+  const int waves = strips * entries >= 1024 ? 4 : 1, lds = T::lds(a.entry_tokens);
+  static LdsLatch latch;
+  const auto kernel = adapter_up_kernel<ACT, RC, LISTED>;
+  const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), lds);
+  if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
+  launch(kernel, dim3((unsigned)((strips + waves - 1) / waves), entries), 64 * waves, lds, st, a);
+  return check_launch(what);
+}
+
 template <int ACT, bool LISTED>
 int launch_up(const AdapterArgs& a, unsigned entries, hipStream_t st, const char* what) {
-  // A wave to a block where columns and entries are few.
-  const int64_t strips = ((int64_t)a.N + 63) / 64;
-  const int waves = strips * entries >= 2048 ? 4 : 1;
-  const dim3 grid((unsigned)((strips + waves - 1) / waves), entries);
-  if (a.rank8 <= 32) launch(adapter_up_kernel<ACT, 1, LISTED>, grid, 64 * waves, 0, st, a);
-  else if (a.rank8 <= 64) launch(adapter_up_kernel<ACT, 2, LISTED>, grid, 64 * waves, 0, st, a);
-  else if (a.rank8 <= 128) launch(adapter_up_kernel<ACT, 4, LISTED>, grid, 64 * waves, 0, st, a);
-  else launch(adapter_up_kernel<ACT, 8, LISTED>, grid, 64 * waves, 0, st, a);
-  return check_launch(what);
+  if (a.rank8 <= 32) return launch_up_tile<ACT, 1, LISTED>(a, entries, st, what);
+  if (a.rank8 <= 64) return launch_up_tile<ACT, 2, LISTED>(a, entries, st, what);
+  if (a.rank8 <= 128) return launch_up_tile<ACT, 4, LISTED>(a, entries, st, what);
+  return launch_up_tile<ACT, 8, LISTED>(a, entries, st, what);
 }
 
 template <int ACT>
 int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipStream_t st, const char* what) {
   a.t = (float*)at;
   if (!space.listed) {
-    const int rc = launch_down<ACT, 1, 1, false>(a, (unsigned)a.M, st, what);
-    return rc != NPAMD_OK ? rc : launch_up<ACT, false>(a, (unsigned)a.M, st, what);
+    // Four waves to a row of A where there are few rows and each wave has columns to read.
+    if ((int64_t)a.M * a.rank8 <= 2048 && a.K > 1024) launch(adapter_few_kernel<ACT, 4>, dim3((unsigned)a.M, (unsigned)a.rank8), 256, 0, st, a);
+    else launch(adapter_few_kernel<ACT, 1>, dim3((unsigned)a.M, (unsigned)a.rank8 / 4), 256, 0, st, a);
+    return launch_up<ACT, false>(a, (unsigned)a.M, st, what);
   }
   int* const count = (int*)(at + space.t);
   Entry* const entries = (Entry*)(at + space.t + 16);
@@ -452,9 +581,9 @@ int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipSt
   a.order = order, a.entries = entries, a.count = count;
   const unsigned blocks = (unsigned)(space.most * (space.tokens / kDownTokens));
   // Up to 64 ranks to a block, so that the tokens' rows are read once.
-  const int rc = a.rank8 <= 16   ? launch_down<ACT, 2, 1, true>(a, blocks, st, what)
-                 : a.rank8 <= 32 ? launch_down<ACT, 2, 2, true>(a, blocks, st, what)
-                                 : launch_down<ACT, 2, 4, true>(a, blocks, st, what);
+  const int rc = a.rank8 <= 16   ? launch_down<ACT, 1>(a, blocks, st, what)
+                 : a.rank8 <= 32 ? launch_down<ACT, 2>(a, blocks, st, what)
+                                 : launch_down<ACT, 4>(a, blocks, st, what);
   return rc != NPAMD_OK ? rc : launch_up<ACT, true>(a, (unsigned)space.most, st, what);
 }
 
@@ -476,10 +605,12 @@ extern "C" int npamd_adapter_linear(const void* x, int64_t ldx, const void* ids,
   NPAMD_REQUIRE(ldx >= K && ldy >= N && (!base || ldbase >= N), "%s: bad row stride", what);
   if (M == 0 || N == 0) return NPAMD_OK;
   NPAMD_REQUIRE(x && ids && a && b && y, "%s: null pointer", what);
-  NPAMD_REQUIRE(((uintptr_t)b & 15) == 0, "%s: b has to lie at a 16-byte address", what);
+  NPAMD_REQUIRE((((uintptr_t)a | (uintptr_t)b) & 15) == 0, "%s: a and b have to lie at 16-byte addresses", what);
+  NPAMD_REQUIRE(M <= kBallotTokens || (((uintptr_t)x & 15) == 0 && ldx % 8 == 0 && K % 8 == 0),
+                "%s: past %d tokens x has to lie at a 16-byte address, K=%d and rows' distances have to be multiples of 8", what, kBallotTokens, K);
   const AdapterSpace space(M, N, K, rank, adapters);
   NPAMD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= space.bytes, "%s: needs %lld bytes of 16-byte aligned workspace", what, (long long)space.bytes);
-  const AdapterArgs args{x, ids, a, b, base, scale, y, ldx, ldbase, ldy, M, N, K, rank, space.rank8, adapters, ids_bits == 64, space.parts, nullptr, nullptr, nullptr, nullptr, space.tokens};
+  const AdapterArgs args{x, ids, a, b, base, scale, y, ldx, ((int64_t)K + 7) / 8 * 8, ldbase, ldy, M, N, K, rank, space.rank8, adapters, ids_bits == 64, space.parts, nullptr, nullptr, nullptr, nullptr, space.tokens};
   hipStream_t st = (hipStream_t)stream;
   if (act_dtype == NPAMD_BF16) return launch_adapters<NPAMD_BF16>(args, space, (uint8_t*)workspace, st, what);
   return launch_adapters<NPAMD_F16>(args, space, (uint8_t*)workspace, st, what);

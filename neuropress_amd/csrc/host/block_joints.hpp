@@ -356,31 +356,35 @@ PyObject* gated_linear_recorded(PyObject*, PyObject* const* args, Py_ssize_t n) 
   });
 }
 
-// adapter_linear(x, ids, a, b, scale, base, columns of y): y, or None; a, b and scale are those of LowRankAdapters, which has checked them
+// adapter_linear(x, ids, a, b, scale, base, columns of x, columns of y): y, or None; a, b and scale are those of LowRankAdapters, which has checked them
 PyObject* adapter_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "adapter_linear(x, ids, a, b, scale, base, columns)");
+  if (n != 8) {
+    PyErr_SetString(PyExc_TypeError, "adapter_linear(x, ids, a, b, scale, base, columns of x, columns of y)");
     return nullptr;
   }
   return translated([&]() -> PyObject* {
     const int device = device_of(args[0]);
     Rows x, base{nullptr, 0, 0, 0, 0};
-    if (!rows_argument(args[0], device, &x) || !PyLong_Check(args[6])) Py_RETURN_NONE;
+    if (!rows_argument(args[0], device, &x) || !PyLong_Check(args[6]) || !PyLong_Check(args[7]) || x.width < 8 || x.width != PyLong_AsLong(args[6])) Py_RETURN_NONE;
     const at::Tensor *ids = readable(args[1], device), *a = readable(args[2], device), *b = readable(args[3], device);
-    if (!ids || !a || !b || !ids->is_contiguous() || ids->sizes() != x.t->sizes().slice(0, x.t->dim() - 1) ||
-        (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong)) Py_RETURN_NONE;
-    if (a->scalar_type() != x.t->scalar_type() || a->size(2) != x.width) Py_RETURN_NONE;
+    if (!ids || !a || !b || !ids->is_contiguous() || ids->sizes() != x.t->sizes().slice(0, x.t->dim() - 1) || (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong))
+      Py_RETURN_NONE;
     const void* scale;
-    if (!vector_of(args[4], device, at::kFloat, a->size(0), &scale)) Py_RETURN_NONE;
+    if (a->scalar_type() != x.t->scalar_type() || !vector_of(args[4], device, at::kFloat, a->size(0), &scale)) Py_RETURN_NONE;
     c10::SmallVector<int64_t, 6> sizes(x.t->sizes().begin(), x.t->sizes().end());
-    sizes.back() = PyLong_AsLong(args[6]);
-    if (sizes.back() < 1 || sizes.back() > INT32_MAX) Py_RETURN_NONE;
+    sizes.back() = PyLong_AsLong(args[7]);
     if (!is_none(args[5]) && (!rows_argument(args[5], device, &base) || base.code != x.code || base.t->sizes() != at::IntArrayRef(sizes))) Py_RETURN_NONE;
-    const int m = (int)x.m, cols = (int)sizes.back(), k = (int)x.width, rank = (int)a->size(1), adapters = (int)a->size(0);
+    const int m = (int)x.m, cols = (int)sizes.back(), rank = (int)a->size(1), adapters = (int)a->size(0);
+    at::Tensor xr = *x.t;
+    int k = (int)x.width;
+    if (m > 64) {  // the entries' tokens come in whole pieces
+      xr = whole_pieces(*x.t, &x.ld);
+      k = (k + 7) / 8 * 8;
+    }
     const int64_t bytes = npamd_adapter_linear_workspace_bytes(m, cols, k, rank, adapters);
     at::Tensor scratch, y = empty(sizes, x.t->scalar_type(), device);
     if (bytes > 0) scratch = floats(bytes, device);
-    TORCH_CHECK(npamd_adapter_linear(x.t->const_data_ptr(), x.ld, ids->const_data_ptr(), ids->scalar_type() == at::kInt ? 32 : 64, a->const_data_ptr(), b->const_data_ptr(),
+    TORCH_CHECK(npamd_adapter_linear(xr.const_data_ptr(), x.ld, ids->const_data_ptr(), ids->scalar_type() == at::kInt ? 32 : 64, a->const_data_ptr(), b->const_data_ptr(),
                                      (const float*)scale, base.t ? base.t->const_data_ptr() : nullptr, base.ld, y.data_ptr(), cols, m, cols, k, rank, adapters, x.code,
                                      out_or_null(scratch), bytes, current_stream(device)) == NPAMD_OK, npamd_last_error());
     return THPVariable_Wrap(std::move(y));

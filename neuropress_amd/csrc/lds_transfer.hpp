@@ -20,6 +20,11 @@ __device__ __forceinline__ void lds_load16(uint32_t dst, uint32_t voff, const vo
   dst = __builtin_amdgcn_readfirstlane(dst);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(voff), "s"(base) : "memory");
 }
+// The same from an address of each lane's own.
+__device__ __forceinline__ void lds_load16_from(uint32_t dst, const void* from) {
+  dst = __builtin_amdgcn_readfirstlane(dst);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(from) : "memory");
+}
 __device__ __forceinline__ void lds_load4(uint32_t dst, uint32_t voff, const void* base) {
   dst = __builtin_amdgcn_readfirstlane(dst);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(voff), "s"(base) : "memory");

@@ -178,8 +178,28 @@ struct ColumnSums {
   void* out;
 };
 
+// Four values of a piece, the first or the second: what is made of a whole piece at a time does not fit the registers next to a row that is on its way.
+template <int DT>
+__device__ __forceinline__ void four(const u32x4& v, int half, float (&f)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == NPAMD_F32) f[e] = __builtin_bit_cast(float, (uint32_t)v[e]);
+    else f[e] = act_bits_to_f32<DT>(e & 1 ? v[2 * half + e / 2] >> 16 : v[2 * half + e / 2] & 0xFFFFu);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void put_four(u32x4& v, int half, const float (&f)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == NPAMD_F32) v[e] = __builtin_bit_cast(uint32_t, f[e]);
+    else if (e & 1) continue;
+    else if constexpr (DT == NPAMD_BF16) v[2 * half + e / 2] = f32_to_bf16_bits(f[e]) | (f32_to_bf16_bits(f[e + 1]) << 16);
+    else v[2 * half + e / 2] = f32_to_f16_bits(f[e]) | (f32_to_f16_bits(f[e + 1]) << 16);
+  }
+}
+
 // Whether the registers hold a team's next rows too.
-constexpr bool rows_ahead(int dt, int nv, bool post, int gate) { return dt == NPAMD_F32 ? nv < 4 : nv < (post && gate ? 1 : 3); }
+constexpr bool rows_ahead(int dt, int nv, bool post, int gate) { return dt == NPAMD_F32 ? nv < 4 : nv < (post && gate ? 2 : 3); }
 
 enum Gate { kNoGate, kSharedGate, kOwnGate };  // own: of a row
 
@@ -188,12 +208,12 @@ enum Gate { kNoGate, kSharedGate, kOwnGate };  // own: of a row
 // sum(c rh), so a row's sums meet in LDS once.  Blocks take parts of a group's rows, so that a shared gate's sums have one place; a team's next row is on its way while
 // this one's sums meet (one piece to a lane; two leave no registers for it).
 template <int DT, int NV, bool POST, int GATE>
-__global__ void __launch_bounds__(512, NV == 1 ? 4 : 2) residual_norm_back_kernel(const ResidualNormBack a, const ColumnSums sum_w, const ColumnSums sum_p, const ColumnSums sum_g, int RW, int teams) {
+__global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kernel(const ResidualNormBack a, const ColumnSums sum_w, const ColumnSums sum_p, const ColumnSums sum_g, int RW, int teams) {
   using P = Pieces<DT>;
   constexpr int V = P::V;
   constexpr bool kAhead = rows_ahead(DT, NV, POST, GATE);
   extern __shared__ __attribute__((aligned(16))) float team_sums[];
-  __shared__ float meet[2][8][3];
+  __shared__ float meet[2][16][3];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave / RW, lanes = 64 * RW;
   const int lane = (int)threadIdx.x - team * lanes, H = a.H, pieces = (H + V - 1) / V;
   const float inv = 1.f / (float)H;
@@ -278,36 +298,33 @@ __global__ void __launch_bounds__(512, NV == 1 ? 4 : 2) residual_norm_back_kerne
       float s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int p = lane + lanes * i;
+        const int p = lane + lanes * i, skip = p * V + V <= H ? 0 : p * V + V - H;  // values that the piece before has too
         if (!live || p >= pieces) continue;
-        float dz[V], rh[V], w[V], ds[V], yh[V], wp[V], g[V];
-        P::unpack(dz_[i], dz);
-        P::unpack(r_[i], rh);
-        P::unpack(wv[i], w);
-        if (POST) {
-          P::unpack(ds_[i], ds);
-          P::unpack(y_[i], yh);
-          P::unpack(pv[i], wp);
-          if (GATE) P::unpack(g_[i], g);
-        }
-        auto value = [&](int e) __attribute__((always_inline)) {
-          const float h = rh[e] * rstd, v = dz[e] * w[e];
-          dw[i][e] = __builtin_fmaf(dz[e], h, dw[i][e]);
-          s1 = __builtin_fmaf(v, h, s1);
+#pragma unroll
+        for (int half = 0; half < V / 4; ++half) {
+          float dz[4], rh[4], w[4], ds[4], yh[4], wp[4], g[4];
+          four<DT>(dz_[i], half, dz);
+          four<DT>(r_[i], half, rh);
+          four<DT>(wv[i], half, w);
           if (POST) {
-            float c = a.scale * wp[e] * (yh[e] * post);
-            if (GATE) c *= g[e];
-            s2 = __builtin_fmaf(c, __builtin_fmaf(rstd, v, ds[e]), s2);
-            s3 = __builtin_fmaf(c, h, s3);
+            four<DT>(ds_[i], half, ds);
+            four<DT>(y_[i], half, yh);
+            four<DT>(pv[i], half, wp);
+            if (GATE) four<DT>(g_[i], half, g);
           }
-        };
-        if (p * V + V <= H) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) value(e);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (e >= p * V + V - H) value(e);
+          for (int e = 0; e < 4; ++e) {
+            const float z = 4 * half + e >= skip ? dz[e] : 0.f, h = rh[e] * rstd, v = z * w[e];
+            dw[i][4 * half + e] = __builtin_fmaf(z, h, dw[i][4 * half + e]);
+            s1 = __builtin_fmaf(v, h, s1);
+            if (POST) {
+              float c = a.scale * wp[e] * (yh[e] * post);
+              if (GATE) c *= g[e];
+              c = 4 * half + e >= skip ? c : 0.f;
+              s2 = __builtin_fmaf(c, __builtin_fmaf(rstd, v, ds[e]), s2);
+              s3 = __builtin_fmaf(c, h, s3);
+            }
+          }
         }
       }
       s1 = wave_sum(s1);
@@ -330,36 +347,43 @@ __global__ void __launch_bounds__(512, NV == 1 ? 4 : 2) residual_norm_back_kerne
       for (int i = 0; i < NV; ++i) {
         const int p = lane + lanes * i, at = min(p * V, H - V);
         if (p >= pieces) continue;
-        float dr[V], f[V], g[V], y[V], wp[V], own[V];
+        const int skip = p * V + V <= H ? 0 : p * V + V - H;
         P::forget(ds_[i]);
         P::forget(dz_[i]);
         P::forget(r_[i]);
         P::forget(y_[i]);
-        P::unpack(ds_[i], dr);
-        P::unpack(dz_[i], f);
-        P::unpack(wv[i], g);
+        u32x4 to_dx, to_dy, to_gate;
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[e] *= g[e];
-        P::unpack(r_[i], g);
+        for (int half = 0; half < V / 4; ++half) {
+          float dr[4], f[4], g[4], y[4], wp[4], own[4];
+          four<DT>(ds_[i], half, dr);
+          four<DT>(dz_[i], half, f);
+          four<DT>(wv[i], half, g);
 #pragma unroll
-        for (int e = 0; e < V; ++e) dr[e] = __builtin_fmaf(rstd, f[e] - g[e] * rstd * c1, dr[e]);
-        if (a.dx) P::store(const_cast<uint8_t*>(P::row_of(a.dx, row, a.lddx)), at, P::pack(dr));
-        P::unpack(y_[i], y);
-        if (POST) P::unpack(pv[i], wp);
-        if (GATE) P::unpack(g_[i], g);
-        const int skip = p * V + V <= H ? 0 : p * V + V - H;  // values that the piece before has too
+          for (int e = 0; e < 4; ++e) f[e] *= g[e];
+          four<DT>(r_[i], half, g);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float d = a.scale * dr[e], u = GATE ? d * g[e] : d, yh = POST ? y[e] * post : y[e];
-          if (GATE == kOwnGate) own[e] = d * (POST ? yh * wp[e] : yh);
-          if (e >= skip) {
-            if (GATE == kSharedGate) dg[i][e] = __builtin_fmaf(d, POST ? yh * wp[e] : yh, dg[i][e]);
-            if (POST) dp[i][e] = __builtin_fmaf(u, yh, dp[i][e]);
+          for (int e = 0; e < 4; ++e) dr[e] = __builtin_fmaf(rstd, f[e] - g[e] * rstd * c1, dr[e]);
+          put_four<DT>(to_dx, half, dr);
+          four<DT>(y_[i], half, y);
+          if (POST) four<DT>(pv[i], half, wp);
+          if (GATE) four<DT>(g_[i], half, g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float d = a.scale * dr[e], u = GATE ? d * g[e] : d, yh = POST ? y[e] * post : y[e];
+            if (GATE == kOwnGate) own[e] = d * (POST ? yh * wp[e] : yh);
+            if (4 * half + e >= skip) {
+              if (GATE == kSharedGate) dg[i][4 * half + e] = __builtin_fmaf(d, POST ? yh * wp[e] : yh, dg[i][4 * half + e]);
+              if (POST) dp[i][4 * half + e] = __builtin_fmaf(u, yh, dp[i][4 * half + e]);
+            }
+            f[e] = POST ? post * __builtin_fmaf(u, wp[e], -yh * c2) : u;
           }
-          f[e] = POST ? post * __builtin_fmaf(u, wp[e], -yh * c2) : u;
+          put_four<DT>(to_dy, half, f);
+          if (GATE == kOwnGate) put_four<DT>(to_gate, half, own);
         }
-        if (a.dy) P::store(const_cast<uint8_t*>(P::row_of(a.dy, row, a.lddy)), at, P::pack(f));
-        if (GATE == kOwnGate && a.dgate) P::store(const_cast<uint8_t*>(P::row_of(a.dgate, row, H)), at, P::pack(own));
+        if (a.dx) P::store(const_cast<uint8_t*>(P::row_of(a.dx, row, a.lddx)), at, to_dx);
+        if (a.dy) P::store(const_cast<uint8_t*>(P::row_of(a.dy, row, a.lddy)), at, to_dy);
+        if (GATE == kOwnGate && a.dgate) P::store(const_cast<uint8_t*>(P::row_of(a.dgate, row, H)), at, to_gate);
       }
     }
     if (GATE == kSharedGate) leave(sum_g, dg, unit, group);
@@ -457,9 +481,9 @@ struct SumParts {
   int parts, gate_parts, H, width, last;
 };
 template <int DT>
-__global__ void __launch_bounds__(1024) residual_norm_back_sum_kernel(const SumParts s, int gates_from) {
+__global__ void __launch_bounds__(1024) residual_norm_back_sum_kernel(const SumParts s) {
   __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane, which = min((int)blockIdx.y, 2), gate = gates_from + (int)blockIdx.y - 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane, which = min((int)blockIdx.y, 2), gate = (int)blockIdx.y - 2;
   const ColumnSums to = which == 0 ? s.w : which == 1 ? s.p : s.g;
   if (!to.partial) return;
   const int parts = which == 2 ? s.gate_parts : s.parts, first = parts * wave / 16, end = parts * (wave + 1) / 16;
@@ -503,7 +527,7 @@ struct BackPlan {
     nv = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
     row_waves = 1;
     while (row_waves * 64 * nv < pieces) row_waves *= 2;
-    teams = std::min(8 / row_waves, std::max(1, M));
+    teams = std::min((nv == 1 ? 16 : 8) / row_waves, std::max(1, M));
     auto count = [&](int turns) { return std::min<int64_t>(256, ((int64_t)M + teams * turns - 1) / (teams * turns)); };
     const int64_t most = count(count(2) > 1 && count(1) * H * 8 <= kMaxSums ? 1 : 2);
     parts = (int)std::clamp<int64_t>(most / groups, 1, std::max<int64_t>(1, (rows + teams - 1) / teams));
@@ -571,12 +595,7 @@ int launch_backward(ResidualNormBack a, void* dw, void* dwp, void* dgate, float*
   if (sw.partial || sp.partial || sg.partial) {
     constexpr int V = Pieces<DT>::V;
     const SumParts s{sw, sp, sg, p.blocks, p.parts, a.H, (int)p.width, p.nv ? a.H / V * V : a.H};
-    int done = 0;
-    do {  // the gates in as many launches as the grid's second dimension asks for
-      const int gates = sg.partial ? std::min(p.groups - done, 65000) : 0;
-      launch(residual_norm_back_sum_kernel<DT>, dim3((unsigned)(a.H + 63) / 64, (unsigned)(2 + gates)), 1024, 0, st, s, done);
-      done += gates;
-    } while (sg.partial && done < p.groups);
+    launch(residual_norm_back_sum_kernel<DT>, dim3((unsigned)(a.H + 63) / 64, (unsigned)(2 + (sg.partial ? p.groups : 0))), 1024, 0, st, s);  // groups in parts: 512 at most
   }
   return check_launch(what);
 }

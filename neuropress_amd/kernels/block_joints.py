@@ -251,7 +251,7 @@ class LowRankAdapters:
     """The adapters of one projection, checked and laid out once, for :func:`adapter_linear`.
 
     *a* ``[L, r, K]`` and *b* ``[L, N, r]`` in float16 or bfloat16, *scale* float32 ``[L]`` or None (1): adapter i adds ``scale[i] * (x @ a[i].T) @ b[i].T``.  Ranks up to 256, up to
-    8192 adapters.  Ranks that are no multiple of eight are padded (a copy of *b*); otherwise the tensors are kept as they are.
+    8192 adapters.  Ranks and columns that are no multiples of eight are padded (a copy); otherwise the tensors are kept as they are.
     """
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor | None = None):
@@ -270,10 +270,10 @@ class LowRankAdapters:
         a, b = a.detach(), b.detach()
         if self.rank % 8:
             b = torch.nn.functional.pad(b, (0, -self.rank % 8))
-        if self.in_features < 8:  # the kernels read pieces of eight columns
-            a = torch.nn.functional.pad(a, (0, 8 - self.in_features))
-        b = b.contiguous()
-        self.a, self.b = a.contiguous(), b if b.data_ptr() % 16 == 0 else b.clone()
+        if self.in_features % 8:
+            a = torch.nn.functional.pad(a, (0, -self.in_features % 8))
+        a, b = a.contiguous(), b.contiguous()
+        self.a, self.b = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (a, b))
         self.scale = None if scale is None else scale.detach().contiguous()
 
 
@@ -285,9 +285,7 @@ def adapter_linear(x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor
     -1, leaves its tokens' base as it is.  Tokens may come in any order; each adapter's weights are read once for up to 16 tokens of a decode step or 128 of a prompt.  For inference: calls that torch
     follows (:func:`tracked`) are refused.
     """
-    y = None
-    if adapters.in_features >= 8:
-        y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, base, adapters.out_features)
+    y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, base, adapters.in_features, adapters.out_features)
     if y is not None:
         return y
     what = "adapter_linear"
@@ -309,8 +307,10 @@ def adapter_linear(x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor
         return x.new_empty((*lead, n))
     with torch.no_grad(), _on_device(x):
         ids = ids.reshape(*ids.shape, *[1] * (len(lead) - ids.dim())).expand(lead).contiguous()
-        x = x.detach().contiguous() if k >= 8 else gather_columns(x.detach().reshape(rows, k), None, 8).view(*lead, 8)
-        y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, None if base is None else base.detach().contiguous(), n)
+        x = x.detach().contiguous()
+        if k < 8:  # the kernels read pieces of eight columns
+            x, k = gather_columns(x.view(rows, k), None, 8).view(*lead, 8), 8
+        y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, None if base is None else base.detach().contiguous(), k, n)
     if y is None:
         raise RuntimeError(f"{what}: no kernel for these tensors")
     return y

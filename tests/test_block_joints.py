@@ -43,9 +43,12 @@ def test_adapter_linear_refuses():
         ok = dict(x=P, ldx=64, ids=P, bits=32, a=P, b=P, scale=P, base=P, ldb=72, y=P, ldy=72, m=m, n=72, k=64, r=12, l=4, dtype=0, ws=P, wsn=need, st=None)
         for change, match in [(dict(m=-1), "bad shape"), (dict(n=-1), "bad shape"), (dict(k=0), "bad shape"), (dict(r=0), "bad shape"), (dict(l=0), "bad shape"), (dict(dtype=2), "f16 or bf16"),
                               (dict(bits=16), "32 or 64"), (dict(ldx=63), "stride"), (dict(ldy=71), "stride"), (dict(ldb=71), "stride"), (dict(x=None), "null"), (dict(ids=None), "null"),
-                              (dict(a=None), "null"), (dict(b=None), "null"), (dict(y=None), "null"), (dict(b=P + 8), "16-byte"), (dict(ws=None), "workspace"), (dict(ws=P + 4), "workspace"),
+                              (dict(a=None), "null"), (dict(b=None), "null"), (dict(y=None), "null"), (dict(b=P + 8), "16-byte"), (dict(a=P + 8), "16-byte"), (dict(ws=None), "workspace"), (dict(ws=P + 4), "workspace"),
                               (dict(wsn=need - 1), "workspace")]:  # fmt: skip
             _refused("npamd_adapter_linear", *{**ok, **change}.values(), match=match)
+        if m > 64:
+            for change in (dict(x=P + 2), dict(ldx=66), dict(k=63)):
+                _refused("npamd_adapter_linear", *{**ok, **change}.values(), match="multiples of 8")
         for change in (dict(k=7), dict(r=257), dict(l=8193), dict(m=2**22 + 1), dict(n=2**24 + 1, ldy=1 << 25, ldb=1 << 25)):
             _refused("npamd_adapter_linear", *{**ok, **change}.values(), match="at most", code=-2)
         for change in (dict(m=0), dict(n=0)):
