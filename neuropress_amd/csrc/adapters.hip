@@ -3,8 +3,8 @@
 // Two products whose weights depend on the token.  Tokens of one adapter meet its weights as the columns of MFMAs (16x16x32), so both kernels work on entries: an adapter and some of its
 // tokens.  Up to 64 tokens every wave finds its entry's tokens by itself from the ids (one comparison of all of them and a count of bits), so a call is two launches; past that a
 // block of one launch more sorts tokens by adapter and lists the entries.
-//   down: t = x A^T, f32.  Few tokens: a wave (or a block's four) streams a row of A into registers, as the dense product of one or two tokens does.  More: a block takes 32 tokens of an entry,
-//         up to 64 ranks and a part of K, x and A come into LDS in whole lines, each wave with steps of its own; the waves' sums meet in LDS.
+//   down: t = x A^T, f32.  A block takes 16 or 32 tokens of an entry, up to 64 ranks and a part of K; x and A come into LDS in whole lines, each wave with steps of its own, and the waves'
+//         sums meet in LDS.
 //   up:   y = base + scale t B^T.  A block brings its entry's t into LDS once, as two parts of B's type, for an MFMA each (t is not rounded to 16 bits: 2^-16 of it is left with bf16; fp16, scaled
 //         by a power of two to the row's largest, 2^-21), and its waves take 64 or 128 columns each.  Column 8 c + b of a wave is row c of MFMA b, so that a lane ends up with eight neighbouring columns
 //         of four tokens and 16 lanes with 256 bytes of a row of base and y, side by side.  (With four tokens' rows in every quarter of the lanes instead, as the MFMAs' own layout
@@ -33,7 +33,7 @@ struct AdapterArgs {
   const void *x, *ids, *a, *b, *base;
   const float* scale;
   void* y;
-  int64_t ldx, lda, ldbase, ldy;
+  int64_t ldx, ldbase, ldy;
   int M, N, K, rank, rank8, adapters, ids_64, parts;
   float* t;              // [parts][M][rank8]
   const int* order;      // listed entries
@@ -74,116 +74,43 @@ __device__ __forceinline__ Tokens listed_entry(const AdapterArgs& a, int e) {
   return {__builtin_amdgcn_readfirstlane(v.adapter), __builtin_amdgcn_readfirstlane(v.first), __builtin_amdgcn_readfirstlane(v.count), 0};
 }
 
-// Few tokens: KS of a block's four waves to a row of A, TB tokens at a time.  Any K of at least eight and any address of x: a row that does not end with a piece of eight has its last one end
-// with the row, and the values that the piece before has too are zeroed in both operands.  blockIdx.x: entry, .y: ranks, those that only fill B's rows up among them.
-template <int ACT, int TB>
-__device__ __forceinline__ void few_sums(const uint16_t* ar, const uint16_t* const (&xr)[TB], int K, int first, int last, float (&acc)[TB]) {
-  constexpr int U = TB == 1 ? 8 : 4;  // pieces on their way
-  const int lane = threadIdx.x & 63, pieces = (K + 7) / 8, tail = pieces * 8 - K;
-  auto at = [&](int p) { return min(p * 8, K - 8); };
-  auto blank = [&](u32x4& v) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < tail) v[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-  };
-#pragma unroll
-  for (int t = 0; t < TB; ++t) acc[t] = 0.f;
-  for (int p0 = first; p0 < last; p0 += U * 64) {
-    u32x4 av[U], xv[U][TB];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int p = p0 + u * 64 + lane;
-      av[u] = u32x4{0, 0, 0, 0};
-      if (p < last) av[u] = *reinterpret_cast<const u32x4_any*>(ar + at(p));
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        xv[u][t] = u32x4{0, 0, 0, 0};
-        if (p < last) xv[u][t] = *reinterpret_cast<const u32x4_any*>(xr[t] + at(p));
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool ends = tail && p0 + u * 64 + lane == pieces - 1;
-      if (ends) blank(av[u]);
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        if (ends) blank(xv[u][t]);
-        acc[t] = add_dot8<ACT>(av[u], xv[u][t], acc[t]);
-      }
-    }
-  }
-}
-
-template <int ACT, int KS>
-__global__ void __launch_bounds__(256) adapter_few_kernel(const AdapterArgs a) {
-  __shared__ float sums[4][4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS;
-  const Tokens e = ballot_entry(a, blockIdx.x);
-  if (e.count <= 0 || e.adapter < 0) return;
-  const int r = blockIdx.y * (4 / KS) + wave / KS;
-  const uint16_t* const ar = (const uint16_t*)a.a + ((int64_t)e.adapter * a.rank + min(r, a.rank - 1)) * a.lda;
-  const int pieces = (a.K + 7) / 8, turns = (pieces + 63) / 64, first = turns * part / KS * 64, last = min(turns * (part + 1) / KS * 64, pieces);
-  for (int j = 0; j < e.count; j += 4) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const uint16_t* xr[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) xr[t] = (const uint16_t*)a.x + __builtin_amdgcn_readlane(e.mine, min(j + t, e.count - 1)) * a.ldx;
-    if (e.count - j == 1) {
-      const uint16_t* const one[1] = {xr[0]};
-      float sum[1];
-      few_sums<ACT, 1>(ar, one, a.K, first, last, sum);
-      acc[0] = sum[0];
-    } else {
-      few_sums<ACT, 4>(ar, xr, a.K, first, last, acc);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const float v = wave_sum_last(acc[t]);
-      if (lane == 63) sums[wave][t] = v;
-    }
-    __syncthreads();
-    const int token = __builtin_amdgcn_ds_bpermute(min(j + lane, e.count - 1) * 4, e.mine);  // of all lanes: those that give have to take part
-    if (part == 0 && lane < 4 && j + lane < e.count && r < a.rank8) {
-      float v = 0.f;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) v += sums[wave + i][lane];
-      a.t[(int64_t)token * a.rank8 + r] = r < a.rank ? v : 0.f;
-    }
-    __syncthreads();
-  }
-}
-
-// Listed entries: RG groups of 16 ranks of 32 tokens; blockIdx.x: entry and its part of 32 tokens, .y: ranks, .z: part of K.  A wave takes every so manieth 64-k step of the part, in two places of its
+// TG groups of 16 tokens, RG of 16 ranks; blockIdx.x: entry (listed: and its part of 32 tokens), .y: ranks, .z: part of K.  A wave takes every so manieth 64-k step of the part, in two places of its
 // own in LDS: rows of 128 bytes, 16-byte piece p of row r in place p ^ ((r >> 1) & 7).  Tokens' rows come from wherever they are.
-template <int RG>
+template <int TG, int RG>
 struct DownTile {
-  static constexpr int kRows = kDownTokens + 16 * RG, kPlace = kRows * 128, kSums = 2 * RG * 1024;
+  static constexpr int kTokens = 16 * TG, kRows = kTokens + 16 * RG, kPlace = kRows * 128, kSums = TG * RG * 1024;
   static constexpr int kWaves = kLdsPerBlockMax / (2 * kPlace) < 8 ? kLdsPerBlockMax / (2 * kPlace) : 8;
   static constexpr int lds(int waves) { return waves * 2 * kPlace; }
   static_assert(2 * kPlace >= kSums);
 };
 
-template <int ACT, int RG>
+template <int ACT, int TG, int RG, bool LISTED>
 __global__ void __launch_bounds__(512) adapter_down_kernel(const AdapterArgs a) {
-  using T = DownTile<RG>;
-  constexpr int TG = kDownTokens / 16, L = T::kRows / 8;
+  using T = DownTile<TG, RG>;
+  constexpr int L = T::kRows / 8;
   extern __shared__ __attribute__((aligned(16))) uint8_t down_lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, c = lane & 15, h = lane >> 4;
-  const int parts_of_entry = a.entry_tokens / kDownTokens, part = blockIdx.x % parts_of_entry;
-  Tokens e = listed_entry(a, blockIdx.x / parts_of_entry);
-  e.first += part * kDownTokens;
-  e.count = min(e.count - part * kDownTokens, kDownTokens);
+  Tokens e;
+  if constexpr (LISTED) {
+    const int parts_of_entry = a.entry_tokens / T::kTokens, part = blockIdx.x % parts_of_entry;
+    e = listed_entry(a, blockIdx.x / parts_of_entry);
+    e.first += part * T::kTokens;
+    e.count = min(e.count - part * T::kTokens, T::kTokens);
+  } else {
+    e = ballot_entry(a, blockIdx.x);
+  }
+  auto token = [&](int at) __attribute__((always_inline)) { return LISTED ? a.order[e.first + at] : __builtin_amdgcn_ds_bpermute(at * 4, e.mine); };  // by all lanes at once
   if (e.count <= 0 || e.adapter < 0) return;
   const int r0 = blockIdx.y * 16 * RG, pieces = a.K / 8, steps = (pieces + 7) / 8;
   const int from = (int)((int64_t)steps * blockIdx.z / a.parts), till = (int)((int64_t)steps * (blockIdx.z + 1) / a.parts);
-  // Load i brings rows 8 i .. 8 i + 7: tokens (past the entry's end: its last one), then ranks (past the last: it again; neither is stored).
+  // Load i brings rows 8 i .. 8 i + 7: tokens (past the entry's end its last one, or what was there), then ranks (past the last: it again); what comes of those is not stored.
   const int row8 = lane >> 3;
   const uint8_t* row[L];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     const int r = 8 * i + row8;
-    if (8 * i < kDownTokens) row[i] = (const uint8_t*)a.x + (int64_t)a.order[e.first + min(r, e.count - 1)] * a.ldx * 2;
-    else row[i] = (const uint8_t*)a.a + ((int64_t)e.adapter * a.rank + min(r0 + r - kDownTokens, a.rank - 1)) * a.lda * 2;
+    if (8 * i < T::kTokens) row[i] = (const uint8_t*)a.x + (int64_t)token(min(r, e.count - 1)) * a.ldx * 2;
+    else row[i] = (const uint8_t*)a.a + ((int64_t)e.adapter * a.rank + min(r0 + r - T::kTokens, a.rank - 1)) * a.K * 2;
   }
   uint8_t* const mine = down_lds + wave * 2 * T::kPlace;
   const uint32_t mine_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
@@ -191,6 +118,7 @@ __global__ void __launch_bounds__(512) adapter_down_kernel(const AdapterArgs a) 
     const int end = pieces - step * 8 - 1;  // pieces past the rows' end: the last one again
 #pragma unroll
     for (int i = 0; i < L; ++i) {
+      if (8 * i < T::kTokens && 8 * i >= e.count) continue;
       const int p = min((lane & 7) ^ (((8 * i + row8) >> 1) & 7), end);
       lds_load16_from(mine_at + (uint32_t)(place * T::kPlace + i * 1024), row[i] + (int64_t)step * 128 + p * 16);
     }
@@ -213,7 +141,7 @@ __global__ void __launch_bounds__(512) adapter_down_kernel(const AdapterArgs a) 
 #pragma unroll
       for (int g = 0; g < TG; ++g) xo[g] = *reinterpret_cast<const u32x4*>(at + (16 * g + c) * 128 + spot);
 #pragma unroll
-      for (int q = 0; q < RG; ++q) ao[q] = *reinterpret_cast<const u32x4*>(at + (kDownTokens + 16 * q + c) * 128 + spot);
+      for (int q = 0; q < RG; ++q) ao[q] = *reinterpret_cast<const u32x4*>(at + (T::kTokens + 16 * q + c) * 128 + spot);
       if (step * 8 + 4 * j + h >= pieces) {  // past the rows' end: counts for nothing, whatever it is
 #pragma unroll
         for (int g = 0; g < TG; ++g) xo[g] = u32x4{0, 0, 0, 0};
@@ -236,13 +164,13 @@ __global__ void __launch_bounds__(512) adapter_down_kernel(const AdapterArgs a) 
     for (int q = 0; q < RG; ++q) *reinterpret_cast<f32x4*>(sums + (((wave * TG + g) * RG + q) * 64 + lane) * 4) = acc[g][q];
   __syncthreads();
   for (int o = wave; o < TG * RG; o += waves) {
-    const int g = o / RG, q = o % RG, r = r0 + 16 * q + 4 * h;
+    const int g = o / RG, q = o % RG, r = r0 + 16 * q + 4 * h, m = token(min(16 * g + c, e.count - 1));
     f32x4 v{0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(sums + ((w * TG * RG + o) * 64 + lane) * 4);
     if (16 * g + c >= e.count || r >= a.rank8) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = r + i < a.rank ? v[i] : 0.f;  // what only fills B's rows up
-    *reinterpret_cast<f32x4*>(a.t + ((int64_t)blockIdx.z * a.M + a.order[e.first + 16 * g + c]) * a.rank8 + r) = v;
+    *reinterpret_cast<f32x4*>(a.t + ((int64_t)blockIdx.z * a.M + m) * a.rank8 + r) = v;
   }
 }
 
@@ -279,7 +207,7 @@ struct UpTile {
 };
 
 template <int ACT, int RC, bool LISTED>
-__global__ void __launch_bounds__(256) adapter_up_kernel(const AdapterArgs a) {
+__global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const AdapterArgs a) {
   using T = UpTile<RC>;
   constexpr int CT = T::kCT, kPieces = 4 * RC;  // of a row of t, eight values each
   typedef uint32_t Columns __attribute__((ext_vector_type(CT / 2)));
@@ -521,9 +449,9 @@ struct AdapterSpace {
     rank8 = (rank + 7) / 8 * 8;
     tokens = listed ? entry_tokens_of(M, N, rank8) : 16;
     most = listed ? (int)std::min<int64_t>(M, ((int64_t)M + tokens - 1) / tokens + adapters + 1) : M;
-    // Parts of K of the down kernel, so that there are as many blocks as compute units.
+    // Parts of K of the down kernel: as many as there are compute units for its blocks; few tokens: two steps for each of a block's waves.
     const int blocks = (M + kDownTokens - 1) / kDownTokens * ((rank8 + 63) / 64);
-    parts = listed ? std::clamp(std::min(256 / blocks, K / 1024), 1, 8) : 1;
+    parts = listed ? std::clamp(std::min(256 / blocks, K / 1024), 1, 8) : std::clamp((K + 1023) / 1024, 1, 8);
     t = (int64_t)parts * M * rank8 * 4;
     entries = listed ? 16 + (int64_t)most * sizeof(Entry) : 0;
     order = listed ? ((int64_t)M * 4 + 15) / 16 * 16 : 0;
@@ -531,12 +459,12 @@ struct AdapterSpace {
   }
 };
 
-template <int ACT, int RG>
+template <int ACT, int TG, int RG, bool LISTED>
 int launch_down(const AdapterArgs& a, unsigned blocks, hipStream_t st, const char* what) {
-  using T = DownTile<RG>;
+  using T = DownTile<TG, RG>;
   const int steps = (a.K + 63) / 64, waves = std::clamp((steps + a.parts - 1) / a.parts, 1, T::kWaves), lds = T::lds(waves);
   static LdsLatch latch;
-  const auto kernel = adapter_down_kernel<ACT, RG>;
+  const auto kernel = adapter_down_kernel<ACT, TG, RG, LISTED>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), lds);
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
   launch(kernel, dim3(blocks, (unsigned)((a.rank8 + 16 * RG - 1) / (16 * RG)), (unsigned)a.parts), 64 * waves, lds, st, a);
@@ -569,10 +497,8 @@ template <int ACT>
 int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipStream_t st, const char* what) {
   a.t = (float*)at;
   if (!space.listed) {
-    // Four waves to a row of A where there are few rows and each wave has columns to read.
-    if ((int64_t)a.M * a.rank8 <= 2048 && a.K > 1024) launch(adapter_few_kernel<ACT, 4>, dim3((unsigned)a.M, (unsigned)a.rank8), 256, 0, st, a);
-    else launch(adapter_few_kernel<ACT, 1>, dim3((unsigned)a.M, (unsigned)a.rank8 / 4), 256, 0, st, a);
-    return launch_up<ACT, false>(a, (unsigned)a.M, st, what);
+    const int rc = launch_down<ACT, 1, 1, false>(a, (unsigned)a.M, st, what);
+    return rc != NPAMD_OK ? rc : launch_up<ACT, false>(a, (unsigned)a.M, st, what);
   }
   int* const count = (int*)(at + space.t);
   Entry* const entries = (Entry*)(at + space.t + 16);
@@ -581,9 +507,9 @@ int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipSt
   a.order = order, a.entries = entries, a.count = count;
   const unsigned blocks = (unsigned)(space.most * (space.tokens / kDownTokens));
   // Up to 64 ranks to a block, so that the tokens' rows are read once.
-  const int rc = a.rank8 <= 16   ? launch_down<ACT, 1>(a, blocks, st, what)
-                 : a.rank8 <= 32 ? launch_down<ACT, 2>(a, blocks, st, what)
-                                 : launch_down<ACT, 4>(a, blocks, st, what);
+  const int rc = a.rank8 <= 16   ? launch_down<ACT, kDownTokens / 16, 1, true>(a, blocks, st, what)
+                 : a.rank8 <= 32 ? launch_down<ACT, kDownTokens / 16, 2, true>(a, blocks, st, what)
+                                 : launch_down<ACT, kDownTokens / 16, 4, true>(a, blocks, st, what);
   return rc != NPAMD_OK ? rc : launch_up<ACT, true>(a, (unsigned)space.most, st, what);
 }
 
@@ -600,17 +526,16 @@ extern "C" int npamd_adapter_linear(const void* x, int64_t ldx, const void* ids,
   NPAMD_REQUIRE(M >= 0 && N >= 0 && K >= 1 && rank >= 1 && adapters >= 1, "%s: bad shape M=%d N=%d K=%d rank=%d adapters=%d", what, M, N, K, rank, adapters);
   NPAMD_REQUIRE(act_dtype == NPAMD_F16 || act_dtype == NPAMD_BF16, "%s: f16 or bf16 only", what);
   NPAMD_REQUIRE(ids_bits == 32 || ids_bits == 64, "%s: ids of 32 or 64 bits, got %d", what, ids_bits);
-  if (K < 8 || rank > kMaxRank || adapters > kMaxAdapters || M > 1 << 22 || N > 1 << 24)
-    return fail(NPAMD_ERR_UNSUPPORTED, "%s: at least 8 columns of x, at most 2^22 tokens, 2^24 columns of y, rank %d and %d adapters", what, kMaxRank, kMaxAdapters);
+  if (rank > kMaxRank || adapters > kMaxAdapters || M > 1 << 22 || N > 1 << 24)
+    return fail(NPAMD_ERR_UNSUPPORTED, "%s: at most 2^22 tokens, 2^24 columns of y, rank %d and %d adapters", what, kMaxRank, kMaxAdapters);
   NPAMD_REQUIRE(ldx >= K && ldy >= N && (!base || ldbase >= N), "%s: bad row stride", what);
   if (M == 0 || N == 0) return NPAMD_OK;
   NPAMD_REQUIRE(x && ids && a && b && y, "%s: null pointer", what);
   NPAMD_REQUIRE((((uintptr_t)a | (uintptr_t)b) & 15) == 0, "%s: a and b have to lie at 16-byte addresses", what);
-  NPAMD_REQUIRE(M <= kBallotTokens || (((uintptr_t)x & 15) == 0 && ldx % 8 == 0 && K % 8 == 0),
-                "%s: past %d tokens x has to lie at a 16-byte address, K=%d and rows' distances have to be multiples of 8", what, kBallotTokens, K);
+  NPAMD_REQUIRE(((uintptr_t)x & 15) == 0 && ldx % 8 == 0 && K % 8 == 0, "%s: x has to lie at a 16-byte address, K=%d and its rows' distance have to be multiples of 8", what, K);
   const AdapterSpace space(M, N, K, rank, adapters);
   NPAMD_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= space.bytes, "%s: needs %lld bytes of 16-byte aligned workspace", what, (long long)space.bytes);
-  const AdapterArgs args{x, ids, a, b, base, scale, y, ldx, ((int64_t)K + 7) / 8 * 8, ldbase, ldy, M, N, K, rank, space.rank8, adapters, ids_bits == 64, space.parts, nullptr, nullptr, nullptr, nullptr, space.tokens};
+  const AdapterArgs args{x, ids, a, b, base, scale, y, ldx, ldbase, ldy, M, N, K, rank, space.rank8, adapters, ids_bits == 64, space.parts, nullptr, nullptr, nullptr, nullptr, space.tokens};
   hipStream_t st = (hipStream_t)stream;
   if (act_dtype == NPAMD_BF16) return launch_adapters<NPAMD_BF16>(args, space, (uint8_t*)workspace, st, what);
   return launch_adapters<NPAMD_F16>(args, space, (uint8_t*)workspace, st, what);

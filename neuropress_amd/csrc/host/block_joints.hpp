@@ -365,7 +365,7 @@ PyObject* adapter_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return translated([&]() -> PyObject* {
     const int device = device_of(args[0]);
     Rows x, base{nullptr, 0, 0, 0, 0};
-    if (!rows_argument(args[0], device, &x) || !PyLong_Check(args[6]) || !PyLong_Check(args[7]) || x.width < 8 || x.width != PyLong_AsLong(args[6])) Py_RETURN_NONE;
+    if (!rows_argument(args[0], device, &x) || !PyLong_Check(args[6]) || !PyLong_Check(args[7]) || x.width != PyLong_AsLong(args[6])) Py_RETURN_NONE;
     const at::Tensor *ids = readable(args[1], device), *a = readable(args[2], device), *b = readable(args[3], device);
     if (!ids || !a || !b || !ids->is_contiguous() || ids->sizes() != x.t->sizes().slice(0, x.t->dim() - 1) || (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong))
       Py_RETURN_NONE;
@@ -375,12 +375,8 @@ PyObject* adapter_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     sizes.back() = PyLong_AsLong(args[7]);
     if (!is_none(args[5]) && (!rows_argument(args[5], device, &base) || base.code != x.code || base.t->sizes() != at::IntArrayRef(sizes))) Py_RETURN_NONE;
     const int m = (int)x.m, cols = (int)sizes.back(), rank = (int)a->size(1), adapters = (int)a->size(0);
-    at::Tensor xr = *x.t;
-    int k = (int)x.width;
-    if (m > 64) {  // the entries' tokens come in whole pieces
-      xr = whole_pieces(*x.t, &x.ld);
-      k = (k + 7) / 8 * 8;
-    }
+    const at::Tensor xr = whole_pieces(*x.t, &x.ld);
+    const int k = ((int)x.width + 7) / 8 * 8;
     const int64_t bytes = npamd_adapter_linear_workspace_bytes(m, cols, k, rank, adapters);
     at::Tensor scratch, y = empty(sizes, x.t->scalar_type(), device);
     if (bytes > 0) scratch = floats(bytes, device);

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from . import ACTIVATIONS, _check_device, _dt, _on_device, _rows_of, gather_columns, tracked
+from . import ACTIVATIONS, _check_device, _dt, _on_device, _rows_of, tracked
 
 __all__ = ["residual_norm", "residual_norm_stats", "residual_norm_backward", "gated_linear", "gated_linear_pre", "gated_linear_backward", "LowRankAdapters",
            "adapter_linear"]  # fmt: skip
@@ -308,8 +308,6 @@ def adapter_linear(x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor
     with torch.no_grad(), _on_device(x):
         ids = ids.reshape(*ids.shape, *[1] * (len(lead) - ids.dim())).expand(lead).contiguous()
         x = x.detach().contiguous()
-        if k < 8:  # the kernels read pieces of eight columns
-            x, k = gather_columns(x.view(rows, k), None, 8).view(*lead, 8), 8
         y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, None if base is None else base.detach().contiguous(), k, n)
     if y is None:
         raise RuntimeError(f"{what}: no kernel for these tensors")
