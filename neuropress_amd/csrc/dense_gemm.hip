@@ -305,6 +305,24 @@ constexpr DenseCost kDenseCost[] = {
 };
 constexpr int kDenseTiles = sizeof(kDenseCost) / sizeof(kDenseCost[0]), kDenseTwoGroups = kDenseTiles - 1;
 
+// The same where W lies with the contracted index as its row and x does not: its reads are twice as many as x's, and tiles whose waves have few MFMAs to a read take longer.  Fitted to 150 shapes of 1 to
+// 4096 rows, 64 to 8192 columns and K of 128 to 28672: the tile and split of least estimate is 1.3 % slower than the best there is in the mean, with the figures above 7 % (1000 x 2184 x 5478
+// 50 / 42 us, 766 x 3360 x 9560 78 / 63).  Where both lie so the figures above are 1.5 % off.
+constexpr DenseCost kTurnedCost[kDenseTiles] = {
+    kDenseCost[0],
+    {64, 64, 1, 1.319f, 0.213f, 0.020f, 2.094f},
+    {64, 128, 1, 1.287f, 0.302f, 0.021f, 2.422f},
+    {128, 128, 1, 1.342f, 0.374f, 0.030f, 3.322f},
+    kDenseCost[4],
+    {256, 128, 1, 1.316f, 0.540f, 0.036f, 4.582f},
+    kDenseCost[6],
+    kDenseCost[7],
+    kDenseCost[8],
+    kDenseCost[9],
+    kDenseCost[10],
+    {256, 256, 1, 2.163f, 0.853f, 0.051f, 6.146f},
+};
+
 template <int ACT>
 int launch_dense(const DenseShape& s, int tile, hipStream_t st) {
   const int rc = tile == 0 ? launch_dense_tile<ACT, 1, 1, 4, false>(s, st)
@@ -407,10 +425,16 @@ void count_tiles(int M, int N, int64_t* tiles, std::index_sequence<I...>) {
 // below (their bytes, their share of the walk and the sum) is less than the best so far.  us on the host, all tiles and parts in turn / so: 384 x 4096 x 4096
 // 0.61 / 0.17, 77 x 3003 x 2176 0.83 / 0.16, 64 x 1024 x 4096 0.87 / 0.32, 528 x 336 x 13440 0.94 / 0.56.
 //
-// `tiles_there`: bit i for tile i of the list, of the forms that not every tile has; 64 x 128 in two groups and the kernel above are in no such list.
-DensePlan plan_dense(int M, int N, int K, int forced_tile, int max_splits, bool wide = true, unsigned tiles_there = ~0u) {
+// `form`: of the wide tiles' other forms.
+struct DenseForm {
+  unsigned tiles;  // bit i: it has tile i of the list; 64 x 128 in two groups and the kernel above are in no such list
+  const DenseCost* cost;
+  float split_fixed, split_per_mb;
+};
+constexpr DenseForm kPlainForm{~0u, kDenseCost, kDenseSplitFixed, kDenseSplitPerMb};
+DensePlan plan_dense(int M, int N, int K, int forced_tile, int max_splits, bool wide = true, const DenseForm& form = kPlainForm) {
   DensePlan best{0, 1, 1e30f};
-  if (forced_tile > 0 && forced_tile <= kDenseTiles && !(tiles_there >> (forced_tile - 1) & 1)) forced_tile = 0;
+  if (forced_tile > 0 && forced_tile <= kDenseTiles && !(form.tiles >> (forced_tile - 1) & 1)) forced_tile = 0;
   const int steps = K / 64;
   const int forced = tuning().dense_splits, most = max_splits < steps ? max_splits : steps;
   const int forced_splits = forced < most ? forced : most;
@@ -419,10 +443,10 @@ DensePlan plan_dense(int M, int N, int K, int forced_tile, int max_splits, bool 
   int64_t tiles[kDenseTiles];
   count_tiles(M, N, tiles, std::make_index_sequence<kDenseTiles>{});
   const bool two_groups = only >= 0 || (M >= N && steps >= 64);
-  auto load = [&](int i) { return (float)tiles[i] * steps * (kDenseCost[i].bm + kDenseCost[i].bn) * 128e-6f * kDenseCost[i].per_mb; };
+  auto load = [&](int i) { return (float)tiles[i] * steps * (kDenseCost[i].bm + kDenseCost[i].bn) * 128e-6f * form.cost[i].per_mb; };
   auto look = [&](int i, int splits, int part, float bytes, float sum) {
-    if (!(tiles_there >> i & 1)) return;
-    const DenseCost& c = kDenseCost[i];
+    if (!(form.tiles >> i & 1)) return;
+    const DenseCost& c = form.cost[i];
     const int64_t rounds = ((tiles[i] * splits + 7) / 8 + 31) / 32;
     if (i == kDenseTwoGroups && only < 0 && (splits == 1 || rounds > 1 || !two_groups)) return;
     const float walk = (float)rounds * ((part + c.groups - 1) / c.groups) * c.per_step;
@@ -436,22 +460,22 @@ DensePlan plan_dense(int M, int N, int K, int forced_tile, int max_splits, bool 
     for (int i = first; i < last; ++i) look(i, 1, steps, load(i), 0.f);
   if (forced_splits == 1 || max_splits < 2) return best;
   const float mb = 4e-6f * M * N;
-  auto per_mb = [](int i) { return i == kDenseTwoGroups ? kDenseTwoGroupsPerMb : kDenseSplitPerMb; };
+  auto per_mb = [&](int i) { return i == kDenseTwoGroups ? kDenseTwoGroupsPerMb : form.split_per_mb; };
   if (forced_splits > 1) {
     const int part = (steps + forced_splits - 1) / forced_splits;
-    for (int i = first; i < last; ++i) look(i, forced_splits, part, load(i), kDenseSplitFixed + per_mb(i) * mb * forced_splits);
+    for (int i = first; i < last; ++i) look(i, forced_splits, part, load(i), form.split_fixed + per_mb(i) * mb * forced_splits);
     return best;
   }
   const int parts = std::min(std::min(max_splits, kDensePlannedSplits), steps / kDenseMinSplitSteps);
   int part_of[kDensePlannedSplits + 1];
   for (int splits = 2; splits <= parts; ++splits) part_of[splits] = (steps + splits - 1) / splits;
   for (int i = first; i < last; ++i) {
-    const DenseCost& c = kDenseCost[i];
-    const float bytes = load(i), least = c.fixed + c.per_round + kDenseSplitFixed + fmaxf(bytes, tiles[i] * steps / (256.f * c.groups) * c.per_step);
+    const DenseCost& c = form.cost[i];
+    const float bytes = load(i), least = c.fixed + c.per_round + form.split_fixed + fmaxf(bytes, tiles[i] * steps / (256.f * c.groups) * c.per_step);
     for (int splits = 2; splits <= parts && tiles[i] * splits <= 512; ++splits) {
       const float sum = per_mb(i) * mb * splits;
       if (least + sum >= best.us) break;
-      look(i, splits, part_of[splits], bytes, kDenseSplitFixed + sum);
+      look(i, splits, part_of[splits], bytes, form.split_fixed + sum);
     }
   }
   return best;
@@ -573,8 +597,13 @@ __global__ void __launch_bounds__(64) splitk_reduce_gated_kernel(const DenseShap
 constexpr unsigned kGatedTiles = 1u << 1 | 1u << 2 | 1u << 3 | 1u << 5 | 1u << 6 | 1u << 7 | 1u << 8 | 1u << 9 | 1u << 11;
 constexpr unsigned kTurnedTiles = 1u << 1 | 1u << 2 | 1u << 3 | 1u << 5 | 1u << 11;
 
-DensePlan plan_gated(int M, int N, int K, int max_splits) { return plan_dense(M, 2 * N, K, tuning().dense_tile, max_splits, true, kGatedTiles); }
-DensePlan plan_turned(int M, int N, int K, int max_splits) { return plan_dense(M, N, K, tuning().dense_tile, max_splits, true, kTurnedTiles); }
+constexpr DenseForm kGatedForm{kGatedTiles, kDenseCost, kDenseSplitFixed, kDenseSplitPerMb};
+constexpr DenseForm kTurnedForm{kTurnedTiles, kTurnedCost, 2.0f, 0.3f}, kBothTurnedForm{kTurnedTiles, kDenseCost, kDenseSplitFixed, kDenseSplitPerMb};
+
+DensePlan plan_gated(int M, int N, int K, int max_splits) { return plan_dense(M, 2 * N, K, tuning().dense_tile, max_splits, true, kGatedForm); }
+DensePlan plan_turned(int M, int N, int K, bool x_too, int max_splits) {
+  return plan_dense(M, N, K, tuning().dense_tile, max_splits, true, x_too ? kBothTurnedForm : kTurnedForm);
+}
 
 int whole_steps(int K) { return (K + 63) / 64 * 64; }
 
@@ -600,15 +629,15 @@ int dense_gemm_gated(const char* what, const DenseShape& shape, int K, int act, 
   return check_launch(what);
 }
 
-int64_t dense_gemm_turned_workspace_bytes(int M, int N, int K, bool) {
-  const DensePlan p = plan_turned(M, N, whole_steps(K), kDenseMaxSplits);
+int64_t dense_gemm_turned_workspace_bytes(int M, int N, int K, bool x_too) {
+  const DensePlan p = plan_turned(M, N, whole_steps(K), x_too, kDenseMaxSplits);
   return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
 }
 
 int dense_gemm_turned(const char* what, const DenseShape& shape, int K, bool x_too, int act, int64_t workspace_bytes, hipStream_t st) {
   DenseShape s = shape;
-  DensePlan p = plan_turned(s.M, s.N, whole_steps(K), kDenseMaxSplits);
-  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * s.N * 4) < p.splits)) p = plan_turned(s.M, s.N, whole_steps(K), 1);
+  DensePlan p = plan_turned(s.M, s.N, whole_steps(K), x_too, kDenseMaxSplits);
+  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * s.N * 4) < p.splits)) p = plan_turned(s.M, s.N, whole_steps(K), x_too, 1);
   s.steps = whole_steps(K) / 64;
   s.splits = p.splits;
   s.K = K;

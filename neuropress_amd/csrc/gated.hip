@@ -121,24 +121,37 @@ __global__ void __launch_bounds__(256) gated_pointwise_kernel(const GatedPointwi
   float sum[2][8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[0][e] = sum[1][e] = 0.f;
-  for (int64_t row = first; row < last; ++row) {
-    const uint8_t* const pr = P::row_of(a.pre, row, a.ldp);
-    float dh[8], g[8], u[8];
-    P::unpack(P::load(P::row_of(a.dh, row, a.lddh), at), dh);
-    P::unpack(P::load(pr, at), g);
-    P::unpack(P::load(pr + (int64_t)a.N * 2, at), u);
+  constexpr int U = 4;  // rows on their way
+  for (int64_t row0 = first; row0 < last; row0 += U) {
+    u32x4 dv[U], gv[U], uv[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float value, slope;
-      activation_and_slope<KIND>(g[e], value, slope);
-      g[e] = dh[e] * u[e] * slope;
-      u[e] = dh[e] * value;
-      sum[0][e] += g[e];
-      sum[1][e] += u[e];
+    for (int i = 0; i < U; ++i) {
+      const int64_t row = min(row0 + i, last - 1);  // past the end: the last row, not stored
+      const uint8_t* const pr = P::row_of(a.pre, row, a.ldp);
+      dv[i] = P::load(P::row_of(a.dh, row, a.lddh), at);
+      gv[i] = P::load(pr, at);
+      uv[i] = P::load(pr + (int64_t)a.N * 2, at);
     }
-    uint8_t* const to = const_cast<uint8_t*>(P::row_of(a.dpre, row, a.ldd));
-    P::store(to, at, P::pack(g));
-    P::store(to + (int64_t)a.N * 2, at, P::pack(u));
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (row0 + i >= last) break;
+      float dh[8], g[8], u[8];
+      P::unpack(dv[i], dh);
+      P::unpack(gv[i], g);
+      P::unpack(uv[i], u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float value, slope;
+        activation_and_slope<KIND>(g[e], value, slope);
+        g[e] = dh[e] * u[e] * slope;
+        u[e] = dh[e] * value;
+        sum[0][e] += g[e];
+        sum[1][e] += u[e];
+      }
+      uint8_t* const to = const_cast<uint8_t*>(P::row_of(a.dpre, row0 + i, a.ldd));
+      P::store(to, at, P::pack(g));
+      P::store(to + (int64_t)a.N * 2, at, P::pack(u));
+    }
   }
   if (!a.partials) return;
   float* const to = a.partials + (int64_t)blockIdx.y * 2 * a.N + at;
