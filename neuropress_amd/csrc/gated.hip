@@ -32,13 +32,14 @@ int launch_some_tile(const FewArgs& a, int waves, hipStream_t st, const char* wh
   return check_launch(what);
 }
 
-// A tile of gate rows and one of up rows to a block.
+// A tile of gate rows and one of up rows to a block; two of each past 4096 columns, where one leaves a second round of blocks mostly empty (us at four tokens, one / two: 4864 x 896 7.6 / 5.9,
+// 5504 x 2048 12.8 / 11.6, 14336 x 4096 49 / 45; 4096 x 1024 5.3 / -).
 template <int ACT>
 int launch_some(const FewArgs& a, hipStream_t st, const char* what) {
-  const int steps = (a.K / 8 + 15) / 16, mt = (a.M + 15) / 16, waves = std::min(std::min(8, steps), 160 * 1024 / ((mt + 2) * 8192));
-  if (mt == 1) return launch_some_tile<ACT, 1, 2>(a, waves, st, what);
-  if (mt == 2) return launch_some_tile<ACT, 2, 2>(a, waves, st, what);
-  return mt == 3 ? launch_some_tile<ACT, 3, 2>(a, waves, st, what) : launch_some_tile<ACT, 4, 2>(a, waves, st, what);
+  const int steps = (a.K / 8 + 15) / 16, mt = (a.M + 15) / 16, r = mt <= 2 && a.N > 4096 ? 4 : 2, waves = std::min(std::min(8, steps), 160 * 1024 / ((mt + r) * 8192));
+  if (mt == 1) return r == 4 ? launch_some_tile<ACT, 1, 4>(a, waves, st, what) : launch_some_tile<ACT, 1, 2>(a, waves, st, what);
+  if (mt == 2) return r == 4 ? launch_some_tile<ACT, 2, 4>(a, waves, st, what) : launch_some_tile<ACT, 2, 2>(a, waves, st, what);
+  return launch_some_tile<ACT, 3, 2>(a, waves, st, what);
 }
 
 // A gate row and its up row to a wave, or (few and long) to a block's four.
@@ -60,12 +61,17 @@ int launch_few(const FewArgs& a, hipStream_t st, const char* what) {
   return check_launch(what);
 }
 
+// Which kernel takes a call; aligned: rows that the tiles can read.  Us with dense_few_kernel / dense_some_kernel / the tiles, silu: two tokens 14336 x 4096 43.5 / 44.2 / 54.5, 1024 x 1024 3.6 / 4.0 / 7.1;
+// three 1024 x 1024 4.0 / 3.9 / 7.1; 16 tokens 8192 x 2048 - / 15.6 / 17.8, 4864 x 896 - / 6.4 / 6.8.  Past 16 tokens a block holds two tiles of them: 32 tokens 14336 x 4096 - / 54 / 59, 8192 x 2048 - /
+// 17.5 / 17.7, 4096 x 1024 - / 6.3 / 7.2, but 5504 x 2048 - / 14.5 / 13.0, 4864 x 896 - / 8.3 / 6.9; 48 tokens 1024 x 1024 - / 5.8 / 7.2, 2752 x 1024 - / 6.5 / 7.1, but 2048 x 4096 - / 14.1 / 12.9; 64 tokens
+// 1024 x 1024 - / 7.6 / 7.2.
 enum Path { kFew, kSome, kTiles };
 Path path_of(int M, int N, int K, bool aligned) {
   if (M <= 2) return kFew;
   if (!aligned) return M <= NPAMD_GEMV_MAX_M ? kFew : kTiles;
-  if (M <= 16 || (M <= 32 && 2 * (int64_t)N * K <= 1 << 24)) return kSome;
-  return M <= 64 && N <= 2048 && K <= std::max(2 * N, 2560) ? kSome : kTiles;
+  const int64_t weights = 2 * (int64_t)N * K;
+  if (M <= 16 || (M <= 32 && (N <= 4096 ? weights <= 1 << 24 : N >= 8192))) return kSome;
+  return M <= 48 && weights <= 1 << 23 ? kSome : kTiles;
 }
 
 bool bad_shape(int M, int N, int K) { return M < 0 || N < 0 || K < 1; }
