@@ -217,26 +217,27 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave / RW, lanes = 64 * RW;
   const int lane = (int)threadIdx.x - team * lanes, H = a.H, pieces = (H + V - 1) / V;
   const float inv = 1.f / (float)H;
+  constexpr bool kHeld = NV < 4 || !POST;  // the weights and a shared gate stay in registers; else they come from the L1 when they are used (2048 x 12288 bf16, shared gate: 254 / 127 us)
   u32x4 dsv[NV], dzv[NV], yv[NV], rv[NV], wv[NV], pv[NV], gv[NV];
   float dw[NV][V], dp[NV][V], dg[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int p = lane + lanes * i, at = min(p * V, H - V);
     dsv[i] = dzv[i] = yv[i] = rv[i] = wv[i] = pv[i] = gv[i] = u32x4{0, 0, 0, 0};
-    if (p < pieces) {
+    if (kHeld && p < pieces) {
       wv[i] = P::load((const uint8_t*)a.w, at);
       if (POST) pv[i] = P::load((const uint8_t*)a.wp, at);
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[i][e] = dp[i][e] = dg[i][e] = 0.f;
   }
-  float next_rstd = 0.f, next_post = 0.f;
+  float next_stats = 0.f;  // rstd in even lanes, post_rstd in odd ones
+  const float* const stats = POST && threadIdx.x % 2 ? a.post_rstd : a.rstd;
   auto request = [&](int64_t row, int64_t end) __attribute__((always_inline)) {
     if (row >= end) return;
     int64_t at_row = row;  // by vector loads: scalar ones would be waited for in front of the barrier
     asm volatile("" : "+v"(at_row));
-    next_rstd = a.rstd[at_row];
-    if (POST) next_post = a.post_rstd[at_row];
+    next_stats = stats[at_row];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int p = lane + lanes * i, at = min(p * V, H - V);
@@ -278,19 +279,26 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
     const int group = unit / a.parts, part = unit - group * a.parts;
     const int64_t from = GATE == kSharedGate ? (int64_t)group * a.gate_every : 0, rows = GATE == kSharedGate ? min((int64_t)a.gate_every, a.M - from) : a.M;
     const int64_t begin = from + rows * part / a.parts, end = from + rows * (part + 1) / a.parts;
-    if (GATE == kSharedGate) {
+    if (GATE == kSharedGate && kHeld) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int p = lane + lanes * i;
         if (p < pieces) gv[i] = P::load(P::row_of(a.gate, group, a.ldg), min(p * V, H - V));
       }
     }
+    auto bring = [&](int i, int at) __attribute__((always_inline)) {  // what is not held
+      if (kHeld) return;
+      wv[i] = P::load((const uint8_t*)a.w, at);
+      if (POST) pv[i] = P::load((const uint8_t*)a.wp, at);
+      if (GATE == kSharedGate) gv[i] = P::load(P::row_of(a.gate, group, a.ldg), at);
+    };
     int64_t row = begin + team;
     if (kAhead) request(row, end);
     for (int64_t first = begin; first < end; first += teams, row += teams, turn ^= 1) {
       if (!kAhead) request(row, end);
       const bool live = row < end;
-      const float rstd = next_rstd, post = next_post;
+      const int stats_bits = __builtin_bit_cast(int, next_stats);
+      const float rstd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(stats_bits, 0)), post = __builtin_bit_cast(float, __builtin_amdgcn_readlane(stats_bits, 1));
       u32x4 ds_[NV], dz_[NV], y_[NV], r_[NV], g_[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) ds_[i] = dsv[i], dz_[i] = dzv[i], y_[i] = yv[i], r_[i] = rv[i], g_[i] = gv[i];
@@ -300,6 +308,8 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
       for (int i = 0; i < NV; ++i) {
         const int p = lane + lanes * i, skip = p * V + V <= H ? 0 : p * V + V - H;  // values that the piece before has too
         if (!live || p >= pieces) continue;
+        bring(i, min(p * V, H - V));
+        if (GATE == kSharedGate && !kHeld) g_[i] = gv[i];
 #pragma unroll
         for (int half = 0; half < V / 4; ++half) {
           float dz[4], rh[4], w[4], ds[4], yh[4], wp[4], g[4];
@@ -348,6 +358,8 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
         const int p = lane + lanes * i, at = min(p * V, H - V);
         if (p >= pieces) continue;
         const int skip = p * V + V <= H ? 0 : p * V + V - H;
+        bring(i, at);
+        if (GATE == kSharedGate && !kHeld) g_[i] = gv[i];
         P::forget(ds_[i]);
         P::forget(dz_[i]);
         P::forget(r_[i]);
