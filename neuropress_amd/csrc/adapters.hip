@@ -69,8 +69,8 @@ __device__ __forceinline__ Tokens ballot_entry(const AdapterArgs& a, int e) {
 }
 
 __device__ __forceinline__ Tokens listed_entry(const AdapterArgs& a, int e) {
+  const Entry v = a.entries[e];  // there for every block, whether it has been written or not: one round trip to memory, not two
   if (e >= *a.count) return {-1, 0, 0, 0};
-  const Entry v = a.entries[e];
   return {__builtin_amdgcn_readfirstlane(v.adapter), __builtin_amdgcn_readfirstlane(v.first), __builtin_amdgcn_readfirstlane(v.count), 0};
 }
 
@@ -264,10 +264,19 @@ __global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const 
     if (e.adapter < 0) continue;
     f32x4 sum[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     if (at < e.count && r < a.rank8) {
-      for (int z = 0; z < a.parts; ++z) {
-        const f32x4* const from = reinterpret_cast<const f32x4*>(a.t + ((int64_t)z * a.M + m) * a.rank8 + r);
-        sum[0] += from[0];
-        sum[1] += from[1];
+      const float* const from = a.t + (int64_t)m * a.rank8 + r;
+      const int64_t part = (int64_t)a.M * a.rank8;
+      for (int z0 = 0; z0 < a.parts; z0 += 4) {  // four parts on their way
+        f32x4 got[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4* const of = reinterpret_cast<const f32x4*>(from + min(z0 + i, a.parts - 1) * part);
+          got[i][0] = of[0];
+          got[i][1] = of[1];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (z0 + i < a.parts) sum[0] += got[i][0], sum[1] += got[i][1];
       }
     }
     float v[8], back = 1.f;  // a power of two
@@ -480,9 +489,9 @@ int launch_down(const AdapterArgs& a, unsigned blocks, hipStream_t st, const cha
 template <int ACT, int RC, bool LISTED>
 int launch_up_tile(const AdapterArgs& a, unsigned entries, hipStream_t st, const char* what) {
   using T = UpTile<RC>;
-  // A wave to a block where columns and entries are few.
+  // Four waves to a block, which bring t in together; one where that is next to nothing and blocks are few.
   const int64_t strips = ((int64_t)a.N + 16 * T::kCT - 1) / (16 * T::kCT);
-  const int waves = strips * entries >= 1024 ? 4 : 1, lds = T::lds(a.entry_tokens);
+  const int waves = LISTED || strips * entries >= 1024 ? 4 : 1, lds = T::lds(a.entry_tokens);
   static LdsLatch latch;
   const auto kernel = adapter_up_kernel<ACT, RC, LISTED>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), lds);
