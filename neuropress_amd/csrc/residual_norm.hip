@@ -278,7 +278,9 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
   for (int unit = blockIdx.x; unit < a.groups * a.parts; unit += gridDim.x) {
     const int group = unit / a.parts, part = unit - group * a.parts;
     const int64_t from = GATE == kSharedGate ? (int64_t)group * a.gate_every : 0, rows = GATE == kSharedGate ? min((int64_t)a.gate_every, a.M - from) : a.M;
-    const int64_t begin = from + rows * part / a.parts, end = from + rows * (part + 1) / a.parts;
+    // The parts' rows in turn: neighbouring blocks read neighbouring rows, where strips of rows would start a power of two of bytes apart (8192 x 4096: 92 / 83 us).
+    const int64_t begin = from + (int64_t)part * teams, end = from + rows;
+    const int step = a.parts * teams;
     if (GATE == kSharedGate && kHeld) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
     };
     int64_t row = begin + team;
     if (kAhead) request(row, end);
-    for (int64_t first = begin; first < end; first += teams, row += teams, turn ^= 1) {
+    for (int64_t first = begin; first < end; first += step, row += step, turn ^= 1) {
       if (!kAhead) request(row, end);
       const bool live = row < end;
       const int stats_bits = __builtin_bit_cast(int, next_stats);
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
       u32x4 ds_[NV], dz_[NV], y_[NV], r_[NV], g_[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) ds_[i] = dsv[i], dz_[i] = dzv[i], y_[i] = yv[i], r_[i] = rv[i], g_[i] = gv[i];
-      if (kAhead) request(row + teams, end);
+      if (kAhead) request(row + step, end);
       float s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
