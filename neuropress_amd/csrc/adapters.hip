@@ -8,7 +8,7 @@
 //   up:   y = base + scale t B^T.  A block brings its entry's t into LDS once, as two parts of B's type, for an MFMA each (t is not rounded to 16 bits: 2^-16 of it is left with bf16; fp16, scaled
 //         by a power of two to the row's largest, 2^-21), and its waves take 64 or 128 columns each.  Column 8 c + b of a wave is row c of MFMA b, so that a lane ends up with eight neighbouring columns
 //         of four tokens and 16 lanes with 256 bytes of a row of base and y, side by side.  (With four tokens' rows in every quarter of the lanes instead, as the MFMAs' own layout
-//         has them, a load touches 64 places: 64 to 86 us in the place of XX for 4096 tokens through 14336 columns.)
+//         has them, a load touches 64 places: 64 to 86 us in the place of 52 for 4096 tokens through 14336 columns of bf16, rank 64.)
 // Bound by the latency of two dependent launches for a decode step, by the bytes of base and y for prompts.
 #include <algorithm>
 
@@ -24,6 +24,7 @@ namespace {
 constexpr int kBallotTokens = 64;  // as many as a wave compares at once
 constexpr int kMaxAdapters = 8192, kMaxRank = 256;
 constexpr int kDownTokens = 32;    // of a listed entry's part in the down kernel
+constexpr int kGridRows = 65535;   // of a launch
 
 struct Entry {
   int adapter, first, count, unused;  // tokens: order[first .. first + count)
@@ -197,7 +198,7 @@ __device__ __forceinline__ void two_parts(const float (&v)[8], u32x4& hi, u32x4&
   for (int i = 0; i < 4; ++i) hi[i] = h16[2 * i] | (h16[2 * i + 1] << 16), lo[i] = l16[2 * i] | (l16[2 * i + 1] << 16);
 }
 
-// RC chunks of 32 ranks, CT columns to a lane; blockIdx.x: 16 CT columns to each of the block's waves, .y: entry.  LDS: t's two parts, rows of 64 RC + 16 bytes, then what each token's sums are
+// RC chunks of 32 ranks, CT columns to a lane; blockIdx.x: 16 CT columns to each of the block's waves, .y and .z: entry.  LDS: t's two parts, rows of 64 RC + 16 bytes, then what each token's sums are
 // multiplied with, and the tokens.
 template <int RC>
 struct UpTile {
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const 
   typedef uint32_t ColumnsAny __attribute__((ext_vector_type(CT / 2), aligned(2)));
   extern __shared__ __attribute__((aligned(16))) uint8_t up_lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
-  const Tokens e = LISTED ? listed_entry(a, blockIdx.y) : ballot_entry(a, blockIdx.y);
+  const Tokens e = LISTED ? listed_entry(a, blockIdx.z * gridDim.y + blockIdx.y) : ballot_entry(a, blockIdx.y);
   if (e.count <= 0) return;
   const int groups = (e.count + 15) / 16;
   const int64_t col0 = ((int64_t)blockIdx.x * (blockDim.x >> 6) + wave) * 16 * CT, n0 = col0 + CT * c;
@@ -362,8 +363,8 @@ __global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const 
 }
 
 // Tokens by adapter, those without one last, and the entries.  One block: counts in LDS, their running sums, then every token to its place.  Where all of a wave's tokens have one
-// adapter, as a prompt's have, they are counted and placed side by side with one atomic addition; else each by itself.  A token's results do not depend on its place.  XX us for 4096 tokens of
-// five prompts, XX for 4096 of 1024 adapters in any order (with a wave's adapters one after the other 8.4 and 91).
+// adapter, as a prompt's have, they are counted and placed side by side with one atomic addition; else each by itself.  A token's results do not depend on its place.  5.9 us for 4096 tokens of
+// five prompts, 7.0 for 4096 of 1024 adapters in any order (with a wave's adapters one after the other 8.4 and 91).
 __global__ void __launch_bounds__(1024) adapter_list_kernel(const AdapterArgs a, int* __restrict__ order, Entry* __restrict__ entries, int* __restrict__ count) {
   extern __shared__ int places[];  // [adapters + 1]
   __shared__ int sums[2][16];
@@ -457,13 +458,15 @@ int entry_tokens_of(int M, int N, int rank8) {
 
 struct AdapterSpace {
   bool listed;
-  int rank8, parts, tokens, most;  // entries at most
+  int rank8, parts, tokens, most, layers;  // entries at most, whole layers of a grid's rows
   int64_t t, entries, order, bytes;
   AdapterSpace(int M, int N, int K, int rank, int adapters) {
     listed = M > kBallotTokens;
     rank8 = (rank + 7) / 8 * 8;
     tokens = listed ? entry_tokens_of(M, N, rank8) : 16;
     most = listed ? (int)std::min<int64_t>(M, ((int64_t)M + tokens - 1) / tokens + adapters + 1) : M;
+    layers = (most + kGridRows - 1) / kGridRows;
+    most = (most + layers - 1) / layers * layers;
     // Parts of K of the down kernel: as many as there are compute units for its blocks; few tokens: two steps for each of a block's waves.
     const int blocks = (M + kDownTokens - 1) / kDownTokens * ((rank8 + 63) / 64);
     parts = listed ? std::clamp(std::min(256 / blocks, K / 1024), 1, 8) : std::clamp((K + 1023) / 1024, 1, 8);
@@ -487,7 +490,7 @@ int launch_down(const AdapterArgs& a, unsigned blocks, hipStream_t st, const cha
 }
 
 template <int ACT, int RC, bool LISTED>
-int launch_up_tile(const AdapterArgs& a, unsigned entries, hipStream_t st, const char* what) {
+int launch_up_tile(const AdapterArgs& a, int entries, int layers, hipStream_t st, const char* what) {
   using T = UpTile<RC>;
   // Four waves to a block, which bring t in together; one where that is next to nothing and blocks are few.
   const int64_t strips = ((int64_t)a.N + 16 * T::kCT - 1) / (16 * T::kCT);
@@ -496,16 +499,16 @@ int launch_up_tile(const AdapterArgs& a, unsigned entries, hipStream_t st, const
   const auto kernel = adapter_up_kernel<ACT, RC, LISTED>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), lds);
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
-  launch(kernel, dim3((unsigned)((strips + waves - 1) / waves), entries), 64 * waves, lds, st, a);
+  launch(kernel, dim3((unsigned)((strips + waves - 1) / waves), (unsigned)(entries / layers), (unsigned)layers), 64 * waves, lds, st, a);
   return check_launch(what);
 }
 
 template <int ACT, bool LISTED>
-int launch_up(const AdapterArgs& a, unsigned entries, hipStream_t st, const char* what) {
-  if (a.rank8 <= 32) return launch_up_tile<ACT, 1, LISTED>(a, entries, st, what);
-  if (a.rank8 <= 64) return launch_up_tile<ACT, 2, LISTED>(a, entries, st, what);
-  if (a.rank8 <= 128) return launch_up_tile<ACT, 4, LISTED>(a, entries, st, what);
-  return launch_up_tile<ACT, 8, LISTED>(a, entries, st, what);
+int launch_up(const AdapterArgs& a, int entries, int layers, hipStream_t st, const char* what) {
+  if (a.rank8 <= 32) return launch_up_tile<ACT, 1, LISTED>(a, entries, layers, st, what);
+  if (a.rank8 <= 64) return launch_up_tile<ACT, 2, LISTED>(a, entries, layers, st, what);
+  if (a.rank8 <= 128) return launch_up_tile<ACT, 4, LISTED>(a, entries, layers, st, what);
+  return launch_up_tile<ACT, 8, LISTED>(a, entries, layers, st, what);
 }
 
 template <int ACT>
@@ -513,7 +516,7 @@ int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipSt
   a.t = (float*)at;
   if (!space.listed) {
     const int rc = launch_down<ACT, 1, 1, false>(a, (unsigned)a.M, st, what);
-    return rc != NPAMD_OK ? rc : launch_up<ACT, false>(a, (unsigned)a.M, st, what);
+    return rc != NPAMD_OK ? rc : launch_up<ACT, false>(a, a.M, 1, st, what);
   }
   int* const count = (int*)(at + space.t);
   Entry* const entries = (Entry*)(at + space.t + 16);
@@ -525,7 +528,7 @@ int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipSt
   const int rc = a.rank8 <= 16   ? launch_down<ACT, kDownTokens / 16, 1, true>(a, blocks, st, what)
                  : a.rank8 <= 32 ? launch_down<ACT, kDownTokens / 16, 2, true>(a, blocks, st, what)
                                  : launch_down<ACT, kDownTokens / 16, 4, true>(a, blocks, st, what);
-  return rc != NPAMD_OK ? rc : launch_up<ACT, true>(a, (unsigned)space.most, st, what);
+  return rc != NPAMD_OK ? rc : launch_up<ACT, true>(a, space.most, space.layers, st, what);
 }
 
 }  // namespace

@@ -244,3 +244,43 @@ def test_refusals(gpu):
     narrow = kernels.LowRankAdapters(a[:, :, :5], b)
     with pytest.raises(RuntimeError, match="x must be"):
         kernels.adapter_linear(x[:, :8], narrow, ids, base)
+
+
+def test_more_entries_than_rows_of_a_grid(gpu):
+    """Entries of 32 tokens, more than 65535 of them."""
+    m, adapters = 2_200_000, 5
+    x, a, b, scale, base = _make(m, 8, 8, 136, adapters, torch.bfloat16)
+    ids = _ids(m, adapters, "any")
+    _check(x, a, b, scale, base, ids, _run(x, a, b, scale, ids, base))
+
+
+@pytest.mark.parametrize("m", [4, 80])
+def test_broadcast_inputs(gpu, m):
+    """One row for all tokens, one number for all, and rows that lie the other way round."""
+    from neuropress_amd import kernels
+
+    x, a, b, scale, base = _make(m, 72, 64, 8, 4, torch.float16)
+    ids = _ids(m, 4, "any")
+    ad = kernels.LowRankAdapters(a, b, scale)
+    for xs, bs, i in ((x[:1].expand(m, -1), base[:1].expand(m, -1), ids), (x.T.contiguous().T, base.T.contiguous().T, ids), (x, base, ids[:1].expand(m)), (x, base, torch.tensor(2, device=gpu))):
+        y = kernels.adapter_linear(xs, ad, i, bs)
+        _check(xs.contiguous(), a, b, scale, bs.contiguous(), i.expand(m).contiguous(), y)
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 90])
+def test_module_beside_quantized_layers(gpu, tokens):
+    """The base of a module is what its projection gives, int4 or codebook, whatever kernels take it."""
+    from neuropress_amd.kernels import LowRankAdapters
+    from neuropress_amd.nn import NPAdapterLinear, NPLinear
+
+    q = cases.q4_layer(5, 96, 128)
+    base = NPLinear(q["blob"], q["scale"], 96, 128, 32, 4, "sym", "cuda", compute_dtype=torch.float16).to(gpu)
+    x, a, b, scale, _ = _make(tokens, 96, 128, 12, 3, torch.float16)
+    layer = NPAdapterLinear(base, LowRankAdapters(a, b, scale))
+    ids = _ids(tokens, 3, "any")
+    with torch.no_grad():
+        _check(x, a, b, scale, base(x), ids, layer(x, ids), "tokens")
+        twice = x[None].expand(2, -1, -1)
+        y, per_sequence = base(twice), layer(twice, torch.tensor([1, -1], device=gpu))  # of so many tokens: the projection's kernels may be others
+    _check(x, a, b, scale, y[0], torch.ones_like(ids), per_sequence[0], "sequences")
+    assert torch.equal(per_sequence[1], y[1])
