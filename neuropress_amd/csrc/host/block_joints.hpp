@@ -309,7 +309,8 @@ PyObject* gated_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t n) 
     Rows dh, x, w, pre;
     if (activation_of(args[4]) < 0 || !rows_argument(args[1], device, &x) || !gated_weight(args[2], x, device, &w)) Py_RETURN_NONE;
     if (!rows_argument(args[0], device, &dh) || !rows_argument(args[3], device, &pre) || dh.code != x.code || pre.code != x.code) Py_RETURN_NONE;
-    if (dh.m != x.m || pre.m != x.m || 2 * dh.width != w.m || pre.width != w.m) Py_RETURN_NONE;
+    const auto lead = [](const Rows& r) { return r.t->sizes().slice(0, r.t->dim() - 1); };
+    if (lead(dh) != lead(x) || lead(pre) != lead(x) || 2 * dh.width != w.m || pre.width != w.m) Py_RETURN_NONE;
     for (int i = 5; i < 9; ++i)
       if (!PyBool_Check(args[i])) Py_RETURN_NONE;
     const bool need[3] = {args[6] == Py_True, args[7] == Py_True, args[8] == Py_True};

@@ -290,3 +290,33 @@ def test_refusals(gpu):
                         ((dh, x.cpu(), w, pre), "GPU"), ((dh.cpu(), x, w, pre), "GPU"), ((dh, x, w, pre, "silu", (True,) * 3, torch.bfloat16), "bias_dtype")]:  # fmt: skip
         with pytest.raises(RuntimeError, match=match):
             kernels.gated_linear_backward(*args)
+
+
+@pytest.mark.parametrize("m", [2, 12, 90])
+def test_broadcast_gradients_and_inputs(gpu, m):
+    """The gradient of a sum, one value for all, and inputs whose rows are one row or lie the other way round."""
+    from neuropress_amd import kernels
+
+    x, w, b, _ = _inputs(m, 40, 72, torch.bfloat16)
+    one = torch.ones(m, 40, dtype=x.dtype, device="cuda")
+    for xs, ws in ((x, w), (x[:1].expand(m, -1), w[:1].expand(80, -1)), (x.T.contiguous().T, w.T.contiguous().T)):
+        h, pre = _check_forward(xs.contiguous(), ws.contiguous(), b, "gelu_tanh")
+        leaves = [t.detach().requires_grad_() for t in (xs, ws, b)]
+        out = kernels.gated_linear(*leaves, "gelu_tanh")
+        assert torch.equal(out, h)
+        got = torch.autograd.grad(out.sum(), leaves)
+        want = kernels.gated_linear_backward(one, xs.contiguous(), ws.contiguous(), pre, "gelu_tanh")
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+def test_gradients_of_other_rows_are_refused(gpu):
+    """As many rows in another shape: which belongs to which is not said."""
+    from neuropress_amd import kernels
+
+    x, w, b, dh = _inputs(6, 16, 64, torch.float16)
+    x = x.view(2, 3, 64)
+    pre = kernels.gated_linear_pre(x, w, b)[1]
+    assert kernels.gated_linear_backward(dh.view(2, 3, 16), x, w, pre)[0].shape == x.shape
+    for wrong in ((dh.view(3, 2, 16), pre), (dh, pre), (dh.view(2, 3, 16), pre.view(6, 32)), (dh.view(2, 3, 16), pre.view(3, 2, 32))):
+        with pytest.raises(RuntimeError, match="dh and pre"):
+            kernels.gated_linear_backward(wrong[0], x, w, wrong[1])
