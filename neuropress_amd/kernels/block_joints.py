@@ -186,7 +186,7 @@ def gated_linear(x: torch.Tensor, gate_up: torch.Tensor, bias: torch.Tensor | No
     """``act(x @ gate.T + bias) * (x @ up.T + bias)`` of an fp16 / bf16 *x* ``[..., K]`` and *gate_up* ``[2 N, K]`` of its dtype, N gate rows before N up rows (as
     :class:`MoEExperts` has them), rounded once (``npamd_gated_linear``): the first half of a gated feed-forward block in one kernel.
 
-    *activation*: as for :func:`dense_linear_act`; *bias* ``[2 N]`` in float32 or x's dtype.  Any sizes.  Where a gradient is recorded both sums are kept, rounded to x's dtype, and the
+    *activation*: as for :func:`dense_linear_act`; *bias* ``[2 N]`` in float32 or x's dtype.  Any number of tokens, N below 2**21 and K below 2**22 (a few tokens: 2**24 and 2**30).  Where a gradient is recorded both sums are kept, rounded to x's dtype, and the
     backward pass is :func:`gated_linear_backward`'s kernels (first derivatives; captured under the terms of :func:`layer_norm`).  Calls that torch follows in other ways go through torch's
     own operations, which round in between.
     """

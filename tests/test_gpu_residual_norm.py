@@ -352,3 +352,79 @@ def test_refusals(gpu):
                           (dict(rstd=rstd.half()), "rstd"), (dict(post_rstd=None), "rstd"), (dict(stream=r.cpu()), "GPU"), (dict(gate=g[:, 0]), "gate")]:  # fmt: skip
         with pytest.raises(RuntimeError, match=match):
             kernels.residual_norm_backward(**{**good, **change})
+
+
+def test_each_input_by_itself(gpu):
+    """One leaf that follows, the others not: its gradient is the one that all of them together give."""
+    from neuropress_amd import kernels
+
+    t = _make((2, 11, 136), torch.bfloat16, True, "sequence")
+    grads = _grads((2, 11, 136), torch.bfloat16)
+    all_leaves = [v.clone().requires_grad_() for v in t]
+    want = torch.autograd.grad(kernels.residual_norm(*all_leaves, scale=0.6), all_leaves, grads)
+    for i in range(5):
+        leaves = [v.clone().requires_grad_(j == i) for j, v in enumerate(t)]
+        got = torch.autograd.grad(kernels.residual_norm(*leaves, scale=0.6), leaves[i], grads)[0]
+        assert torch.equal(got, want[i])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_broadcast_gradients_and_inputs(gpu, dtype):
+    """The gradient of a sum, one value for all, and inputs whose rows are one row or lie the other way round."""
+    from neuropress_amd import kernels
+
+    t = _make((6, 10, 72), dtype, True, "channel")
+    one = torch.ones((6, 10, 72), dtype=dtype, device="cuda")
+    for x, y in ((t[0], t[1]), (t[0][:1].expand(6, -1, -1), t[1][:, :1].expand(-1, 10, -1)), (t[0].transpose(0, 1).contiguous().transpose(0, 1), t[1].permute(2, 0, 1).contiguous().permute(1, 2, 0))):
+        same = [x.contiguous(), y.contiguous(), *t[2:]]
+        stats = _check_forward(same, 0.9)
+        leaves = [v.detach().requires_grad_() for v in (x, y, *t[2:])]
+        r, z = kernels.residual_norm(*leaves, scale=0.9)
+        assert torch.equal(r, stats[0]) and torch.equal(z, stats[1])
+        got = torch.autograd.grad(r.sum() + z.sum(), leaves)
+        want = kernels.residual_norm_backward(one, one, same[1], stats[0], *t[2:], 0.9, stats[2], stats[3])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_one_tensor_as_both_inputs(gpu):
+    from neuropress_amd import kernels
+
+    t = _make((7, 264), torch.float32, True, "none")
+    stats = _check_forward([t[0], t[0], *t[2:]], 0.5)
+    leaf = t[0].clone().requires_grad_()
+    ds, dz = _grads((7, 264), torch.float32)
+    got = torch.autograd.grad(kernels.residual_norm(leaf, leaf, t[2], t[3], scale=0.5), leaf, (ds, dz))[0]
+    want = kernels.residual_norm_backward(ds, dz, t[0], stats[0], t[2], t[3], None, 0.5, stats[2], stats[3])
+    assert torch.equal(got, want[0] + want[1])
+
+
+@pytest.mark.parametrize("rows,every", [(1000, 1000), (1000, 37), (777, 300), (513, 512)])
+def test_rows_of_a_part_lie_apart(gpu, rows, every):
+    """Blocks take every so manieth row of a gate's: the last gate has fewer rows than there are parts."""
+    from neuropress_amd import _lib, kernels
+
+    t = _make((rows, 200), torch.float32, True, "none")
+    gate = torch.randn((rows + every - 1) // every, 200, generator=cases.gen(rows)).cuda()
+    wide = gate.repeat_interleave(every, 0)[:rows].contiguous()
+    stats = kernels.residual_norm_stats(*t[:4], wide, 0.8)
+    ds, dz = _grads((rows, 200), torch.float32)
+    _check_backward([*t[:4], wide], 0.8, stats, ds, dz)
+    whole = rows // every * every
+    if whole:  # as sequences, with the rows of the last, shorter one left out
+        seq = [v[:whole].view(-1, every, 200) for v in t[:2]]
+        _check_backward([*seq, t[2], t[3], gate[: rows // every, None]], 0.8, [s[:whole].view(-1, every, *s.shape[1:]) for s in stats],
+                        *(d[:whole].view(-1, every, 200) for d in (ds, dz)))  # fmt: skip
+    # through the C interface, whose last gate may have fewer rows
+    out = [torch.empty_like(t[0]), torch.empty_like(t[0]), torch.empty(200, device="cuda"), torch.empty(200, device="cuda"), torch.empty_like(gate)]
+    lib = _lib.load()
+    need = lib.npamd_residual_norm_workspace_bytes(rows, 200, every, 2)
+    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    p = lambda v: v.data_ptr()
+    rc = lib.npamd_residual_norm_backward(p(ds), 200, p(dz), 200, p(t[1]), 200, p(stats[0]), 200, p(t[2]), p(t[3]), p(gate), 200, every, 0.8, p(stats[2]), p(stats[3]), p(out[0]), 200, p(out[1]),
+                                          200, p(out[2]), p(out[3]), p(out[4]), rows, 200, 2, p(scratch), need, torch.cuda.current_stream().cuda_stream)  # fmt: skip
+    assert rc == 0
+    dr, edr, dy, dw, dp, dg = _backward(ds, dz, t[1], stats[0], t[2], t[3], wide, 0.8, stats[2], stats[3])
+    seg = lambda v: torch.stack([v[i : i + every].sum(0) for i in range(0, rows, every)])
+    k = (rows / 32 + 80) * U
+    for got, ref in zip(out, ((dr, edr), dy, dw, dp, (seg(dg[0]), seg(dg[1]) + k * seg(dg[0].abs())))):
+        _within(got, *ref, torch.float32, f"{rows} rows, a gate for {every}")
