@@ -24,6 +24,7 @@ namespace {
 constexpr int kBallotTokens = 64;  // as many as a wave compares at once
 constexpr int kMaxAdapters = 8192, kMaxRank = 256;
 constexpr int kDownTokens = 32;    // of a listed entry's part in the down kernel
+constexpr int kManyWaves = 1024;   // of the up kernel: four for each compute unit
 constexpr int kGridRows = 65535;   // of a launch
 
 struct Entry {
@@ -200,17 +201,17 @@ __device__ __forceinline__ void two_parts(const float (&v)[8], u32x4& hi, u32x4&
 
 // RC chunks of 32 ranks, CT columns to a lane; blockIdx.x: 16 CT columns to each of the block's waves, .y and .z: entry.  LDS: t's two parts, rows of 64 RC + 16 bytes, then what each token's sums are
 // multiplied with, and the tokens.
-template <int RC>
+template <int RC, int CT>
 struct UpTile {
-  static constexpr int kRow = 64 * RC + 16, kCT = RC <= 2 ? 8 : 4;
+  static constexpr int kRow = 64 * RC + 16;
   static constexpr int kTokens = RC <= 2 ? 128 : 256 / RC;  // of an entry, at most
   static constexpr int lds(int tokens) { return tokens * (2 * kRow + 8); }
 };
 
-template <int ACT, int RC, bool LISTED>
+template <int ACT, int RC, int CT, bool LISTED>
 __global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const AdapterArgs a) {
-  using T = UpTile<RC>;
-  constexpr int CT = T::kCT, kPieces = 4 * RC;  // of a row of t, eight values each
+  using T = UpTile<RC, CT>;
+  constexpr int kPieces = 4 * RC;  // of a row of t, eight values each
   typedef uint32_t Columns __attribute__((ext_vector_type(CT / 2)));
   typedef uint32_t ColumnsAny __attribute__((ext_vector_type(CT / 2), aligned(2)));
   extern __shared__ __attribute__((aligned(16))) uint8_t up_lds[];
@@ -489,26 +490,31 @@ int launch_down(const AdapterArgs& a, unsigned blocks, hipStream_t st, const cha
   return check_launch(what);
 }
 
-template <int ACT, int RC, bool LISTED>
+template <int ACT, int RC, int CT, bool LISTED>
 int launch_up_tile(const AdapterArgs& a, int entries, int layers, hipStream_t st, const char* what) {
-  using T = UpTile<RC>;
+  using T = UpTile<RC, CT>;
   // Four waves to a block, which bring t in together; one where that is next to nothing and blocks are few.
-  const int64_t strips = ((int64_t)a.N + 16 * T::kCT - 1) / (16 * T::kCT);
-  const int waves = LISTED || strips * entries >= 1024 ? 4 : 1, lds = T::lds(a.entry_tokens);
+  const int64_t strips = ((int64_t)a.N + 16 * CT - 1) / (16 * CT);
+  const int waves = LISTED || strips * entries >= kManyWaves ? 4 : 1, lds = T::lds(a.entry_tokens);
   static LdsLatch latch;
-  const auto kernel = adapter_up_kernel<ACT, RC, LISTED>;
+  const auto kernel = adapter_up_kernel<ACT, RC, CT, LISTED>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), lds);
   if (e != hipSuccess) return fail(NPAMD_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
   launch(kernel, dim3((unsigned)((strips + waves - 1) / waves), (unsigned)(entries / layers), (unsigned)layers), 64 * waves, lds, st, a);
   return check_launch(what);
 }
 
+// Four columns to a lane where registers allow no more and, of up to 64 tokens, where waves are few: there is less to a wave then (us of a call, eight / four: one token 4096 x 4096 of rank 16 7.3 / 6.9,
+// 16 of rank 64 8.8 / 8.0; but 32 tokens of as many adapters 14336 x 4096 9.8 / 11.5).
 template <int ACT, bool LISTED>
 int launch_up(const AdapterArgs& a, int entries, int layers, hipStream_t st, const char* what) {
-  if (a.rank8 <= 32) return launch_up_tile<ACT, 1, LISTED>(a, entries, layers, st, what);
-  if (a.rank8 <= 64) return launch_up_tile<ACT, 2, LISTED>(a, entries, layers, st, what);
-  if (a.rank8 <= 128) return launch_up_tile<ACT, 4, LISTED>(a, entries, layers, st, what);
-  return launch_up_tile<ACT, 8, LISTED>(a, entries, layers, st, what);
+  if (a.rank8 > 128) return launch_up_tile<ACT, 8, 4, LISTED>(a, entries, layers, st, what);
+  if (a.rank8 > 64) return launch_up_tile<ACT, 4, 4, LISTED>(a, entries, layers, st, what);
+  if constexpr (!LISTED) {
+    if (((int64_t)a.N + 127) / 128 * entries < kManyWaves)
+      return a.rank8 <= 32 ? launch_up_tile<ACT, 1, 4, false>(a, entries, layers, st, what) : launch_up_tile<ACT, 2, 4, false>(a, entries, layers, st, what);
+  }
+  return a.rank8 <= 32 ? launch_up_tile<ACT, 1, 8, LISTED>(a, entries, layers, st, what) : launch_up_tile<ACT, 2, 8, LISTED>(a, entries, layers, st, what);
 }
 
 template <int ACT>
