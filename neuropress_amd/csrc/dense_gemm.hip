@@ -648,6 +648,84 @@ int dense_gemm_turned(const char* what, const DenseShape& shape, int K, bool x_t
   return check_launch(what);
 }
 
+namespace {
+
+// Two products in one launch (wide_gemm_pair.hip), on one tile, the second's tiles whole: us as for one, the rounds counted until the last block of both is done, and the bytes of the second's result,
+// which is the gradient of weights and as large as they are.  Together they are taken where the estimate is 5 % less than that of one after the other, which have a launch's gap and one more
+// last round.  240 shapes of 1 to 4096 rows, 64 to 14336 and 64 to 8192 columns were looked at on every tile and in 1 to 8 parts; of 151 others the whole backward pass takes 0.82 of the time
+// in the mean, five take 3 to 7 % longer (one after the other / together, us: 1000 x 2739 x 2184 85 / 78, 512 x 1024 x 1024 25.4 / 21.6, 2048 x 1024 x 512 31.8 / 24.4, 300 x 4864 x 896 40 / 35,
+// 29 x 188 x 152 10.9 / 7.8, 4096 x 14336 x 4096 1569 / 1540; 1 x 5236 x 1232 25.7 / 27.5).
+constexpr float kPairOutPerMb = 0.15f, kPairGap = 4.f, kPairWorth = 0.95f;
+
+// b1 blocks of r1 us, then b2 of r2, on 256 compute units, each of which takes the next as soon as it has none.
+float time_of_blocks(int64_t b1, float r1, int64_t b2, float r2) {
+  const int64_t late = b1 % 256, early = 256 - late;  // units of the first product's last round, and those that are free in it
+  const float start = (float)(b1 / 256) * r1;
+  if (late == 0) return start + (float)((b2 + 255) / 256) * r2;
+  const int64_t turns = (int64_t)(r1 / r2);  // of the early ones, meanwhile
+  if (b2 <= early * turns) return start + r1;
+  const int64_t rest = b2 - early * turns, rounds = rest / 256, left = rest % 256;
+  return left == 0 ? start + r1 + (float)rounds * r2 : left <= early ? start + (float)(turns + 1 + rounds) * r2 : start + r1 + (float)(rounds + 1) * r2;
+}
+
+struct PairPlan {
+  bool together, both_first;
+  int tile, splits;
+};
+PairPlan plan_pair(int M, int N, int K2) {
+  if (tuning().dense_pair < 0) return {false, false, 0, 1};
+  const int steps = whole_steps(K2) / 64, second_steps = whole_steps(M) / 64;
+  const int forced = tuning().dense_tile, only = forced > 0 && forced <= kDenseTiles && (kTurnedTiles >> (forced - 1) & 1) ? forced - 1 : -1;
+  const int parts = std::min(tuning().dense_splits, std::min(steps, kDenseMaxSplits));  // 0: planned
+  int64_t tiles[kDenseTiles], second_tiles[kDenseTiles];
+  count_tiles(M, N, tiles, std::make_index_sequence<kDenseTiles>{});
+  count_tiles(K2, N, second_tiles, std::make_index_sequence<kDenseTiles>{});
+  PairPlan best{tuning().dense_pair > 0, false, 0, 1};
+  float least = 1e30f;
+  for (int i = 0; i < kDenseTiles; ++i) {
+    if (only >= 0 ? i != only : !(kTurnedTiles >> i & 1)) continue;
+    const DenseCost &a = kTurnedCost[i], &b = kDenseCost[i];
+    const float bytes = ((float)tiles[i] * steps * a.per_mb + (float)second_tiles[i] * second_steps * b.per_mb) * (a.bm + a.bn) * 128e-6f + kPairOutPerMb * 2e-6f * K2 * N;
+    const float second = b.per_round + (float)second_steps * b.per_step;
+    for (int splits = parts > 0 ? parts : 1; splits <= (parts > 0 ? parts : kDensePlannedSplits); ++splits) {
+      if (!parts && splits > 1 && (steps < splits * kDenseMinSplitSteps || tiles[i] * splits > 512)) break;
+      const float first = a.per_round + (float)((steps + splits - 1) / splits) * a.per_step;
+      const bool turn = second > first;  // the longer blocks first
+      const float walk = turn ? time_of_blocks(second_tiles[i], second, tiles[i] * splits, first) : time_of_blocks(tiles[i] * splits, first, second_tiles[i], second);
+      const float us = a.fixed + sqrtf(walk * walk + bytes * bytes) + (splits > 1 ? kTurnedForm.split_fixed + kTurnedForm.split_per_mb * 4e-6f * M * N * splits : 0.f);
+      if (us < least) least = us, best.both_first = turn, best.tile = i, best.splits = splits;
+    }
+  }
+  if (!best.together)
+    best.together = least < kPairWorth * (plan_turned(M, N, whole_steps(K2), false, kDenseMaxSplits).us + plan_turned(K2, N, whole_steps(M), true, kDenseMaxSplits).us + kPairGap);
+  return best;
+}
+
+}  // namespace
+
+int64_t dense_gemm_turned_pair_workspace_bytes(int M, int N, int K2) {
+  const PairPlan p = plan_pair(M, N, K2);
+  if (p.together) return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
+  return std::max(dense_gemm_turned_workspace_bytes(M, N, K2, false), dense_gemm_turned_workspace_bytes(K2, N, M, true));
+}
+
+int dense_gemm_turned_pair(const char* what, const DenseShape& one, const DenseShape& both, int act, int64_t workspace_bytes, hipStream_t st) {
+  const int M = one.M, N = one.N, K2 = both.M;
+  const PairPlan p = plan_pair(M, N, K2);
+  if (!p.together) {
+    const int rc = dense_gemm_turned(what, one, K2, false, act, workspace_bytes, st);
+    return rc != NPAMD_OK ? rc : dense_gemm_turned(what, both, M, true, act, workspace_bytes, st);
+  }
+  DenseShape a = one, b = both;
+  a.steps = whole_steps(K2) / 64, a.splits = p.splits, a.K = K2;
+  b.steps = whole_steps(M) / 64, b.splits = 1, b.K = M;
+  const int rc = launch_wide_pair(a, b, act, p.tile, p.both_first, st);
+  if (rc != NPAMD_OK || a.splits == 1) return rc;
+  if (act == NPAMD_BF16) launch_splitk_reduce<NPAMD_BF16>(a.partials, a.splits, M, N, nullptr, a.y, a.ldy, st);
+  else launch_splitk_reduce<NPAMD_F16>(a.partials, a.splits, M, N, nullptr, a.y, a.ldy, st);
+  return check_launch(what);
+}
+
 }  // namespace npamd
 
 // Rows of x and w that end inside a 64-k step, K a multiple of 8: neither is copied to whole steps first.

@@ -5,8 +5,8 @@
 // keeps of them, half of what f32 would take.
 // Backward, from those sums g and u and the gradient dh: dg = dh u act'(g), du = dh act(g) in f32, rounded to x's type as the matrix pipes' operands (one rounding of 2^-9 or
 // 2^-12 of each of the terms that dx and dW add up, as in a training step whose pointwise part stands by itself; two parts of each would double the products, which are nearly
-// all of the time); then dx = [dg du] W and dW = [dg du]^T x on the wide tiles whose operands lie with the contracted index as their rows (nothing is transposed in memory), and the bias's gradient as sums of the
-// f32 values over strips of rows, added in their order.
+// all of the time); then dx = [dg du] W and dW = [dg du]^T x on the wide tiles whose operands lie with the contracted index as their rows (nothing is transposed in memory), both
+// in one launch where that is estimated to take less time (dense_gemm.hip), and the bias's gradient as sums of the f32 values over strips of rows, added in their order.
 #include <algorithm>
 #include <type_traits>
 
@@ -226,7 +226,7 @@ struct BackSpace {
     dpre = (int64_t)M * ldd * 2;
     dpre = (dpre + 15) / 16 * 16;
     partials = db ? ((int64_t)strips_of(M, N, true) * 2 * N * 4 + 15) / 16 * 16 : 0;
-    parts = std::max(dx ? dense_gemm_turned_workspace_bytes(M, K, 2 * N, false) : 0, dw ? dense_gemm_turned_workspace_bytes(2 * N, K, M, true) : 0);
+    parts = dx && dw ? dense_gemm_turned_pair_workspace_bytes(M, K, 2 * N) : std::max(dx ? dense_gemm_turned_workspace_bytes(M, K, 2 * N, false) : 0, dw ? dense_gemm_turned_workspace_bytes(2 * N, K, M, true) : 0);
   }
 };
 
@@ -316,16 +316,15 @@ extern "C" int npamd_gated_linear_backward(const void* dh, int64_t lddh, const v
     else if (act_dtype == NPAMD_BF16) launch(gated_bias_kernel<NPAMD_BF16>, blocks, 1024, 0, st, partials, a.strips, 2 * N, dbias);
     else launch(gated_bias_kernel<NPAMD_F16>, blocks, 1024, 0, st, partials, a.strips, 2 * N, dbias);
   }
-  int rc = check_launch(what);
-  DenseShape s{};
-  s.partials = (float*)(at + space.dpre + space.partials);
-  if (rc == NPAMD_OK && dx) {
-    s.x = at, s.ldx = space.ldd, s.w = gate_up, s.ldw = ldw, s.y = dx, s.ldy = lddx, s.M = M, s.N = K;
-    rc = dense_gemm_turned(what, s, 2 * N, false, act_dtype, space.parts, st);
-  }
-  if (rc == NPAMD_OK && dgate_up) {
-    s.x = at, s.ldx = space.ldd, s.w = x, s.ldw = ldx, s.y = dgate_up, s.ldy = lddw, s.M = 2 * N, s.N = K;
-    rc = dense_gemm_turned(what, s, M, true, act_dtype, space.parts, st);
-  }
+  const int rc = check_launch(what);
+  DenseShape one{}, both{};
+  one.partials = both.partials = (float*)(at + space.dpre + space.partials);
+  one.x = both.x = at, one.ldx = both.ldx = space.ldd;
+  one.w = gate_up, one.ldw = ldw, one.y = dx, one.ldy = lddx, one.M = M, one.N = K;
+  both.w = x, both.ldw = ldx, both.y = dgate_up, both.ldy = lddw, both.M = 2 * N, both.N = K;
+  if (rc != NPAMD_OK) return rc;
+  if (dx && dgate_up) return dense_gemm_turned_pair(what, one, both, act_dtype, space.parts, st);
+  if (dx) return dense_gemm_turned(what, one, 2 * N, false, act_dtype, space.parts, st);
+  if (dgate_up) return dense_gemm_turned(what, both, M, true, act_dtype, space.parts, st);
   return rc;
 }

@@ -89,17 +89,17 @@ __device__ __forceinline__ void store_rows(const uint8_t* ep, int lane, void* y,
   }
 }
 
-template <int ACT, class T, int FORM = kWidePlain, bool XK = false, bool WK = false>
-__global__ void __launch_bounds__(T::kThreads, T::kThreads == 256 ? 2 : 1)
-wide_gemm_kernel(const DenseShape s) {
+// Block `block` of a launch for the product.
+template <int ACT, class T, int FORM, bool XK, bool WK>
+__device__ __forceinline__ void wide_gemm_block(const DenseShape& s, int block) {
   constexpr int MT = T::MT, NT = T::NT, ST = T::ST, L = T::kLoads, kM = T::kMfmas, SPAN = T::SPAN;
   constexpr bool EPILOGUE = FORM == kWideEpilogue, GATED = FORM == kWideGated, TURNED = XK || WK;
   static_assert(!GATED || (NT % 2 == 0 && !TURNED));
   static_assert(!(XK && (MT & (MT - 1) || (T::kBM != 64 && T::kBM != 128 && T::kBM != 256))), "places of a turned row");
   static_assert(!(WK && (NT & (NT - 1) || (T::kBN != 64 && T::kBN != 128 && T::kBN != 256))), "places of a turned row");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  // blockIdx.x % 8 names the die; a die takes an eighth of the units, counted down the columns of a group of row tiles (launch_wide_tile).
-  const int unit = (blockIdx.x & 7) * s.units_per_die + (blockIdx.x >> 3), columns = s.col_tiles * s.splits;
+  // block % 8 names the die; a die takes an eighth of the units, counted down the columns of a group of row tiles (launch_wide_tile).
+  const int unit = (block & 7) * s.units_per_die + (block >> 3), columns = s.col_tiles * s.splits;
   if (unit >= s.row_tiles * columns) return;
   const int group = unit / (s.group * columns), in = unit - group * (s.group * columns), group_rows = min(s.group, s.row_tiles - group * s.group);
   const int column = in / group_rows, rt = group * s.group + in - column * group_rows;
@@ -484,18 +484,31 @@ wide_gemm_kernel(const DenseShape s) {
 }
 
 template <int ACT, class T, int FORM = kWidePlain, bool XK = false, bool WK = false>
-int launch_wide_tile(DenseShape s, hipStream_t st) {
+__global__ void __launch_bounds__(T::kThreads, T::kThreads == 256 ? 2 : 1)
+wide_gemm_kernel(const DenseShape s) {
+  wide_gemm_block<ACT, T, FORM, XK, WK>(s, blockIdx.x);
+}
+
+// Counts the units, a tile or a part of one each; returns how many blocks they take, a whole number for each die.
+template <class T, int FORM>
+int64_t count_units(DenseShape& s) {
   constexpr int kColumns = FORM == kWideGated ? T::kBN / 2 : T::kBN;  // of y
   s.row_tiles = (s.M + T::kBM - 1) / T::kBM;
   s.col_tiles = (s.N + kColumns - 1) / kColumns;
   const int64_t units = (int64_t)s.col_tiles * s.row_tiles * s.splits, blocks = (units + 7) / 8 * 8;
-  if (blocks > 0x7FFFFFFF) return fail(NPAMD_ERR_UNSUPPORTED, "npamd_dense_gemm: too many tiles");
   s.units_per_die = (int)(blocks / 8);
   // Units are counted down the columns of 2048 rows, so that the rows of W that a die's decode wrote (see die_block) are read through its L2 and, past
   // 2048 rows, x does not come into the L2s again for every column tile; where x is the longer side, down four row tiles, as then it is what each die would
   // bring whole.  Decode + product of int4 layers with groups of 4 tiles / of 2048 rows, us: 656 x 1452 x 4608 27.2 / 22.7, 304 x 3690 x 2048 22.9 / 18.1, 1104 x 2714
   // x 1024 19.2 / 15.3; 1440 x 970 x 8832 53.4 / 59.2, 1956 x 1532 x 11008 102.2 / 108.5, 3575 x 703 x 1536 17.3 / 20.3.
   s.group = s.M > 1.2f * s.N * (FORM == kWideGated ? 2 : 1) ? 4 : 2048 / T::kBM;
+  return blocks;
+}
+
+template <int ACT, class T, int FORM = kWidePlain, bool XK = false, bool WK = false>
+int launch_wide_tile(DenseShape s, hipStream_t st) {
+  const int64_t blocks = count_units<T, FORM>(s);
+  if (blocks > 0x7FFFFFFF) return fail(NPAMD_ERR_UNSUPPORTED, "npamd_dense_gemm: too many tiles");
   static LdsLatch latch;
   const auto kernel = wide_gemm_kernel<ACT, T, FORM, XK, WK>;
   const hipError_t e = enable_dynamic_lds(latch, reinterpret_cast<const void*>(kernel), T::kLds);

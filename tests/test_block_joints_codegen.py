@@ -48,6 +48,14 @@ def test_wide_tiles(tmp_path, source, count):
             assert [ln for ln in loop if "ds_read_b64_tr_b16" in ln], name
 
 
+def test_wide_pair(tmp_path):
+    kernels = list(_kernels(tmp_path, "wide_gemm_pair.hip", "wide_gemm_pair_kernel"))
+    assert len(kernels) == 2 * 5
+    for name, code in kernels:
+        assert _m0_is_the_transfers(code) and not _spills(code), name
+        assert not [ln for ln in code if re.search(r"v_accvgpr_(mov|read|write)", ln)], name
+
+
 def test_adapters(tmp_path):
     kernels = list(_kernels(tmp_path, "adapters.hip", "adapter_\\w+_kernel"))
     assert len(kernels) == 1 + 2 * (1 + 3) + 2 * (6 + 4)  # the list; down; up by the ballot and by the list

@@ -320,3 +320,45 @@ def test_gradients_of_other_rows_are_refused(gpu):
     for wrong in ((dh.view(3, 2, 16), pre), (dh, pre), (dh.view(2, 3, 16), pre.view(6, 32)), (dh.view(2, 3, 16), pre.view(3, 2, 32))):
         with pytest.raises(RuntimeError, match="dh and pre"):
             kernels.gated_linear_backward(wrong[0], x, w, wrong[1])
+
+
+@pytest.fixture
+def paired(tuned, monkeypatch):
+    """Both products of the backward pass in one launch (1) or one after the other (-1)."""
+    from neuropress_amd import _lib
+
+    def force(pair, tile, splits):
+        monkeypatch.setenv("NPAMD_DENSE_PAIR", str(pair))
+        tuned(tile, splits)
+
+    yield force
+    monkeypatch.delenv("NPAMD_DENSE_PAIR", raising=False)
+    _lib.load().npamd_diag_reload_tuning()
+
+
+@pytest.mark.parametrize("tile", [2, 3, 4, 6, 12])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_both_products_in_one_launch(gpu, paired, tile, splits, dtype):
+    from neuropress_amd import kernels
+
+    bm, bn = cases.DENSE_TILES[tile]
+    shapes = [(bm + 65, bn // 2 + 1, 200), (70, 36, 8 * bn + 8), (1, 130, 9), (9, bm // 2 + 5, bn + 24), (455, 20, 40), (2 * bm + 15, bn + 4, 320), (1300, 40, 24), (6, 900, 330)]
+    for m, n, k in shapes:
+        x, w, b, dh = _inputs(m, n, k, dtype)
+        pre = torch.cat((dh, dh.flip(0)), -1)
+        paired(1, tile, splits)
+        together = _check_backward(dh, x, w, pre, "silu", what=(m, n, k))
+        paired(-1, tile, splits)
+        for a, e in zip(together[:1], kernels.gated_linear_backward(dh, x, w, pre)):
+            assert torch.equal(a, e), "of the same tile and parts"
+
+
+def test_products_one_after_the_other(gpu, paired):
+    """What is planned for both, or for one of them by itself, agrees with the formulas whichever way they go."""
+    for m, n, k in ((3, 700, 520), (64, 512, 1024), (700, 300, 1160), (2500, 96, 264)):
+        x, w, b, dh = _inputs(m, n, k, torch.float16)
+        pre = torch.cat((dh, dh.flip(0)), -1)
+        for pair in (-1, 0, 1):
+            paired(pair, 0, 0)
+            _check_backward(dh, x, w, pre, "gelu", what=(m, n, k, pair))
