@@ -3,7 +3,7 @@
 // Two products whose weights depend on the token.  Tokens of one adapter meet its weights as the columns of MFMAs (16x16x32), so both kernels work on entries: an adapter and some of its
 // tokens.  Up to 64 tokens every wave finds its entry's tokens by itself from the ids (one comparison of all of them and a count of bits), so a call is two launches; past that a
 // block of one launch more sorts tokens by adapter and lists the entries.
-//   down: t = x A^T, f32.  A block takes 16 or 32 tokens of an entry, up to 64 ranks and a part of K; x and A come into LDS in whole lines, each wave with steps of its own, and the waves'
+//   down: t = x A^T, f32.  A block takes 16, 32 or 64 tokens of an entry, up to 64 ranks and a part of K; x and A come into LDS in whole lines, each wave with steps of its own, and the waves'
 //         sums meet in LDS.
 //   up:   y = base + scale t B^T.  A block brings its entry's t into LDS once, as two parts of B's type, for an MFMA each (t is not rounded to 16 bits: 2^-16 of it is left with bf16; fp16, scaled
 //         by a power of two to the row's largest, 2^-21), and its waves take 64 or 128 columns each.  Column 8 c + b of a wave is row c of MFMA b, so that a lane ends up with eight neighbouring columns
@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kBallotTokens = 64;  // as many as a wave compares at once
 constexpr int kMaxAdapters = 8192, kMaxRank = 256;
-constexpr int kDownTokens = 32;    // of a listed entry's part in the down kernel
+constexpr int kDownTokens = 32, kDownMost = 64;  // of a listed entry's part in the down kernel
 constexpr int kManyWaves = 1024;   // of the up kernel: four for each compute unit
 constexpr int kGridRows = 65535;   // of a launch
 
@@ -76,7 +76,7 @@ __device__ __forceinline__ Tokens listed_entry(const AdapterArgs& a, int e) {
   return {__builtin_amdgcn_readfirstlane(v.adapter), __builtin_amdgcn_readfirstlane(v.first), __builtin_amdgcn_readfirstlane(v.count), 0};
 }
 
-// TG groups of 16 tokens, RG of 16 ranks; blockIdx.x: entry (listed: and its part of 32 tokens), .y: ranks, .z: part of K.  A wave takes every so manieth 64-k step of the part, in two places of its
+// TG groups of 16 tokens, RG of 16 ranks; blockIdx.x: entry (listed: and its part of 32 or 64 tokens), .y: ranks, .z: part of K.  A wave takes every so manieth 64-k step of the part, in two places of its
 // own in LDS: rows of 128 bytes, 16-byte piece p of row r in place p ^ ((r >> 1) & 7).  Tokens' rows come from wherever they are.
 template <int TG, int RG>
 struct DownTile {
@@ -459,7 +459,7 @@ int entry_tokens_of(int M, int N, int rank8) {
 
 struct AdapterSpace {
   bool listed;
-  int rank8, parts, tokens, most, layers;  // entries at most, whole layers of a grid's rows
+  int rank8, parts, tokens, down_tokens, most, layers;  // entries at most, whole layers of a grid's rows
   int64_t t, entries, order, bytes;
   AdapterSpace(int M, int N, int K, int rank, int adapters) {
     listed = M > kBallotTokens;
@@ -468,9 +468,13 @@ struct AdapterSpace {
     most = listed ? (int)std::min<int64_t>(M, ((int64_t)M + tokens - 1) / tokens + adapters + 1) : M;
     layers = (most + kGridRows - 1) / kGridRows;
     most = (most + layers - 1) / layers * layers;
-    // Parts of K of the down kernel: as many as there are compute units for its blocks; few tokens: two steps for each of a block's waves.
-    const int blocks = (M + kDownTokens - 1) / kDownTokens * ((rank8 + 63) / 64);
-    parts = listed ? std::clamp(std::min(256 / blocks, K / 1024), 1, 8) : std::clamp((K + 1023) / 1024, 1, 8);
+    // Parts of K of the down kernel: as many as there are compute units for its blocks, of which an eighth more are counted, as entries end inside; few tokens: two steps for each of a
+    // block's waves.  64 tokens to a block, which A's rows are read for once, where there are blocks enough (us of a call, 32 tokens / 64, 4096 tokens of five prompts through 4096 columns: rank
+    // 64, K = 4096 53.7 / 50.1; rank 32, K = 14336 70.5 / 56.9; five prompts through 14336 columns, rank 64, K = 4096 91.1 / 88.4).
+    const int ranks = (rank8 + 63) / 64, parts_most = std::max(1, K / 1024);
+    down_tokens = tokens >= kDownMost && (int64_t)(M / kDownMost) * ranks * parts_most >= 128 ? kDownMost : kDownTokens;
+    const int blocks = (M + down_tokens - 1) / down_tokens * ranks, counted = blocks + blocks / 8;
+    parts = listed ? std::clamp(std::min(256 / counted, parts_most), 1, 8) : std::clamp((K + 1023) / 1024, 1, 8);
     t = (int64_t)parts * M * rank8 * 4;
     entries = listed ? 16 + (int64_t)most * sizeof(Entry) : 0;
     order = listed ? ((int64_t)M * 4 + 15) / 16 * 16 : 0;
@@ -517,6 +521,13 @@ int launch_up(const AdapterArgs& a, int entries, int layers, hipStream_t st, con
   return a.rank8 <= 32 ? launch_up_tile<ACT, 1, 8, LISTED>(a, entries, layers, st, what) : launch_up_tile<ACT, 2, 8, LISTED>(a, entries, layers, st, what);
 }
 
+template <int ACT, int TG>
+int launch_listed_down(const AdapterArgs& a, unsigned blocks, hipStream_t st, const char* what) {
+  // Up to 64 ranks to a block, so that the tokens' rows are read once.
+  if (a.rank8 <= 16) return launch_down<ACT, TG, 1, true>(a, blocks, st, what);
+  return a.rank8 <= 32 ? launch_down<ACT, TG, 2, true>(a, blocks, st, what) : launch_down<ACT, TG, 4, true>(a, blocks, st, what);
+}
+
 template <int ACT>
 int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipStream_t st, const char* what) {
   a.t = (float*)at;
@@ -529,11 +540,8 @@ int launch_adapters(AdapterArgs a, const AdapterSpace& space, uint8_t* at, hipSt
   int* const order = (int*)(at + space.t + space.entries);
   launch(adapter_list_kernel, 1, 1024, (unsigned)(a.adapters + 1) * 4, st, a, order, entries, count);
   a.order = order, a.entries = entries, a.count = count;
-  const unsigned blocks = (unsigned)(space.most * (space.tokens / kDownTokens));
-  // Up to 64 ranks to a block, so that the tokens' rows are read once.
-  const int rc = a.rank8 <= 16   ? launch_down<ACT, kDownTokens / 16, 1, true>(a, blocks, st, what)
-                 : a.rank8 <= 32 ? launch_down<ACT, kDownTokens / 16, 2, true>(a, blocks, st, what)
-                                 : launch_down<ACT, kDownTokens / 16, 4, true>(a, blocks, st, what);
+  const unsigned blocks = (unsigned)(space.most * (space.tokens / space.down_tokens));
+  const int rc = space.down_tokens == kDownMost ? launch_listed_down<ACT, kDownMost / 16>(a, blocks, st, what) : launch_listed_down<ACT, kDownTokens / 16>(a, blocks, st, what);
   return rc != NPAMD_OK ? rc : launch_up<ACT, true>(a, space.most, space.layers, st, what);
 }
 
