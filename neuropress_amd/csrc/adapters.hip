@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const 
         f32x4 got[4][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x4* const of = reinterpret_cast<const f32x4*>(from + min(z0 + i, a.parts - 1) * part);
+          if (z0 + i >= a.parts) break;
+          const f32x4* const of = reinterpret_cast<const f32x4*>(from + (z0 + i) * part);
           got[i][0] = of[0];
           got[i][1] = of[1];
         }
