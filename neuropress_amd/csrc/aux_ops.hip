@@ -458,12 +458,12 @@ int launch_q_embedding(const int64_t* ids, int64_t n_ids, const uint8_t* w_pack,
 }
 
 // The gather of gather_columns.hpp, one block's share per block.
-template <bool PERM, bool LDS, int ROWS>
+template <bool LDS, int ROWS>
 __global__ void __launch_bounds__(256)
 gather_columns_kernel(const uint16_t* __restrict__ x, int64_t ldx, const int32_t* __restrict__ perm,
                       uint16_t* __restrict__ out, int64_t ldo, int M, int K, bool vec, bool perm_vec) {
   extern __shared__ __attribute__((aligned(16))) uint16_t row_lds[];
-  gather_columns_block<PERM, LDS, ROWS>(x, ldx, perm, out, ldo, M, K, vec, perm_vec, blockIdx.x, gridDim.x, blockIdx.y, row_lds);
+  gather_columns_block<true, LDS, ROWS>(x, ldx, perm, out, ldo, M, K, vec, perm_vec, blockIdx.x, gridDim.x, blockIdx.y, row_lds);
 }
 
 // Rows padded with zeros, as they lie otherwise: a piece of eight columns to a thread, rows one behind the other, read in one load at whatever address.  19308 x 2614 31 us;
@@ -514,9 +514,9 @@ extern "C" int npamd_gather_columns(const void* x, int64_t ldx, const int32_t* p
     const uint16_t* xm = xs + (int64_t)m0 * ldx;
     uint16_t* om = os + (int64_t)m0 * ldo;
     const auto go = [&](auto kernel) { launch(kernel, grid, 256, plan.lds_bytes, st, xm, ldx, perm, om, ldo, rows, K, vec, pv); };
-    if (plan.pair) go(gather_columns_kernel<true, true, 2>);
-    else if (plan.lds) go(gather_columns_kernel<true, true, 1>);
-    else go(gather_columns_kernel<true, false, 1>);
+    if (plan.pair) go(gather_columns_kernel<true, 2>);
+    else if (plan.lds) go(gather_columns_kernel<true, 1>);
+    else go(gather_columns_kernel<false, 1>);
   }
   return check_launch("npamd_gather_columns");
 }

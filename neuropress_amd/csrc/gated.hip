@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(64) gated_pointwise_narrow_kernel(const GatedP
   a.partials[(int64_t)blockIdx.y * 2 * a.N + a.N + n] = sum_u;
 }
 
-// The strips' sums in their order: 64 columns to a block, its 16 waves each a sixteenth of the strips.
+// The strips' sums in their order: 64 columns to a block, its 16 waves each a sixteenth of the strips.  5478 columns of 250 strips 4.7 us, latency.
 template <int DT>
 __global__ void __launch_bounds__(1024) gated_bias_kernel(const float* __restrict__ partials, int strips, int columns, void* __restrict__ out) {
   __shared__ float sums[16][64];

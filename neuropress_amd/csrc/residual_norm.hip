@@ -27,7 +27,7 @@ struct ResidualNorm {
 __device__ __forceinline__ float rsqrt_mean(float sum, int H, float eps) { return 1.0f / __builtin_sqrtf(sum / (float)H + eps); }
 
 // RW waves to a row, NV pieces to a lane: x and y are read once, r stays in registers between its sum and its norm.  x and y are read by all of a row's waves before the first of
-// them stores, so that r and z may take their places.
+// them stores, so that r and z may take their places.  Bound by HBM: 4096 x 4096 bf16 with both norms 23.4 us, 5.7 TB/s of 134 MB (a copy: 4.9), one row 2.0.
 template <int DT, int NV, int RW>
 __global__ void __launch_bounds__(RW < 4 ? 256 : 64 * RW) residual_norm_row_kernel(const ResidualNorm a, int64_t first) {
   using P = Pieces<DT>;
@@ -206,7 +206,8 @@ enum Gate { kNoGate, kSharedGate, kOwnGate };  // own: of a row
 // One pass over the four rows: RW waves to a row, `teams` rows to a block at a time, a lane has NV pieces of every row that its team meets and adds up its columns' part of the
 // weights' and the gate's gradients in registers.  sum(u wp yh) is taken apart so that it needs no dr: with c = scale gate wp yh it is sum(c (ds + rstd v)) - rstd sum(v rh) / H
 // sum(c rh), so a row's sums meet in LDS once.  Blocks take parts of a group's rows, so that a shared gate's sums have one place; a team's next row is on its way while
-// this one's sums meet (one piece to a lane; two leave no registers for it).
+// this one's sums meet (one piece to a lane; two leave no registers for it).  Bound by HBM: 8192 x 4096 bf16 with both norms and a gate 82 us, 4.9 TB/s of 403 MB; 513 x 3003 fp16 12.4, the latency
+// of one row's chain.
 template <int DT, int NV, bool POST, int GATE>
 __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kernel(const ResidualNormBack a, const ColumnSums sum_w, const ColumnSums sum_p, const ColumnSums sum_g, int RW, int teams) {
   using P = Pieces<DT>;
@@ -489,7 +490,7 @@ residual_norm_back_columns_kernel(const ResidualNormBack a, const float* __restr
 }
 
 // The parts' sums, in the order of the parts: 64 columns of one vector (blockIdx.y: the first weight's, the other's, the gates') to a block, its 16 waves each a sixteenth of the parts.
-// A part has `width` columns, whole pieces: the last one's lie at its end.
+// A part has `width` columns, whole pieces: the last one's lie at its end.  Three vectors of 4096 in 256 parts 5.3 us, latency.
 struct SumParts {
   ColumnSums w, p, g;
   int parts, gate_parts, H, width, last;

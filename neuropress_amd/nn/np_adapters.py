@@ -18,7 +18,7 @@ class NPAdapterLinear(nn.Module):
     """``base(x)`` plus each token's adapter (:func:`neuropress_amd.kernels.adapter_linear`).
 
     *ids*: which adapter each token or each sequence of x has, -1 for none; given with the call, or left on the module by :func:`set_adapter_ids`.  Without either the module is
-    ``base``.  The adapters are no parameters: ``state_dict`` and moves leave them where they are.
+    ``base``.  The adapters are no parameters: ``state_dict`` and moves leave them where they are; the projection's own entries lie under ``base.``.
     """
 
     def __init__(self, base: nn.Module, adapters: LowRankAdapters) -> None:
