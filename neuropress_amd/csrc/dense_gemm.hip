@@ -668,10 +668,8 @@ float time_of_blocks(int64_t b1, float r1, int64_t b2, float r2) {
   return left == 0 ? start + r1 + (float)rounds * r2 : left <= early ? start + (float)(turns + 1 + rounds) * r2 : start + r1 + (float)(rounds + 1) * r2;
 }
 
-struct PairPlan {
-  bool together, both_first;
-  int tile, splits;
-};
+}  // namespace
+
 PairPlan plan_pair(int M, int N, int K2) {
   if (tuning().dense_pair < 0) return {false, false, 0, 1};
   const int steps = whole_steps(K2) / 64, second_steps = whole_steps(M) / 64;
@@ -701,28 +699,16 @@ PairPlan plan_pair(int M, int N, int K2) {
   return best;
 }
 
-}  // namespace
+int64_t dense_gemm_pair_workspace_bytes(const PairPlan& p, int M, int N) { return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0; }
 
-int64_t dense_gemm_turned_pair_workspace_bytes(int M, int N, int K2) {
-  const PairPlan p = plan_pair(M, N, K2);
-  if (p.together) return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
-  return std::max(dense_gemm_turned_workspace_bytes(M, N, K2, false), dense_gemm_turned_workspace_bytes(K2, N, M, true));
-}
-
-int dense_gemm_turned_pair(const char* what, const DenseShape& one, const DenseShape& both, int act, int64_t workspace_bytes, hipStream_t st) {
-  const int M = one.M, N = one.N, K2 = both.M;
-  const PairPlan p = plan_pair(M, N, K2);
-  if (!p.together) {
-    const int rc = dense_gemm_turned(what, one, K2, false, act, workspace_bytes, st);
-    return rc != NPAMD_OK ? rc : dense_gemm_turned(what, both, M, true, act, workspace_bytes, st);
-  }
+int dense_gemm_pair(const char* what, const PairPlan& p, const DenseShape& one, const DenseShape& both, const StripSums& sums, int act, hipStream_t st) {
   DenseShape a = one, b = both;
-  a.steps = whole_steps(K2) / 64, a.splits = p.splits, a.K = K2;
-  b.steps = whole_steps(M) / 64, b.splits = 1, b.K = M;
-  const int rc = launch_wide_pair(a, b, act, p.tile, p.both_first, st);
+  a.steps = whole_steps(b.M) / 64, a.splits = p.splits, a.K = b.M;
+  b.steps = whole_steps(a.M) / 64, b.splits = 1, b.K = a.M;
+  const int rc = launch_wide_pair(a, b, sums, act, p.tile, p.both_first, st);
   if (rc != NPAMD_OK || a.splits == 1) return rc;
-  if (act == NPAMD_BF16) launch_splitk_reduce<NPAMD_BF16>(a.partials, a.splits, M, N, nullptr, a.y, a.ldy, st);
-  else launch_splitk_reduce<NPAMD_F16>(a.partials, a.splits, M, N, nullptr, a.y, a.ldy, st);
+  if (act == NPAMD_BF16) launch_splitk_reduce<NPAMD_BF16>(a.partials, a.splits, a.M, a.N, nullptr, a.y, a.ldy, st);
+  else launch_splitk_reduce<NPAMD_F16>(a.partials, a.splits, a.M, a.N, nullptr, a.y, a.ldy, st);
   return check_launch(what);
 }
 

@@ -48,11 +48,25 @@ int64_t dense_gemm_gated_workspace_bytes(int M, int N, int K);
 int dense_gemm_turned(const char* what, const DenseShape& s, int K, bool x_too, int act, int64_t workspace_bytes, hipStream_t st);
 int64_t dense_gemm_turned_workspace_bytes(int M, int N, int K, bool x_too);
 
-// The two products behind a gradient dp [M][K2]: dx [M][N] = dp w, w [K2][N], and dw [K2][N] = dp^T x, x [M][N] (`one` and `both` as for dense_gemm_turned), in one launch or two.
-int dense_gemm_turned_pair(const char* what, const DenseShape& one, const DenseShape& both, int act, int64_t workspace_bytes, hipStream_t st);
-int64_t dense_gemm_turned_pair_workspace_bytes(int M, int N, int K2);
+// Sums over strips of rows, [strips][columns] in f32, that are still to be added up, in their order: out in f32 or the activations' type.  columns 0: none.
+struct StripSums {
+  const float* partials;
+  int strips, columns;
+  void* out;
+  int out_f32;
+};
 
-int launch_wide_pair(const DenseShape& one, const DenseShape& both, int act, int tile, bool both_first, hipStream_t st);
+// The two products behind a gradient dp [M][K2] in one launch: dx [M][N] = dp w, w [K2][N], and dw [K2][N] = dp^T x, x [M][N] (`one` and `both` as for dense_gemm_turned), and the sums.
+// The plan says whether that takes less time than one after the other.
+struct PairPlan {
+  bool together, both_first;
+  int tile, splits;
+};
+PairPlan plan_pair(int M, int N, int K2);
+int64_t dense_gemm_pair_workspace_bytes(const PairPlan& p, int M, int N);
+int dense_gemm_pair(const char* what, const PairPlan& p, const DenseShape& one, const DenseShape& both, const StripSums& sums, int act, hipStream_t st);
+
+int launch_wide_pair(const DenseShape& one, const DenseShape& both, const StripSums& sums, int act, int tile, bool both_first, hipStream_t st);
 int launch_wide_gated(const DenseShape& s, int act, int tile, hipStream_t st);
 int launch_wide_turned(const DenseShape& s, int act, int tile, bool x_too, hipStream_t st);
 

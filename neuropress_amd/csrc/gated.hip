@@ -15,6 +15,7 @@
 #include "dense_gemm.hpp"
 #include "dense_rows.hpp"
 #include "row_pieces.hpp"
+#include "strip_sums.hpp"
 #include "wave_ops.hpp"
 
 using namespace npamd;
@@ -193,23 +194,11 @@ __global__ void __launch_bounds__(64) gated_pointwise_narrow_kernel(const GatedP
   a.partials[(int64_t)blockIdx.y * 2 * a.N + a.N + n] = sum_u;
 }
 
-// The strips' sums in their order: 64 columns to a block, its 16 waves each a sixteenth of the strips.  5478 columns of 250 strips 4.7 us, latency.
-template <int DT>
-__global__ void __launch_bounds__(1024) gated_bias_kernel(const float* __restrict__ partials, int strips, int columns, void* __restrict__ out) {
-  __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-  const int first = strips * wave / 16, last = strips * (wave + 1) / 16;
-  float v = 0.f;
-  if (col < columns) {
-#pragma unroll 8
-    for (int i = first; i < last; ++i) v += partials[(int64_t)i * columns + col];
-  }
-  sums[wave][lane] = v;
-  __syncthreads();
-  if (wave || col >= columns) return;
-#pragma unroll
-  for (int i = 1; i < 16; ++i) v += sums[i][lane];
-  store_from_f32<DT>(out, col, v);
+// The strips' sums.  5478 columns of 250 strips 4.7 us, latency.
+template <int ACT>
+__global__ void __launch_bounds__(1024) gated_bias_kernel(const StripSums s) {
+  __shared__ float meet[kStripShares * kStripColumns];
+  add_strips<ACT, 16>(s, blockIdx.x, meet);
 }
 
 // Strips of rows: some 8192 waves where there are as many rows; 256 strips at most where their sums are kept.
@@ -220,13 +209,16 @@ int strips_of(int M, int N, bool sums) {
 
 struct BackSpace {
   int64_t ldd, dpre, partials, parts;  // row distance and bytes
+  PairPlan pair{false, false, 0, 1};
   int64_t bytes() const { return dpre + partials + parts; }
   BackSpace(int M, int N, int K, bool dx, bool dw, bool db) {
     ldd = (2 * (int64_t)N + 7) / 8 * 8;
     dpre = (int64_t)M * ldd * 2;
     dpre = (dpre + 15) / 16 * 16;
     partials = db ? ((int64_t)strips_of(M, N, true) * 2 * N * 4 + 15) / 16 * 16 : 0;
-    parts = dx && dw ? dense_gemm_turned_pair_workspace_bytes(M, K, 2 * N) : std::max(dx ? dense_gemm_turned_workspace_bytes(M, K, 2 * N, false) : 0, dw ? dense_gemm_turned_workspace_bytes(2 * N, K, M, true) : 0);
+    if (dx && dw) pair = plan_pair(M, K, 2 * N);
+    parts = pair.together ? dense_gemm_pair_workspace_bytes(pair, M, K)
+                          : std::max(dx ? dense_gemm_turned_workspace_bytes(M, K, 2 * N, false) : 0, dw ? dense_gemm_turned_workspace_bytes(2 * N, K, M, true) : 0);
   }
 };
 
@@ -310,21 +302,22 @@ extern "C" int npamd_gated_linear_backward(const void* dh, int64_t lddh, const v
   const GatedPointwise a{dh, pre, at, lddh, ldp, space.ldd, partials, M, N, strips_of(M, N, dbias != nullptr)};
   if (act_dtype == NPAMD_BF16) launch_pointwise<NPAMD_BF16>(a, activation, st);
   else launch_pointwise<NPAMD_F16>(a, activation, st);
-  if (dbias) {
-    const unsigned blocks = (unsigned)((2 * (int64_t)N + 63) / 64);
-    if (bias_dtype == NPAMD_F32) launch(gated_bias_kernel<NPAMD_F32>, blocks, 1024, 0, st, partials, a.strips, 2 * N, dbias);
-    else if (act_dtype == NPAMD_BF16) launch(gated_bias_kernel<NPAMD_BF16>, blocks, 1024, 0, st, partials, a.strips, 2 * N, dbias);
-    else launch(gated_bias_kernel<NPAMD_F16>, blocks, 1024, 0, st, partials, a.strips, 2 * N, dbias);
-  }
-  const int rc = check_launch(what);
   DenseShape one{}, both{};
   one.partials = both.partials = (float*)(at + space.dpre + space.partials);
   one.x = both.x = at, one.ldx = both.ldx = space.ldd;
   one.w = gate_up, one.ldw = ldw, one.y = dx, one.ldy = lddx, one.M = M, one.N = K;
   both.w = x, both.ldw = ldx, both.y = dgate_up, both.ldy = lddw, both.M = 2 * N, both.N = K;
-  if (rc != NPAMD_OK) return rc;
-  if (dx && dgate_up) return dense_gemm_turned_pair(what, one, both, act_dtype, space.parts, st);
-  if (dx) return dense_gemm_turned(what, one, 2 * N, false, act_dtype, space.parts, st);
-  if (dgate_up) return dense_gemm_turned(what, both, M, true, act_dtype, space.parts, st);
+  const StripSums sums{partials, a.strips, dbias ? 2 * N : 0, dbias, bias_dtype == NPAMD_F32};
+  if (space.pair.together) {
+    const int rc = check_launch(what);
+    return rc != NPAMD_OK ? rc : dense_gemm_pair(what, space.pair, one, both, sums, act_dtype, st);
+  }
+  if (dbias) {
+    if (act_dtype == NPAMD_BF16) launch(gated_bias_kernel<NPAMD_BF16>, (unsigned)strip_blocks(sums), 1024, 0, st, sums);
+    else launch(gated_bias_kernel<NPAMD_F16>, (unsigned)strip_blocks(sums), 1024, 0, st, sums);
+  }
+  int rc = check_launch(what);
+  if (rc == NPAMD_OK && dx) rc = dense_gemm_turned(what, one, 2 * N, false, act_dtype, space.parts, st);
+  if (rc == NPAMD_OK && dgate_up) rc = dense_gemm_turned(what, both, M, true, act_dtype, space.parts, st);
   return rc;
 }

@@ -70,7 +70,7 @@ def test_adapters(tmp_path):
 
 def test_gated(tmp_path):
     kernels = list(_kernels(tmp_path, "gated.hip", "gated_\\w+_kernel|dense_few_kernel|dense_some_kernel"))
-    assert len(kernels) == 2 * (5 + 6 + 5 + 5) + 3  # some, few, pointwise and narrow of each activation; the bias's sums
+    assert len(kernels) == 2 * (5 + 6 + 5 + 5 + 1)  # some, few, pointwise and narrow of each activation; the bias's sums
     for name, code in kernels:
         assert not _spills(code), name
         if "dense_some" in name:
