@@ -368,8 +368,17 @@ PyObject* adapter_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Rows x, base{nullptr, 0, 0, 0, 0};
     if (!rows_argument(args[0], device, &x) || !PyLong_Check(args[6]) || !PyLong_Check(args[7]) || x.width != PyLong_AsLong(args[6])) Py_RETURN_NONE;
     const at::Tensor *ids = readable(args[1], device), *a = readable(args[2], device), *b = readable(args[3], device);
-    if (!ids || !a || !b || !ids->is_contiguous() || ids->sizes() != x.t->sizes().slice(0, x.t->dim() - 1) || (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong))
-      Py_RETURN_NONE;
+    if (!ids || !a || !b || !ids->is_contiguous() || (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong)) Py_RETURN_NONE;
+    const at::IntArrayRef lead = x.t->sizes().slice(0, x.t->dim() - 1);
+    if (ids->dim() > (int64_t)lead.size() || ids->sizes() != lead.slice(0, ids->dim())) Py_RETURN_NONE;
+    at::Tensor spread;  // one for each token, where there is one for each sequence of several
+    if (ids->numel() != x.m) {
+      c10::SmallVector<int64_t, 6> ones(ids->sizes().begin(), ids->sizes().end());
+      ones.resize(lead.size(), 1);
+      const c10::DeviceGuard guard(x.t->device());
+      spread = ids->view(ones).expand(lead).contiguous();
+      ids = &spread;
+    }
     const void* scale;
     if (a->scalar_type() != x.t->scalar_type() || !vector_of(args[4], device, at::kFloat, a->size(0), &scale)) Py_RETURN_NONE;
     c10::SmallVector<int64_t, 6> sizes(x.t->sizes().begin(), x.t->sizes().end());
