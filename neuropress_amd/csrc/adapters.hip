@@ -201,16 +201,15 @@ __device__ __forceinline__ void two_parts(const float (&v)[8], u32x4& hi, u32x4&
 
 // RC chunks of 32 ranks, CT columns to a lane; blockIdx.x: 16 CT columns to each of the block's waves, .y and .z: entry.  LDS: t's two parts, rows of 64 RC + 16 bytes, then what each token's sums are
 // multiplied with, and the tokens.
-template <int RC, int CT>
+template <int RC>
 struct UpTile {
   static constexpr int kRow = 64 * RC + 16;
-  static constexpr int kTokens = RC <= 2 ? 128 : 256 / RC;  // of an entry, at most
   static constexpr int lds(int tokens) { return tokens * (2 * kRow + 8); }
 };
 
 template <int ACT, int RC, int CT, bool LISTED>
 __global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const AdapterArgs a) {
-  using T = UpTile<RC, CT>;
+  using T = UpTile<RC>;
   constexpr int kPieces = 4 * RC;  // of a row of t, eight values each
   typedef uint32_t Columns __attribute__((ext_vector_type(CT / 2)));
   typedef uint32_t ColumnsAny __attribute__((ext_vector_type(CT / 2), aligned(2)));
@@ -449,9 +448,13 @@ __global__ void __launch_bounds__(1024) adapter_list_kernel(const AdapterArgs a,
   });
 }
 
+// Whether a lane of the up kernel has eight columns of listed tokens, not four: past rank 64, where they leave the registers of a wave two blocks to a compute unit, with blocks enough (us of a call of
+// rank 128, four / eight: 4096 tokens through 14336 columns 135 / 112, 2000 through 14336 68 / 62, 1024 47.5 / 44.5; 4096 through 4096 65 / 67, 300 through 4096 22.6 / 25.0).
+bool eight_columns(int M, int N, int rank8) { return rank8 <= 64 || (rank8 <= 128 && ((int64_t)N + 511) / 512 * ((M + kDownTokens - 1) / kDownTokens) >= 512); }
+
 // Tokens of a listed entry: as many as leave two rounds of the up kernel's blocks, B being read once for each.
 int entry_tokens_of(int M, int N, int rank8) {
-  const int most = rank8 <= 64 ? 128 : rank8 <= 128 ? 64 : 32;
+  const int most = eight_columns(M, N, rank8) ? 128 : rank8 <= 128 ? 64 : 32;
   const int64_t columns = ((int64_t)N + 511) / 512;
   int tokens = most;
   while (tokens > kDownTokens && columns * ((M + tokens - 1) / tokens) < 512) tokens /= 2;
@@ -497,7 +500,7 @@ int launch_down(const AdapterArgs& a, unsigned blocks, hipStream_t st, const cha
 
 template <int ACT, int RC, int CT, bool LISTED>
 int launch_up_tile(const AdapterArgs& a, int entries, int layers, hipStream_t st, const char* what) {
-  using T = UpTile<RC, CT>;
+  using T = UpTile<RC>;
   // Four waves to a block, which bring t in together; one where that is next to nothing and blocks are few.
   const int64_t strips = ((int64_t)a.N + 16 * CT - 1) / (16 * CT);
   const int waves = LISTED || strips * entries >= kManyWaves ? 4 : 1, lds = T::lds(a.entry_tokens);
@@ -514,6 +517,9 @@ int launch_up_tile(const AdapterArgs& a, int entries, int layers, hipStream_t st
 template <int ACT, bool LISTED>
 int launch_up(const AdapterArgs& a, int entries, int layers, hipStream_t st, const char* what) {
   if (a.rank8 > 128) return launch_up_tile<ACT, 8, 4, LISTED>(a, entries, layers, st, what);
+  if constexpr (LISTED) {
+    if (a.rank8 > 64 && eight_columns(a.M, a.N, a.rank8)) return launch_up_tile<ACT, 4, 8, true>(a, entries, layers, st, what);
+  }
   if (a.rank8 > 64) return launch_up_tile<ACT, 4, 4, LISTED>(a, entries, layers, st, what);
   if constexpr (!LISTED) {
     if (((int64_t)a.N + 127) / 128 * entries < kManyWaves)

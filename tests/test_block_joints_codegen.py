@@ -58,7 +58,7 @@ def test_wide_pair(tmp_path):
 
 def test_adapters(tmp_path):
     kernels = list(_kernels(tmp_path, "adapters.hip", "adapter_\\w+_kernel"))
-    assert len(kernels) == 1 + 2 * (1 + 2 * 3) + 2 * (6 + 4)  # the list; down; up by the ballot and by the list
+    assert len(kernels) == 1 + 2 * (1 + 2 * 3) + 2 * (6 + 5)  # the list; down; up by the ballot and by the list
     for name, code in kernels:
         assert not _spills(code), name
         if "adapter_down_kernel" in name:

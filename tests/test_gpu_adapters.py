@@ -284,3 +284,13 @@ def test_module_beside_quantized_layers(gpu, tokens):
         y, per_sequence = base(twice), layer(twice, torch.tensor([1, -1], device=gpu))  # of so many tokens: the projection's kernels may be others
     _check(x, a, b, scale, y[0], torch.ones_like(ids), per_sequence[0], "sequences")
     assert torch.equal(per_sequence[1], y[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,rank", [(1030, 8192 + 8, 128), (1030, 8192 + 3, 66), (4100, 4096, 100), (300, 4096, 128), (4100, 2048, 200)])
+def test_wide_ranks_of_long_prompts(gpu, dtype, m, n, rank):
+    """Both widths of a lane's columns past rank 64, entries of 32 to 128 tokens."""
+    x, a, b, scale, base = _make(m, n, 72, rank, 5, dtype)
+    for how in ("runs", "any"):
+        ids = _ids(m, 5, how)
+        _check(x, a, b, scale, base, ids, _run(x, a, b, scale, ids, base), how)
