@@ -11,6 +11,7 @@
 //         has them, a load touches 64 places: 64 to 86 us in the place of 52 for 4096 tokens through 14336 columns of bf16, rank 64.)
 // Bound by the latency of two dependent launches for a decode step, by the bytes of base and y for prompts.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "gemm_tile.hpp"
@@ -364,8 +365,8 @@ __global__ void __launch_bounds__(256, RC == 1 ? 4 : 2) adapter_up_kernel(const 
 }
 
 // Tokens by adapter, those without one last, and the entries.  One block: counts in LDS, their running sums, then every token to its place.  Where all of a wave's tokens have one
-// adapter, as a prompt's have, they are counted and placed side by side with one atomic addition; else each by itself.  A token's results do not depend on its place.  5.9 us for 4096 tokens of
-// five prompts, 7.0 for 4096 of 1024 adapters in any order (with a wave's adapters one after the other 8.4 and 91).
+// adapter, as a prompt's have, they are counted and placed side by side with one atomic addition; else each by itself.  A token's results do not depend on its place.  5.6 us for 4096 tokens of
+// five prompts, 6.4 for 4096 of 1024 adapters in any order (with a wave's adapters one after the other 8.4 and 91).
 __global__ void __launch_bounds__(1024) adapter_list_kernel(const AdapterArgs a, int* __restrict__ order, Entry* __restrict__ entries, int* __restrict__ count) {
   extern __shared__ int places[];  // [adapters + 1]
   __shared__ int sums[2][16];
@@ -373,22 +374,31 @@ __global__ void __launch_bounds__(1024) adapter_list_kernel(const AdapterArgs a,
   // f(the lane's token, its bucket, whether there is one) for all tokens.  The first turns' ids are read once, all at a time.
   constexpr int kKept = 8;
   int kept[kKept];
-  auto bucket_of = [&](int64_t m) __attribute__((always_inline)) {
-    const int id = m < a.M ? adapter_of(a, (int)m) : -1;
-    return id < 0 ? a.adapters : id;
+  auto bucket_of = [&](int64_t id) __attribute__((always_inline)) { return id >= 0 && id < a.adapters ? (int)id : a.adapters; };
+  auto bucket_at = [&](int64_t m) __attribute__((always_inline)) {  // past the end: the last one's
+    m = min(m, (int64_t)a.M - 1);
+    return bucket_of(a.ids_64 ? ((const int64_t*)a.ids)[m] : ((const int*)a.ids)[m]);
   };
+  // All of them on their way at a time: without a branch between them.
+  auto keep = [&](const auto* ids) __attribute__((always_inline)) {
+    std::remove_cv_t<std::remove_reference_t<decltype(*ids)>> raw[kKept];
 #pragma unroll
-  for (int i = 0; i < kKept; ++i) kept[i] = bucket_of(i * 1024 + threadIdx.x);
+    for (int i = 0; i < kKept; ++i) raw[i] = ids[min(i * 1024 + (int)threadIdx.x, a.M - 1)];
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) kept[i] = bucket_of(raw[i]);
+  };
+  if (a.ids_64) keep((const int64_t*)a.ids);
+  else keep((const int*)a.ids);
   for (int i = threadIdx.x; i < buckets; i += 1024) places[i] = 0;
   __syncthreads();
   auto each = [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kKept; ++i)
       if (i * 1024 < a.M) f(i * 1024 + (int)threadIdx.x, kept[i]);
-    int next = bucket_of(kKept * 1024 + threadIdx.x);
+    int next = bucket_at(kKept * 1024 + threadIdx.x);
     for (int64_t at = kKept * 1024; at < a.M; at += 1024) {
       const int bucket = next;
-      next = bucket_of(at + 1024 + threadIdx.x);
+      next = bucket_at(at + 1024 + threadIdx.x);
       f((int)at + (int)threadIdx.x, bucket);
     }
   };
