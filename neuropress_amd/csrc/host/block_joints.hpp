@@ -238,11 +238,13 @@ at::Tensor last_dimension(const at::Tensor& t, int64_t n) {
 // h and, with keep, pre; of tensors that have been checked.
 std::array<at::Tensor, 2> gated_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, int activation, bool keep) {
   const int k = (int)x.size(-1), m = (int)(x.numel() / k), n = (int)(w.size(0) / 2), code = dtype_code(x.scalar_type()), device = x.get_device();
-  const bool tiles = m > NPAMD_GEMV_MAX_M;
+  // Odd K or row distances: few tokens read W as it lies, once for every four of them; past that a copy in whole pieces takes less (us as it lies / with the copy: 8 tokens 14336 x 4095 118 / 140,
+  // 8192 x 2047 34 / 38; 9 tokens 148 / 141, 46 / 38, 2739 x 2183 23 / 20, but 515 x 2311 8.9 / 13.0; 20 tokens 255 / 143, 75 / 39, 35 / 21, 13.3 / 13.8).
+  const bool pieces = m > ((int64_t)n * k >= 1 << 21 ? 8 : 20);
   int64_t ldx, ldw;
-  const at::Tensor xr = tiles ? whole_pieces(x, &ldx) : as_rows(x, &ldx), wr = tiles ? whole_pieces(w, &ldw) : as_rows(w, &ldw);
+  const at::Tensor xr = pieces ? whole_pieces(x, &ldx) : as_rows(x, &ldx), wr = pieces ? whole_pieces(w, &ldw) : as_rows(w, &ldw);
   const at::Tensor b = bias.defined() ? bias.contiguous() : at::Tensor();
-  const int columns = tiles ? (k + 7) / 8 * 8 : k;
+  const int columns = pieces ? (k + 7) / 8 * 8 : k;
   std::array<at::Tensor, 2> out{last_dimension(x, n), keep ? last_dimension(x, 2 * (int64_t)n) : at::Tensor()};
   const int64_t bytes = npamd_gated_linear_workspace_bytes(m, n, columns);
   at::Tensor scratch;
