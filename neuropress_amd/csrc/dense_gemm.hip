@@ -533,65 +533,82 @@ int npamd::dense_gemm_epilogue(const char* what, const DenseShape& shape, int K,
 namespace npamd {
 namespace {
 
-// The sums of the parts of the gated product and what becomes of them: four columns of y to a thread, the parts' loads of the gate's and the up projection's columns in batches.
-template <int ACT>
-__global__ void __launch_bounds__(64) splitk_reduce_gated_kernel(const DenseShape s) {
-  const int n = ((int)blockIdx.x * 64 + (int)threadIdx.x) * 4, last = min(3, s.N - 1 - n);  // columns past N: the last one again, not stored
+// Sums of parts whose rows are whole 16 bytes, of the gated product with what becomes of them: four columns of y to a thread, the parts' loads (of the gate's and the up projection's
+// columns) in batches, four values to a store at whatever address.  1000 x 2183 in two parts 6 us, a value at a time 19.
+template <int ACT, bool GATED>
+__global__ void __launch_bounds__(64) splitk_reduce_rows_kernel(const DenseShape s) {
+  constexpr int U = GATED ? 2 : 1;
+  typedef uint32_t Four __attribute__((ext_vector_type(2), aligned(2)));
+  const int n = ((int)blockIdx.x * 64 + (int)threadIdx.x) * 4, last = min(3, s.N - 1 - n), columns4 = parts_row(s.N);
   if (n >= s.N) return;
-  const bool vec = s.N % 4 == 0 && (reinterpret_cast<uintptr_t>(s.partials) & 15) == 0;
-  float bias[2][4] = {};
-  if (s.ep.bias) {
+  auto leave = [&](void* to, int64_t at, const float (&v)[4]) __attribute__((always_inline)) {
+    if (last == 3) {
+      uint32_t bits[4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int j = 0; j < 4; ++j) bits[j] = ACT == NPAMD_BF16 ? f32_to_bf16_bits(v[j]) : f32_to_f16_bits(v[j]);
+      Four out;
+      out[0] = bits[0] | (bits[1] << 16);
+      out[1] = bits[2] | (bits[3] << 16);
+      *reinterpret_cast<Four*>((uint16_t*)to + at) = out;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j <= last) store_from_f32<ACT>(to, at + j, v[j]);
+    }
+  };
+  float bias[U][4] = {};
+  if (GATED && s.ep.bias) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = u * s.N + n + min(j, last);
         bias[u][j] = s.ep.bias_16 ? load_as_f32<ACT>(s.ep.bias, at) : ((const float*)s.ep.bias)[at];
       }
   }
+  const int64_t part = (int64_t)s.M * U * columns4;
   for (int m = blockIdx.y; m < s.M; m += gridDim.y) {
-    const float* const p = s.partials + (size_t)m * 2 * s.N + n;
-    float sum[2][4] = {};
+    const float* const p = s.partials + (int64_t)m * U * columns4 + n;
+    float sum[U][4] = {};
     for (int z0 = 0; z0 < s.splits; z0 += kReduceBatch) {
-      float v[kReduceBatch][2][4];
+      f32x4 v[kReduceBatch][U];
 #pragma unroll
       for (int i = 0; i < kReduceBatch; ++i)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float* const q = p + (size_t)min(z0 + i, s.splits - 1) * s.M * 2 * s.N + (size_t)u * s.N;
-          if (vec) {
-            const f32x4 t = *reinterpret_cast<const f32x4*>(q);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][u][j] = t[j];
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][u][j] = q[min(j, last)];
-          }
-        }
+        for (int u = 0; u < U; ++u) v[i][u] = *reinterpret_cast<const f32x4*>(p + min(z0 + i, s.splits - 1) * part + u * columns4);
 #pragma unroll
       for (int i = 0; i < kReduceBatch; ++i)
         if (z0 + i < s.splits) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum[u][j] += v[i][u][j];
         }
     }
+    if constexpr (GATED) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sum[u][j] += bias[u][j];
-        if (s.ep.pre && j <= last) store_from_f32<ACT>(s.ep.pre, (int64_t)m * s.ep.ldp + (int64_t)u * s.N + n + j, sum[u][j]);
+        for (int j = 0; j < 4; ++j) sum[u][j] += bias[u][j];
+        if (s.ep.pre) leave(s.ep.pre, (int64_t)m * s.ep.ldp + (int64_t)u * s.N + n, sum[u]);
       }
-    activate_all(s.ep.act, [&](auto f) {
+      activate_all(s.ep.act, [&](auto f) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[0][j] = f(sum[0][j]);
-    });
+        for (int j = 0; j < 4; ++j) sum[0][j] = f(sum[0][j]);
+      });
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j <= last) store_from_f32<ACT>(s.y, (int64_t)m * s.ldy + n + j, sum[0][j] * sum[1][j]);
+      for (int j = 0; j < 4; ++j) sum[0][j] *= sum[U - 1][j];
+    }
+    leave(s.y, (int64_t)m * s.ldy + n, sum[0]);
   }
+}
+
+template <bool GATED>
+int launch_reduce_rows(const char* what, const DenseShape& s, int act, hipStream_t st) {
+  const dim3 grid((unsigned)(((s.N + 3) / 4 + 63) / 64), (unsigned)(s.M < 65535 ? s.M : 65535));
+  if (act == NPAMD_BF16) launch(splitk_reduce_rows_kernel<NPAMD_BF16, GATED>, grid, 64, 0, st, s);
+  else launch(splitk_reduce_rows_kernel<NPAMD_F16, GATED>, grid, 64, 0, st, s);
+  return check_launch(what);
 }
 
 constexpr unsigned kGatedTiles = 1u << 1 | 1u << 2 | 1u << 3 | 1u << 5 | 1u << 6 | 1u << 7 | 1u << 8 | 1u << 9 | 1u << 11;
@@ -611,41 +628,36 @@ int whole_steps(int K) { return (K + 63) / 64 * 64; }
 
 int64_t dense_gemm_gated_workspace_bytes(int M, int N, int K) {
   const DensePlan p = plan_gated(M, N, whole_steps(K), kDenseMaxSplits);
-  return p.splits > 1 ? (int64_t)p.splits * M * 2 * N * 4 : 0;
+  return p.splits > 1 ? (int64_t)p.splits * M * 2 * parts_row(N) * 4 : 0;
 }
 
 int dense_gemm_gated(const char* what, const DenseShape& shape, int K, int act, int64_t workspace_bytes, hipStream_t st) {
   DenseShape s = shape;
   DensePlan p = plan_gated(s.M, s.N, whole_steps(K), kDenseMaxSplits);
-  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * 2 * s.N * 4) < p.splits)) p = plan_gated(s.M, s.N, whole_steps(K), 1);
+  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * 2 * parts_row(s.N) * 4) < p.splits)) p = plan_gated(s.M, s.N, whole_steps(K), 1);
   s.steps = whole_steps(K) / 64;
   s.splits = p.splits;
   s.pieces = K / 8;
   const int rc = launch_wide_gated(s, act, p.tile, st);
   if (rc != NPAMD_OK || s.splits == 1) return rc;
-  const dim3 grid((unsigned)(((s.N + 3) / 4 + 63) / 64), (unsigned)(s.M < 65535 ? s.M : 65535));
-  if (act == NPAMD_BF16) launch(splitk_reduce_gated_kernel<NPAMD_BF16>, grid, 64, 0, st, s);
-  else launch(splitk_reduce_gated_kernel<NPAMD_F16>, grid, 64, 0, st, s);
-  return check_launch(what);
+  return launch_reduce_rows<true>(what, s, act, st);
 }
 
 int64_t dense_gemm_turned_workspace_bytes(int M, int N, int K, bool x_too) {
   const DensePlan p = plan_turned(M, N, whole_steps(K), x_too, kDenseMaxSplits);
-  return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
+  return p.splits > 1 ? (int64_t)p.splits * M * parts_row(N) * 4 : 0;
 }
 
 int dense_gemm_turned(const char* what, const DenseShape& shape, int K, bool x_too, int act, int64_t workspace_bytes, hipStream_t st) {
   DenseShape s = shape;
   DensePlan p = plan_turned(s.M, s.N, whole_steps(K), x_too, kDenseMaxSplits);
-  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * s.N * 4) < p.splits)) p = plan_turned(s.M, s.N, whole_steps(K), x_too, 1);
+  if (p.splits > 1 && (!s.partials || workspace_bytes / ((int64_t)s.M * parts_row(s.N) * 4) < p.splits)) p = plan_turned(s.M, s.N, whole_steps(K), x_too, 1);
   s.steps = whole_steps(K) / 64;
   s.splits = p.splits;
   s.K = K;
   const int rc = launch_wide_turned(s, act, p.tile, x_too, st);
   if (rc != NPAMD_OK || s.splits == 1) return rc;
-  if (act == NPAMD_BF16) launch_splitk_reduce<NPAMD_BF16>(s.partials, s.splits, s.M, s.N, nullptr, s.y, s.ldy, st);
-  else launch_splitk_reduce<NPAMD_F16>(s.partials, s.splits, s.M, s.N, nullptr, s.y, s.ldy, st);
-  return check_launch(what);
+  return launch_reduce_rows<false>(what, s, act, st);
 }
 
 namespace {
@@ -699,7 +711,7 @@ PairPlan plan_pair(int M, int N, int K2) {
   return best;
 }
 
-int64_t dense_gemm_pair_workspace_bytes(const PairPlan& p, int M, int N) { return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0; }
+int64_t dense_gemm_pair_workspace_bytes(const PairPlan& p, int M, int N) { return p.splits > 1 ? (int64_t)p.splits * M * parts_row(N) * 4 : 0; }
 
 int dense_gemm_pair(const char* what, const PairPlan& p, const DenseShape& one, const DenseShape& both, const StripSums& sums, int act, hipStream_t st) {
   DenseShape a = one, b = both;
@@ -707,9 +719,7 @@ int dense_gemm_pair(const char* what, const PairPlan& p, const DenseShape& one, 
   b.steps = whole_steps(a.M) / 64, b.splits = 1, b.K = a.M;
   const int rc = launch_wide_pair(a, b, sums, act, p.tile, p.both_first, st);
   if (rc != NPAMD_OK || a.splits == 1) return rc;
-  if (act == NPAMD_BF16) launch_splitk_reduce<NPAMD_BF16>(a.partials, a.splits, a.M, a.N, nullptr, a.y, a.ldy, st);
-  else launch_splitk_reduce<NPAMD_F16>(a.partials, a.splits, a.M, a.N, nullptr, a.y, a.ldy, st);
-  return check_launch(what);
+  return launch_reduce_rows<false>(what, a, act, st);
 }
 
 }  // namespace npamd

@@ -32,6 +32,9 @@ struct DenseShape {
   int K;             // of the kernels with an operand whose rows are the contracted ones
 };
 
+// Values of a row of the parts of the gated products and those with turned operands: whole 16 bytes.
+__host__ __device__ constexpr int parts_row(int N) { return (N + 3) / 4 * 4; }
+
 // The product on wide tile `tile` of the plan's list; splits > 1: its parts, without their sum.
 int launch_wide(const DenseShape& s, int act, int tile, hipStream_t st);
 int launch_wide_epilogue(const DenseShape& s, int act, int tile, hipStream_t st);

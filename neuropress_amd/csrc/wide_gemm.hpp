@@ -295,17 +295,18 @@ __device__ __forceinline__ void wide_gemm_block(const DenseShape& s, int block) 
   const int wm0 = m0 + wm * 16 * MT, wn0 = n0 + wn * (GATED ? 8 : 16) * NT, rows = s.M - wm0, cols = s.N - wn0;  // of the wave's tile
   // A lane has the columns 16 b + 4 h .. + 3 of row 16 a + c.  Gated: those of the gate and, NT / 2 column groups later, of the up projection.
   if (s.splits > 1) {
-    const int row_values = GATED ? 2 * s.N : s.N;
+    constexpr bool kWholeRows = GATED || TURNED;  // the parts' rows are padded to whole 16 bytes, at 16-byte addresses
+    const int columns4 = parts_row(s.N), row_values = GATED ? 2 * columns4 : TURNED ? columns4 : s.N;
     float* const to = s.partials + ((int64_t)part * s.M + wm0) * row_values + wn0;
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)kBuffer, kRaw);
-    const bool whole = s.N % 4 == 0 && (reinterpret_cast<uintptr_t>(s.partials) & 15) == 0;
+    const bool whole = kWholeRows || (s.N % 4 == 0 && (reinterpret_cast<uintptr_t>(s.partials) & 15) == 0);
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
       for (int b = 0; b < NT; ++b) {
         const bool up = GATED && b >= NT / 2;
         const int m = 16 * a + c, n = 16 * (up ? b - NT / 2 : b) + 4 * h;
-        const uint32_t off = (uint32_t)(m * row_values + n + (up ? s.N : 0)) * 4u;
+        const uint32_t off = (uint32_t)(m * row_values + n + (up ? columns4 : 0)) * 4u;
         if (whole) {
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[a][b]), rsrc, m < rows && n < cols ? off : kNowhere, 0, 0);
         } else {
