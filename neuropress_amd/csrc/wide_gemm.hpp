@@ -77,14 +77,21 @@ __device__ __forceinline__ void store_rows(const uint8_t* ep, int lane, void* y,
     }
     return;
   }
-  // Rows at odd addresses: a value at a time, a row's side by side.
-#pragma unroll 8
-  for (int m = 0; m < 16 * MT; ++m) {
+  // Rows at odd addresses: whole pieces wherever they come to lie, the last piece of a row value by value (2556 x 8526 with both sums, K = 304: all of it by value 84 us, so 65; 8528 60).
+  constexpr int kPerRow = 2 * NC, kRowsAtOnce = 64 / kPerRow;
+  const int r = lane / kPerRow, p = lane % kPerRow;
+#pragma unroll 4
+  for (int i = 0; i < (16 * MT + kRowsAtOnce - 1) / kRowsAtOnce; ++i) {
+    const int m = i * kRowsAtOnce + r;
+    if (r >= kRowsAtOnce || m >= min(rows, 16 * MT) || p * 8 >= cols) continue;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(ep + m * kRow + p * 16);
+    uint16_t* const at = to + (int64_t)m * ldy64 + p * 8;
+    if (p * 8 + 8 <= cols) {
+      *reinterpret_cast<u32x4_any*>(at) = v;
+    } else {
 #pragma unroll
-    for (int n0 = 0; n0 < 16 * NC; n0 += 64) {
-      const int n = n0 + lane;
-      const uint16_t v = *reinterpret_cast<const uint16_t*>(ep + m * kRow + min(n, 16 * NC - 1) * 2);
-      __builtin_amdgcn_raw_buffer_store_b16(v, rsrc, m < rows && n < 16 * NC && n < cols ? ((uint32_t)m * ldy + (uint32_t)n) * 2u : kNowhere, 0, 0);
+      for (int e = 0; e < 8; ++e)
+        if (p * 8 + e < cols) at[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
     }
   }
 }
