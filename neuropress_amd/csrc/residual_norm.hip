@@ -198,6 +198,9 @@ __device__ __forceinline__ void put_four(u32x4& v, int half, const float (&f)[4]
   }
 }
 
+// The piece has been read when this has been passed: what stands behind it, a barrier too, may let others overwrite where it came from.
+__device__ __forceinline__ void arrived(const u32x4& v) { asm volatile("; arrived %0" ::"v"(v) : "memory"); }
+
 // Whether the registers hold a team's next rows too.
 constexpr bool rows_ahead(int dt, int nv, bool post, int gate) { return dt == NPAMD_F32 ? nv < 4 : nv < (post && gate ? 2 : 3); }
 
@@ -343,6 +346,11 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kerne
       s1 = wave_sum(s1);
       if (POST) s2 = wave_sum(s2), s3 = wave_sum(s3);
       if (RW > 1) {
+        // dx and dy may take the places of ds and y, and a row's last two pieces overlap, also where they are two waves': every value of the row has to be here before any is stored.  The sums
+        // have used dz and, with POST, these two.
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (!POST) arrived(ds_[i]), arrived(y_[i]);
         if ((threadIdx.x & 63) == 0) {
           meet[turn][wave][0] = s1;
           if (POST) meet[turn][wave][1] = s2, meet[turn][wave][2] = s3;

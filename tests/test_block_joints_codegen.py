@@ -84,3 +84,23 @@ def test_residual_norm(tmp_path):
         # 16-bit rows with both norms: 8 bytes of a shared gate's form, and rows of four pieces to a lane
         known = re.search(r"residual_norm_back_kernelILi[01]ELi(1ELb1ELi1|4ELb[01]ELi[12])E", name)
         assert not _spills(code) or known, name
+
+
+def test_a_row_has_arrived_before_it_is_overwritten(tmp_path):
+    """dx and dy may take the places of ds and y: without the norm behind, whose sums use both, a row's waves meet only when they have them, whatever else is on its way."""
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not build.Path(hipcc).exists():
+        pytest.skip("needs hipcc")
+    out = tmp_path / "kernels.s"
+    res = subprocess.run([hipcc, *build.CXXFLAGS, *build.DEVICE_FLAGS, "-S", "--cuda-device-only", str(build.CSRC / "residual_norm.hip"), "-o", str(out)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr[-2000:]
+    lines, forms = out.read_text().split("\n"), 0
+    for i, pieces in ((i, int(m[1])) for i, ln in enumerate(lines) if (m := re.match(r"^_ZN\S*residual_norm_back_kernelILi\dELi(\d)ELb0ELi\dE\S*: *;", ln))):
+        body = lines[i : next(j for j in range(i, len(lines)) if lines[j].startswith(".Lfunc_end"))]
+        meets = next(k for k, ln in enumerate(body) if "s_barrier" in ln and "lgkmcnt(0)" in body[k - 1] and "#ASM" in body[k - 2])
+        used = [k for k, ln in enumerate(body[:meets]) if re.match(r"\s+; arrived v\[\d+:\d+\]", ln)]
+        assert len(used) == 2 * pieces, lines[i]
+        between = body[used[0] : meets]
+        assert not [ln for ln in between if re.match(r"\s+(global|flat|buffer|scratch)_load", ln)], lines[i]
+        forms += 1
+    assert forms == 3 * 3 * 3

@@ -428,3 +428,29 @@ def test_rows_of_a_part_lie_apart(gpu, rows, every):
     k = (rows / 32 + 80) * U
     for got, ref in zip(out, ((dr, edr), dy, dw, dp, (seg(dg[0]), seg(dg[1]) + k * seg(dg[0].abs())))):
         _within(got, *ref, torch.float32, f"{rows} rows, a gate for {every}")
+
+
+@pytest.mark.parametrize("dtype,h", [(torch.bfloat16, 513), (torch.bfloat16, 1025), (torch.float16, 4100), (torch.bfloat16, 8193), (torch.float32, 257), (torch.float32, 4099)])
+@pytest.mark.parametrize("gate", ["none", "channel", "token"])
+def test_gradients_in_the_place_of_inputs_without_the_norm_behind(gpu, dtype, h, gate):
+    """The last two pieces of these rows overlap and are those of two waves: what one of them stores the other may not read any more."""
+    from neuropress_amd import _lib, kernels
+
+    rows, code = 300, {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}[dtype]
+    x, y, w, _, g = _make((rows, h), dtype, False, gate)
+    r, _, _, rstd = kernels.residual_norm_stats(x, y, w, None, g)
+    ds, dz = _grads((rows, h), dtype)
+    ref = kernels.residual_norm_backward(ds, dz, y, r, w, None, g, 1.0, None, rstd)
+    every = 0 if g is None else 1 if gate == "token" else rows
+    need = _lib.load().npamd_residual_norm_workspace_bytes(rows, h, every, code)
+    ws = torch.empty(max(4, need), dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    for into_y in (False, True):
+        ds2, dz2, y2, dw = ds.clone(), dz.clone(), y.clone(), torch.empty(h, device="cuda", dtype=dtype)
+        dg = None if g is None else torch.empty_like(g)
+        dy = y2 if into_y else dz2
+        _lib.call("npamd_residual_norm_backward", ds2.data_ptr(), h, dz2.data_ptr(), h, y2.data_ptr(), h, r.data_ptr(), h, w.data_ptr(), None, None if g is None else g.data_ptr(), h,
+                  max(1, every), 1.0, None, rstd.data_ptr(), ds2.data_ptr(), h, dy.data_ptr(), h, dw.data_ptr(), None, None if g is None else dg.data_ptr(), rows, h, code,
+                  ws.data_ptr(), need, st)  # fmt: skip
+        for a, b in zip((ds2, dy, dw, None, dg), ref):
+            assert a is None and b is None or torch.equal(a, b)
