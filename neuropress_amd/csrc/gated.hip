@@ -65,13 +65,13 @@ int launch_few(const FewArgs& a, hipStream_t st, const char* what) {
 // Which kernel takes a call; aligned: rows that the tiles can read.  Us with dense_few_kernel / dense_some_kernel / the tiles, silu: two tokens 14336 x 4096 43.5 / 44.2 / 54.5, 1024 x 1024 3.6 / 4.0 / 7.1;
 // three 1024 x 1024 4.0 / 3.9 / 7.1; 16 tokens 8192 x 2048 - / 15.6 / 17.8, 4864 x 896 - / 6.4 / 6.8.  Past 16 tokens a block holds two tiles of them: 32 tokens 14336 x 4096 - / 54 / 59, 8192 x 2048 - /
 // 17.5 / 17.7, 4096 x 1024 - / 6.3 / 7.2, but 5504 x 2048 - / 14.5 / 13.0, 4864 x 896 - / 8.3 / 6.9; 48 tokens 1024 x 1024 - / 5.8 / 7.2, 2752 x 1024 - / 6.5 / 7.1, but 2048 x 4096 - / 14.1 / 12.9; 64 tokens
-// 1024 x 1024 - / 7.6 / 7.2.
+// 1024 x 1024 - / 7.6 / 7.2.  far: outputs whose rows are too far apart for the tiles.
 enum Path { kFew, kSome, kTiles };
-Path path_of(int M, int N, int K, bool aligned) {
+Path path_of(int M, int N, int K, bool aligned, bool far) {
   if (M <= 2) return kFew;
   if (!aligned) return M <= NPAMD_GEMV_MAX_M ? kFew : kTiles;
   const int64_t weights = 2 * (int64_t)N * K;
-  if (M <= 16 || (M <= 32 && (N <= 4096 ? weights <= 1 << 24 : N >= 8192))) return kSome;
+  if (M <= 16 || (M <= NPAMD_GEMV_MAX_M && (far || (N <= 4096 ? weights <= 1 << 24 : N >= 8192)))) return kSome;
   return M <= 48 && weights <= 1 << 23 ? kSome : kTiles;
 }
 
@@ -243,7 +243,7 @@ void launch_pointwise(const GatedPointwise& a, int act, hipStream_t st) {
 }  // namespace
 
 extern "C" int64_t npamd_gated_linear_workspace_bytes(int M, int N, int K) {
-  return M < 1 || N < 1 || K < 1 || past_kernels(M, N, K) || path_of(M, N, K, true) != kTiles ? 0 : dense_gemm_gated_workspace_bytes(M, N, K);
+  return M < 1 || N < 1 || K < 1 || past_kernels(M, N, K) || path_of(M, N, K, true, false) != kTiles ? 0 : dense_gemm_gated_workspace_bytes(M, N, K);
 }
 
 extern "C" int npamd_gated_linear(const void* x, int64_t ldx, const void* gate_up, int64_t ldw, const void* bias, int bias_dtype, int activation, void* y, int64_t ldy,
@@ -261,12 +261,13 @@ extern "C" int npamd_gated_linear(const void* x, int64_t ldx, const void* gate_u
   const DenseEpilogue ep{bias, nullptr, 0, activation, bias_dtype != NPAMD_F32, pre, ldp};
   const bool tiles = tiles_take(x, ldx, gate_up, ldw, K);
   const FewArgs a{x, gate_up, y, ldx, ldw, ldy, M, N, K, ep};
-  const Path path = path_of(M, N, K, tiles);
+  const bool far = ldy >= NPAMD_TILE_MAX_STRIDE || (pre && ldp >= NPAMD_TILE_MAX_STRIDE);
+  const Path path = path_of(M, N, K, tiles, far);
   if (path == kSome) return act_dtype == NPAMD_BF16 ? launch_some<NPAMD_BF16>(a, st, what) : launch_some<NPAMD_F16>(a, st, what);
   if (path == kFew) return act_dtype == NPAMD_BF16 ? launch_few<NPAMD_BF16>(a, st, what) : launch_few<NPAMD_F16>(a, st, what);
   NPAMD_REQUIRE(tiles, "%s: past %d tokens x and gate_up have to lie at 16-byte addresses, K=%d and rows' distances have to be multiples of 8", what, NPAMD_GEMV_MAX_M, K);
   NPAMD_REQUIRE(!workspace || ((uintptr_t)workspace & 15) == 0, "%s: the workspace has to lie at a 16-byte address", what);
-  if (ldy >= NPAMD_TILE_MAX_STRIDE || (pre && ldp >= NPAMD_TILE_MAX_STRIDE))
+  if (far)
     return fail(NPAMD_ERR_UNSUPPORTED, "%s: past %d tokens the outputs' rows have to be less than 2^22 apart", what, NPAMD_GEMV_MAX_M);
   DenseShape s{};
   s.x = x, s.w = gate_up, s.y = y, s.ldx = ldx, s.ldw = ldw, s.ldy = ldy, s.M = M, s.N = N, s.partials = (float*)workspace, s.ep = ep;

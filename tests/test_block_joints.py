@@ -82,6 +82,17 @@ def test_gated_linear_refuses():
 
 
 @no_gpu
+def test_gated_linear_takes_outputs_far_apart_up_to_32_tokens():
+    """Whatever the sizes would be best served by: outputs' rows may be any distance apart up to there."""
+    far = 1 << 22
+    for m in (3, 16, 17, 20, 32):
+        for n, k in ((32, 64), (2048, 4096), (4864, 896), (5504, 2048), (8192, 2048)):
+            for ldy, ldp in ((far, 2 * n), (n, far), (far + 1, far + 3)):
+                code = _lib.load().npamd_gated_linear(P, k, P, k, P, 2, 4, P, ldy, P, ldp, m, n, k, 0, None, 0, None)
+                assert code not in (0, -1, -2), (m, n, k, _lib.load().npamd_last_error())  # nothing here to launch on
+
+
+@no_gpu
 def test_gated_linear_backward_refuses():
     size = _lib.load().npamd_gated_linear_backward_workspace_bytes
     need = size(70, 32, 64, 1, 1, 1)

@@ -362,3 +362,32 @@ def test_products_one_after_the_other(gpu, paired):
         for pair in (-1, 0, 1):
             paired(pair, 0, 0)
             _check_backward(dh, x, w, pre, "gelu", what=(m, n, k, pair))
+
+
+def _formula(x, w, b):
+    """((h, its tolerance), (both sums, theirs)) with SiLU, as in _check_forward."""
+    v, spread = x.double() @ w.double().T + b.double(), x.double().abs() @ w.double().abs().T + b.double().abs()
+    e = (x.shape[-1] / 16 + 40) * U * spread
+    (g, u), (eg, eu) = v.chunk(2, -1), e.chunk(2, -1)
+    a, ea = _act("silu", g), 1.13 * eg + 2.0**-20 * g.abs()
+    return (a * u, ea * u.abs() + (a.abs() + ea) * eu + 2 * U * (a * u).abs()), (v, e)
+
+
+@pytest.mark.parametrize("m,n,k", [(20, 5504, 264), (32, 3000, 2992), (17, 6000, 72)])
+def test_outputs_far_apart(gpu, m, n, k):
+    """Rows of y and of the sums further apart than the tiles take, at sizes that go there otherwise."""
+    from neuropress_amd import _lib
+
+    x, w, b, _ = _inputs(m, n, k, torch.bfloat16)
+    refs = _formula(x, w, b)
+    far, bits = 1 << 22, dict(device="cuda", dtype=torch.int16)
+    for ldy, ldp in ((far, 2 * n), (n, far), (far + 1, far + 3)):
+        wide = [torch.full((m - 1, ld), 77, **bits) for ld in (ldy, ldp)]
+        wide = [torch.cat((t.view(-1), torch.full((c,), 77, **bits))) for t, c in zip(wide, (n, 2 * n))]
+        _lib.call("npamd_gated_linear", x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), _lib.BF16, 4, wide[0].data_ptr(), ldy, wide[1].data_ptr(), ldp, m, n, k, _lib.BF16, None, 0,
+                  torch.cuda.current_stream().cuda_stream)  # fmt: skip
+        for t, ld, (ref, tol) in zip(wide, (ldy, ldp), refs):
+            got = t.view(torch.bfloat16).as_strided(ref.shape, (ld, 1))
+            _within(got, ref, tol, torch.bfloat16, (ldy, ldp))
+            got.view(torch.int16).fill_(77)
+            assert bool((t == 77).all()), "between the rows"
