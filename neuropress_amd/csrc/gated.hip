@@ -90,12 +90,12 @@ struct GatedPointwise {
   int M, N, strips;
 };
 
-// act(g) and act'(g).
+// act(g) and act'(g); both are NaN where g is.
 template <int KIND>
 __device__ __forceinline__ void activation_and_slope(float g, float& value, float& slope) {
   if constexpr (KIND == NPAMD_ACT_RELU) {
     value = g < 0.f ? 0.f : g;
-    slope = g > 0.f ? 1.f : 0.f;
+    slope = g > 0.f ? 1.f : g <= 0.f ? 0.f : g;
   } else if constexpr (KIND == NPAMD_ACT_GELU) {
     const float cdf = gelu_cdf_f32(g);
     value = g * cdf;
@@ -106,6 +106,7 @@ __device__ __forceinline__ void activation_and_slope(float g, float& value, floa
     const float e = __expf(-1.5957691216f * w), s = __builtin_amdgcn_rcpf(1.f + e);
     value = gelu_tanh_f32(g);
     slope = __builtin_fmaf(c * s * (1.f - s), 1.5957691216f * __builtin_fmaf(0.134145f * c, c, 1.f), s);
+    slope = g == g ? slope : g;  // fmaxf drops a NaN
   } else if constexpr (KIND == NPAMD_ACT_SILU) {
     const float p = __builtin_amdgcn_rcpf(1.f + __expf(-g));
     value = g * p;

@@ -391,3 +391,23 @@ def test_outputs_far_apart(gpu, m, n, k):
             _within(got, ref, tol, torch.bfloat16, (ldy, ldp))
             got.view(torch.int16).fill_(77)
             assert bool((t == 77).all()), "between the rows"
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,n,k", [(9, 5, 40), (70, 61, 72)])
+def test_sums_that_are_not_numbers(gpu, act, m, n, k):
+    """A NaN among the gate's sums or the other ones goes on into every gradient that the formula multiplies it into, and no other: the slope of an activation is NaN there."""
+    from neuropress_amd import kernels
+
+    for dtype in DTYPES:
+        x, w, b, dh = _inputs(m, n, k, dtype)
+        clean = kernels.gated_linear_pre(x, w, b, act)[1]
+        assert bool(clean.isfinite().all())
+        for row, column, bad in ((2, 1, {1, n + 1} if act else {n + 1}), (m - 1, n + 3, {3})):
+            pre = clean.clone()
+            pre[row, column] = float("nan")
+            dx, dw, db = kernels.gated_linear_backward(dh, x, w, pre, act)
+            rows, columns = torch.zeros(m, dtype=torch.bool, device="cuda"), torch.zeros(2 * n, dtype=torch.bool, device="cuda")
+            rows[row] = True
+            columns[list(bad)] = True
+            assert torch.equal(dx.isnan(), rows[:, None].expand(m, k)) and torch.equal(dw.isnan(), columns[:, None].expand(2 * n, k)) and torch.equal(db.isnan(), columns)
