@@ -606,9 +606,9 @@ int64_t npamd_gated_linear_backward_workspace_bytes(int M, int N, int K, int dx,
 /*
  * Low-rank adapters of many requests beside a projection that they share: y[m] = base[m] + scale[i] * (x[m] A_i^T) B_i^T with i = ids[m]; y[m] = base[m], bit for bit, where ids[m] is not in
  * 0 .. adapters - 1.  x [M, K], base (NULL: zero), y [M, N], a [adapters, rank, K], b: act_dtype (NPAMD_F16 or NPAMD_BF16); ids [M]: integers of ids_bits 32 or 64; scale: NULL (1), or f32
- * [adapters].  b: [adapters, N, rank rounded up to a multiple of eight] with zeros past the rank.  f32 sums; x A^T is held to 2^-16 (bf16) or 2^-21 (f16); y is rounded once.  y may be base
- * (with the same row distance).  x, a and b lie at 16-byte addresses, K and ldx are multiples of 8; base and y lie anywhere.  Rank at most 256, at most 8192 adapters, 2^22 tokens, 2^24 columns
- * of y.
+ * [adapters].  b: [adapters, N, rank rounded up to a multiple of eight] with zeros past the rank.  f32 sums; x A^T is held to 2^-16 of each value (bf16), or to 2^-21 of it and 2^-37 of a
+ * token's largest (f16); y is rounded once.  y may be base (with the same row distance).  x, a and b lie at 16-byte addresses, K and ldx are multiples of 8; base and y lie anywhere.  Rank at
+ * most 256, at most 8192 adapters, 2^22 tokens, 2^24 columns of y.
  * workspace: npamd_adapter_linear_workspace_bytes bytes of 16-byte aligned device memory, contents irrelevant; calls that overlap must not share one.
  */
 int npamd_adapter_linear(const void* x, int64_t ldx, const void* ids, int ids_bits, const void* a, const void* b, const float* scale, const void* base, int64_t ldbase,

@@ -6,7 +6,7 @@
 //   down: t = x A^T, f32.  A block takes 16, 32 or 64 tokens of an entry, up to 64 ranks and a part of K; x and A come into LDS in whole lines, each wave with steps of its own, and the waves'
 //         sums meet in LDS.
 //   up:   y = base + scale t B^T.  A block brings its entry's t into LDS once, as two parts of B's type, for an MFMA each (t is not rounded to 16 bits: 2^-16 of it is left with bf16; fp16, scaled
-//         by a power of two to the row's largest, 2^-21), and its waves take 64 or 128 columns each.  Column 8 c + b of a wave is row c of MFMA b, so that a lane ends up with eight neighbouring columns
+//         by a power of two to the row's largest, 2^-21 of it and 2^-37 of the largest), and its waves take 64 or 128 columns each.  Column 8 c + b of a wave is row c of MFMA b, so that a lane ends up with eight neighbouring columns
 //         of four tokens and 16 lanes with 256 bytes of a row of base and y, side by side.  (With four tokens' rows in every quarter of the lanes instead, as the MFMAs' own layout
 //         has them, a load touches 64 places: 64 to 86 us in the place of 52 for 4096 tokens through 14336 columns of bf16, rank 64.)
 // Bound by the latency of two dependent launches for a decode step, by the bytes of base and y for prompts.
@@ -178,10 +178,11 @@ __global__ void __launch_bounds__(512) adapter_down_kernel(const AdapterArgs a) 
 }
 
 // Eight values as two parts of the operands' type, both of the value's sign: the first cut off, the second what is left.  A part that would be zero where the value is not is the smallest
-// normal number instead, so that a product with an infinite weight is infinite and not NaN.
+// number there is instead (bf16: the smallest normal one), so that a product with an infinite weight is infinite and not NaN.  The matrix pipes take fp16's subnormal numbers as they are: of a row
+// whose largest value is 2^14 and more, two parts are off by 2 x 2^-24 at most where they are that small, 2^-37 of the largest (with the smallest normal number, 2^-14, in both parts 2^-27).
 template <int ACT>
 __device__ __forceinline__ void two_parts(const float (&v)[8], u32x4& hi, u32x4& lo) {
-  constexpr float kTiny = ACT == NPAMD_BF16 ? 1.17549435e-38f : 6.103515625e-5f;
+  constexpr float kTiny = ACT == NPAMD_BF16 ? 1.17549435e-38f : 5.9604644775390625e-8f;
   uint32_t h16[8], l16[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

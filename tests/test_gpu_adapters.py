@@ -294,3 +294,29 @@ def test_wide_ranks_of_long_prompts(gpu, dtype, m, n, rank):
     for how in ("runs", "any"):
         ids = _ids(m, 5, how)
         _check(x, a, b, scale, base, ids, _run(x, a, b, scale, ids, base), how)
+
+
+@pytest.mark.parametrize("m", [3, 150])
+@pytest.mark.parametrize("rank", [8, 24, 60, 128, 200])
+def test_small_values_beside_large_ones(gpu, m, rank):
+    """float16, values of x A^T of one token 2^22 apart, and columns of y that meet only the small ones: x A^T is held to 2^-21 of each and 2^-37 of the token's largest."""
+    k, n = 256, 136
+    x, a, b, _, _ = _make(m, n, k, rank, 2, torch.float16)
+    a = torch.cat((a[:, :1] * 2.0**10, a[:, 1:] * 2.0**-12), 1)
+    b[:, ::2, 0] = 0.0
+    ids = _ids(m, 2, "random")
+    scale = torch.tensor([2.0**6, 2.0**7], device="cuda")
+    y = _run(x, a, b, scale, ids, None)
+    tried = 0
+    for i in range(2):
+        rows = ids == i
+        xd, ad, bd = x[rows].double(), a[i].double(), b[i, ::2].double()
+        t = xd @ ad.T
+        et = (k / 16 + 40) * U * (xd.abs() @ ad.abs().T) + 2.0**-21 * t.abs() + 2.0**-37 * t.abs().amax(-1, keepdim=True)
+        ref = scale[i].double() * (t @ bd.T)
+        tol = scale[i].double() * (et @ bd.abs().T + (rank / 16 + 40) * U * (t[:, 1:].abs() @ bd[:, 1:].abs().T)) + 3 * U * ref.abs()
+        eps = torch.finfo(torch.float16).eps
+        bad = (y[rows, ::2].double() - ref).abs() / (tol + ref.abs() * (eps / 2) * 1.0001 + torch.finfo(torch.float16).smallest_normal * eps / 2)
+        assert bool((bad <= 1).all()), f"{bad.max().item():.2f} of the tolerance"
+        tried += int(rows.sum())
+    assert tried
