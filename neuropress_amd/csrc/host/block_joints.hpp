@@ -179,8 +179,7 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
     const c10::DeviceGuard guard(x.device());
     const auto out = ResidualNormCall(x, y, weight, post.value_or(at::Tensor()), gate.value_or(at::Tensor()), scale, eps).forward(true);
     ctx->set_materialize_grads(false);
-    // x itself is needed only where it is a leaf, which a capture asks about.
-    ctx->save_for_backward({y, out[0], weight, post.value_or(at::Tensor()), gate.value_or(at::Tensor()), out[2], out[3], x.is_leaf() && x.requires_grad() ? x : at::Tensor()});
+    ctx->save_for_backward({y, out[0], weight, post.value_or(at::Tensor()), gate.value_or(at::Tensor()), out[2], out[3]});
     ctx->saved_data["scale"] = scale;
     return {out[0], out[1]};
   }
@@ -191,7 +190,7 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
     if (!grads[0].defined() && !grads[1].defined()) return result;
     const at::Tensor &y = saved[0], &stream = saved[1], &weight = saved[2], &post = saved[3], &gate = saved[4];
     const c10::DeviceGuard guard(y.device());
-    refuse_foreign_leaves("residual_norm", {saved[7], y, weight, post, gate});
+    refuse_foreign_leaves("residual_norm");
     std::array<at::Tensor, 5> out;
     {
       const c10::AutoGradMode off(false);
@@ -335,7 +334,7 @@ struct GatedLinearNode : torch::autograd::Function<GatedLinearNode> {
     const bool recorded = c10::GradMode::is_enabled();
     const at::Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &pre = saved[3];
     const c10::DeviceGuard guard(x.device());
-    refuse_foreign_leaves("gated_linear", {x, w, bias});
+    refuse_foreign_leaves("gated_linear");
     torch::autograd::variable_list result(4);
     std::array<at::Tensor, 3> out;
     {

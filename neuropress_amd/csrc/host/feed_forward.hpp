@@ -129,15 +129,17 @@ at::Tensor as_rows(const at::Tensor& t, int64_t* ld) { return rows_of(t, ld) ? t
 
 const void* data_or_null(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
-// Inside a capture torch would go on to leaves whose nodes another graph that is still alive has made on another stream: waiting for that stream there ends the process.
-void refuse_foreign_leaves(const char* what, std::initializer_list<at::Tensor> inputs) {
+// Inside a capture torch would go on to leaves whose nodes another graph that is still alive has made on another stream: waiting for that stream there ends the process.  Called in
+// a node's backward pass: the leaves are those that its edges lead to, whether it keeps them or not.
+void refuse_foreign_leaves(const char* what) {
   const auto stream = c10::hip::getCurrentHIPStream();
   hipStreamCaptureStatus status;
   if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) return (void)hipGetLastError();
   if (status == hipStreamCaptureStatusNone) return;
-  for (const at::Tensor& t : inputs) {
-    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) continue;
-    const auto leaf = torch::autograd::impl::try_get_grad_accumulator(t);
+  const auto node = torch::autograd::get_current_node();
+  TORCH_CHECK(node, what, ": a backward pass cannot be captured outside torch's engine");
+  for (const torch::autograd::Edge& edge : node->next_edges()) {
+    const auto leaf = std::dynamic_pointer_cast<torch::autograd::AccumulateGrad>(edge.function);
     TORCH_CHECK(!leaf || !leaf->stream() || leaf->stream()->id() == stream.id(), what,
                 ": a backward pass cannot be captured while a graph of the same leaves from another stream is alive: free it, or make it on the stream of the capture");
   }
@@ -164,7 +166,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     torch::autograd::variable_list out(4);
     const at::Tensor &x = saved[0], &mean = saved[3], &rstd = saved[4];
     const c10::DeviceGuard guard(x.device());
-    refuse_foreign_leaves("layer_norm", {saved[0], saved[1], saved[2]});
+    refuse_foreign_leaves("layer_norm");
     {
       const c10::AutoGradMode off(false);
       const bool with_w = saved[1].defined(), with_b = saved[2].defined();

@@ -454,3 +454,24 @@ def test_gradients_in_the_place_of_inputs_without_the_norm_behind(gpu, dtype, h,
                   ws.data_ptr(), need, st)  # fmt: skip
         for a, b in zip((ds2, dy, dw, None, dg), ref):
             assert a is None and b is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("post", [False, True])
+def test_the_stream_may_change_between_the_passes(gpu, post):
+    """No gradient needs x's values: a leaf that an optimizer, say, has changed meanwhile is no error; y's values are needed, and torch says so."""
+    from neuropress_amd import kernels
+
+    t = _make((6, 515), torch.bfloat16, post, "none")
+    ds, dz = _grads((6, 515), torch.bfloat16)
+    x, y, w = (v.clone().requires_grad_() for v in t[:3])
+    want = torch.autograd.grad(kernels.residual_norm(x, y, w, t[3]), (x, y, w), (ds, dz))
+    out = kernels.residual_norm(x, y, w, t[3])
+    with torch.no_grad():
+        x.mul_(3.0)
+    for a, b in zip(torch.autograd.grad(out, (x, y, w), (ds, dz)), want):
+        assert torch.equal(a, b)
+    out = kernels.residual_norm(x, y, w, t[3])
+    with torch.no_grad():
+        y.mul_(3.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, (x, y, w), (ds, dz))

@@ -165,3 +165,30 @@ def test_capture_beside_an_eager_graph_of_the_same_leaves(gpu):
         assert torch.equal(x.grad, want)
         for t in leaves:
             t.grad = None
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_capture_beside_an_eager_graph_of_one_leaf(gpu, which):
+    """The same where x, y, a weight or the gate is the only leaf, kept by the node or not."""
+    from neuropress_amd import kernels
+
+    g = cases.gen(which)
+    given = [torch.randn(s, generator=g).bfloat16().to(gpu) for s in ((20, 64), (20, 64), (64,), (64,), (64,))]
+    leaf = given[which].requires_grad_()
+    make = lambda: kernels.residual_norm(*given, 0.7)[1]
+    back = torch.ones(20, 64, device=gpu, dtype=torch.bfloat16)
+    alive = make()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            make().backward(back)
+    torch.cuda.synchronize()
+    assert leaf.grad is None
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        make().backward(back)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(leaf.grad, torch.autograd.grad(make(), leaf, back)[0])
