@@ -325,22 +325,25 @@ struct GatedLinearNode : torch::autograd::Function<GatedLinearNode> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation) {
     const c10::DeviceGuard guard(x.device());
     const auto out = gated_forward(x, w, bias.value_or(at::Tensor()), (int)activation, true);
-    ctx->save_for_backward({x, w, bias.value_or(at::Tensor()), out[1]});
+    ctx->save_for_backward({x, w, out[1]});
     ctx->saved_data["activation"] = activation;
+    if (bias) ctx->saved_data["bias"] = (int64_t)bias->scalar_type();  // all that its gradient needs of it
     return out[0];
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const torch::autograd::variable_list saved = ctx->get_saved_variables();
     const bool recorded = c10::GradMode::is_enabled();
-    const at::Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &pre = saved[3];
+    const at::Tensor &x = saved[0], &w = saved[1], &pre = saved[2];
+    const auto bias = ctx->saved_data.find("bias");
+    const bool biased = bias != ctx->saved_data.end();
     const c10::DeviceGuard guard(x.device());
     refuse_foreign_leaves("gated_linear");
     torch::autograd::variable_list result(4);
     std::array<at::Tensor, 3> out;
     {
       const c10::AutoGradMode off(false);
-      const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), bias.defined() && ctx->needs_input_grad(2)};
-      out = gated_backward(grads[0], x, w, pre, (int)ctx->saved_data["activation"].toInt(), bias.defined() ? bias.scalar_type() : at::kFloat, need);
+      const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), biased && ctx->needs_input_grad(2)};
+      out = gated_backward(grads[0], x, w, pre, (int)ctx->saved_data["activation"].toInt(), biased ? (at::ScalarType)bias->second.toInt() : at::kFloat, need);
     }
     for (int i = 0; i < 3; ++i) result[i] = recorded ? final_gradient("gated_linear: its backward pass cannot be differentiated", out[i]) : out[i];
     return result;

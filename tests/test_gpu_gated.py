@@ -411,3 +411,18 @@ def test_sums_that_are_not_numbers(gpu, act, m, n, k):
             rows[row] = True
             columns[list(bad)] = True
             assert torch.equal(dx.isnan(), rows[:, None].expand(m, k)) and torch.equal(dw.isnan(), columns[:, None].expand(2 * n, k)) and torch.equal(db.isnan(), columns)
+
+
+@pytest.mark.parametrize("bias_dtype", [torch.float16, torch.float32])
+def test_the_bias_may_change_between_the_passes(gpu, bias_dtype):
+    """Its gradient needs none of its values."""
+    from neuropress_amd import kernels
+
+    x, w, b, dh = _inputs(12, 40, 72, torch.float16)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b.to(bias_dtype))]
+    want = torch.autograd.grad(kernels.gated_linear(*leaves), leaves, dh)
+    out = kernels.gated_linear(*leaves)
+    with torch.no_grad():
+        leaves[2].mul_(3.0)
+    got = torch.autograd.grad(out, leaves, dh)
+    assert got[2].dtype == bias_dtype and all(torch.equal(a, e) for a, e in zip(got, want))
