@@ -23,7 +23,12 @@ class NPAdapterLinear(nn.Module):
 
     def __init__(self, base: nn.Module, adapters: LowRankAdapters) -> None:
         super().__init__()
+        for side in ("in_features", "out_features"):
+            theirs, ours = getattr(base, side, None), getattr(adapters, side, None)
+            if isinstance(theirs, int) and isinstance(ours, int) and theirs != ours:
+                raise RuntimeError(f"NPAdapterLinear: the adapters have {side} of {ours}, the projection of {theirs}")
         self.base = base
+        self.training = base.training  # without a word to what is inside it
         self.adapters = adapters
         self.ids: torch.Tensor | None = None
 
@@ -38,7 +43,8 @@ class NPAdapterLinear(nn.Module):
 
 
 def attach_adapters(model: nn.Module, adapters: dict[str, LowRankAdapters]) -> int:
-    """Put an :class:`NPAdapterLinear` in the place of every module of *model* that *adapters* names; returns how many.  Names that *model* does not have are an error."""
+    """Put an :class:`NPAdapterLinear` in the place of every module of *model* that *adapters* names; returns how many.  Names that *model* does not have, and adapters
+    of other sizes than the layer's, are an error, and nothing is replaced."""
     places = []
     for name, those in adapters.items():
         parent_name, _, attr = name.rpartition(".")
@@ -49,9 +55,13 @@ def attach_adapters(model: nn.Module, adapters: dict[str, LowRankAdapters]) -> i
             raise RuntimeError(f"attach_adapters: the model has no module {name!r}") from None
         if not attr:
             raise RuntimeError("attach_adapters: the model itself cannot be replaced: wrap it in an NPAdapterLinear")
-        places.append((parent, attr, base.base if isinstance(base, NPAdapterLinear) else base, those))
-    for parent, attr, base, those in places:
-        setattr(parent, attr, NPAdapterLinear(base, those).train(base.training))
+        base = base.base if isinstance(base, NPAdapterLinear) else base
+        try:
+            places.append((parent, attr, NPAdapterLinear(base, those)))
+        except RuntimeError as e:
+            raise RuntimeError(f"attach_adapters: {name}: {e}") from None
+    for parent, attr, layer in places:
+        setattr(parent, attr, layer)
     return len(places)
 
 

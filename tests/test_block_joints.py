@@ -131,3 +131,34 @@ def test_attaching_adapters_to_what_is_not_there():
     set_adapter_ids(torch.nn.Sequential(layer), None)
     x = torch.randn(3, 4)
     assert torch.equal(layer(x), model[0](x)) and set(layer.state_dict()) == {"base.weight", "base.bias"}
+
+
+def test_attaching_adapters_of_other_sizes():
+    """Found when they are attached, not at the first call; nothing has been replaced then."""
+    from types import SimpleNamespace
+
+    from neuropress_amd.nn import NPAdapterLinear, attach_adapters
+
+    model = torch.nn.Sequential(torch.nn.Linear(4, 8), torch.nn.Linear(8, 6, bias=False), torch.nn.ReLU())
+    sizes = lambda k, n: SimpleNamespace(in_features=k, out_features=n)
+    for wrong in (sizes(8, 4), sizes(4, 7), sizes(5, 8)):
+        with pytest.raises(RuntimeError, match="0: .*_features"):
+            attach_adapters(model, {"1": sizes(8, 6), "0": wrong})
+        assert not any(isinstance(layer, NPAdapterLinear) for layer in model)
+        with pytest.raises(RuntimeError, match="_features"):
+            NPAdapterLinear(model[0], wrong)
+    assert attach_adapters(model, {"0": sizes(4, 8), "1": sizes(8, 6), "2": sizes(1, 1)}) == 3  # a layer that says nothing of its sizes
+    first = model[0].base
+    assert attach_adapters(model, {"0": sizes(4, 8)}) == 1 and model[0].base is first
+    with pytest.raises(RuntimeError, match="_features"):
+        attach_adapters(model, {"0": sizes(8, 4)})
+
+
+def test_attaching_adapters_leaves_modes_alone():
+    from neuropress_amd.nn import NPAdapterLinear
+
+    inner = torch.nn.Dropout().eval()
+    base = torch.nn.Sequential(inner).train()
+    inner.eval()
+    assert NPAdapterLinear(base, None).training and base.training and not inner.training
+    assert not NPAdapterLinear(base.eval(), None).training
