@@ -62,17 +62,21 @@ int launch_few(const FewArgs& a, hipStream_t st, const char* what) {
   return check_launch(what);
 }
 
-// Which kernel takes a call; aligned: rows that the tiles can read.  Us with dense_few_kernel / dense_some_kernel / the tiles, silu: two tokens 14336 x 4096 43.5 / 44.2 / 54.5, 1024 x 1024 3.6 / 4.0 / 7.1;
-// three 1024 x 1024 4.0 / 3.9 / 7.1; 16 tokens 8192 x 2048 - / 15.6 / 17.8, 4864 x 896 - / 6.4 / 6.8.  Past 16 tokens a block holds two tiles of them: 32 tokens 14336 x 4096 - / 54 / 59, 8192 x 2048 - /
-// 17.5 / 17.7, 4096 x 1024 - / 6.3 / 7.2, but 5504 x 2048 - / 14.5 / 13.0, 4864 x 896 - / 8.3 / 6.9; 48 tokens 1024 x 1024 - / 5.8 / 7.2, 2752 x 1024 - / 6.5 / 7.1, but 2048 x 4096 - / 14.1 / 12.9; 64 tokens
-// 1024 x 1024 - / 7.6 / 7.2.  far: outputs whose rows are too far apart for the tiles.
+// Which kernel takes a call; aligned: rows that the tiles can read.  One and two tokens: dense_few_kernel (us, silu, with it / dense_some_kernel / the tiles: 14336 x 4096 43.5 / 44.2 / 54.5,
+// 1024 x 1024 3.6 / 4.0 / 7.1).  From three on dense_some_kernel, whose blocks have all of K, or the tiles, which may have parts of it.  Up to 4096 columns K has to be long for so few of them before the tiles are
+// ahead; past them blocks of dense_some_kernel have 32 columns, and what decides is how full their last round is and, past 16 tokens, whether rows of W lie a multiple of 4096 bytes apart, which the tiles read more
+// slowly.  Us, dense_some_kernel / the tiles: 16 tokens 512 x 2560 5.8 / 7.9, 512 x 14336 26.4 / 13.9, 8192 x 2048 15.8 / 18.0, 9728 x 512 9.7 / 8.2; 24 tokens 1024 x 2560 8.9 / 9.7, 1024 x 8192 18.9 / 12.8,
+// 3584 x 3584 13.4 / 16.2, 4288 x 1024 8.4 / 8.0, 8192 x 2560 19.2 / 18.9, 8192 x 4096 29.3 / 31.3, 9728 x 4096 44.2 / 40.3, 14336 x 4096 49.5 / 57.2; 40 tokens 2048 x 2048 9.3 / 11.8, 2048 x 4096 14.5 / 12.9,
+// 4096 x 4096 17.2 / 21.4, 8192 x 4096 32.1 / 31.6.  Over 180 shapes of 512 to 28672 columns and K of 512 to 14336, at nine numbers of tokens from 3 to 48, the kernel taken is 0.2 to 1.2 % slower than the better
+// one in the mean, 26 % at most; over 110 others 0.3 to 1.8 %, 35 % at most.  far: outputs whose rows are too far apart for the tiles.
 enum Path { kFew, kSome, kTiles };
 Path path_of(int M, int N, int K, bool aligned, bool far) {
   if (M <= 2) return kFew;
   if (!aligned) return M <= NPAMD_GEMV_MAX_M ? kFew : kTiles;
-  const int64_t weights = 2 * (int64_t)N * K;
-  if (M <= 16 || (M <= NPAMD_GEMV_MAX_M && (far || (N <= 4096 ? weights <= 1 << 24 : N >= 8192)))) return kSome;
-  return M <= 48 && weights <= 1 << 23 ? kSome : kTiles;
+  if (far && M <= NPAMD_GEMV_MAX_M) return kSome;
+  if (N <= 4096) return M <= 48 && K <= std::max(M <= 16 ? 4096 : 2560, N * N >> (M <= 16 ? 9 : M <= 32 ? 10 : 11)) ? kSome : kTiles;
+  const int blocks = (N + 31) / 32, rounds = (blocks + 255) / 256;
+  return (M <= 16 && N <= 8192) || (M <= 32 && K % 2048 == 0 && 6 * blocks >= 5 * 256 * rounds) ? kSome : kTiles;
 }
 
 bool bad_shape(int M, int N, int K) { return M < 0 || N < 0 || K < 1; }

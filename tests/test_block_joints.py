@@ -81,6 +81,15 @@ def test_gated_linear_refuses():
     assert size(0, 32, 64) == 0 == size(70, 2**24 + 1, 64) == size(1, 32, 64) and size(70, 64, 8192) > 0
 
 
+def test_gated_linear_of_some_tokens_goes_where_it_was_measured_to_be_faster():
+    """The tiles split a long K over blocks and need workspace for it; the kernel for some tokens needs none."""
+    size = _lib.load().npamd_gated_linear_workspace_bytes
+    for m, n, k in ((16, 512, 14336), (24, 512, 8192), (24, 1024, 8192), (40, 512, 8192), (48, 2048, 8192)):
+        assert size(m, n, k) > 0, (m, n, k)
+    for m, n, k in ((16, 512, 2560), (16, 8192, 2048), (24, 3584, 3584), (32, 4096, 4096), (40, 4096, 4096), (24, 14336, 4096)):
+        assert size(m, n, k) == 0, (m, n, k)
+
+
 @no_gpu
 def test_gated_linear_takes_outputs_far_apart_up_to_32_tokens():
     """Whatever the sizes would be best served by: outputs' rows may be any distance apart up to there."""
