@@ -5,8 +5,9 @@
 // keeps of them, half of what f32 would take.
 // Backward, from those sums g and u and the gradient dh: dg = dh u act'(g), du = dh act(g) in f32, rounded to x's type as the matrix pipes' operands (one rounding of 2^-9 or
 // 2^-12 of each of the terms that dx and dW add up, as in a training step whose pointwise part stands by itself; two parts of each would double the products, which are nearly
-// all of the time); then dx = [dg du] W and dW = [dg du]^T x on the wide tiles whose operands lie with the contracted index as their rows (nothing is transposed in memory), both
-// in one launch where that is estimated to take less time (dense_gemm.hip), and the bias's gradient as sums of the f32 values over strips of rows, added in their order.
+// all of the time; past 65504 they are infinite with fp16); then dx = [dg du] W and dW = [dg du]^T x on the wide tiles whose operands lie with the contracted index as their rows (nothing
+// is transposed in memory), both in one launch where that is estimated to take less time (dense_gemm.hip), and the bias's gradient as f32 sums of the f32 values over strips of rows, added in
+// their order.
 #include <algorithm>
 #include <type_traits>
 

@@ -4,7 +4,9 @@
 // Backward, from the gradients ds of r and dz of z, with rh = r rstd, yh = y rstd_y, v = dz w:
 //   dr = ds + rstd (v - rh sum(v rh) / H) = dx,  dw = sum over rows of dz rh,  dgate = sum over the gate's rows of scale dr b,
 //   u = scale gate dr:  without wp dy = u;  with it dwp = sum over rows of u yh,  dy = rstd_y (u wp - yh sum(u wp yh) / H).
-// All arithmetic in f32 (but f64 in the sums over rows that do not fit the registers), one rounding at the store.
+// All arithmetic in f32 (but f64 in the sums over rows that do not fit the registers), one rounding at the store.  The backward pass takes r as the forward pass rounded it, which is what a
+// training step keeps of it, next to the rstd of the unrounded one: rh is then off by half a step of r's type, as dz and ds are.  Sums over rows that fit the registers are chains of M / 256 additions and less
+// (as many as a block's rows have turns), then those over teams and blocks.
 #include <algorithm>
 
 #include "common.hpp"
@@ -209,8 +211,9 @@ enum Gate { kNoGate, kSharedGate, kOwnGate };  // own: of a row
 // One pass over the four rows: RW waves to a row, `teams` rows to a block at a time, a lane has NV pieces of every row that its team meets and adds up its columns' part of the
 // weights' and the gate's gradients in registers.  sum(u wp yh) is taken apart so that it needs no dr: with c = scale gate wp yh it is sum(c (ds + rstd v)) - rstd sum(v rh) / H
 // sum(c rh), so a row's sums meet in LDS once.  Blocks take parts of a group's rows, so that a shared gate's sums have one place; a team's next row is on its way while
-// this one's sums meet (one piece to a lane; two leave no registers for it).  Bound by HBM: 8192 x 4096 bf16 with both norms and a gate 82 us, 4.9 TB/s of 403 MB; 513 x 3003 fp16 12.4, the latency
-// of one row's chain.
+// this one's sums meet where the registers hold it (rows_ahead: one piece to a lane; two of 16 bits but with both norms and a gate, three of f32).  Bound by HBM: 8192 x 4096 bf16 with both norms and a gate 82 us,
+// 4.9 TB/s of 403 MB.  Few rows: by the sums over rows, column by column through LDS and then a second launch (513 x 3003 fp16 with a gate of each sequence 13.8 us in both launches, 8.2 when neither dweight nor dgate is
+// asked for; two rows of 8192 with both norms and a gate 15.2, 6.2 without any of its three sums).
 template <int DT, int NV, bool POST, int GATE>
 __global__ void __launch_bounds__(NV == 1 ? 1024 : 512) residual_norm_back_kernel(const ResidualNormBack a, const ColumnSums sum_w, const ColumnSums sum_p, const ColumnSums sum_g, int RW, int teams) {
   using P = Pieces<DT>;

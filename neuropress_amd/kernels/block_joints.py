@@ -119,7 +119,8 @@ def residual_norm_backward(
     needs: tuple[bool, bool, bool, bool, bool] = (True, True, True, True, True),
 ) -> tuple[torch.Tensor | None, ...]:
     """Gradients of x, y, weight, post_weight and gate (``npamd_residual_norm_backward``) from those of r and z (None for one of them: zero), in y's dtype; None where *needs* says
-    no or there is no such input.  *stream*, *post_rstd*, *rstd*: r and the statistics of :func:`residual_norm_stats`.  The same bits from run to run."""
+    no or there is no such input.  *stream*, *post_rstd*, *rstd*: r as it was rounded and the statistics of :func:`residual_norm_stats`.  The sums over rows are float32 (float64 past 16384 columns, 8192 of
+    float32).  The same bits from run to run."""
     out = _lib.host().residual_norm_backward(dstream, dnormed, y, stream, weight, post_weight, gate, scale, post_rstd, rstd, *needs)
     if out is not None:
         return out
@@ -223,7 +224,8 @@ def gated_linear_backward(
     bias_dtype: torch.dtype | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
     """Gradients of x, gate_up and the bias (``npamd_gated_linear_backward``) from that of the output, in x's dtype (the bias's in *bias_dtype*, float32 or x's); None where *needs* says
-    no.  *pre*: of :func:`gated_linear_pre`.  What goes into the products is rounded to x's dtype, the products' sums are float32.  The same bits from run to run."""
+    no.  *pre*: of :func:`gated_linear_pre`.  The gradients of both sums go into the products rounded to x's dtype (float16: infinite past 65504), the products' and the bias's sums are float32.  The same bits from run to
+    run."""
     what = "gated_linear_backward"
     code = ACTIVATIONS.get(activation)
     wide = bias_dtype == torch.float32
@@ -282,7 +284,7 @@ def adapter_linear(x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor
     ``[..., K]`` that they share, whose output is *base* ``[..., N]`` (None: zero).
 
     *ids*: int32 or int64, one for each token (x's dimensions but the last) or for each of the first of x's dimensions (``[B]`` for x ``[B, T, K]``); a number that is no adapter's, such as
-    -1, leaves its tokens' base as it is.  Tokens may come in any order; each adapter's weights are read once for up to 16 tokens of a decode step or 128 of a prompt.  For inference: calls that torch
+    -1, leaves its tokens' base as it is.  Tokens may come in any order; an adapter's weights are read once for up to 16 of its tokens in a decode step, in a prompt *a* for up to 32 or 64 and *b* for up to 32 to 128.  For inference: calls that torch
     follows (:func:`tracked`) are refused.
     """
     y = _lib.host().adapter_linear(x, ids, adapters.a, adapters.b, adapters.scale, base, adapters.in_features, adapters.out_features)

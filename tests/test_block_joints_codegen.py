@@ -86,6 +86,12 @@ def test_residual_norm(tmp_path):
         assert not _spills(code) or known, name
 
 
+def test_which_forms_of_the_residual_norm_spill(tmp_path):
+    """16-bit rows: one piece to a lane with both norms and a shared gate; four pieces with a gate, but a row's own without the norm behind."""
+    spilled = {m[0] for name, code in _kernels(tmp_path, "residual_norm.hip", "residual_norm_\\w*kernel") if _spills(code) and (m := re.search(r"ILi[012]ELi\dELb[01]ELi[012]E", name))}
+    assert spilled <= {f"ILi{dt}ELi{rest}E" for dt in (0, 1) for rest in ("1ELb1ELi1", "4ELb1ELi1", "4ELb1ELi2", "4ELb0ELi1")}
+
+
 def test_a_row_has_arrived_before_it_is_overwritten(tmp_path):
     """dx and dy may take the places of ds and y: without the norm behind, whose sums use both, a row's waves meet only when they have them, whatever else is on its way."""
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
