@@ -137,7 +137,7 @@ void refuse_foreign_leaves(const char* what) {
   if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) return (void)hipGetLastError();
   if (status == hipStreamCaptureStatusNone) return;
   const auto node = torch::autograd::get_current_node();
-  TORCH_CHECK(node, what, ": a backward pass cannot be captured outside torch's engine");
+  if (!node) return;  // called by itself, not by torch's engine: nothing goes on to the leaves
   for (const torch::autograd::Edge& edge : node->next_edges()) {
     const auto leaf = std::dynamic_pointer_cast<torch::autograd::AccumulateGrad>(edge.function);
     TORCH_CHECK(!leaf || !leaf->stream() || leaf->stream()->id() == stream.id(), what,

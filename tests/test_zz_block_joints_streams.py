@@ -192,3 +192,24 @@ def test_capture_beside_an_eager_graph_of_one_leaf(gpu, which):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(leaf.grad, torch.autograd.grad(make(), leaf, back)[0])
+
+
+def test_captured_call_of_a_node_by_itself(gpu):
+    """Nothing goes on to the leaves there, so another stream's graph of them is no hindrance."""
+    from neuropress_amd import kernels
+
+    g = cases.gen(4)
+    x, y, w = (torch.randn(s, generator=g).bfloat16().to(gpu).requires_grad_() for s in ((20, 64), (20, 64), (64,)))
+    ds, dz = (torch.randn(20, 64, generator=g).bfloat16().to(gpu) for _ in range(2))
+    out = kernels.residual_norm(x, y, w)
+    want = torch.autograd.grad(out, (x, y, w), (ds, dz), retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = out[0].grad_fn(ds, dz)[:3]
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
