@@ -426,3 +426,10 @@ def test_the_bias_may_change_between_the_passes(gpu, bias_dtype):
         leaves[2].mul_(3.0)
     got = torch.autograd.grad(out, leaves, dh)
     assert got[2].dtype == bias_dtype and all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+@pytest.mark.parametrize("m,n,k", [(16, 512, 4096), (16, 512, 4104), (24, 3584, 3584), (32, 4096, 8192), (33, 2730, 3584), (48, 4096, 8192), (40, 4096, 8200), (17, 6912, 2048), (32, 9728, 2048), (3, 8200, 1024)])
+def test_some_tokens_of_long_rows(gpu, m, n, k):
+    """Both sides of the lines between the kernel for some tokens and the tiles."""
+    x, w, b, _ = _inputs(m, n, k, torch.bfloat16)
+    _check_forward(x, w, b, "silu")
