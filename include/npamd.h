@@ -570,8 +570,8 @@ int npamd_residual_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, 
 /*
  * Its backward pass, from the gradients of both outputs (one of dstream and dnormed may be NULL: zero), y, stream_out as it was rounded, and the statistics; formulas at the
  * kernels (residual_norm.hip).  M at least 1.  dx, dy, dweight, dpost_weight [H] and dgate (a row of H for every row of the gate, one behind the other) may be NULL: not asked for.
- * dx may be dstream, dy may be y or dnormed (with the same row distance).  The sums over rows are added in a fixed order: the same from run to run; in f32 in chains of M / 256 additions and fewer
- * up to 16384 columns (f32: 8192), in f64 past them.
+ * dx may be dstream, dy may be y or dnormed (with the same row distance).  The sums over rows are added in a fixed order: the same from run to run; from 8 to 16384 columns (f32: 4 to 8192)
+ * in f32, in chains of M / 128 additions and fewer, in f64 otherwise.
  * workspace: npamd_residual_norm_workspace_bytes(M, H, gate_every, dtype) bytes (gate_every 0 without a gate) of 16-byte aligned device memory, contents irrelevant; calls
  * that overlap must not share one.
  */
@@ -592,7 +592,8 @@ int npamd_gated_linear(const void* x, int64_t ldx, const void* gate_up, int64_t 
 int64_t npamd_gated_linear_workspace_bytes(int M, int N, int K);
 
 /*
- * Its backward pass from dh [M, N], x, gate_up and pre: with g and u the halves of pre, dg = dh u act'(g) and du = dh act(g) (f32, rounded to act_dtype as operands, with f16 infinite past 65504; NaN where g is),
+ * Its backward pass from dh [M, N], x, gate_up and pre: with g and u the halves of pre, dg = dh u act'(g) and du = dh act(g) (f32, rounded to act_dtype as operands, with f16 infinite past
+ * 65504; NaN where g is, but dg without an activation),
  *   dx = [dg du] gate_up,  dgate_up = [dg du]^T x,  dbias = sums over rows of the unrounded [dg du] (of bias_dtype), f32 sums, each rounded once.
  * dx [M, K], dgate_up [2 N, K], dbias [2 N] may be NULL: not asked for; then what only they need may be, too.  M at least 1.  dh and pre lie at any address; x and gate_up at 16-byte
  * addresses with row distances that are multiples of 8, and their rows are readable up to a multiple of eight columns (the last one too); row distances below

@@ -5,8 +5,8 @@
 //   dr = ds + rstd (v - rh sum(v rh) / H) = dx,  dw = sum over rows of dz rh,  dgate = sum over the gate's rows of scale dr b,
 //   u = scale gate dr:  without wp dy = u;  with it dwp = sum over rows of u yh,  dy = rstd_y (u wp - yh sum(u wp yh) / H).
 // All arithmetic in f32 (but f64 in the sums over rows that do not fit the registers), one rounding at the store.  The backward pass takes r as the forward pass rounded it, which is what a
-// training step keeps of it, next to the rstd of the unrounded one: rh is then off by half a step of r's type, as dz and ds are.  Sums over rows that fit the registers are chains of M / 256 additions and less
-// (as many as a block's rows have turns), then those over teams and blocks.
+// training step keeps of it, next to the rstd of the unrounded one: rh is then off by half a step of r's type, as dz and ds are.  Sums over rows that fit the registers are chains of M / 128 additions and
+// fewer, as many as a team has rows (129 to 256 gates have a block each), then those over teams and blocks.
 #include <algorithm>
 
 #include "common.hpp"

@@ -119,8 +119,8 @@ def residual_norm_backward(
     needs: tuple[bool, bool, bool, bool, bool] = (True, True, True, True, True),
 ) -> tuple[torch.Tensor | None, ...]:
     """Gradients of x, y, weight, post_weight and gate (``npamd_residual_norm_backward``) from those of r and z (None for one of them: zero), in y's dtype; None where *needs* says
-    no or there is no such input.  *stream*, *post_rstd*, *rstd*: r as it was rounded and the statistics of :func:`residual_norm_stats`.  The sums over rows are float32 (float64 past 16384 columns, 8192 of
-    float32).  The same bits from run to run."""
+    no or there is no such input.  *stream*, *post_rstd*, *rstd*: r as it was rounded and the statistics of :func:`residual_norm_stats`.  The sums over rows are float32 from 8 to 16384 columns
+    (float32 rows: 4 to 8192), float64 otherwise.  The same bits from run to run."""
     out = _lib.host().residual_norm_backward(dstream, dnormed, y, stream, weight, post_weight, gate, scale, post_rstd, rstd, *needs)
     if out is not None:
         return out
